@@ -1666,8 +1666,10 @@ extern "C" rg_status rg_debug_hook(rg_ctx* ctx, rg_gpt* m, int what, long long v
             RG_CUDA(cudaMalloc(&da, std::max<size_t>(ha.size(), (size_t)128 * K) * 2));
             RG_CUDA(cudaMalloc(&dw, hw.size() * 2));
             RG_CUDA(cudaMalloc(&dc, (size_t)M * N * 4));
-            RG_CUDA(cudaMemcpy(da, ha.data(), ha.size() * 2, cudaMemcpyHostToDevice));
-            RG_CUDA(cudaMemcpy(dw, hw.data(), hw.size() * 2, cudaMemcpyHostToDevice));
+            // on the context's stream: a pageable cudaMemcpy on the default stream may return before its data has arrived,
+            // and the context's stream does not wait for the default stream
+            RG_CUDA(cudaMemcpyAsync(da, ha.data(), ha.size() * 2, cudaMemcpyHostToDevice, ctx->stream));
+            RG_CUDA(cudaMemcpyAsync(dw, hw.data(), hw.size() * 2, cudaMemcpyHostToDevice, ctx->stream));
             std::vector<float> got((size_t)M * N), parts_sum((size_t)M * N, 0.f);
             rg_status rs = rg_gemm_bf16_tc(ctx, da, M, K, dw, N, dc, N, nullptr, nullptr, 0, -1);
             if (rs == RG_OK && cudaStreamSynchronize(ctx->stream) != cudaSuccess) rs = RG_ERR_BACKEND;
