@@ -56,6 +56,11 @@ typedef struct rg_gpt rg_gpt;         /* GPTModel, src/models/gpt.rs:17-24      
 RG_API int rg_device_count(void);
 /* CudaBackend::new(device_index), src/backend/cuda.rs:87-125; Device::cuda(index), src/backend/mod.rs:72-77 */
 RG_API rg_status rg_ctx_create(int device, rg_ctx** out);
+/* The same on a stream of the caller (a cudaStream_t of that device, NULL for its default stream), for the ops of this
+ * header next to another owner of the GPU: every call enqueues on it, so arrays of that owner that are ordered on the
+ * stream need no further synchronisation in either direction.  The stream must outlive the context and its storages.
+ * rg_gpt_create refuses such a context (RG_ERR_UNSUPPORTED). */
+RG_API rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** out);
 RG_API rg_status rg_ctx_destroy(rg_ctx* ctx);
 /* Backend::synchronize, src/backend/mod.rs:137-138 */
 RG_API rg_status rg_synchronize(rg_ctx* ctx);
@@ -71,12 +76,27 @@ RG_API rg_status rg_ones(rg_ctx* ctx, const size_t* shape, int ndim, rg_storage*
 /* Backend::from_slice(&[f32], &[usize]); len != prod(shape) is RG_ERR_SHAPE (src/backend/cpu.rs:54-57) */
 RG_API rg_status rg_from_slice(rg_ctx* ctx, const float* data, size_t len, const size_t* shape, int ndim,
                         rg_storage** out);
-/* Backend::to_vec: copies prod(shape) floats to out (cap = capacity in floats) and synchronises */
+/* Backend::to_vec: copies prod(shape) floats to out (cap = capacity in floats) and synchronises; bf16 values are widened */
 RG_API rg_status rg_to_vec(rg_ctx* ctx, const rg_storage* st, float* out, size_t cap);
 /* Backend::shape */
 RG_API rg_status rg_shape(const rg_storage* st, size_t* shape_out, int cap, int* ndim_out);
 RG_API size_t rg_storage_len(const rg_storage* st); /* CudaStorage::len, src/backend/cuda.rs:65-67 */
-RG_API rg_status rg_storage_free(rg_storage* st);   /* Drop of the Storage value         */
+RG_API rg_status rg_storage_free(rg_storage* st);   /* Drop of the Storage value; in stream order, without waiting */
+/* DType of a storage (TensorV2::dtype, src/tensor_v2.rs:16-23): RG_DTYPE_F32, or RG_DTYPE_BF16.  Storages are created as
+ * f32; bf16 ones come from rg_cast, rg_from_device and the training ops below.  Ops whose comment does not name bf16 return
+ * RG_ERR_UNSUPPORTED for them. */
+RG_API int rg_storage_dtype(const rg_storage* st);
+/* Values of `a` as `dtype`; bf16 rounds to nearest even.  The same dtype shares the buffer, like rg_reshape. */
+RG_API rg_status rg_cast(rg_ctx* ctx, const rg_storage* a, int dtype, rg_storage** out);
+/* A storage over a contiguous row-major array that the caller owns on the context's GPU.  Nothing is copied when `data` is
+ * 16-byte aligned (otherwise the values are copied on the context's stream).  The array must hold its values in the order of
+ * the context's stream, stay unchanged, and outlive the storage, its reshapes and the work enqueued on them. */
+RG_API rg_status rg_from_device(rg_ctx* ctx, void* data, int dtype, const size_t* shape, int ndim, rg_storage** out);
+/* The storage as a DLPack DLManagedTensor* (kDLCUDA, compact strides) that shares its buffer; its deleter may be called from
+ * any thread.  The consumer reads it in the order of the context's stream, and work on it that another stream enqueued must
+ * be complete (or ordered before the context's stream) when the deleter is called.  A storage made by rg_from_device is
+ * RG_ERR_UNSUPPORTED. */
+RG_API rg_status rg_to_dlpack(const rg_storage* st, void** out);
 
 /* ---- ops: one per Backend trait method, src/backend/mod.rs:157-226.  Each
  * returns a new owned storage; inputs are never modified. ------------------ */
@@ -114,6 +134,40 @@ RG_API rg_status rg_layer_norm(rg_ctx* ctx, const rg_storage* x, const rg_storag
 /* sparse_cross_entropy: mean over rows of -log softmax(logits)[target] (src/backend/cpu.rs:377-427) */
 RG_API rg_status rg_sparse_cross_entropy(rg_ctx* ctx, const rg_storage* logits, const rg_storage* targets,
                                   rg_storage** out);
+
+/* ---- training ops: the device side of the steps between the last block and the optimizer of
+ * WasmGptTrainer::train_step (src/wasm_api.rs:62-94): final LayerNorm, LM head with its loss, their gradients, gradient
+ * clipping.  Activations and matrices are f32 or bf16 (one type per call where not said otherwise); LayerNorm parameters,
+ * biases, targets, statistics, losses and their gradients are f32, as in bf16-weight mode of the model below.  Every sum and
+ * statistic is held in 32 bits or more; results do not depend on timing (no atomics on values).  These calls are not
+ * enqueued into a stream capture (RG_ERR_UNSUPPORTED). ------------------------------------------------------------- */
+/* layer_norm that keeps its statistics for the gradient: y as rg_layer_norm (type of x), mean and rstd = 1/sqrt(var + eps)
+ * f32, one per row (the leading axes of x).  No row is not an error; an empty last axis is RG_ERR_SHAPE. */
+RG_API rg_status rg_layer_norm_fwd(rg_ctx* ctx, const rg_storage* x, const rg_storage* gamma, const rg_storage* beta, float epsilon,
+                                   rg_storage** y, rg_storage** mean, rg_storage** rstd);
+/* Its gradient (the backward closure of the layernorm op, src/ops/): with xh = (x - mean) rstd and a = dy gamma,
+ * dx = rstd (a - mean(a) - xh mean(a xh)) in the type of x; dgamma = sum over rows of dy xh and dbeta = sum over rows of dy,
+ * f32 in the shape of gamma.  dy has the shape and type of x. */
+RG_API rg_status rg_layer_norm_bwd(rg_ctx* ctx, const rg_storage* dy, const rg_storage* x, const rg_storage* gamma, const rg_storage* mean,
+                                   const rg_storage* rstd, rg_storage** dx, rg_storage** dgamma, rg_storage** dbeta);
+/* rg_sparse_cross_entropy of the logits z = x w + bias, without a buffer of all logits: x [R,D], w [D,V] (the Linear layout,
+ * src/nn/linear.rs:14-19; same type as x), bias V values f32 or NULL, targets R values f32 (ids, as rg_sparse_cross_entropy).
+ * Rows whose target equals ignore_index are left out of the mean; any other target outside 0..V-1 is RG_ERR_SHAPE.
+ * loss [1] = mean over the remaining rows of lse - z[target] (0 when none remains); lse [R] = log sum exp z of every row.
+ * The host waits until the targets are checked, not for the result. */
+RG_API rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, const rg_storage* w, const rg_storage* bias,
+                                         const rg_storage* targets, int64_t ignore_index, rg_storage** loss, rg_storage** lse);
+/* Its gradient for an upstream gradient dloss ([1] f32, NULL for 1): with n the number of rows that have a target and
+ * dz = (exp(z - lse) - onehot(target)) dloss / n (0 in ignored rows), dx = dz w^T and dw = x^T dz in the type of x,
+ * dbias [V] = sum over rows of dz, f32 (NULL when bias is NULL; dbias may then be NULL).  lse is what the forward call returned. */
+RG_API rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* x, const rg_storage* w, const rg_storage* bias,
+                                             const rg_storage* targets, int64_t ignore_index, const rg_storage* lse,
+                                             const rg_storage* dloss, rg_storage** dx, rg_storage** dw, rg_storage** dbias);
+/* clip_gradients (src/wasm_api.rs:202-224): norm [1] = sqrt of the sum of squares over all n gradients (f32 and bf16 may be
+ * mixed; sums in f64) and, in out[i], gradient i times min(1, max_norm / norm) in its own type.  max_norm must be positive
+ * (infinity only measures); a NaN anywhere makes norm and every output NaN. */
+RG_API rg_status rg_clip_grad_norm(rg_ctx* ctx, const rg_storage* const* grads, size_t n, float max_norm, rg_storage** out,
+                                   rg_storage** norm);
 
 /* ---- GPT model: src/models/gpt.rs ---------------------------------------- */
 enum { RG_ACT_RELU = 0, RG_ACT_GELU_TANH = 1 };

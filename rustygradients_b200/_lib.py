@@ -83,6 +83,7 @@ SIGNATURES = {
     "rg_version": (C.c_char_p, []),
     "rg_device_count": (C.c_int, []),
     "rg_ctx_create": (None, [C.c_int, _PP]),
+    "rg_ctx_create_on_stream": (None, [C.c_int, _P, _PP]),
     "rg_ctx_destroy": (None, [_P]),
     "rg_synchronize": (None, [_P]),
     "rg_ctx_stream": (C.c_void_p, [_P]),
@@ -94,6 +95,10 @@ SIGNATURES = {
     "rg_shape": (None, [_P, _SZP, C.c_int, C.POINTER(C.c_int)]),
     "rg_storage_len": (C.c_size_t, [_P]),
     "rg_storage_free": (None, [_P]),
+    "rg_storage_dtype": (C.c_int, [_P]),
+    "rg_cast": (None, [_P, _P, C.c_int, _PP]),
+    "rg_from_device": (None, [_P, _P, C.c_int, _SZP, C.c_int, _PP]),
+    "rg_to_dlpack": (None, [_P, _PP]),
     "rg_add": (None, [_P, _P, _P, _PP]),
     "rg_sub": (None, [_P, _P, _P, _PP]),
     "rg_mul": (None, [_P, _P, _P, _PP]),
@@ -112,6 +117,11 @@ SIGNATURES = {
     "rg_embedding": (None, [_P, _P, _P, _PP]),
     "rg_layer_norm": (None, [_P, _P, _P, _P, C.c_float, _PP]),
     "rg_sparse_cross_entropy": (None, [_P, _P, _P, _PP]),
+    "rg_layer_norm_fwd": (None, [_P, _P, _P, _P, C.c_float, _PP, _PP, _PP]),
+    "rg_layer_norm_bwd": (None, [_P, _P, _P, _P, _P, _P, _PP, _PP, _PP]),
+    "rg_linear_cross_entropy": (None, [_P, _P, _P, _P, _P, C.c_int64, _PP, _PP]),
+    "rg_linear_cross_entropy_bwd": (None, [_P, _P, _P, _P, _P, C.c_int64, _P, _P, _PP, _PP, _PP]),
+    "rg_clip_grad_norm": (None, [_P, _PP, _SZ, C.c_float, _PP, _PP]),
     "rg_gpt_create": (None, [_P, C.POINTER(GptConfigC), _PP]),
     "rg_gpt_destroy": (None, [_P]),
     "rg_gpt_num_params": (C.c_int, [_P]),

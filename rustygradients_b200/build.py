@@ -3,16 +3,18 @@ sm_100a with nvcc.  Run as `python -m rustygradients_b200.build` (add -v to see
 ptxas resource usage)."""
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "librg_b200.so")
 SOURCES = ["rg_api.cu", "rg_gpt.cu", "rg_mega.cu", "rg_cloop.cu", "rg_gemm_tc.cu", "rg_attn_tc.cu", "rg_noalloc.cu", "rg_ingest.cu",
-           "rg_tokenizer.cu"]
+           "rg_tokenizer.cu", "rg_train.cu", "rg_lce.cu", "rg_lce_tc.cu"]
 
 
 def _newest_source_mtime() -> float:
@@ -29,17 +31,27 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "nvcc")
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-           "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden", "--use_fast_math" if False else "-DRG_NO_FAST_MATH",
-           "-o", LIB_PATH] + [os.path.join(CSRC, s) for s in SOURCES]
+    arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
+    flags = arch + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-DRG_NO_FAST_MATH"]
     if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+        flags = ["-Xptxas", "-v"] + flags
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+        return res.stderr
+
+    # one object per source, compiled side by side; the library appears only when it is complete
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            logs = list(pool.map(lambda so: run([nvcc] + flags + ["-c", os.path.join(CSRC, so[0]), "-o", so[1]]), zip(SOURCES, objs)))
+        part = LIB_PATH + f".{os.getpid()}.tmp"
+        logs.append(run([nvcc] + arch + ["-shared", "-o", part] + objs))
+        os.replace(part, LIB_PATH)
     if verbose:
-        sys.stderr.write(res.stderr)
+        sys.stderr.write("".join(logs))
     return LIB_PATH
 
 

@@ -6,6 +6,8 @@
 
 #include <string.h>
 
+#include <algorithm>
+
 // ---------------------------------------------------------------------------
 // errors
 // ---------------------------------------------------------------------------
@@ -26,18 +28,32 @@ extern "C" const char* rg_last_error(void) { return g_last_error.c_str(); }
 extern "C" const char* rg_version(void) { return "rg_b200 0.1 (sm_100a)"; }
 
 rg_devbuf::~rg_devbuf() {
-    if (ptr) {
-        int cur = 0;
-        cudaGetDevice(&cur);
-        if (cur != device) cudaSetDevice(device);
-        // the context's stream still exists: stream-ordered free; else (context destroyed first, which synchronised
-        // the stream) a plain free
-        if (!(ctx_alive && *ctx_alive && cudaFreeAsync(ptr, stream) == cudaSuccess)) {
+    if (!ptr || borrowed) return;
+    int cur = 0;
+    cudaGetDevice(&cur);
+    if (cur != device) cudaSetDevice(device);
+    // the context's stream still exists: stream-ordered free; else (context destroyed first, which synchronised
+    // the stream) a plain free.  A stream that is being captured takes no free of this buffer: it waits in `parked`.
+    bool done = false;
+    if (life && life->alive) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
             cudaGetLastError();
-            cudaFree(ptr);
+            life->parked.push_back(ptr);
+            done = true;
+        } else {
+            while (!life->parked.empty()) {
+                cudaFreeAsync(life->parked.back(), stream);
+                life->parked.pop_back();
+            }
+            done = cudaFreeAsync(ptr, stream) == cudaSuccess;
         }
-        if (cur != device) cudaSetDevice(cur);
     }
+    if (!done) {
+        cudaGetLastError();
+        cudaFree(ptr);
+    }
+    if (cur != device) cudaSetDevice(cur);
 }
 
 // ---------------------------------------------------------------------------
@@ -52,7 +68,7 @@ extern "C" int rg_device_count(void) {
     return n;
 }
 
-extern "C" rg_status rg_ctx_create(int device, rg_ctx** out) {
+static rg_status ctx_create(int device, bool own_stream, cudaStream_t stream, rg_ctx** out) {
     if (!out) return rg_fail(RG_ERR_INVALID_INPUT, "rg_ctx_create: out is NULL");
     *out = nullptr;
     int n = rg_device_count();
@@ -67,7 +83,9 @@ extern "C" rg_status rg_ctx_create(int device, rg_ctx** out) {
     rg_ctx* c = new rg_ctx();
     c->device = device;
     c->sm_count = prop.multiProcessorCount;
-    cudaError_t e = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
+    c->own_stream = own_stream;
+    c->stream = stream;
+    cudaError_t e = own_stream ? cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) : cudaSuccess;
     if (e == cudaSuccess) {
         // keep freed op outputs in the device's pool instead of returning them to the driver at every synchronise
         cudaMemPool_t pool = nullptr;
@@ -77,9 +95,13 @@ extern "C" rg_status rg_ctx_create(int device, rg_ctx** out) {
         cudaGetLastError();
     }
     if (e == cudaSuccess) e = cudaMalloc(&c->d_flag, sizeof(int) * 4);
-    if (e == cudaSuccess) e = cudaMemset(c->d_flag, 0, sizeof(int) * 4);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->d_flag, 0, sizeof(int) * 4, c->stream);
     if (e == cudaSuccess) e = cudaMallocHost(&c->h_flag, sizeof(int) * 4);
+    if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->check_ev, cudaEventDisableTiming);
     if (e != cudaSuccess) {
+        cudaFree(c->d_flag);
+        cudaFreeHost(c->h_flag);
+        if (own_stream && c->stream) cudaStreamDestroy(c->stream);
         delete c;
         return rg_fail(RG_ERR_BACKEND, "rg_ctx_create: %s", cudaGetErrorString(e));
     }
@@ -87,15 +109,26 @@ extern "C" rg_status rg_ctx_create(int device, rg_ctx** out) {
     return RG_OK;
 }
 
+extern "C" rg_status rg_ctx_create(int device, rg_ctx** out) { return ctx_create(device, true, nullptr, out); }
+extern "C" rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** out) {
+    return ctx_create(device, false, (cudaStream_t)stream, out);
+}
+
 extern "C" rg_status rg_ctx_destroy(rg_ctx* ctx) {
     if (!ctx) return RG_OK;
-    cudaSetDevice(ctx->device);
-    cudaStreamSynchronize(ctx->stream);
-    *ctx->alive = false;
-    cudaStreamDestroy(ctx->stream);
-    cudaFree(ctx->d_flag);
-    cudaFree(ctx->tc_ws);
-    cudaFreeHost(ctx->h_flag);
+    {
+        std::lock_guard<std::mutex> lock(ctx->life->mu);
+        cudaSetDevice(ctx->device);
+        cudaStreamSynchronize(ctx->stream);
+        ctx->life->alive = false;
+        for (void* p : ctx->life->parked) cudaFree(p);
+        ctx->life->parked.clear();
+        if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
+        cudaEventDestroy(ctx->check_ev);
+        cudaFree(ctx->d_flag);
+        cudaFree(ctx->tc_ws);
+        cudaFreeHost(ctx->h_flag);
+    }
     delete ctx;
     return RG_OK;
 }
@@ -131,27 +164,35 @@ static size_t shape_len(const size_t* shape, int ndim) {
     return n;
 }
 
-rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storage** out) {
-    if (ndim < 0 || ndim > 8) return rg_fail(RG_ERR_DIMENSION, "storage rank %d not in 0..8", ndim);
-    rg_storage* s = new rg_storage();
-    s->ctx = ctx;
-    s->shape.assign(shape, shape + ndim);
-    s->len = shape_len(shape, ndim);
-    s->buf = std::make_shared<rg_devbuf>();
-    s->buf->device = ctx->device;
-    s->buf->bytes = (s->len ? s->len : 1) * sizeof(float);
-    s->buf->stream = ctx->stream;
-    s->buf->ctx_alive = ctx->alive;
-    cudaError_t e = cudaMallocAsync(&s->buf->ptr, s->buf->bytes, ctx->stream);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        const size_t want = s->buf->bytes;
-        s->buf->ptr = nullptr;
-        delete s;
-        return rg_fail(RG_ERR_BACKEND, "Failed to allocate %zu bytes of CUDA memory: %s", want, cudaGetErrorString(e));
-    }
-    *out = s;
+rg_status rg_need_f32(const char* op, const rg_storage* a, const rg_storage* b, const rg_storage* c) {
+    for (const rg_storage* s : {a, b, c})
+        if (s && s->dtype != RG_DTYPE_F32)
+            return rg_fail(RG_ERR_UNSUPPORTED, "%s takes f32 storages; this one holds bf16 (rg_cast converts)", op);
     return RG_OK;
+}
+
+rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storage** out, int dtype) {
+    if (ndim < 0 || ndim > 8) return rg_fail(RG_ERR_DIMENSION, "storage rank %d not in 0..8", ndim);
+    return rg_no_throw([&] {
+        std::unique_ptr<rg_storage> s(new rg_storage());
+        s->ctx = ctx;
+        s->shape.assign(shape, shape + ndim);
+        s->len = shape_len(shape, ndim);
+        s->dtype = dtype;
+        s->buf = std::make_shared<rg_devbuf>();
+        s->buf->device = ctx->device;
+        s->buf->bytes = (s->len ? s->len : 1) * rg_dtype_size(dtype);
+        s->buf->stream = ctx->stream;
+        s->buf->life = ctx->life;
+        cudaError_t e = cudaMallocAsync(&s->buf->ptr, s->buf->bytes, ctx->stream);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            s->buf->ptr = nullptr;
+            return rg_fail(RG_ERR_BACKEND, "Failed to allocate %zu bytes of CUDA memory: %s", s->buf->bytes, cudaGetErrorString(e));
+        }
+        *out = s.release();
+        return RG_OK;
+    });
 }
 
 __global__ void rg_fill_kernel(float* p, size_t n, float v) {
@@ -205,10 +246,138 @@ extern "C" rg_status rg_from_slice(rg_ctx* ctx, const float* data, size_t len, c
 extern "C" rg_status rg_to_vec(rg_ctx* ctx, const rg_storage* st, float* outp, size_t cap) {
     if (!ctx || !st || (!outp && st->len)) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
     if (cap < st->len) return rg_fail(RG_ERR_SHAPE, "rg_to_vec: capacity %zu < %zu elements", cap, st->len);
-    rg_ctx_guard g(ctx);
-    if (st->len) RG_CUDA(cudaMemcpyAsync(outp, st->data(), st->len * sizeof(float), cudaMemcpyDeviceToHost, ctx->stream));
-    RG_CUDA(cudaStreamSynchronize(ctx->stream));
-    return rg_tc_wait_check(ctx);
+    rg_storage* wide = nullptr;  // bf16 values are read as f32
+    if (st->dtype != RG_DTYPE_F32) RG_TRY(rg_cast(ctx, st, RG_DTYPE_F32, &wide));
+    rg_status rs = RG_OK;
+    {
+        rg_ctx_guard g(ctx);
+        const float* src = wide ? wide->data() : st->data();
+        cudaError_t e = cudaSuccess;
+        if (st->len) e = cudaMemcpyAsync(outp, src, st->len * sizeof(float), cudaMemcpyDeviceToHost, ctx->stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+        delete wide;
+        if (e != cudaSuccess)
+            return rg_fail(RG_ERR_BACKEND, "Failed to copy from CUDA: %s", cudaGetErrorString(e));
+        rs = rg_tc_wait_check(ctx);
+    }
+    return rs;
+}
+
+// ---- other arrays on the same GPU ----
+extern "C" rg_status rg_from_device(rg_ctx* ctx, void* data, int dtype, const size_t* shape, int ndim, rg_storage** out) {
+    if (!ctx || !out || (ndim > 0 && !shape)) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    *out = nullptr;
+    if (ndim < 0 || ndim > 8) return rg_fail(RG_ERR_DIMENSION, "storage rank %d not in 0..8", ndim);
+    if (dtype != RG_DTYPE_F32 && dtype != RG_DTYPE_BF16) return rg_fail(RG_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
+    const size_t esize = rg_dtype_size(dtype);
+    size_t len = 1;
+    for (int i = 0; i < ndim; i++) {
+        if (shape[i] && len > ((size_t)1 << 62) / shape[i]) return rg_fail(RG_ERR_SHAPE, "rg_from_device: the shape overflows");
+        len *= shape[i];
+    }
+    rg_op_guard g(ctx);
+    if (!len) return rg_alloc_storage(ctx, shape, ndim, out, dtype);
+    if (!data || (reinterpret_cast<uintptr_t>(data) % esize)) return rg_fail(RG_ERR_INVALID_INPUT, "rg_from_device: not a device array");
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, data) != cudaSuccess) {
+        cudaGetLastError();
+        return rg_fail(RG_ERR_INVALID_INPUT, "rg_from_device: not a device array");
+    }
+    if ((at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) || at.device != ctx->device)
+        return rg_fail(RG_ERR_INVALID_INPUT, "rg_from_device: the array is not in the memory of device %d", ctx->device);
+    if (reinterpret_cast<uintptr_t>(data) & 15) {  // kernels move 16 bytes at a time from the start of a storage: copy
+        RG_TRY(rg_alloc_storage(ctx, shape, ndim, out, dtype));
+        cudaError_t e = cudaMemcpyAsync((*out)->raw(), data, len * esize, cudaMemcpyDeviceToDevice, ctx->stream);
+        if (e != cudaSuccess) {
+            delete *out;
+            *out = nullptr;
+            return rg_fail(RG_ERR_BACKEND, "rg_from_device: %s", cudaGetErrorString(e));
+        }
+        return RG_OK;
+    }
+    return rg_no_throw([&] {
+        std::unique_ptr<rg_storage> s(new rg_storage());
+        s->ctx = ctx;
+        s->shape.assign(shape, shape + ndim);
+        s->len = len;
+        s->dtype = dtype;
+        s->buf = std::make_shared<rg_devbuf>();
+        s->buf->ptr = data;
+        s->buf->bytes = len * esize;
+        s->buf->device = ctx->device;
+        s->buf->borrowed = true;
+        s->buf->life = ctx->life;
+        *out = s.release();
+        return RG_OK;
+    });
+}
+
+extern "C" int rg_storage_dtype(const rg_storage* st) { return st ? st->dtype : RG_DTYPE_F32; }
+
+// The DLPack exchange structures (dlpack.h of the array API standard), version without flags.
+struct dl_device { int32_t type, id; };
+struct dl_dtype { uint8_t code, bits; uint16_t lanes; };
+struct dl_tensor { void* data; dl_device device; int32_t ndim; dl_dtype dtype; int64_t *shape, *strides; uint64_t byte_offset; };
+struct dl_managed { dl_tensor t; void* manager; void (*deleter)(dl_managed*); };
+struct dl_export {
+    dl_managed m;
+    std::shared_ptr<rg_devbuf> buf;
+    int64_t dims[8], strides[8];
+};
+static void dl_release(dl_managed* m) {
+    if (!m) return;
+    dl_export* x = static_cast<dl_export*>(m->manager);
+    std::shared_ptr<rg_ctx_life> life = x->buf->life;
+    std::lock_guard<std::mutex> lock(life->mu);
+    delete x;
+}
+
+extern "C" rg_status rg_to_dlpack(const rg_storage* st, void** out) {
+    if (!st || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    *out = nullptr;
+    if (st->buf->borrowed)
+        return rg_fail(RG_ERR_UNSUPPORTED, "this storage borrows a caller's array (rg_from_device): use that array itself");
+    return rg_no_throw([&] {
+        dl_export* x = new dl_export();
+        x->buf = st->buf;
+        int64_t stride = 1;
+        for (int i = (int)st->shape.size() - 1; i >= 0; i--) {
+            x->dims[i] = (int64_t)st->shape[i], x->strides[i] = stride;
+            stride *= std::max<int64_t>(1, x->dims[i]);
+        }
+        dl_tensor& t = x->m.t;
+        t.data = st->buf->ptr, t.device = {2 /* CUDA */, st->buf->device}, t.ndim = (int32_t)st->shape.size();
+        t.dtype = {(uint8_t)(st->dtype == RG_DTYPE_BF16 ? 4 : 2) /* bfloat, float */, (uint8_t)(8 * rg_dtype_size(st->dtype)), 1};
+        t.shape = x->dims, t.strides = x->strides, t.byte_offset = 0;
+        x->m.manager = x, x->m.deleter = dl_release;
+        *out = &x->m;
+        return RG_OK;
+    });
+}
+
+// f32 -> bf16 rounds to nearest even; bf16 -> f32 is exact
+template <typename A, typename B>
+__global__ void rg_cast_kernel(const A* __restrict__ a, B* __restrict__ b, size_t n) {
+    const size_t stride = (size_t)gridDim.x * blockDim.x;
+    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) b[i] = rg_from_float<B>(rg_to_float(a[i]));
+}
+
+extern "C" rg_status rg_cast(rg_ctx* ctx, const rg_storage* a, int dtype, rg_storage** out) {
+    if (!ctx || !a || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    *out = nullptr;
+    if (dtype != RG_DTYPE_F32 && dtype != RG_DTYPE_BF16) return rg_fail(RG_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
+    RG_TRY(rg_same_ctx(ctx, {a}));
+    if (dtype == a->dtype) return rg_reshape(ctx, a, a->shape.data(), (int)a->shape.size(), out);
+    rg_op_guard g(ctx);
+    RG_TRY(rg_alloc_storage(ctx, a->shape.data(), (int)a->shape.size(), out, dtype));
+    if (!a->len) return RG_OK;
+    const int grid = (int)std::min<size_t>((a->len + 255) / 256, (size_t)ctx->sm_count * 16);
+    if (dtype == RG_DTYPE_BF16)
+        rg_cast_kernel<<<grid, 256, 0, ctx->stream>>>(a->data(), static_cast<__nv_bfloat16*>((*out)->raw()), a->len);
+    else
+        rg_cast_kernel<<<grid, 256, 0, ctx->stream>>>(static_cast<const __nv_bfloat16*>(a->raw()), (*out)->data(), a->len);
+    RG_LAUNCHED(ctx);
+    return rg_launched_ok(out);
 }
 
 extern "C" rg_status rg_shape(const rg_storage* st, size_t* shape_out, int cap, int* ndim_out) {
@@ -223,14 +392,10 @@ extern "C" size_t rg_storage_len(const rg_storage* st) { return st ? st->len : 0
 
 extern "C" rg_status rg_storage_free(rg_storage* st) {
     if (!st) return RG_OK;
-    if (st->ctx) {
-        // the buffer may still be read by kernels queued on the context's stream
-        rg_ctx_guard g(st->ctx);
-        if (st->buf.use_count() == 1) cudaStreamSynchronize(st->ctx->stream);
-        delete st;
-    } else {
-        delete st;
-    }
+    // kernels queued on the context's stream may still use the buffer: it is freed in that stream's order
+    std::shared_ptr<rg_ctx_life> life = st->buf->life;
+    std::lock_guard<std::mutex> lock(life->mu);
+    delete st;
     return RG_OK;
 }
 
@@ -293,6 +458,7 @@ static int grid_for(size_t n, int per_thread = 1) {
 
 static rg_status binary_op(rg_ctx* ctx, const rg_storage* a, const rg_storage* b, rg_storage** out, int op) {
     if (!ctx || !a || !b || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("add / sub / mul", a, b));
     rg_ctx_guard g(ctx);
     const int na = (int)a->shape.size(), nb = (int)b->shape.size(), nd = std::max(na, nb);
     bcast_dims d;
@@ -364,6 +530,7 @@ __global__ void rg_unary_kernel(const float* __restrict__ a, float* __restrict__
 
 static rg_status unary_op(rg_ctx* ctx, const rg_storage* a, rg_storage** out, int op, float param) {
     if (!ctx || !a || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("an elementwise op", a));
     rg_ctx_guard g(ctx);
     RG_TRY(rg_alloc_storage(ctx, a->shape.data(), (int)a->shape.size(), out));
     const size_t n = a->len;
@@ -434,6 +601,7 @@ __global__ void __launch_bounds__(256) rg_softmax_rows_kernel(const float* __res
 
 extern "C" rg_status rg_softmax(rg_ctx* ctx, const rg_storage* a, rg_storage** out) {
     if (!ctx || !a || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("softmax", a));
     if (a->shape.empty()) return rg_fail(RG_ERR_DIMENSION, "softmax requires at least 1 dimension, got 0");
     rg_ctx_guard g(ctx);
     RG_TRY(rg_alloc_storage(ctx, a->shape.data(), (int)a->shape.size(), out));
@@ -466,6 +634,7 @@ __global__ void __launch_bounds__(256) rg_layernorm_rows_kernel(const float* __r
 extern "C" rg_status rg_layer_norm(rg_ctx* ctx, const rg_storage* x, const rg_storage* gamma, const rg_storage* beta,
                                    float epsilon, rg_storage** out) {
     if (!ctx || !x || !gamma || !beta || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("layer_norm", x, gamma, beta));
     if (x->shape.empty()) return rg_fail(RG_ERR_DIMENSION, "layer_norm requires at least 1 dimension, got 0");
     const size_t n = x->shape.back();
     if (gamma->len != n)
@@ -507,6 +676,7 @@ __global__ void __launch_bounds__(1024) rg_sum_all_kernel(const float* __restric
 
 extern "C" rg_status rg_sum(rg_ctx* ctx, const rg_storage* a, rg_storage** out) {
     if (!ctx || !a || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("sum", a));
     rg_ctx_guard g(ctx);
     size_t one = 1;
     RG_TRY(rg_alloc_storage(ctx, &one, 1, out));
@@ -518,6 +688,7 @@ extern "C" rg_status rg_sum(rg_ctx* ctx, const rg_storage* a, rg_storage** out) 
 
 extern "C" rg_status rg_sum_axis(rg_ctx* ctx, const rg_storage* a, size_t axis, rg_storage** out) {
     if (!ctx || !a || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("sum_axis", a));
     if (axis >= a->shape.size())
         return rg_fail(RG_ERR_SHAPE, "Axis %zu out of bounds for array of dimension %zu", axis, a->shape.size());
     rg_ctx_guard g(ctx);
@@ -572,6 +743,7 @@ static rg_status read_flag(rg_ctx* ctx, int* value) {
 extern "C" rg_status rg_sparse_cross_entropy(rg_ctx* ctx, const rg_storage* logits, const rg_storage* targets,
                                              rg_storage** out) {
     if (!ctx || !logits || !targets || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("sparse_cross_entropy", logits, targets));
     if (logits->shape.size() != 2) return rg_fail(RG_ERR_SHAPE, "Logits must be 2D, got %zuD", logits->shape.size());
     const size_t rows = logits->shape[0], n = logits->shape[1];
     if (targets->len != rows)
@@ -619,6 +791,7 @@ extern "C" rg_status rg_reshape(rg_ctx* ctx, const rg_storage* a, const size_t* 
     s->buf = a->buf;
     s->shape.assign(new_shape, new_shape + ndim);
     s->len = a->len;
+    s->dtype = a->dtype;
     *out = s;
     return RG_OK;
 }
@@ -644,6 +817,7 @@ __global__ void rg_permute_kernel(const float* __restrict__ x, float* __restrict
 
 extern "C" rg_status rg_transpose(rg_ctx* ctx, const rg_storage* a, size_t axis1, size_t axis2, rg_storage** out) {
     if (!ctx || !a || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("transpose", a));
     const int nd = (int)a->shape.size();
     if (axis1 >= (size_t)nd || axis2 >= (size_t)nd)
         return rg_fail(RG_ERR_SHAPE, "Transpose axes (%zu, %zu) out of bounds for array of dimension %d", axis1, axis2, nd);
@@ -689,6 +863,7 @@ __global__ void rg_embedding_rows_kernel(const float* __restrict__ idx, const fl
 
 extern "C" rg_status rg_embedding(rg_ctx* ctx, const rg_storage* indices, const rg_storage* weights, rg_storage** out) {
     if (!ctx || !indices || !weights || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("embedding", indices, weights));
     if (weights->shape.size() != 2)
         return rg_fail(RG_ERR_SHAPE, "Embedding weights must be 2D, got %zuD", weights->shape.size());
     if (indices->shape.size() != 1 && indices->shape.size() != 2)
@@ -716,6 +891,7 @@ extern "C" rg_status rg_embedding(rg_ctx* ctx, const rg_storage* indices, const 
 
 extern "C" rg_status rg_matmul(rg_ctx* ctx, const rg_storage* a, const rg_storage* b, rg_storage** out) {
     if (!ctx || !a || !b || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
+    RG_TRY(rg_need_f32("matmul", a, b));
     const int na = (int)a->shape.size(), nb = (int)b->shape.size();
     rg_ctx_guard g(ctx);
     rg_gemm_args p;

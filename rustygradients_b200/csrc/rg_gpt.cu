@@ -353,6 +353,8 @@ static void set_smem_attr(F f, int bytes) {
 extern "C" rg_status rg_gpt_create(rg_ctx* ctx, const rg_gpt_config* cfg, rg_gpt** out) {
     if (!ctx || !cfg || !out) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
     *out = nullptr;
+    if (!ctx->own_stream)  // the token step is captured into a graph and runs beside host copies on the model's stream
+        return rg_fail(RG_ERR_UNSUPPORTED, "a model needs a context with a stream of its own (rg_ctx_create)");
     if (!cfg->block_size || !cfg->vocab_size || !cfg->num_layers || !cfg->num_heads || !cfg->embedding_dim)
         return rg_fail(RG_ERR_INVALID_INPUT, "GptConfig fields must be non-zero");
     if (cfg->embedding_dim % cfg->num_heads != 0)

@@ -9,6 +9,8 @@
 #include <stdio.h>
 
 #include <cstring>
+#include <exception>
+#include <initializer_list>
 #include <memory>
 #include <utility>
 #include <mutex>
@@ -40,19 +42,27 @@ void rg_clear_error();
 // ---------------------------------------------------------------------------
 // handles
 // ---------------------------------------------------------------------------
+// What outlives a context: buffers that left the library (rg_to_dlpack) are released under its lock, from any thread.
+struct rg_ctx_life {
+    std::mutex mu;               // one call at a time per context
+    bool alive = true;           // the context (and its stream) still exists
+    std::vector<void*> parked;   // buffers released while the stream was being captured: freed by the next release outside
+};
+
 struct rg_ctx {
     int device = 0;
     int sm_count = 148;
     cudaStream_t stream = nullptr;
-    std::mutex mu;
+    bool own_stream = true;  // false: the caller's stream (rg_ctx_create_on_stream)
     uint64_t launches = 0;
     int* d_flag = nullptr;  // device word kernels raise on invalid input
     int* h_flag = nullptr;  // pinned mirror
     bool pdl = false;        // launch with programmatic stream serialization (inside a chain of rg_pdl_sync kernels)
     float* tc_ws = nullptr;  // split-k workspace of the tensor-core GEMM (this context's stream only)
     size_t tc_ws_bytes = 0;
-    // storages outlive nothing they need: a buffer frees itself on `stream` only while this is still true
-    std::shared_ptr<bool> alive = std::make_shared<bool>(true);
+    cudaEvent_t check_ev = nullptr;  // the host waits for an op's argument check here, not for the op itself
+    // storages outlive nothing they need: a buffer frees itself on `stream` only while the context is alive
+    std::shared_ptr<rg_ctx_life> life = std::make_shared<rg_ctx_life>();
 };
 
 // Op outputs come from the device's stream-ordered pool (cudaMallocAsync on the context's stream: a few microseconds
@@ -63,8 +73,9 @@ struct rg_devbuf {
     size_t bytes = 0;
     int device = 0;
     cudaStream_t stream = nullptr;
-    std::shared_ptr<bool> ctx_alive;
-    ~rg_devbuf();
+    bool borrowed = false;  // the caller's memory (rg_from_device): never freed here
+    std::shared_ptr<rg_ctx_life> life;
+    ~rg_devbuf();  // the caller holds life->mu
 };
 
 struct rg_storage {
@@ -72,23 +83,72 @@ struct rg_storage {
     std::shared_ptr<rg_devbuf> buf;  // reshape views alias the same buffer
     std::vector<size_t> shape;
     size_t len = 0;
+    int dtype = RG_DTYPE_F32;  // RG_DTYPE_BF16: only where a declaration in rg_b200.h says so
+    const void* raw() const { return buf->ptr; }
+    void* raw() { return buf->ptr; }
     const float* data() const { return static_cast<const float*>(buf->ptr); }
     float* data() { return static_cast<float*>(buf->ptr); }
 };
 
-rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storage** out);
+static inline size_t rg_dtype_size(int dtype) { return dtype == RG_DTYPE_BF16 ? 2 : 4; }
+
+rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storage** out, int dtype = RG_DTYPE_F32);
+// RG_ERR_UNSUPPORTED when one of the (non-NULL) operands of `op` does not hold f32 values
+rg_status rg_need_f32(const char* op, const rg_storage* a, const rg_storage* b = nullptr, const rg_storage* c = nullptr);
 rg_status rg_tc_wait_check(rg_ctx* ctx);  // after a synchronise: did a wait of a tensor-core kernel give up?
 
 struct rg_ctx_guard {
     rg_ctx* c;
     explicit rg_ctx_guard(rg_ctx* ctx) : c(ctx) {
-        c->mu.lock();
+        c->life->mu.lock();
         cudaSetDevice(c->device);
     }
-    ~rg_ctx_guard() { c->mu.unlock(); }
+    ~rg_ctx_guard() { c->life->mu.unlock(); }
+};
+
+// The same for the ops that work next to another owner of the GPU (rg_ctx_create_on_stream): the thread's current
+// device is put back.
+struct rg_op_guard {
+    rg_ctx* c;
+    int before = -1;
+    explicit rg_op_guard(rg_ctx* ctx) : c(ctx) {
+        c->life->mu.lock();
+        cudaGetDevice(&before);
+        if (before != c->device) cudaSetDevice(c->device);
+    }
+    ~rg_op_guard() {
+        if (before >= 0 && before != c->device) cudaSetDevice(before);
+        c->life->mu.unlock();
+    }
 };
 
 #define RG_LAUNCHED(ctx) ((ctx)->launches++)
+
+// Every storage of an op belongs to its context (NULL entries are skipped).
+static inline rg_status rg_same_ctx(const rg_ctx* ctx, std::initializer_list<const rg_storage*> all) {
+    for (const rg_storage* s : all)
+        if (s && s->ctx != ctx) return rg_fail(RG_ERR_INVALID_INPUT, "a storage belongs to another context");
+    return RG_OK;
+}
+
+// C++ exceptions end at the C entry points.
+template <typename F>
+static inline rg_status rg_no_throw(F f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return rg_fail(RG_ERR_BACKEND, "%s", e.what());
+    }
+}
+
+// After the launches of an op: a launch that was refused deletes the outputs and is reported.
+static inline rg_status rg_launched_ok(rg_storage** out) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return RG_OK;
+    delete *out;
+    *out = nullptr;
+    return rg_fail(RG_ERR_BACKEND, "CUDA error %d (%s): %s", (int)e, cudaGetErrorName(e), cudaGetErrorString(e));
+}
 
 #ifdef __CUDACC__
 // Kernel launch that, when pdl is set, may begin before the previous kernel of the stream has finished (the kernel
@@ -205,5 +265,11 @@ __device__ __forceinline__ void rg_pdl_sync() {
 
 __device__ __forceinline__ float rg_to_float(float v) { return v; }
 __device__ __forceinline__ float rg_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T rg_from_float(float v);
+template <>
+__device__ __forceinline__ float rg_from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 rg_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 #endif  // __CUDACC__

@@ -1,0 +1,745 @@
+// Linear cross entropy on the tensor cores (sm_100a): the three contractions of rg_lce.cuh for many rows.
+//
+//   logits  z[R,V]  = x[R,D] w[D,V]      -> (maximum, sum) per row and tile, or dz of a piece of the vocabulary
+//   dx      [R,D]   = dz[R,V] w[D,V]^T
+//   dw      [D,V]   = x[R,D]^T dz[R,V]
+//
+// Every operand is used as it lies in memory: tcgen05 takes a shared-memory tile either with the contraction axis
+// contiguous ("K-major") or with the other axis contiguous ("MN-major"), so no transposed copy of x, w or dz exists.  TMA
+// brings 64-element wide boxes (128-byte swizzle) of three-dimensional arrays [plane][row][column]; what lies outside is
+// filled with zeros, which handles every ragged edge of R, D and V.
+//
+// bf16 inputs are one plane and are multiplied as they are.  f32 inputs are split into three bf16 planes that hold all 24
+// bits (x = x0 + x1 + x2 exactly, each the leading 8 bits of what the planes before leave), and six of the nine products
+// are accumulated; the three left out are below 2^-23 of the product of magnitudes.  The tensor core truncates when it adds
+// to its f32 accumulator, so a long chain loses about 2^-25 of the running sum per step (measured: a relative error of
+// 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32 inputs the chain is therefore cut every 256 elements
+// of K: x0 w0 and the five small products have an accumulator each, and the epilogue warps add both to f32 registers with
+// rounding.
+#include "rg_lce.cuh"
+
+#include <cuda.h>
+
+#include <algorithm>
+
+#define LT_BM 128
+#define LT_BK 64
+#define LT_THREADS 320  // TMA warp, MMA warp, 8 epilogue warps
+#define LT_SPIN_LIMIT (1u << 22)
+#define LT_STAGE_ALL 196608   // bytes of the operand ring
+#define LT_SMEM_BYTES (LT_STAGE_ALL + 8 * 32 * 33 * 4 + 1024 + 256)
+#define LT_SEG 4              // k-blocks per accumulator chain for f32 inputs
+
+template <int PLANES>
+struct lt_shape {
+    static constexpr int BN = PLANES == 1 ? 256 : 128;
+    static constexpr int A_BYTES = LT_BM * LT_BK * 2, B_BYTES = BN * LT_BK * 2;
+    static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
+    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 4 or 2
+};
+
+// One contraction of a launch: C[M,N] = sum over K of A[m,k] B[n,k]
+struct lt_prob {
+    int M, N, K;
+    int tiles_m, tiles_n, splits, kb_per;  // the K axis is cut into `splits` runs of kb_per 64-wide blocks
+    int a_mn, b_mn;                        // 1: the M (N) axis is the contiguous one
+    int b_k0, b_n0;                        // where the piece of the vocabulary starts in B
+};
+
+enum { LT_FWD = 0, LT_DZ = 1, LT_GRAD = 2 };
+
+struct lt_args {
+    lt_prob p[2];
+    int nprobs;
+    int* counter;  // tiles handed out beyond the first of each CTA
+    int* err;
+    int R, D, V;
+    int v0, vn;    // piece of the vocabulary: first column, number of columns
+    const float* bias;
+    const int* tgt;
+    float2* parts;            // LT_FWD
+    float* tz;
+    const float* lse;         // LT_DZ
+    __nv_bfloat16* dz;        // [plane][R][dz_pitch]
+    long long dz_pitch;
+    float* dbparts;           // [4 * tiles_m][V] or NULL
+    float* dxparts;           // LT_GRAD: [splits][R][D]
+    int dx_add;               // add to what the pieces before left there
+    void* dw;                 // [D][V]
+    int dw_bf16;
+    const float* scal;
+};
+
+__device__ __forceinline__ uint32_t lt_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void lt_bar_init(uint64_t* b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(lt_smem(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void lt_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lt_smem(b)) : "memory");
+}
+__device__ __forceinline__ bool lt_wait(uint64_t* bar, uint32_t parity, int* err) {
+    uint32_t ok = 0, spins = 0;
+    while (true) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(lt_smem(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (++spins > LT_SPIN_LIMIT) {
+            atomicExch(err, 1);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ void lt_tma(const CUtensorMap* map, void* dst, uint64_t* bar, int x, int y, int plane) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(lt_smem(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(plane), "r"(lt_smem(bar))
+        : "memory");
+}
+// Shared-memory descriptors, 128-byte swizzle.  K-major: rows of 64 elements (128 bytes), groups of 8 rows 1024 bytes
+// apart.  MN-major: rows of 64 M (N) elements, one per k; groups of 8 k 1024 bytes apart, the next 64 M (N) elements 64
+// rows (8192 bytes) further.
+__device__ __forceinline__ uint64_t lt_desc(uint32_t addr, int mn) {
+    uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
+    if (mn) d |= (uint64_t)(8192 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ void lt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+        "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void lt_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lt_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void lt_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void lt_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// The leading 8 bits of a finite value as bf16 (truncated, so it cannot overflow); what is left is exact in f32.  Infinity
+// and NaN go to the first plane as they are and leave nothing.
+__device__ __forceinline__ void lt_split3(float v, uint32_t& h0, uint32_t& h1, uint32_t& h2) {
+    const uint32_t b0 = __float_as_uint(v) & 0xffff0000u;
+    const bool fin = (b0 & 0x7f800000u) != 0x7f800000u;
+    const float r1 = fin ? v - __uint_as_float(b0) : 0.f;
+    const uint32_t b1 = __float_as_uint(r1) & 0xffff0000u;
+    const float r2 = r1 - __uint_as_float(b1);
+    // a NaN whose leading bits alone would read as infinity stays a NaN
+    h0 = (v != v) ? 0x7fc0u : b0 >> 16, h1 = b1 >> 16, h2 = __float_as_uint(r2) >> 16;
+}
+
+struct lt_tile {
+    int prob, m, n, split;
+};
+template <int EPI>
+__device__ __forceinline__ lt_tile lt_decode(const lt_args& e, int t) {
+    lt_tile r;
+    const int n0 = e.p[0].tiles_m * e.p[0].tiles_n * e.p[0].splits;
+    if (EPI == LT_GRAD && t < n0) {  // dx: the column tiles of one row tile together (they share dz), one run of K after the other
+        r.prob = 0;
+        r.n = t % e.p[0].tiles_n, t /= e.p[0].tiles_n;
+        r.m = t % e.p[0].tiles_m, r.split = t / e.p[0].tiles_m;
+        return r;
+    }
+    // logits and dw: the row tiles of one column tile together (they share w, dz)
+    r.prob = EPI == LT_GRAD ? 1 : 0;
+    if (EPI == LT_GRAD) t -= n0;
+    r.m = t % e.p[r.prob].tiles_m, r.n = t / e.p[r.prob].tiles_m, r.split = 0;
+    return r;
+}
+
+// What a thread keeps of its row while the columns of a tile pass by.
+struct lt_row {
+    int row;        // row of C
+    bool live;      // inside the matrix
+    int tgt;
+    float lse;
+    lce_ms ms;
+};
+
+// 32 consecutive columns of one row per thread (32 rows per warp), starting at column `col` of the tile's matrix.
+template <int PLANES, int EPI>
+__device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, lt_row& w, float (&v)[32], int col, float* stage) {
+    const int lane = threadIdx.x & 31;
+    if (EPI == LT_FWD || EPI == LT_DZ) {
+        const int c = e.v0 + col, left = e.v0 + e.vn - c;  // vocabulary column of v[0]; columns inside the piece
+        if (left <= 0 && EPI == LT_FWD) return;
+        if (e.bias) {
+            if (left >= 32) {
+                const float4* b = reinterpret_cast<const float4*>(e.bias + c);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float4 q = __ldg(b + j);
+                    v[4 * j] += q.x, v[4 * j + 1] += q.y, v[4 * j + 2] += q.z, v[4 * j + 3] += q.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (j < left) v[j] += e.bias[c + j];
+            }
+        }
+        const bool here = w.live && w.tgt >= c && w.tgt < c + 32;
+        const bool any = __any_sync(RG_FULL_MASK, here);
+        if (EPI == LT_FWD) {
+            if (left < 32) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (j >= left) v[j] = -INFINITY;
+            }
+            if (any && here) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (w.tgt == c + j) e.tz[w.row] = v[j];
+            }
+            float m = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; j++) m = fmaxf(m, v[j]);
+            m = fmaxf(m, w.ms.m);
+            const float ref = m == -INFINITY ? 0.f : m;
+            float s = w.ms.s * expf(w.ms.m - ref);
+#pragma unroll
+            for (int j = 0; j < 32; j++) s += expf(v[j] - ref);
+            w.ms = {m, s};
+        } else {
+            const bool dead = !w.live || w.tgt < 0;
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = (dead || j >= left) ? 0.f : expf(v[j] - w.lse);
+            if (any && here) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (w.tgt == c + j) v[j] -= 1.f;
+            }
+            if (w.live && col < e.dz_pitch) {
+                __nv_bfloat16* o = e.dz + (long long)w.row * e.dz_pitch + col;
+                const long long plane = (long long)e.R * e.dz_pitch;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    uint32_t h[3][4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (PLANES == 1) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * k], v[j + 2 * k + 1]);
+                            h[0][k] = *reinterpret_cast<const uint32_t*>(&b);
+                        } else {
+                            uint32_t a0, a1, a2, b0, b1, b2;
+                            lt_split3(v[j + 2 * k], a0, a1, a2);
+                            lt_split3(v[j + 2 * k + 1], b0, b1, b2);
+                            h[0][k] = a0 | (b0 << 16), h[1][k] = a1 | (b1 << 16), h[2][k] = a2 | (b2 << 16);
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < PLANES; p++)
+                        *reinterpret_cast<uint4*>(o + p * plane + j) = make_uint4(h[p][0], h[p][1], h[p][2], h[p][3]);
+                }
+            }
+            if (e.dbparts) {
+                // sums over the warp's 32 rows: 31 halving exchanges leave column `lane` in each lane
+#pragma unroll
+                for (int half = 16; half >= 1; half >>= 1) {
+                    const bool up = lane & half;
+#pragma unroll
+                    for (int i = 0; i < half; i++) {
+                        const float keep = up ? v[i + half] : v[i], send = up ? v[i] : v[i + half];
+                        v[i] = keep + __shfl_xor_sync(RG_FULL_MASK, send, half);
+                    }
+                }
+                const int q = (threadIdx.x >> 5) & 3;
+                if (lane < left) e.dbparts[(size_t)(t.m * 4 + q) * e.V + c + lane] = v[0];
+            }
+        }
+        return;
+    }
+    // gradients: through shared memory, so that a warp stores 32 consecutive columns of one row at a time whatever the
+    // alignment of the rows (the GPT-2 vocabulary is odd)
+#pragma unroll
+    for (int j = 0; j < 32; j++) stage[lane * 33 + j] = v[j];
+    __syncwarp();
+    const int row0 = w.row - lane;
+    const int n = col + lane;
+    const lt_prob& p = e.p[t.prob];
+    const int rows = min(32, p.M - row0);
+    if (n < p.N) {
+        if (t.prob == 0) {
+            float* o = e.dxparts + ((size_t)t.split * e.R + row0) * e.D + n;
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) {
+                float s = stage[r * 33 + lane];
+                if (e.dx_add) s += o[(size_t)r * e.D];
+                o[(size_t)r * e.D] = s;
+            }
+        } else {
+            const float scale = e.scal[1];
+            const size_t at = (size_t)row0 * e.V + e.v0 + n;
+            if (e.dw_bf16) {
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(e.dw) + at;
+#pragma unroll 8
+                for (int r = 0; r < rows; r++) o[(size_t)r * e.V] = __float2bfloat16_rn(stage[r * 33 + lane] * scale);
+            } else {
+                float* o = static_cast<float*>(e.dw) + at;
+#pragma unroll 8
+                for (int r = 0; r < rows; r++) o[(size_t)r * e.V] = stage[r * 33 + lane] * scale;
+            }
+        }
+    }
+    __syncwarp();
+}
+
+template <int PLANES, int EPI>
+__global__ void __launch_bounds__(LT_THREADS, 1)
+lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmA1,
+              const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ lt_args e) {
+    typedef lt_shape<PLANES> S;
+    extern __shared__ unsigned char lt_raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~(uintptr_t)1023);
+    float* stage_all = reinterpret_cast<float*>(ring + LT_STAGE_ALL);
+    uint64_t* full = reinterpret_cast<uint64_t*>(stage_all + 8 * 32 * 33);
+    uint64_t* empty = full + 4;
+    uint64_t* acc_full = empty + 4;     // [2]
+    uint64_t* acc_empty = acc_full + 2; // [2]
+    uint64_t* sched_full = acc_empty + 2;
+    uint64_t* sched_empty = sched_full + 2;
+    uint64_t* drain = sched_empty + 2;
+    volatile int* sched_tile = reinterpret_cast<volatile int*>(drain + 1);  // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int total = 0;
+    for (int i = 0; i < e.nprobs; i++) total += e.p[i].tiles_m * e.p[i].tiles_n * e.p[i].splits;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 4; s++) lt_bar_init(&full[s], 1), lt_bar_init(&empty[s], 1);
+        for (int b = 0; b < 2; b++) {
+            lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 8);
+            lt_bar_init(&sched_full[b], 1), lt_bar_init(&sched_empty[b], 9);
+        }
+        lt_bar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(lt_smem(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ===== one thread hands out tiles and brings their operands =====
+        if (lane == 0) {
+            uint32_t it = 0, ti = 0;
+            bool ok = true;
+            int tile = blockIdx.x;
+            while (true) {
+                const uint32_t slot = ti & 1u;
+                ok = lt_wait(&sched_empty[slot], ((ti >> 1) & 1u) ^ 1u, e.err);
+                if (!ok) break;
+                sched_tile[slot] = tile;
+                lt_arrive(&sched_full[slot]);
+                ti++;
+                if (tile >= total) break;
+                const int next = (int)gridDim.x + atomicAdd(e.counter, 1);  // arrives while this tile is loaded
+                const lt_tile t = lt_decode<EPI>(e, tile);
+                const lt_prob& p = e.p[t.prob];
+                const CUtensorMap* ma = (EPI == LT_GRAD && t.prob) ? &tmA1 : &tmA0;
+                const CUtensorMap* mb = (EPI == LT_GRAD && t.prob) ? &tmB1 : &tmB0;
+                const int m0 = t.m * LT_BM, n0 = t.n * S::BN;
+                const int kb0 = t.split * p.kb_per, kb1 = min(kb0 + p.kb_per, (p.K + LT_BK - 1) / LT_BK);
+                for (int kb = kb0; kb < kb1; kb++, it++) {
+                    const int s = it % S::STAGES;
+                    ok = lt_wait(&empty[s], ((it / S::STAGES) & 1u) ^ 1u, e.err);
+                    if (!ok) break;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lt_smem(&full[s])),
+                                 "r"((uint32_t)S::STAGE_BYTES)
+                                 : "memory");
+                    unsigned char* a = ring + s * S::STAGE_BYTES;
+                    unsigned char* b = a + PLANES * S::A_BYTES;
+                    const int k = kb * LT_BK;
+#pragma unroll
+                    for (int pl = 0; pl < PLANES; pl++) {
+                        if (p.a_mn) {
+                            lt_tma(ma, a + pl * S::A_BYTES, &full[s], m0, k, pl);
+                            lt_tma(ma, a + pl * S::A_BYTES + 8192, &full[s], m0 + 64, k, pl);
+                        } else {
+                            lt_tma(ma, a + pl * S::A_BYTES, &full[s], k, m0, pl);
+                        }
+                        if (p.b_mn) {
+#pragma unroll
+                            for (int j = 0; j < S::BN / 64; j++)
+                                lt_tma(mb, b + pl * S::B_BYTES + j * 8192, &full[s], p.b_n0 + n0 + j * 64, k, pl);
+                        } else {
+                            lt_tma(mb, b + pl * S::B_BYTES, &full[s], p.b_k0 + k, n0, pl);
+                        }
+                    }
+                }
+                if (!ok) break;
+                tile = next;
+            }
+            if (!ok)  // a wait gave up: the copies in flight land before the CTA's memory goes away
+                for (uint32_t i = it > (uint32_t)S::STAGES ? it - S::STAGES : 0; i < it; i++)
+                    lt_wait(&full[i % S::STAGES], (i / S::STAGES) & 1u, e.err);
+        }
+    } else if (warp == 1) {
+        // ===== one thread issues the MMAs =====
+        if (lane == 0) {
+            uint32_t it = 0, ti = 0, seg = 0;
+            bool ok = true;
+            while (true) {
+                const uint32_t slot = ti & 1u;
+                ok = lt_wait(&sched_full[slot], (ti >> 1) & 1u, e.err);
+                if (!ok) break;
+                const int tile = sched_tile[slot];
+                lt_arrive(&sched_empty[slot]);
+                ti++;
+                if (tile >= total) break;
+                const lt_tile t = lt_decode<EPI>(e, tile);
+                const lt_prob& p = e.p[t.prob];
+                const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
+                // D f32, A and B bf16, their majors, N, M
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
+                                       ((uint32_t)(S::BN >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
+                const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
+                const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
+                for (int sg = 0; sg < segs && ok; sg++, seg++) {
+                    const uint32_t buf = seg & 1u;
+                    ok = lt_wait(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, e.err);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d0 = tmem + buf * 256, d1 = d0 + 128;
+                    const int kn = PLANES == 1 ? nkb : min(LT_SEG, nkb - sg * LT_SEG);
+                    for (int kb = 0; kb < kn; kb++, it++) {
+                        const int s = it % S::STAGES;
+                        ok = lt_wait(&full[s], (it / S::STAGES) & 1u, e.err);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t a = lt_smem(ring + s * S::STAGE_BYTES), b = a + PLANES * S::A_BYTES;
+                        if (PLANES == 1) {
+#pragma unroll
+                            for (int k = 0; k < LT_BK / 16; k++)
+                                lt_mma(d0, lt_desc(a + k * astep, p.a_mn), lt_desc(b + k * bstep, p.b_mn), idesc, kb > 0 || k > 0);
+                        } else {
+#pragma unroll
+                            for (int pr = 0; pr < 6; pr++) {
+                                constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
+#pragma unroll
+                                for (int k = 0; k < LT_BK / 16; k++)
+                                    lt_mma(pr == 0 ? d0 : d1, lt_desc(a + pa[pr] * S::A_BYTES + k * astep, p.a_mn),
+                                           lt_desc(b + pb[pr] * S::B_BYTES + k * bstep, p.b_mn), idesc, kb > 0 || k > 0 || pr > 1);
+                            }
+                        }
+                        lt_commit(&empty[s]);
+                    }
+                    if (ok) lt_commit(&acc_full[buf]);
+                }
+                if (!ok) break;
+            }
+            if (!ok) {  // MMAs in flight finish before the tensor memory is given back
+                lt_commit(drain);
+                lt_wait(drain, 0, e.err);
+            }
+        }
+    } else {
+        // ===== epilogue warps: TMEM lane quarter = warp % 4, warps 2..5 the left half of the columns, 6..9 the right =====
+        constexpr int HALF = S::BN / 2;
+        const int q = warp & 3, half = warp < 6 ? 0 : 1;
+        float* stage = stage_all + (warp - 2) * 32 * 33;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + half * HALF;
+        uint32_t ti = 0, seg = 0;
+        bool ok = true;
+        while (true) {
+            const uint32_t slot = ti & 1u;
+            ok = lt_wait(&sched_full[slot], (ti >> 1) & 1u, e.err);
+            if (!ok) break;
+            const int tile = sched_tile[slot];
+            __syncwarp();
+            if (lane == 0) lt_arrive(&sched_empty[slot]);
+            ti++;
+            if (tile >= total) break;
+            const lt_tile t = lt_decode<EPI>(e, tile);
+            const lt_prob& p = e.p[t.prob];
+            lt_row w;
+            w.row = t.m * LT_BM + q * 32 + lane;
+            w.live = w.row < p.M;
+            w.ms = {-INFINITY, 0.f};
+            w.tgt = (EPI != LT_GRAD && w.live) ? e.tgt[w.row] : -1;
+            w.lse = (EPI == LT_DZ && w.live) ? e.lse[w.row] : 0.f;
+            const int c0 = t.n * S::BN + half * HALF;
+            const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
+            const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
+            float acc[PLANES == 1 ? 1 : HALF / 32][32];
+            for (int sg = 0; sg < segs; sg++, seg++) {
+                const uint32_t buf = seg & 1u;
+                ok = lt_wait(&acc_full[buf], (seg >> 1) & 1u, e.err);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t ta = taddr + buf * 256;
+                if (PLANES == 1) {
+#pragma unroll 1
+                    for (int c = 0; c < HALF / 32; c++) {
+                        lt_ld32(ta + c * 32, acc[0]);
+                        lt_ld_wait();
+                        if (c == HALF / 32 - 1) {  // the accumulator has been read: hand it back before the last columns are worked on
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) lt_arrive(&acc_empty[buf]);
+                        }
+                        lt_columns<PLANES, EPI>(e, t, w, acc[0], c0 + c * 32, stage);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < HALF / 32; c++) {
+                        float big[32], small[32];
+                        lt_ld32(ta + c * 32, big);
+                        lt_ld32(ta + 128 + c * 32, small);
+                        lt_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) acc[c][j] = (sg ? acc[c][j] : 0.f) + (big[j] + small[j]);
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) lt_arrive(&acc_empty[buf]);
+                }
+            }
+            if (!ok) break;
+            if (PLANES != 1) {
+#pragma unroll
+                for (int c = 0; c < HALF / 32; c++) lt_columns<PLANES, EPI>(e, t, w, acc[c], c0 + c * 32, stage);
+            }
+            if (EPI == LT_FWD && w.live) e.parts[(size_t)(t.n * 2 + half) * e.R + w.row] = make_float2(w.ms.m, w.ms.s);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// operands
+// ---------------------------------------------------------------------------
+// bf16 planes [plane][rows][pitch] of a matrix whose rows TMA cannot address (f32 values, or rows that do not start on
+// 16-byte boundaries).  A thread writes 16 bytes of each plane.
+template <int PLANES, typename T>
+__global__ void __launch_bounds__(256) lt_pack_kernel(const T* __restrict__ src, long long rows, int cols, int pitch,
+                                                      __nv_bfloat16* __restrict__ dst) {
+    const int groups = pitch / 8;
+    const long long n = rows * groups, stride = (long long)gridDim.x * 256;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+        const long long r = i / groups;
+        const int c = (int)(i - r * groups) * 8;
+        uint32_t h[3][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float a = c + 2 * k < cols ? rg_to_float(src[r * cols + c + 2 * k]) : 0.f;
+            const float b = c + 2 * k + 1 < cols ? rg_to_float(src[r * cols + c + 2 * k + 1]) : 0.f;
+            if (PLANES == 1) {
+                const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);  // exact: the values are bf16
+                h[0][k] = *reinterpret_cast<const uint32_t*>(&q);
+            } else {
+                uint32_t a0, a1, a2, b0, b1, b2;
+                lt_split3(a, a0, a1, a2);
+                lt_split3(b, b0, b1, b2);
+                h[0][k] = a0 | (b0 << 16), h[1][k] = a1 | (b1 << 16), h[2][k] = a2 | (b2 << 16);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PLANES; p++)
+            *reinterpret_cast<uint4*>(dst + (p * rows + r) * pitch + c) = make_uint4(h[p][0], h[p][1], h[p][2], h[p][3]);
+    }
+}
+
+struct lt_operand {
+    const void* base;
+    int rows, cols, planes;
+    long long pitch;  // elements
+};
+
+typedef CUresult (*lt_encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+
+static rg_status lt_encoder(lt_encode_fn* fn) {
+    static lt_encode_fn found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<lt_encode_fn>(f);
+    }();
+    if (!found) return rg_fail(RG_ERR_BACKEND, "cuTensorMapEncodeTiled is not available");
+    *fn = found;
+    return RG_OK;
+}
+
+static rg_status lt_map(CUtensorMap* map, const lt_operand& o, int box_rows) {
+    lt_encode_fn encode = nullptr;
+    RG_TRY(lt_encoder(&encode));
+    const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)o.pitch * 2, (cuuint64_t)o.pitch * 2 * o.rows};
+    const cuuint32_t box[3] = {LT_BK, (cuuint32_t)box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return rg_fail(RG_ERR_BACKEND, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return RG_OK;
+}
+
+// The operand as TMA reads it: the caller's matrix itself, or packed planes in `scratch`.
+static rg_status lt_operand_of(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, rg_storage** scratch, lt_operand* o) {
+    const int planes = dtype == RG_DTYPE_F32 ? 3 : 1;
+    *o = {src, rows, cols, planes, cols};
+    if (planes == 1 && cols % 8 == 0) return RG_OK;
+    const int pitch = (cols + 7) / 8 * 8;
+    const size_t halves = (size_t)planes * rows * pitch;
+    RG_TRY(rg_alloc_storage(ctx, &halves, 1, scratch, RG_DTYPE_BF16));
+    o->base = (*scratch)->raw(), o->pitch = pitch;
+    const int grid = (int)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>((*scratch)->raw());
+    if (planes == 3) lt_pack_kernel<3, float><<<grid, 256, 0, ctx->stream>>>((const float*)src, rows, cols, pitch, dst);
+    else lt_pack_kernel<1, __nv_bfloat16><<<grid, 256, 0, ctx->stream>>>((const __nv_bfloat16*)src, rows, cols, pitch, dst);
+    RG_LAUNCHED(ctx);
+    return RG_OK;
+}
+
+static int lt_bn(int dtype) { return dtype == RG_DTYPE_F32 ? lt_shape<3>::BN : lt_shape<1>::BN; }
+int lce_tc_nparts(int V, int dtype) { return 2 * rg_cdiv(V, lt_bn(dtype)); }
+
+static lt_prob lt_problem(int M, int N, int K, int bn, int a_mn, int b_mn) {
+    lt_prob p;
+    memset(&p, 0, sizeof(p));
+    p.M = M, p.N = N, p.K = K;
+    p.tiles_m = rg_cdiv(M, LT_BM), p.tiles_n = rg_cdiv(N, bn), p.splits = 1, p.kb_per = rg_cdiv(K, LT_BK);
+    p.a_mn = a_mn, p.b_mn = b_mn;
+    return p;
+}
+
+template <int PLANES, int EPI>
+static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
+    RG_CUDA(cudaFuncSetAttribute(lce_tc_kernel<PLANES, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_SMEM_BYTES));
+    long long total = 0;
+    for (int i = 0; i < e.nprobs; i++) total += (long long)e.p[i].tiles_m * e.p[i].tiles_n * e.p[i].splits;
+    if (total > 0x3fffffff) return rg_fail(RG_ERR_SHAPE, "linear_cross_entropy: too many tiles");
+    RG_CUDA(cudaMemsetAsync(e.counter, 0, sizeof(int), ctx->stream));
+    const int grid = (int)std::min<long long>(total, ctx->sm_count);
+    lce_tc_kernel<PLANES, EPI><<<grid, LT_THREADS, LT_SMEM_BYTES, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], e);
+    RG_CUDA(cudaGetLastError());
+    RG_LAUNCHED(ctx);
+    return RG_OK;
+}
+template <int EPI>
+static rg_status lt_run(rg_ctx* ctx, const lce_call& c, const CUtensorMap* maps, lt_args& e) {
+    return c.dtype == RG_DTYPE_F32 ? lt_launch<3, EPI>(ctx, maps, e) : lt_launch<1, EPI>(ctx, maps, e);
+}
+
+static void lt_common(rg_ctx* ctx, const lce_call& c, rg_storage* counter, lt_args* e) {
+    memset(e, 0, sizeof(*e));
+    e->counter = reinterpret_cast<int*>(counter->raw()), e->err = ctx->d_flag + 1;
+    e->R = c.R, e->D = c.D, e->V = c.V, e->v0 = 0, e->vn = c.V;
+    e->bias = c.bias, e->tgt = c.tgt, e->lse = c.lse, e->scal = c.scal;
+    e->parts = c.parts, e->tz = c.tz;
+}
+
+rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
+    rg_outputs<3> o;  // packed x, packed w, counter
+    lt_operand x, w;
+    const size_t one = 1;
+    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[2]));
+    RG_TRY(lt_operand_of(ctx, c.x, c.R, c.D, c.dtype, &o[0], &x));
+    RG_TRY(lt_operand_of(ctx, c.w, c.D, c.V, c.dtype, &o[1], &w));
+    CUtensorMap maps[4];
+    RG_TRY(lt_map(&maps[0], x, LT_BM));
+    RG_TRY(lt_map(&maps[1], w, LT_BK));
+    maps[2] = maps[0], maps[3] = maps[1];
+    lt_args e;
+    lt_common(ctx, c, o[2], &e);
+    e.nprobs = 1;
+    e.p[0] = lt_problem(c.R, c.V, c.D, lt_bn(c.dtype), 0, 1);
+    return lt_run<LT_FWD>(ctx, c, maps, e);
+}
+
+// The gradient goes over pieces of the vocabulary: dz of a piece (at most LT_DZ_BYTES, whatever R and V are) is written as
+// bf16 planes, then one launch multiplies it with w and with x.
+#define LT_DZ_BYTES ((size_t)512 << 20)
+
+rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
+    rg_outputs<6> o;  // packed x, packed w, counter, dz, partial dx, partial dbias
+    lt_operand x, w;
+    const size_t one = 1;
+    const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = lt_bn(c.dtype);
+    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[2]));
+    RG_TRY(lt_operand_of(ctx, c.x, c.R, c.D, c.dtype, &o[0], &x));
+    RG_TRY(lt_operand_of(ctx, c.w, c.D, c.V, c.dtype, &o[1], &w));
+
+    const long long most = std::max<long long>(1, (long long)(LT_DZ_BYTES / ((size_t)planes * 2 * c.R)) / 256) * 256;
+    const int pieces = (int)((c.V + most - 1) / most);
+    const int piece = (int)std::min<long long>(most, (rg_cdiv(c.V, pieces) + 255) / 256 * 256);
+    const int width = std::min(piece, (c.V + 63) / 64 * 64);  // columns of dz that are stored
+    const size_t zlen = (size_t)planes * c.R * width;
+    RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[3], RG_DTYPE_BF16));
+
+    // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
+    lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(c.D, piece, c.R, bn, 1, 1);
+    const long long load = (long long)pdx.tiles_m * pdx.tiles_n * pdx.kb_per + (long long)pdw.tiles_m * pdw.tiles_n * pdw.kb_per;
+    const int fair = (int)std::max<long long>(LT_SEG, load / ctx->sm_count / 2);
+    // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
+    const int run = rg_cdiv(pdx.kb_per, std::min(16, rg_cdiv(pdx.kb_per, fair))), splits = rg_cdiv(pdx.kb_per, run);
+    const size_t plen = (size_t)splits * c.R * c.D;
+    RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[4]));
+    const int dbrows = 4 * rg_cdiv(c.R, LT_BM);
+    if (c.dbias) {
+        const size_t blen = (size_t)dbrows * c.V;
+        RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[5]));
+    }
+
+    CUtensorMap mz[4], mg[4];
+    lt_operand z = {o[3]->raw(), c.R, width, planes, width};
+    RG_TRY(lt_map(&mz[0], x, LT_BM));
+    RG_TRY(lt_map(&mz[1], w, LT_BK));
+    mz[2] = mz[0], mz[3] = mz[1];
+    RG_TRY(lt_map(&mg[0], z, LT_BM));
+    RG_TRY(lt_map(&mg[1], w, bn));
+    RG_TRY(lt_map(&mg[2], x, LT_BK));
+    RG_TRY(lt_map(&mg[3], z, LT_BK));
+
+    for (int i = 0; i < pieces; i++) {
+        lt_args e;
+        lt_common(ctx, c, o[2], &e);
+        e.v0 = i * piece, e.vn = std::min(piece, c.V - e.v0);
+        e.dz = static_cast<__nv_bfloat16*>(o[3]->raw()), e.dz_pitch = width;
+        e.dbparts = c.dbias ? o[5]->data() : nullptr;
+        e.dxparts = o[4]->data(), e.dx_add = i > 0;
+        e.dw = c.dw, e.dw_bf16 = c.dtype == RG_DTYPE_BF16;
+        e.nprobs = 1;
+        e.p[0] = lt_problem(c.R, e.vn, c.D, bn, 0, 1);
+        e.p[0].b_n0 = e.v0;
+        RG_TRY(lt_run<LT_DZ>(ctx, c, mz, e));
+        e.nprobs = 2;
+        e.p[0] = lt_problem(c.R, c.D, e.vn, bn, 0, 0);
+        e.p[0].splits = rg_cdiv(e.p[0].kb_per, run), e.p[0].kb_per = run;
+        e.p[0].b_k0 = e.v0;
+        e.p[1] = lt_problem(c.D, e.vn, c.R, bn, 1, 1);
+        RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
+    }
+    lce_dx_finish_launch(ctx, o[4]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
+    if (c.dbias) lce_dbias_finish_launch(ctx, o[5]->data(), dbrows, c.V, c.scal, c.dbias);
+    return RG_OK;
+}

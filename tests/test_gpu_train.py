@@ -1,0 +1,444 @@
+"""GPU parity of the training ops (LayerNorm with statistics and gradient, linear cross entropy with gradient, clipping
+by the global norm) against their formulas in 64 bits.
+
+Tolerances are worst-case bounds of the arithmetic, worked out per element beside each check: U is half a step of the
+output type (relative), E32 = 2^-23 one step of f32."""
+import numpy as np
+import pytest
+
+import rustygradients_b200 as rg
+
+pytestmark = pytest.mark.gpu
+
+E32 = 2.0 ** -23
+U = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8}
+EPS = 1e-5
+
+
+def rounded(a, dtype):
+    """The f32 array whose values are exactly representable in dtype."""
+    a = np.ascontiguousarray(a, np.float32)
+    if dtype == "f32":
+        return a
+    b = a.view(np.uint32).astype(np.uint64)
+    b = ((b + 0x7FFF + ((b >> 16) & 1)) & 0xFFFF0000).astype(np.uint32)
+    return b.view(np.float32).reshape(a.shape)
+
+
+def put(be, a, dtype="f32"):
+    st = be.from_slice(a, list(a.shape))
+    return st if dtype == "f32" else be.cast(st, dtype)
+
+
+def get(be, st):
+    return be.to_array(st).astype(np.float64)
+
+
+def within(got, want, tol, what=""):
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float(np.nanmax(np.abs(got - want) / tol)), np.argwhere(bad)[:3].tolist())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# storages: types and other owners' memory
+# ---------------------------------------------------------------------------------------------------------------------
+def test_cast_and_dtype(backend):
+    be = backend
+    x = np.array([0.0, -0.0, 1.0, 1.00390625, 1.01171875, 3.4e38, np.inf, -np.inf, 1e-40], np.float32)   # ties both ways
+    s = be.from_slice(x, [9])
+    h = be.cast(s, "bf16")
+    assert (s.dtype, h.dtype) == ("f32", "bf16") and h.shape == [9] and len(h) == 9
+    assert np.array_equal(be.to_vec(h), rounded(x, "bf16"))
+    assert np.isnan(be.to_vec(be.cast(be.from_slice([np.nan], [1]), "bf16")))[0]
+    assert np.array_equal(be.to_vec(be.cast(h, "f32")), be.to_vec(h))
+    assert be.cast(h, "bf16").dtype == "bf16" and be.reshape(h, [3, 3]).dtype == "bf16"
+    for op in (lambda: be.add(h, h), lambda: be.relu(h), lambda: be.softmax(h), lambda: be.sum(h), lambda: be.sum_axis(h, 0),
+               lambda: be.transpose(be.reshape(h, [3, 3]), 0, 1), lambda: be.matmul(be.reshape(h, [3, 3]), be.reshape(h, [3, 3])),
+               lambda: be.layer_norm(h, s, s, EPS), lambda: be.embedding(s, be.reshape(h, [3, 3])),
+               lambda: be.sparse_cross_entropy(be.reshape(h, [3, 3]), be.zeros([3]))):
+        with pytest.raises(rg.Unsupported):
+            op()
+    with pytest.raises(rg.Unsupported):
+        be.cast(s, "f16")
+
+
+def test_arrays_of_another_owner():
+    import torch
+    torch.cuda.set_device(0)
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            be = rg.B200Backend(0, stream=stream.cuda_stream)
+            t = torch.arange(24, dtype=torch.float32, device="cuda").reshape(4, 6)
+            s = be.from_device(t)
+            assert s.shape == [4, 6] and np.array_equal(be.to_array(s), t.cpu().numpy())
+            back = torch.from_dlpack(be.add(s, s))
+            assert torch.equal(back, 2 * t) and back.is_cuda
+            # a slice that starts off a 16-byte boundary is copied: later writes to the tensor are not seen
+            odd = be.from_device(t.reshape(-1)[1:])
+            t.add_(1)
+            assert np.array_equal(be.to_vec(odd), np.arange(1, 24, dtype=np.float32))
+            assert np.array_equal(be.to_vec(s), t.reshape(-1).cpu().numpy())
+            t16 = torch.randn(5, 7, device="cuda").bfloat16()
+            h = be.from_device(t16)
+            assert h.dtype == "bf16" and torch.equal(torch.from_dlpack(be.cast(h, "f32")), t16.float())
+            assert torch.equal(torch.utils.dlpack.from_dlpack(be.cast(be.from_device(t16.float()), "bf16").to_dlpack()), t16)
+            # views keep the borrowed tensor alive
+            view = be.reshape(be.from_device(torch.full((8,), 3.0, device="cuda")), [2, 4])
+            torch.full((8,), 5.0, device="cuda")
+            assert np.all(be.to_vec(view) == 3)
+            assert be.from_device(torch.empty(0, 3, device="cuda")).shape == [0, 3]
+            # capsules nobody takes, and tensors that outlive their storage and the backend object
+            be.ones([1 << 20]).to_dlpack()
+            keep = torch.from_dlpack(be.ones([3]))
+            with pytest.raises(BufferError):
+                be.ones([1]).__dlpack__(stream=12345)
+            with pytest.raises(rg.Unsupported):
+                s.to_dlpack()
+            for bad, err in ((t.t(), rg.InvalidInput), (t.cpu(), rg.InvalidInput), (t.double(), rg.Unsupported),
+                             (np.ones(3, np.float32), rg.InvalidInput), (t.reshape((1,) * 7 + (4, 6)), rg.DimensionError)):
+                with pytest.raises(err):
+                    be.from_device(bad)
+            with pytest.raises(rg.Unsupported):
+                rg.GPTModel(be, rg.GptConfig(16, 30, 1, 2, 64))
+            stream.synchronize()
+            be.close()
+            assert keep.sum().item() == 3
+
+
+def test_a_context_refuses_storages_of_another(backend):
+    other = rg.B200Backend(0)
+    x, g = other.ones([2, 4]), backend.ones([4])
+    for call in (lambda: backend.layer_norm_fwd(x, g, g, EPS), lambda: backend.clip_grad_norm([x], 1.0), lambda: backend.cast(x, "bf16"),
+                 lambda: backend.linear_cross_entropy(x, backend.ones([4, 3]), None, backend.zeros([2]))):
+        with pytest.raises(rg.InvalidInput):
+            call()
+
+
+def test_calls_inside_a_capture_are_refused():
+    import torch
+    torch.cuda.set_device(0)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        be = rg.B200Backend(0, stream=stream.cuda_stream)
+        x, g, w, t = be.ones([2, 4]), be.ones([4]), be.ones([4, 3]), be.zeros([2])
+        y, m, r = be.layer_norm_fwd(x, g, g, EPS)
+        dead = be.ones([5])
+        graph = torch.cuda.CUDAGraph()
+        a = torch.zeros(4, device="cuda")
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            a.add_(1)
+            for call in (lambda: be.layer_norm_fwd(x, g, g, EPS), lambda: be.layer_norm_bwd(y, x, g, m, r),
+                         lambda: be.linear_cross_entropy(x, w, None, t), lambda: be.linear_cross_entropy_bwd(x, w, None, t, t),
+                         lambda: be.clip_grad_norm([x], 1.0)):
+                with pytest.raises(rg.Unsupported):
+                    call()
+            del dead      # its memory is given back after the capture
+        graph.replay()
+        stream.synchronize()
+        assert a.sum().item() == 4
+        assert np.allclose(be.to_vec(be.layer_norm_fwd(x, g, g, EPS)[0]), be.to_vec(y))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# LayerNorm
+# ---------------------------------------------------------------------------------------------------------------------
+def ln_inputs(rows, n, dtype, seed=0):
+    rng = np.random.default_rng(seed + 31 * rows + n)
+    x = rounded(rng.standard_normal((rows, n)) * rng.uniform(0.3, 4, (rows, 1)) + rng.uniform(-5, 5, (rows, 1)), dtype)
+    dy = rounded(rng.standard_normal((rows, n)), dtype)
+    g = (1 + 0.3 * rng.standard_normal((1, n))).astype(np.float32)
+    b = (0.5 * rng.standard_normal((1, n))).astype(np.float32)
+    return x, dy, g, b
+
+
+def ln_exact(x, g, b):
+    x = x.astype(np.float64)
+    mean = x.mean(-1, keepdims=True)
+    rstd = 1 / np.sqrt(((x - mean) ** 2).mean(-1, keepdims=True) + np.float64(np.float32(EPS)))
+    return (x - mean) * rstd * g + b, mean, rstd
+
+
+LN_SHAPES = [(1, 1), (3, 1), (1, 768), (2, 2), (5, 7), (64, 8), (33, 192), (9, 255), (17, 256), (4, 257), (6, 514), (300, 768),
+             (37, 1023), (8, 1024), (3, 1026), (650, 1600), (5, 2050), (3, 4097), (2, 4104), (2, 8192), (3, 8200), (2, 12001),
+             (2, 16384), (3, 16386), (70, 20001)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", LN_SHAPES)
+def test_layer_norm_forward_and_gradient(backend, rows, n, dtype):
+    be = backend
+    x, dy, g, b = ln_inputs(rows, n, dtype)
+    X, DY, G, B = put(be, x, dtype), put(be, dy, dtype), put(be, g), put(be, b)
+    y, mean, rstd = be.layer_norm_fwd(X, G, B, EPS)
+    assert (y.dtype, mean.dtype, y.shape, mean.shape, rstd.shape) == (dtype, "f32", [rows, n], [rows], [rows])
+    wy, wm, wr = ln_exact(x, g, b)
+    # a sum of n terms: per-thread chains of at most 40 terms (n <= 20001 over 512 threads), then <= 10 levels
+    chain = 52 * 2.0 ** -24
+    tm = chain * np.abs(x).mean(-1, keepdims=True) + 2 * E32 * np.abs(wm)
+    within(get(be, mean), wm[:, 0], tm[:, 0] + 1e-45, "mean")
+    # variance: relative chain error, 3 roundings a term, and the mean's error squared; half of it in rstd
+    dev = np.abs(x - wm).max(-1, keepdims=True) + tm
+    tr = wr * ((chain + 4 * E32) + 0.5 * wr ** 2 * (tm ** 2 + 2 * E32 * dev ** 2) + 2 * E32)
+    within(get(be, rstd), wr[:, 0], tr[:, 0], "rstd")
+    xh = np.abs((x - wm) * wr)
+    ty = np.abs(g) * (tm * wr + xh * (tr / wr) + 4 * E32 * (xh + np.abs(x) * wr)) + E32 * (np.abs(wy) + np.abs(b))
+    within(get(be, y), wy, ty + U[dtype] * (np.abs(wy) + ty), "y")
+    if n == 1 or rows * n < 3:
+        assert np.all(np.isfinite(get(be, y)))
+    # gradient, from exact statistics rounded to f32
+    m32, r32 = wm[:, 0].astype(np.float32), wr[:, 0].astype(np.float32)
+    dx, dg, db = be.layer_norm_bwd(DY, X, G, put(be, m32), put(be, r32))
+    assert (dx.dtype, dg.dtype, dx.shape, dg.shape, db.shape) == (dtype, "f32", [rows, n], [1, n], [1, n])
+    x6, d6, m6, r6 = x.astype(np.float64), dy.astype(np.float64), m32[:, None].astype(np.float64), r32[:, None].astype(np.float64)
+    h = (x6 - m6) * r6
+    a = d6 * g
+    wdx = r6 * (a - a.mean(-1, keepdims=True) - h * (a * h).mean(-1, keepdims=True))
+    th = 2 * E32 * (np.abs(h) + np.abs(x6) * 0)                 # one subtraction (exact to half a step of x - m) and one product
+    mag = np.abs(a) + np.abs(a).mean(-1, keepdims=True) + np.abs(h) * np.abs(a * h).mean(-1, keepdims=True)
+    tdx = np.abs(r6) * mag * (2 * chain + 8 * E32)
+    within(get(be, dx), wdx, tdx + U[dtype] * (np.abs(wdx) + tdx), "dx")
+    # columns: a chain of at most rows / partial rows terms, then the partial rows (32 slices)
+    steps = (rows + 40) * 2.0 ** -24
+    within(get(be, dg), (d6 * h).sum(0, keepdims=True), (steps + 4 * E32) * np.abs(d6 * h).sum(0, keepdims=True) +
+           (np.abs(d6) * th).sum(0, keepdims=True) + 1e-45, "dgamma")
+    within(get(be, db), d6.sum(0, keepdims=True), steps * np.abs(d6).sum(0, keepdims=True) + 1e-45, "dbeta")
+
+
+def test_layer_norm_gradient_against_differences(backend):
+    be = backend
+    x, dy, g, b = ln_inputs(4, 96, "f32", 5)
+    y, mean, rstd = be.layer_norm_fwd(put(be, x), put(be, g), put(be, b), EPS)
+    dx, dg, db = (get(be, s) for s in be.layer_norm_bwd(put(be, dy), put(be, x), put(be, g), mean, rstd))
+    rng = np.random.default_rng(3)
+
+    def f(x_, g_, b_):
+        return float((ln_exact(x_, g_, b_)[0] * dy).sum())
+
+    for k in range(3):
+        vx, vg, vb = rng.standard_normal(x.shape), rng.standard_normal(g.shape), rng.standard_normal(b.shape)
+        e = 1e-5
+        num = (f(x + e * vx, g + e * vg, b + e * vb) - f(x - e * vx, g - e * vg, b - e * vb)) / (2 * e)
+        ana = (dx * vx).sum() + (dg * vg).sum() + (db * vb).sum()
+        # differences: O(e^2) third derivatives ~ 1e-10 of scale 1e3, cancellation 2^-52 * 1e3 / e ~ 2e-8; f32 gradient 1e-5
+        assert abs(num - ana) <= 2e-4 * (1 + np.abs(dx * vx).sum())
+
+
+def test_layer_norm_far_from_zero_and_not_finite(backend):
+    """Rows whose mean is far from zero keep their variance; a row with a NaN or infinity leaves the other rows alone."""
+    be = backend
+    x = np.random.default_rng(9).standard_normal((4, 768)).astype(np.float32) + np.array([[1e4], [0], [0], [-3e3]], np.float32)
+    x[1, 5], x[2, 700] = np.nan, np.inf
+    g, b = np.ones((1, 768), np.float32), np.zeros((1, 768), np.float32)
+    y, mean, rstd = (get(be, s) for s in be.layer_norm_fwd(put(be, x), put(be, g), put(be, b), EPS))
+    for r in (0, 3):
+        wy, wm, wr = ln_exact(x[r:r + 1], g, b)
+        # the mean is off by its chain (16 terms a thread, 6 levels) relative to 1e4; the deviations from it are exact
+        tm = 24 * 2.0 ** -24 * np.abs(x[r]).mean() + E32 * abs(float(wm[0, 0]))
+        assert abs(mean[r] - wm[0, 0]) <= tm and abs(rstd[r] / wr[0, 0] - 1) <= 1e-5 + tm ** 2
+        assert np.abs(y[r] - wy[0]).max() <= 2 * tm + 1e-4
+    assert np.isnan(y[1]).all() and np.isnan(mean[1])
+    assert np.isnan(y[2]).any() and not np.isfinite(mean[2])
+
+
+def test_layer_norm_ranks_empty_and_refusals(backend):
+    be = backend
+    x, dy, g, b = ln_inputs(6, 10, "f32")
+    G, B = put(be, g), put(be, b)
+    y3, m3, r3 = be.layer_norm_fwd(be.from_slice(x, [2, 3, 10]), G, B, EPS)
+    y2, m2, r2 = be.layer_norm_fwd(put(be, x), G, B, EPS)
+    assert y3.shape == [2, 3, 10] and m3.shape == [2, 3] and np.array_equal(be.to_vec(y3), be.to_vec(y2))
+    y1, m1, r1 = be.layer_norm_fwd(be.from_slice(x[0], [10]), G, B, EPS)
+    assert m1.shape == [] and np.array_equal(be.to_vec(y1), be.to_vec(y2)[:10])
+    dx, dg, db = be.layer_norm_bwd(be.from_slice(dy[0], [10]), be.from_slice(x[0], [10]), G, m1, r1)
+    assert dx.shape == [10] and dg.shape == [1, 10]
+    y0, m0, r0 = be.layer_norm_fwd(be.zeros([0, 10]), G, B, EPS)
+    assert y0.shape == [0, 10] and m0.shape == [0]
+    dx, dg, db = be.layer_norm_bwd(be.zeros([0, 10]), be.zeros([0, 10]), G, m0, r0)
+    assert dx.shape == [0, 10] and not be.to_vec(dg).any() and not be.to_vec(db).any()
+    X, M, R = put(be, x), m2, r2
+    H = be.cast(X, "bf16")
+    for call, err in ((lambda: be.layer_norm_fwd(X, be.ones([9]), B, EPS), rg.ShapeError),
+                      (lambda: be.layer_norm_fwd(X, G, be.ones([11]), EPS), rg.ShapeError),
+                      (lambda: be.layer_norm_fwd(be.zeros([3, 0]), be.zeros([0]), be.zeros([0]), EPS), rg.ShapeError),
+                      (lambda: be.layer_norm_fwd(be.from_slice([1.0], []), G, B, EPS), rg.DimensionError),
+                      (lambda: be.layer_norm_fwd(X, be.cast(G, "bf16"), B, EPS), rg.Unsupported),
+                      (lambda: be.layer_norm_bwd(H, X, G, M, R), rg.Unsupported),
+                      (lambda: be.layer_norm_bwd(be.zeros([10, 6]), X, G, M, R), rg.ShapeError),
+                      (lambda: be.layer_norm_bwd(X, X, G, be.zeros([5]), R), rg.ShapeError),
+                      (lambda: be.layer_norm_bwd(X, X, G, M, be.zeros([7])), rg.ShapeError)):
+        with pytest.raises(err):
+            call()
+
+
+def test_layer_norm_gives_the_same_bits_again(backend):
+    be = backend
+    x, dy, g, b = ln_inputs(4000, 768, "f32")
+    X, DY, G, B = put(be, x), put(be, dy), put(be, g), put(be, b)
+    y, m, r = be.layer_norm_fwd(X, G, B, EPS)
+    first = [be.to_vec(s) for s in be.layer_norm_bwd(DY, X, G, m, r)]
+    for _ in range(3):
+        again = [be.to_vec(s) for s in be.layer_norm_bwd(DY, X, G, m, r)]
+        assert all(np.array_equal(p, q) for p, q in zip(first, again))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# linear cross entropy
+# ---------------------------------------------------------------------------------------------------------------------
+IGNORE = -100
+
+
+def ce_inputs(R, D, V, dtype, bias=True, ignored=0.2, seed=0, scale=2.5):
+    rng = np.random.default_rng(seed + R * 7 + D * 3 + V)
+    x = rounded(rng.standard_normal((R, D)), dtype)
+    w = rounded(rng.standard_normal((D, V)) * scale / np.sqrt(D), dtype)
+    b = (0.5 * rng.standard_normal(V)).astype(np.float32) if bias else None
+    t = rng.integers(0, V, R).astype(np.float32)
+    t[rng.random(R) < ignored] = IGNORE
+    return x, w, b, t
+
+
+def ce_exact(x, w, b, t, dloss=1.0, ignore=IGNORE):
+    x, w = x.astype(np.float64), w.astype(np.float64)
+    z = x @ w + (0 if b is None else b.astype(np.float64))
+    m = z.max(-1, keepdims=True)
+    lse = (m + np.log(np.exp(z - m).sum(-1, keepdims=True)))[:, 0]
+    live = t != ignore
+    at = np.where(live, t, 0).astype(int)
+    n = max(1, int(live.sum()))
+    loss = float(np.where(live, lse - z[np.arange(len(t)), at], 0).sum() / n)
+    p = np.exp(z - lse[:, None])
+    dz = p.copy()
+    dz[np.arange(len(t)), at] -= 1
+    scale = dloss / n if live.any() else 0.0
+    dz *= live[:, None]
+    return {"z": z, "lse": lse, "loss": loss, "p": p, "dz": dz, "scale": scale, "dx": scale * dz @ w.T, "dw": scale * x.T @ dz,
+            "db": scale * dz.sum(0)}
+
+
+def ce_bounds(x, w, b, dtype, ex, live):
+    """Worst cases.  A logit: one chain of additions that truncate (D / 16 steps of a step each, doubled for the additions
+    inside a step) in bf16; in f32 chains of 16 steps, the products left out (2^-21 of the magnitudes) and the additions of the
+    pieces; relative to the sum of magnitudes.  exp: 2 steps and the rounding of its argument."""
+    ax, aw = np.abs(x).astype(np.float64), np.abs(w).astype(np.float64)
+    D = x.shape[1]
+    steps = (2 * (D / 16 + 2) if dtype == "bf16" else 2 * 18 + 4 + D / 256)
+    steps = max(steps, D / 8 + 8)           # the form for few rows: 8 chains of D / 8 terms
+    ez = steps * E32 * (ax @ aw) + E32 * (np.abs(ex["z"]) + (0 if b is None else np.abs(b)))
+    ez_row = ez.max(-1)
+    elsum = 300 * 2.0 ** -24                # chains of at most 128 terms, then partial sums over slices of the vocabulary
+    elogs = E32 * (np.abs(ex["lse"]) + 1)
+    tlse = ez_row + elsum + 2 * elogs + 2 * E32 * np.abs(ex["z"]).max(-1)
+    tloss = float((tlse + ez_row)[live].mean() if live.any() else 0) + E32 * (abs(ex["loss"]) + 1)
+    # gradient, from an lse that is given rounded to f32
+    earg = ez + 2 * E32 * (np.abs(ex["z"]) + np.abs(ex["lse"])[:, None])
+    edz = live[:, None] * (ex["p"] * (earg + 4 * E32) * 1.01 + E32 * np.abs(ex["dz"]))
+    if dtype == "bf16":
+        store = U["bf16"]                   # dz is multiplied as bf16
+    else:
+        store = 2.0 ** -21
+    ez2 = edz + store * (np.abs(ex["dz"]) + edz)
+    V, R, s = w.shape[1], x.shape[0], abs(ex["scale"])
+    chain_v = 2 * (V / 16 + 2) if dtype == "bf16" else 2 * 18 + 4 + V / 256
+    chain_r = 2 * (R / 16 + 2) if dtype == "bf16" else 2 * 18 + 4 + R / 256
+    adz = np.abs(ex["dz"])
+    tdx = s * (ez2 @ aw.T + max(chain_v, 60) * E32 * (adz @ aw.T)) + 3 * E32 * np.abs(ex["dx"])
+    tdw = s * (ax.T @ ez2 + max(chain_r, 24) * E32 * (ax.T @ adz)) + 3 * E32 * np.abs(ex["dw"])
+    tdb = s * (edz.sum(0) + (R / 32 + 40) * E32 * adz.sum(0))
+    return tlse, tloss, tdx + U[dtype] * (np.abs(ex["dx"]) + tdx), tdw + U[dtype] * (np.abs(ex["dw"]) + tdw), tdb
+
+
+def ce_check(be, R, D, V, dtype, bias=True, ignored=0.2, dloss=None, seed=0):
+    x, w, b, t = ce_inputs(R, D, V, dtype, bias, ignored, seed)
+    X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b) if bias else None, put(be, t)
+    ex = ce_exact(x, w, b, t, 1.0 if dloss is None else dloss)
+    live = t != IGNORE
+    tlse, tloss, tdx, tdw, tdb = ce_bounds(x, w, b, dtype, ex, live)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    assert (loss.shape, lse.shape, loss.dtype, lse.dtype) == ([1], [R], "f32", "f32")
+    within(get(be, lse), ex["lse"], tlse, "lse")
+    within(get(be, loss), np.array([ex["loss"]]), tloss + 1e-45, "loss")
+    L = put(be, ex["lse"].astype(np.float32))
+    dx, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, L, None if dloss is None else put(be, np.array([dloss], np.float32)))
+    assert (dx.shape, dw.shape, dx.dtype, dw.dtype) == ([R, D], [D, V], dtype, dtype) and (db is None) == (not bias)
+    within(get(be, dx), ex["dx"], tdx + 1e-45, "dx")
+    within(get(be, dw), ex["dw"], tdw + 1e-45, "dw")
+    if bias:
+        assert db.shape == [V]
+        within(get(be, db), ex["db"], tdb + 1e-45, "dbias")
+    return ex
+
+
+FEW = [(1, 1, 1), (1, 8, 2), (1, 64, 1000), (2, 13, 97), (3, 768, 257), (4, 32, 128), (5, 300, 1025), (8, 128, 129), (9, 31, 63),
+       (16, 257, 2047), (13, 520, 333)]
+MANY = [(17, 1, 1), (17, 8, 2), (33, 13, 97), (64, 64, 64), (64, 192, 97), (127, 65, 255), (128, 128, 256), (129, 72, 257), (200, 100, 1000),
+        (300, 320, 513), (511, 257, 775), (640, 768, 1024), (1025, 40, 2049), (260, 520, 5003)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", FEW + MANY)
+def test_linear_cross_entropy(backend, R, D, V, dtype):
+    ce_check(backend, R, D, V, dtype, bias=(R + V) % 3 != 0, dloss=None if R % 2 else 0.25)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# clipping by the global norm
+# ---------------------------------------------------------------------------------------------------------------------
+def clip_check(be, arrays, dtypes, max_norm):
+    arrays = [rounded(a, t) for a, t in zip(arrays, dtypes)]
+    out, norm = be.clip_grad_norm([put(be, a, t) for a, t in zip(arrays, dtypes)], max_norm)
+    n = float(np.sqrt(sum(float((a.astype(np.float64) ** 2).sum()) for a in arrays)))
+    c = min(1.0, float(np.float32(max_norm)) / n) if n else 1.0
+    assert norm.shape == [1] and norm.dtype == "f32"
+    if n > np.finfo(np.float32).max:                    # no f32 holds it (each of the gradients does)
+        assert np.isinf(get(be, norm)[0])
+    else:
+        within(get(be, norm), np.array([n]), E32 * n + 1e-45, "norm")       # f64 sums, one rounding
+    for a, t, o in zip(arrays, dtypes, out):
+        assert o.shape == list(a.shape) and o.dtype == t
+        want = a.astype(np.float64) * c
+        # the factor is off by 2 steps; 2^-149 / 2^-133: the smallest steps of f32 and bf16
+        within(get(be, o), want, (2 * E32 + U[t]) * np.abs(want) + (1.5e-45 if t == "f32" else 9.2e-41), "gradient")
+        if c == 1.0:
+            assert np.array_equal(be.to_vec(o).reshape(a.shape), a)
+    return n
+
+
+@pytest.mark.parametrize("sizes", [[1], [7], [8191, 8192, 8193], [3, 0, 5, 65536 + 1], [20000] * 3 + [1] * 40, [33] * 600,
+                                   [1000003]])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mixed"])
+def test_clip_grad_norm(backend, sizes, kind):
+    rng = np.random.default_rng(len(sizes) + sizes[0])
+    arrays = [rng.standard_normal(n).astype(np.float32) for n in sizes]
+    dtypes = [kind if kind != "mixed" else ("f32", "bf16")[i % 2] for i in range(len(sizes))]
+    n = clip_check(backend, arrays, dtypes, 0.5)
+    clip_check(backend, arrays, dtypes, 2 * n)          # nothing to clip: the values themselves
+    clip_check(backend, arrays, dtypes, float("inf"))
+
+
+def test_clip_grad_norm_extremes(backend):
+    be = backend
+    # squares beyond the range of f32 both ways
+    clip_check(be, [np.full(100, 1e30, np.float32), np.full(5, -3e38, np.float32)], ["f32", "f32"], 1.0)
+    clip_check(be, [np.full(100, 1e-30, np.float32)], ["f32"], 1e-30)
+    clip_check(be, [np.zeros(64, np.float32)], ["bf16"], 1.0)
+    out, norm = be.clip_grad_norm([], 1.0)
+    assert out == [] and be.to_vec(norm)[0] == 0
+    for bad, where in ((np.nan, 3), (np.nan, 9)):
+        a = np.ones(10, np.float32)
+        a[where] = bad
+        out, norm = be.clip_grad_norm([put(be, a), put(be, np.ones(4, np.float32), "bf16")], 1.0)
+        assert np.isnan(be.to_vec(norm)[0]) and np.isnan(be.to_vec(out[0])).all() and np.isnan(be.to_vec(out[1])).all()
+    a = np.ones(10, np.float32)
+    a[2] = np.inf
+    out, norm = be.clip_grad_norm([put(be, a)], 1.0)     # 1 / inf = 0
+    v = be.to_vec(out[0])
+    assert np.isinf(be.to_vec(norm)[0]) and np.isnan(v[2]) and not v[:2].any() and not v[3:].any()
+    g = put(be, np.array([3.0, 4.0], np.float32))        # the same tensor twice is two tensors of the list
+    out, norm = be.clip_grad_norm([g, g], 5.0)
+    assert abs(be.to_vec(norm)[0] - np.sqrt(50.0)) < 1e-6 and np.array_equal(be.to_vec(g), [3, 4])
+    for m in (0.0, -1.0, float("nan")):
+        with pytest.raises(rg.InvalidInput):
+            be.clip_grad_norm([g], m)
