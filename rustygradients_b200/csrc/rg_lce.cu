@@ -45,45 +45,53 @@ __global__ void __launch_bounds__(1024) lce_check_kernel(const float* __restrict
     }
 }
 
-// lse of 32 rows per CTA (8 threads of different warps walk each row's slices), and the loss: the sum of a CTA's rows in
-// f64, then the last CTA to finish adds the CTAs in order and divides.
+// lse of 8 rows per CTA: 32 threads share the slices of a row, lanes of 8 rows read 64 contiguous bytes.  The maximum of
+// all slices comes first, so the sum is one exponential per slice with no chain between them.  Then the loss: the sum of a
+// CTA's rows in f64; the last CTA to finish adds the CTAs in order and divides.
 __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict__ parts, int nparts, int R, const int* __restrict__ tgt,
                                                        const float* __restrict__ tz, const float* __restrict__ scal,
                                                        int* __restrict__ ticket, double* __restrict__ sums, float* __restrict__ lse_out,
                                                        float* __restrict__ loss) {
-    __shared__ lce_ms red[8][32];
+    __shared__ float red[32][9];
+    __shared__ double rows_s[8];
     __shared__ bool last;
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int r = blockIdx.x * 32 + lane;
-    lce_ms a = {-INFINITY, 0.f};
-    if (r < R) {
-        int p = w;
-        for (; p + 24 < nparts; p += 32) {  // four loads in flight
-            float2 v[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = parts[(size_t)(p + u * 8) * R + r];
-#pragma unroll
-            for (int u = 0; u < 4; u++) a = lce_merge(a, {v[u].x, v[u].y});
-        }
-        for (; p < nparts; p += 8) {
-            const float2 v = parts[(size_t)p * R + r];
-            a = lce_merge(a, {v.x, v.y});
-        }
-    }
-    red[w][lane] = a;
+    const int row = threadIdx.x & 7, slice = threadIdx.x >> 3;
+    const int r = blockIdx.x * 8 + row;
+    const float2* mine = parts + (size_t)slice * R + r;
+    float m = -INFINITY, s = 0.f;
+    if (r < R)
+#pragma unroll 8
+        for (int p = slice; p < nparts; p += 32) m = fmaxf(m, parts[(size_t)p * R + r].x);
+    red[slice][row] = m;
     __syncthreads();
-    if (w == 0) {
-        for (int k = 1; k < 8; k++) a = lce_merge(a, red[k][lane]);
-        double row = 0.0;
-        if (r < R) {
-            const float lse = a.m + logf(a.s);
-            lse_out[r] = lse;
-            if (tgt[r] >= 0) row = (double)lse - (double)tz[r];
-        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) row += __shfl_xor_sync(RG_FULL_MASK, row, o);
-        if (lane == 0) {
-            sums[blockIdx.x] = row;
+    for (int k = 0; k < 32; k++) m = fmaxf(m, red[k][row]);
+    const float ref = m == -INFINITY ? 0.f : m;  // a row of -inf only: every term below is 0
+    if (r < R)
+#pragma unroll 8
+        for (int p = slice; p < nparts; p += 32, mine += (size_t)32 * R) {
+            const float2 v = *mine;
+            s += v.y * expf(v.x - ref);
+        }
+    __syncthreads();
+    red[slice][row] = s;
+    __syncthreads();
+    if (threadIdx.x < 8) {
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; k++) s += red[k][row];
+        double off = 0.0;
+        if (r < R) {
+            const float lse = m + logf(s);
+            lse_out[r] = lse;
+            if (tgt[r] >= 0) off = (double)lse - (double)tz[r];
+        }
+        rows_s[row] = off;
+        __syncwarp(0xff);
+        if (threadIdx.x == 0) {
+            double t = 0.0;
+            for (int k = 0; k < 8; k++) t += rows_s[k];
+            sums[blockIdx.x] = t;
             __threadfence();
             last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
         }
@@ -92,9 +100,9 @@ __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict_
     if (!last) return;
     __threadfence();
     __shared__ double tot[256];
-    double s = 0.0;
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) s += __ldcg(sums + i);
-    tot[threadIdx.x] = s;
+    double t = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) t += __ldcg(sums + i);
+    tot[threadIdx.x] = t;
     __syncthreads();
     for (int o = 128; o > 0; o >>= 1) {
         if ((int)threadIdx.x < o) tot[threadIdx.x] += tot[threadIdx.x + o];
@@ -142,7 +150,7 @@ void lce_dbias_finish_launch(rg_ctx* ctx, const float* parts, int nparts, int V,
 // A CTA owns 128 columns, a lane the columns lane + 32 j: no alignment of the rows of w is needed.  Its 8 warps share the D
 // axis and add their sums through shared memory.  x lies in shared memory as [d][row], so the RB values of one d are one or
 // a few broadcast loads.
-#define LCE_DC 256  // rows of w between two refills of x
+#define LCE_DC 1024  // rows of w between two refills of x
 template <int RB>
 constexpr size_t lce_few_smem() {
     return sizeof(float) * (LCE_DC * RB > 8 * RB * 128 ? LCE_DC * RB : 8 * RB * 128);
@@ -436,7 +444,7 @@ extern "C" rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, c
     RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, nullptr, &o[2]));
     const bool few = c.R <= LCE_FEW_ROWS;
     c.nparts = few ? rg_cdiv(c.V, 128) : lce_tc_nparts(c.V, c.dtype);
-    const size_t pwords = 2 * (size_t)c.nparts * rows, blocks = (size_t)rg_cdiv(c.R, 32), swords = 2 * blocks;
+    const size_t pwords = 2 * (size_t)c.nparts * rows, blocks = (size_t)rg_cdiv(c.R, 8), swords = 2 * blocks;
     RG_TRY(rg_alloc_storage(ctx, &pwords, 1, &o[3]));
     RG_TRY(rg_alloc_storage(ctx, &swords, 1, &o[4]));
     c.parts = static_cast<float2*>(o[3]->raw());

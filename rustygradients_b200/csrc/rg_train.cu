@@ -42,68 +42,98 @@ __device__ __forceinline__ void ln_store(T* __restrict__ p, const float (&v)[VEC
     *reinterpret_cast<V*>(p) = raw;
 }
 
+// VEC parameters (f32, storages start on 16-byte boundaries and c is a multiple of VEC)
+template <int VEC>
+__device__ __forceinline__ void ln_param(const float* __restrict__ p, float (&v)[VEC]) {
+    if (VEC >= 4) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(p + i));
+            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        }
+    } else if (VEC == 2) {
+        const float2 q = __ldg(reinterpret_cast<const float2*>(p));
+        v[0] = q.x, v[VEC - 1] = q.y;
+    } else {
+        v[0] = __ldg(p);
+    }
+}
+
 // Sums of two values over the WPR warps of a row group, in a fixed order; every thread of the group gets them.  red: two
-// slots of [groups][WPR] pairs, used in turn so that one barrier per call is enough.
+// slots of WPR pairs for this group, used in turn, so that one barrier per call - of this group alone - is enough.
 template <int WPR>
 __device__ __forceinline__ float2 ln_group_sum(float a, float b, float2* red, int group, int gwarp) {
     a = rg_warp_sum(a), b = rg_warp_sum(b);
     if (WPR == 1) return make_float2(a, b);
-    if ((threadIdx.x & 31) == 0) red[group * WPR + gwarp] = make_float2(a, b);
-    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[gwarp] = make_float2(a, b);
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(32 * WPR) : "memory");
     float2 r = make_float2(0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < WPR; w++) {
-        const float2 p = red[group * WPR + w];
+        const float2 p = red[w];
         r.x += p.x, r.y += p.y;
     }
     return r;
 }
 
 // y = (x - mean) rstd gamma + beta.  One read of x: the mean, then the squared deviations from it, are summed over the
-// registers, so the variance does not cancel however far the row is from zero.
-// Memory bound: x in, y out.
+// registers, so the variance does not cancel however far the row is from zero.  Memory bound: x in, y out.  A group walks
+// rows with the next row's loads in flight behind the two sums of this one.
 template <typename T, int VEC, int PER, int WPR, int THREADS>
 __global__ void __launch_bounds__(THREADS) rg_ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
                                                             const float* __restrict__ beta, T* __restrict__ y,
                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows,
                                                             int n, float eps) {
     constexpr int GROUPS = THREADS / 32 / WPR;
-    __shared__ float2 red[2][GROUPS * WPR];
+    typedef typename ln_vec<T, VEC>::type V;
+    __shared__ float2 red[2][GROUPS][WPR];
     const int group = threadIdx.x / (32 * WPR), t = threadIdx.x % (32 * WPR), gwarp = t >> 5;
-    const long long row = (long long)blockIdx.x * GROUPS + group;
-    const bool live = row < rows;
-    float v[PER][VEC];
-    float s = 0.f;
+    const long long step = (long long)gridDim.x * GROUPS;
+    V next[PER];
+    long long row = (long long)blockIdx.x * GROUPS + group;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
         const int c = (t + j * 32 * WPR) * VEC;
-        if (live && c < n) {
-            ln_load<T, VEC>(x + row * n + c, v[j]);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) s += v[j][i];
-        }
+        if (row < rows && c < n) next[j] = __ldcs(reinterpret_cast<const V*>(x + row * n + c));
     }
-    const float mean = ln_group_sum<WPR>(s, 0.f, red[0], group, gwarp).x / (float)n;
-    float q = 0.f;
+    for (; row < rows; row += step) {  // the same number of turns for every thread of the group
+        float v[PER][VEC];
+        float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < PER; j++)
-        if ((t + j * 32 * WPR) * VEC < n)
+        for (int j = 0; j < PER; j++) {
+            const int c = (t + j * 32 * WPR) * VEC;
+            const T* e = reinterpret_cast<const T*>(&next[j]);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                const float d = v[j][i] - mean;
-                q += live ? d * d : 0.f;
+                v[j][i] = c < n ? rg_to_float(e[i]) : 0.f;
+                s += v[j][i];
             }
-    const float var = ln_group_sum<WPR>(q, 0.f, red[1], group, gwarp).x / (float)n;
-    const float rstd = 1.f / sqrtf(var + eps);
-    if (!live) return;
-    if (t == 0) mean_out[row] = mean, rstd_out[row] = rstd;
+            if (row + step < rows && c < n) next[j] = __ldcs(reinterpret_cast<const V*>(x + (row + step) * n + c));
+        }
+        const float mean = ln_group_sum<WPR>(s, 0.f, red[0][group], group, gwarp).x / (float)n;
+        float q = 0.f;
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int c = (t + j * 32 * WPR) * VEC;
-        if (c < n) {
+        for (int j = 0; j < PER; j++)
+            if ((t + j * 32 * WPR) * VEC < n)
 #pragma unroll
-            for (int i = 0; i < VEC; i++) v[j][i] = (v[j][i] - mean) * rstd * gamma[c + i] + beta[c + i];
-            ln_store<T, VEC>(y + row * n + c, v[j]);
+                for (int i = 0; i < VEC; i++) {
+                    const float d = v[j][i] - mean;
+                    q += d * d;
+                }
+        const float var = ln_group_sum<WPR>(q, 0.f, red[1][group], group, gwarp).x / (float)n;
+        const float rstd = 1.f / sqrtf(var + eps);
+        if (t == 0) mean_out[row] = mean, rstd_out[row] = rstd;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int c = (t + j * 32 * WPR) * VEC;
+            if (c < n) {
+                float gm[VEC], bt[VEC];
+                ln_param<VEC>(gamma + c, gm);
+                ln_param<VEC>(beta + c, bt);
+#pragma unroll
+                for (int i = 0; i < VEC; i++) v[j][i] = (v[j][i] - mean) * rstd * gm[i] + bt[i];
+                ln_store<T, VEC>(y + row * n + c, v[j]);
+            }
         }
     }
 }
@@ -129,65 +159,81 @@ __global__ void __launch_bounds__(512) rg_ln_fwd_long_kernel(const T* __restrict
         y[(long long)blockIdx.x * n + c] = rg_from_float<T>((rg_to_float(xr[c]) - mean) * rstd * gamma[c] + beta[c]);
 }
 
+// Resident CTAs per SM of the gradient: registers for 8 values a thread (two column sums, this row and the next one)
+#define LN_BWD_CTAS(threads) ((threads) == 256 ? 3 : 1)
+
 // dx = rstd (a - mean(a) - xh mean(a xh)), and the two column sums dgamma = sum dy xh, dbeta = sum dy.  One read of dy and
-// x serves all three: a CTA walks rows blockIdx.x * GROUPS + group, + gridDim.x * GROUPS, ..., every thread always on the
-// same columns, so the column sums stay in its registers until the end; then the CTA's groups are added and the CTA leaves
-// one partial row of sums, which rg_colsum_kernel adds over the CTAs.  Memory bound: dy and x in, dx out.
+// x serves all three: a group walks rows, every thread always on the same columns, so the column sums stay in its registers
+// until the end; then the CTA's groups are added and the CTA leaves one partial row of sums, which rg_colsum_kernel adds over
+// the CTAs.  Memory bound: dy and x in, dx out; the next row's loads are in flight behind the sums of this one.
 template <typename T, int VEC, int PER, int WPR, int THREADS>
-__global__ void __launch_bounds__(THREADS) rg_ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+__global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                             const float* __restrict__ gamma, const float* __restrict__ mean,
                                                             const float* __restrict__ rstd, T* __restrict__ dx,
                                                             float* __restrict__ parts, long long rows, int n) {
-    constexpr int GROUPS = THREADS / 32 / WPR;
-    __shared__ float2 red[2][GROUPS * WPR];
-    __shared__ float comb[GROUPS > 1 ? THREADS * PER * VEC : 1];
+    constexpr int GROUPS = THREADS / 32 / WPR, COLS = 32 * WPR * PER * VEC;
+    constexpr bool AHEAD = PER * VEC <= 8;  // room in the registers for the next row
+    typedef typename ln_vec<T, VEC>::type V;
+    __shared__ float2 red[2][GROUPS][WPR];
+    __shared__ float comb[GROUPS > 1 ? GROUPS * COLS : 1];
     const int group = threadIdx.x / (32 * WPR), t = threadIdx.x % (32 * WPR), gwarp = t >> 5;
-    float dg[PER][VEC], db[PER][VEC], gm[PER][VEC];
+    const long long step = (long long)gridDim.x * GROUPS;
+    float dg[PER][VEC], db[PER][VEC];
 #pragma unroll
     for (int j = 0; j < PER; j++)
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int c = (t + j * 32 * WPR) * VEC;
-            dg[j][i] = db[j][i] = 0.f;
-            gm[j][i] = c < n ? gamma[c + i] : 0.f;
-        }
+        for (int i = 0; i < VEC; i++) dg[j][i] = db[j][i] = 0.f;
     const float inv_n = 1.f / (float)n;
-    int turn = 0;
-    // every group makes the same number of turns (they share the barrier of the row sums); a turn without a row adds nothing
-    for (long long r0 = (long long)blockIdx.x * GROUPS; r0 < rows; r0 += (long long)gridDim.x * GROUPS, turn ^= 1) {
-        const long long row = r0 + group;
-        const bool live = row < rows;
-        float xv[PER][VEC], gv[PER][VEC];
-        const float m = live ? mean[row] : 0.f, r = live ? rstd[row] : 0.f;
+    long long row = (long long)blockIdx.x * GROUPS + group;
+    V nx[PER], ng[PER];
+    float nm = 0.f, nr = 0.f;
+    auto fetch = [&](long long at) {
+        if (at >= rows) return;
+        nm = mean[at], nr = rstd[at];
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int c = (t + j * 32 * WPR) * VEC;
-            if (live && c < n) {
-                ln_load<T, VEC>(x + row * n + c, xv[j]);
-                ln_load<T, VEC>(dy + row * n + c, gv[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) xv[j][i] = m, gv[j][i] = 0.f;
+            if (c < n) {
+                nx[j] = __ldcs(reinterpret_cast<const V*>(x + at * n + c));
+                ng[j] = __ldcs(reinterpret_cast<const V*>(dy + at * n + c));
             }
         }
+    };
+    if (AHEAD) fetch(row);
+    for (int turn = 0; row < rows; row += step, turn ^= 1) {
+        if (!AHEAD) fetch(row);
+        float xv[PER][VEC], gv[PER][VEC];
+        const float m = nm, r = nr;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int c = (t + j * 32 * WPR) * VEC;
+            const T *ex = reinterpret_cast<const T*>(&nx[j]), *eg = reinterpret_cast<const T*>(&ng[j]);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) xv[j][i] = c < n ? rg_to_float(ex[i]) : m, gv[j][i] = c < n ? rg_to_float(eg[i]) : 0.f;
+        }
+        if (AHEAD) fetch(row + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int j = 0; j < PER; j++)
+        for (int j = 0; j < PER; j++) {
+            const int c = (t + j * 32 * WPR) * VEC;
+            float gm[VEC];
+            ln_param<VEC>(gamma + (c < n ? c : 0), gm);  // dy is 0 beyond the row
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
                 const float xh = (xv[j][i] - m) * r;
                 db[j][i] += gv[j][i];
                 dg[j][i] += gv[j][i] * xh;
-                const float a = gv[j][i] * gm[j][i];
+                const float a = gv[j][i] * gm[i];
                 s1 += a, s2 += a * xh;
                 xv[j][i] = xh, gv[j][i] = a;
             }
-        const float2 s = ln_group_sum<WPR>(s1, s2, red[turn], group, gwarp);
+        }
+        const float2 s = ln_group_sum<WPR>(s1, s2, red[turn][group], group, gwarp);
         s1 = s.x * inv_n, s2 = s.y * inv_n;
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int c = (t + j * 32 * WPR) * VEC;
-            if (live && c < n) {
+            if (c < n) {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) gv[j][i] = r * (gv[j][i] - s1 - xv[j][i] * s2);
                 ln_store<T, VEC>(dx + row * n + c, gv[j]);
@@ -203,13 +249,12 @@ __global__ void __launch_bounds__(THREADS) rg_ln_bwd_kernel(const T* __restrict_
 #pragma unroll
             for (int j = 0; j < PER; j++)
 #pragma unroll
-                for (int i = 0; i < VEC; i++)
-                    comb[group * (32 * WPR * PER * VEC) + (t + j * 32 * WPR) * VEC + i] = which ? db[j][i] : dg[j][i];
+                for (int i = 0; i < VEC; i++) comb[group * COLS + (t + j * 32 * WPR) * VEC + i] = which ? db[j][i] : dg[j][i];
             __syncthreads();
             for (int c = threadIdx.x; c < n; c += THREADS) {
                 float s = 0.f;
 #pragma unroll
-                for (int g = 0; g < GROUPS; g++) s += comb[g * (32 * WPR * PER * VEC) + c];
+                for (int g = 0; g < GROUPS; g++) s += comb[g * COLS + c];
                 out[which * n + c] = s;
             }
         } else {
@@ -305,17 +350,17 @@ struct ln_args {
 };
 
 #define LN_MAX_N 16384   // 512 threads with 32 values each
-#define LN_BWD_CTAS 2    // resident CTAs per SM that share the rows of the gradient
 
-template <typename T, int VEC, int PER, int WPR, int THREADS>
-static void ln_launch_one(rg_ctx* ctx, const ln_args& a, bool bwd, int* nparts) {
+template <bool BWD, typename T, int VEC, int PER, int WPR, int THREADS>
+static void ln_launch_one(rg_ctx* ctx, const ln_args& a, int* nparts) {
     constexpr int GROUPS = THREADS / 32 / WPR;
     const long long groups = (a.rows + GROUPS - 1) / GROUPS;
-    if (!bwd) {
-        rg_ln_fwd_kernel<T, VEC, PER, WPR, THREADS><<<(unsigned)groups, THREADS, 0, ctx->stream>>>(
+    if constexpr (!BWD) {
+        const int grid = (int)std::min<long long>(groups, (long long)ctx->sm_count * (2048 / THREADS));
+        rg_ln_fwd_kernel<T, VEC, PER, WPR, THREADS><<<grid, THREADS, 0, ctx->stream>>>(
             (const T*)a.x, a.gamma, a.beta, (T*)a.out, a.mean_out, a.rstd_out, a.rows, a.n, a.eps);
     } else {
-        *nparts = (int)std::min<long long>(groups, (long long)ctx->sm_count * LN_BWD_CTAS);
+        *nparts = (int)std::min<long long>(groups, (long long)ctx->sm_count * LN_BWD_CTAS(THREADS));
         if (!a.parts) return;  // the caller asks for the number of partial rows first
         rg_ln_bwd_kernel<T, VEC, PER, WPR, THREADS><<<*nparts, THREADS, 0, ctx->stream>>>((const T*)a.dy, (const T*)a.x, a.gamma, a.mean,
                                                                                          a.rstd, (T*)a.out, a.parts, a.rows, a.n);
@@ -323,27 +368,39 @@ static void ln_launch_one(rg_ctx* ctx, const ln_args& a, bool bwd, int* nparts) 
     RG_LAUNCHED(ctx);
 }
 
-// The smallest group whose threads hold at most 16 values each (32 from 8192 on, where a group is the largest CTA).
-template <typename T, int VEC>
-static void ln_launch_vec(rg_ctx* ctx, const ln_args& a, bool bwd, int* nparts) {
-    constexpr int P = 16 / VEC;
-    if (a.n <= 256) ln_launch_one<T, VEC, (P + 1) / 2, 1, 256>(ctx, a, bwd, nparts);
-    else if (a.n <= 512) ln_launch_one<T, VEC, P, 1, 256>(ctx, a, bwd, nparts);
-    else if (a.n <= 1024) ln_launch_one<T, VEC, P, 2, 256>(ctx, a, bwd, nparts);
-    else if (a.n <= 2048) ln_launch_one<T, VEC, P, 4, 256>(ctx, a, bwd, nparts);
-    else if (a.n <= 4096) ln_launch_one<T, VEC, P, 8, 256>(ctx, a, bwd, nparts);
-    else if (a.n <= 8192) ln_launch_one<T, VEC, P, 16, 512>(ctx, a, bwd, nparts);
-    else ln_launch_one<T, VEC, 2 * P, 16, 512>(ctx, a, bwd, nparts);
+// Values per thread: 8 in the gradient (two column sums each stay in registers), up to 32 forward; more only where a group
+// is the whole CTA.
+template <bool BWD, typename T, int VEC>
+static void ln_launch_vec(rg_ctx* ctx, const ln_args& a, int* nparts) {
+    constexpr int P = 8 / VEC;
+    if constexpr (BWD) {
+        if (a.n <= 256) ln_launch_one<true, T, VEC, P, 1, 256>(ctx, a, nparts);
+        else if (a.n <= 512) ln_launch_one<true, T, VEC, P, 2, 256>(ctx, a, nparts);
+        else if (a.n <= 1024) ln_launch_one<true, T, VEC, P, 4, 256>(ctx, a, nparts);
+        else if (a.n <= 2048) ln_launch_one<true, T, VEC, P, 8, 256>(ctx, a, nparts);
+        else if (a.n <= 4096) ln_launch_one<true, T, VEC, P, 16, 512>(ctx, a, nparts);
+        else if (a.n <= 8192) ln_launch_one<true, T, VEC, 2 * P, 16, 512>(ctx, a, nparts);
+        else ln_launch_one<true, T, VEC, 4 * P, 16, 512>(ctx, a, nparts);
+    } else {
+        if (a.n <= 256) ln_launch_one<false, T, VEC, P, 1, 256>(ctx, a, nparts);
+        else if (a.n <= 512) ln_launch_one<false, T, VEC, 2 * P, 1, 256>(ctx, a, nparts);
+        else if (a.n <= 1024) ln_launch_one<false, T, VEC, 4 * P, 1, 256>(ctx, a, nparts);
+        else if (a.n <= 2048) ln_launch_one<false, T, VEC, 4 * P, 2, 256>(ctx, a, nparts);
+        else if (a.n <= 4096) ln_launch_one<false, T, VEC, 4 * P, 4, 256>(ctx, a, nparts);
+        else if (a.n <= 8192) ln_launch_one<false, T, VEC, 4 * P, 8, 256>(ctx, a, nparts);
+        else ln_launch_one<false, T, VEC, 4 * P, 16, 512>(ctx, a, nparts);
+    }
 }
 
-static void ln_launch(rg_ctx* ctx, const ln_args& a, int dtype, bool bwd, int* nparts) {
+template <bool BWD>
+static void ln_launch(rg_ctx* ctx, const ln_args& a, int dtype, int* nparts) {
     if (dtype == RG_DTYPE_F32) {
-        if (a.n % 4 == 0) ln_launch_vec<float, 4>(ctx, a, bwd, nparts);
-        else ln_launch_vec<float, 1>(ctx, a, bwd, nparts);
+        if (a.n % 4 == 0) ln_launch_vec<BWD, float, 4>(ctx, a, nparts);
+        else ln_launch_vec<BWD, float, 1>(ctx, a, nparts);
     } else {
-        if (a.n % 8 == 0) ln_launch_vec<__nv_bfloat16, 8>(ctx, a, bwd, nparts);
-        else if (a.n % 2 == 0) ln_launch_vec<__nv_bfloat16, 2>(ctx, a, bwd, nparts);
-        else ln_launch_vec<__nv_bfloat16, 1>(ctx, a, bwd, nparts);
+        if (a.n % 8 == 0) ln_launch_vec<BWD, __nv_bfloat16, 8>(ctx, a, nparts);
+        else if (a.n % 2 == 0) ln_launch_vec<BWD, __nv_bfloat16, 2>(ctx, a, nparts);
+        else ln_launch_vec<BWD, __nv_bfloat16, 1>(ctx, a, nparts);
     }
 }
 
@@ -391,7 +448,7 @@ extern "C" rg_status rg_layer_norm_fwd(rg_ctx* ctx, const rg_storage* x, const r
             memset(&a, 0, sizeof(a));
             a.x = x->raw(), a.gamma = gamma->data(), a.beta = beta->data(), a.out = o[0]->raw();
             a.mean_out = o[1]->data(), a.rstd_out = o[2]->data(), a.rows = (long long)rows, a.n = (int)n, a.eps = epsilon;
-            ln_launch(ctx, a, x->dtype, false, nullptr);
+            ln_launch<false>(ctx, a, x->dtype, nullptr);
         }
     }
     RG_CUDA(cudaGetLastError());
@@ -427,12 +484,12 @@ extern "C" rg_status rg_layer_norm_bwd(rg_ctx* ctx, const rg_storage* dy, const 
         a.x = x->raw(), a.dy = dy->raw(), a.gamma = gamma->data(), a.mean = mean->data(), a.rstd = rstd->data(), a.out = o[0]->raw();
         a.rows = (long long)rows, a.n = (int)n;
         int nparts = (int)std::min<size_t>(rows, 64);
-        if (n <= LN_MAX_N) ln_launch(ctx, a, x->dtype, true, &nparts);  // a.parts is NULL: only counts
+        if (n <= LN_MAX_N) ln_launch<true>(ctx, a, x->dtype, &nparts);  // a.parts is NULL: only counts
         const size_t pshape[2] = {(size_t)nparts, 2 * n};
         RG_TRY(rg_alloc_storage(ctx, pshape, 2, &o[3]));
         a.parts = o[3]->data();
         if (n <= LN_MAX_N) {
-            ln_launch(ctx, a, x->dtype, true, &nparts);
+            ln_launch<true>(ctx, a, x->dtype, &nparts);
         } else {
             const dim3 cols((unsigned)((n + 255) / 256), (unsigned)nparts);
             if (x->dtype == RG_DTYPE_F32) {
@@ -463,8 +520,8 @@ extern "C" rg_status rg_layer_norm_bwd(rg_ctx* ctx, const rg_storage* dy, const 
 // write per value is what has to move; what the last-level cache still holds of the first pass is read from there, because
 // a CTA walks its pieces backwards in the second one).  The tensors are one list of pieces of CLIP_PIECE values; the table
 // of tensors travels as a kernel parameter, so no copy precedes the launch.
-// Squares are added in f64: an f32 square overflows from 1.8e19 and vanishes below 1e-23, and the sum of hundreds of
-// millions of terms would lose digits.
+// The sum is held in f64: an f32 square overflows from 1.8e19 and vanishes below 1e-23, and the sum of hundreds of millions
+// of terms would lose digits.
 #define CLIP_PIECE 8192
 #define CLIP_TENSORS 256
 struct clip_entry {
@@ -500,9 +557,22 @@ __device__ __forceinline__ double clip_block_sum(double v, double* red) {
     return s;
 }
 
-__device__ __forceinline__ void clip_add4(double& acc, float4 v) {
-    const double a = v.x, b = v.y, c = v.z, d = v.w;
-    acc = fma(a, a, acc), acc = fma(b, b, acc), acc = fma(c, c, acc), acc = fma(d, d, acc);
+// Eight squares are added in f32 as a tree (at most 4 roundings on the way of each) and their sum joins the f64 total:
+// one conversion and one f64 addition for eight values (a conversion for each bounded the kernel at 3.7 TB/s).  Where the
+// f32 sum is zero or anywhere near the ends of its range, the eight go through f64 one by one.
+__device__ __forceinline__ void clip_add8(double& acc, const float (&v)[8]) {
+    const float a = fmaf(v[1], v[1], v[0] * v[0]), b = fmaf(v[3], v[3], v[2] * v[2]);
+    const float c = fmaf(v[5], v[5], v[4] * v[4]), d = fmaf(v[7], v[7], v[6] * v[6]);
+    const float s = (a + b) + (c + d);
+    if (s > 0x1p-90f && s < 0x1p120f) {
+        acc += (double)s;
+    } else {
+#pragma unroll 1
+        for (int k = 0; k < 8; k++) {
+            const double w = v[k];
+            acc = fma(w, w, acc);
+        }
+    }
 }
 
 __global__ void __launch_bounds__(256) rg_clip_sumsq_kernel(const __grid_constant__ clip_table t, double* __restrict__ parts) {
@@ -514,27 +584,40 @@ __global__ void __launch_bounds__(256) rg_clip_sumsq_kernel(const __grid_constan
         const int len = (int)min((long long)CLIP_PIECE, e.len - at);
         if (e.bf16) {
             const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(e.in) + at;
-#pragma unroll 4
-            for (int i = threadIdx.x * 8; i + 8 <= len; i += 256 * 8) {
-                const uint4 raw = *reinterpret_cast<const uint4*>(src + i);
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            if (len == CLIP_PIECE) {
+                uint4 raw[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) raw[k] = reinterpret_cast<const uint4*>(src)[threadIdx.x + k * 256];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const double a = __uint_as_float(w[k] << 16), b = __uint_as_float(w[k] & 0xffff0000u);
-                    acc = fma(a, a, acc), acc = fma(b, b, acc);
+                    const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    clip_add8(acc, v);
                 }
-            }
-            for (int i = (len & ~7) + threadIdx.x; i < len; i += 256) {
-                const double a = __bfloat162float(src[i]);
-                acc = fma(a, a, acc);
+            } else {
+                for (int i = threadIdx.x; i < len; i += 256) {
+                    const double w = __bfloat162float(src[i]);
+                    acc = fma(w, w, acc);
+                }
             }
         } else {
             const float* src = static_cast<const float*>(e.in) + at;
-#pragma unroll 8
-            for (int i = threadIdx.x * 4; i + 4 <= len; i += 256 * 4) clip_add4(acc, *reinterpret_cast<const float4*>(src + i));
-            for (int i = (len & ~3) + threadIdx.x; i < len; i += 256) {
-                const double a = src[i];
-                acc = fma(a, a, acc);
+            if (len == CLIP_PIECE) {
+                float4 raw[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) raw[k] = reinterpret_cast<const float4*>(src)[threadIdx.x + k * 256];
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {
+                    const float v[8] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w, raw[k + 1].x, raw[k + 1].y, raw[k + 1].z, raw[k + 1].w};
+                    clip_add8(acc, v);
+                }
+            } else {
+                for (int i = threadIdx.x; i < len; i += 256) {
+                    const double w = src[i];
+                    acc = fma(w, w, acc);
+                }
             }
         }
     }
