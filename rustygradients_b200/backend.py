@@ -39,13 +39,18 @@ def _capsule_gone(capsule):
         C.CFUNCTYPE(None, C.c_void_p)(C.c_void_p.from_address(m + _DL_DELETER_OFFSET).value)(m)
 
 
+_capsule_gone_ptr = C.cast(_capsule_gone, C.c_void_p).value
+
+
 class Storage:
     """CudaStorage {data, shape, device} (src/backend/cuda.rs:29-33): an immutable
     device buffer owned by the library; freed when the Python object dies."""
 
+    __slots__ = ("_backend", "_h", "_keep", "__weakref__")
+
     def __init__(self, backend: "B200Backend", handle: int, keep=None):
         self._backend = backend
-        self._h = C.c_void_p(handle)
+        self._h = handle
         self._keep = keep     # the array whose memory this storage borrows
 
     @property
@@ -68,8 +73,10 @@ class Storage:
         """A DLPack capsule that shares the buffer (`torch.utils.dlpack.from_dlpack(st.to_dlpack())`).  It is read in the
         order of the backend's stream; a storage of `from_device` cannot be exported."""
         m = C.c_void_p()
-        check(self._backend._lib.rg_to_dlpack(self._h, C.byref(m)))
-        return _capsule_new(m, b"dltensor", C.cast(_capsule_gone, C.c_void_p))
+        status = self._backend._lib.rg_to_dlpack(self._h, C.byref(m))
+        if status:
+            check(status)
+        return _capsule_new(m, b"dltensor", _capsule_gone_ptr)
 
     def __dlpack__(self, stream=None, **_):
         """`torch.from_dlpack(st)`: for consumers on the backend's own stream (BufferError elsewhere)."""
@@ -83,8 +90,9 @@ class Storage:
 
     def __del__(self):
         try:
-            if self._h and self._backend._ctx:
-                _lib.load().rg_storage_free(self._h)
+            be = self._backend
+            if self._h and be._ctx:
+                be._free(self._h)
         except Exception:
             pass
         self._h = None
@@ -103,6 +111,7 @@ class B200Backend:
             check(lib.rg_ctx_create_on_stream(int(device_index), C.c_void_p(int(stream)), C.byref(ctx)))
         self._ctx = ctx
         self._lib = lib
+        self._free = lib.rg_storage_free
         self.device_index = device_index
 
     # -- CudaBackend::device_count / is_available (cuda.rs:127-135)
@@ -187,7 +196,9 @@ class B200Backend:
         if n > 8:
             raise _lib.DimensionError(f"storage rank {n} not in 0..8")
         h = C.c_void_p()
-        check(self._lib.rg_from_device(self._ctx, ptr, code, _SHAPES[n](*shape), n, C.byref(h)))
+        status = self._lib.rg_from_device(self._ctx, ptr, code, _SHAPES[n](*shape), n, C.byref(h))
+        if status:
+            check(status)
         return Storage(self, h.value, array)
 
     def cast(self, a: Storage, dtype: str) -> Storage:

@@ -29,6 +29,10 @@ extern "C" const char* rg_version(void) { return "rg_b200 0.1 (sm_100a)"; }
 
 rg_devbuf::~rg_devbuf() {
     if (!ptr || borrowed) return;
+    if (small >= 0 && life && life->alive && life->small[small].size() < RG_SMALL_KEPT) {
+        life->small[small].push_back(ptr);  // capacity was reserved with the context
+        return;
+    }
     int cur = 0;
     cudaGetDevice(&cur);
     if (cur != device) cudaSetDevice(device);
@@ -85,6 +89,7 @@ static rg_status ctx_create(int device, bool own_stream, cudaStream_t stream, rg
     c->sm_count = prop.multiProcessorCount;
     c->own_stream = own_stream;
     c->stream = stream;
+    for (std::vector<void*>& v : c->life->small) v.reserve(RG_SMALL_KEPT);
     cudaError_t e = own_stream ? cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) : cudaSuccess;
     if (e == cudaSuccess) {
         // keep freed op outputs in the device's pool instead of returning them to the driver at every synchronise
@@ -123,6 +128,10 @@ extern "C" rg_status rg_ctx_destroy(rg_ctx* ctx) {
         ctx->life->alive = false;
         for (void* p : ctx->life->parked) cudaFree(p);
         ctx->life->parked.clear();
+        for (std::vector<void*>& v : ctx->life->small) {
+            for (void* p : v) cudaFree(p);
+            v.clear();
+        }
         if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
         cudaEventDestroy(ctx->check_ev);
         cudaFree(ctx->d_flag);
@@ -184,6 +193,19 @@ rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storag
         s->buf->bytes = (s->len ? s->len : 1) * rg_dtype_size(dtype);
         s->buf->stream = ctx->stream;
         s->buf->life = ctx->life;
+        if (s->buf->bytes <= RG_SMALL_MAX) {
+            int k = 0;
+            while (((size_t)1 << (RG_SMALL_MIN_LOG2 + k)) < s->buf->bytes) k++;
+            s->buf->small = k;
+            s->buf->bytes = (size_t)1 << (RG_SMALL_MIN_LOG2 + k);
+            std::vector<void*>& kept = ctx->life->small[k];
+            if (!kept.empty()) {
+                s->buf->ptr = kept.back();
+                kept.pop_back();
+                *out = s.release();
+                return RG_OK;
+            }
+        }
         cudaError_t e = cudaMallocAsync(&s->buf->ptr, s->buf->bytes, ctx->stream);
         if (e != cudaSuccess) {
             cudaGetLastError();

@@ -42,11 +42,19 @@ void rg_clear_error();
 // ---------------------------------------------------------------------------
 // handles
 // ---------------------------------------------------------------------------
+#define RG_SMALL_MIN_LOG2 9
+#define RG_SMALL_CLASSES 12
+#define RG_SMALL_MAX ((size_t)1 << (RG_SMALL_MIN_LOG2 + RG_SMALL_CLASSES - 1))  // 1 MiB
+#define RG_SMALL_KEPT 64  // buffers kept per size
+
 // What outlives a context: buffers that left the library (rg_to_dlpack) are released under its lock, from any thread.
 struct rg_ctx_life {
     std::mutex mu;               // one call at a time per context
     bool alive = true;           // the context (and its stream) still exists
     std::vector<void*> parked;   // buffers released while the stream was being captured: freed by the next release outside
+    // Small buffers (powers of two up to RG_SMALL_MAX bytes) are kept and handed out again without a call to CUDA: everything
+    // of a context runs on one stream, so whoever gets a buffer next comes after whoever used it before.
+    std::vector<void*> small[RG_SMALL_CLASSES];
 };
 
 struct rg_ctx {
@@ -73,6 +81,7 @@ struct rg_devbuf {
     size_t bytes = 0;
     int device = 0;
     cudaStream_t stream = nullptr;
+    int small = -1;         // size class of a small buffer
     bool borrowed = false;  // the caller's memory (rg_from_device): never freed here
     std::shared_ptr<rg_ctx_life> life;
     ~rg_devbuf();  // the caller holds life->mu

@@ -479,8 +479,8 @@ extern "C" rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* 
     if (bias) RG_TRY(rg_alloc_storage(ctx, bias->shape.data(), (int)bias->shape.size(), &o[2]));
     c.lse = lse->data(), c.dx = o[0]->raw(), c.dw = o[1]->raw(), c.dbias = bias ? o[2]->data() : nullptr;
     if (!c.R) {
-        RG_CUDA(cudaMemsetAsync(o[1]->raw(), 0, o[1]->buf->bytes, ctx->stream));
-        if (bias) RG_CUDA(cudaMemsetAsync(o[2]->raw(), 0, o[2]->buf->bytes, ctx->stream));
+        RG_CUDA(cudaMemsetAsync(o[1]->raw(), 0, o[1]->len * rg_dtype_size(o[1]->dtype), ctx->stream));
+        if (bias) RG_CUDA(cudaMemsetAsync(o[2]->raw(), 0, o[2]->len * 4, ctx->stream));
     } else {
         RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, dloss, &o[3]));
         if (c.R <= LCE_FEW_ROWS) {

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(512) rg_ln_fwd_long_kernel(const T* __restrict
 }
 
 // Resident CTAs per SM of the gradient: registers for 8 values a thread (two column sums, this row and the next one)
-#define LN_BWD_CTAS(threads) ((threads) == 256 ? 3 : 1)
+#define LN_BWD_CTAS(threads) ((threads) == 256 ? 2 : 1)
 
 // dx = rstd (a - mean(a) - xh mean(a xh)), and the two column sums dgamma = sum dy xh, dbeta = sum dy.  One read of dy and
 // x serves all three: a group walks rows, every thread always on the same columns, so the column sums stay in its registers
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kerne
                                                             const float* __restrict__ rstd, T* __restrict__ dx,
                                                             float* __restrict__ parts, long long rows, int n) {
     constexpr int GROUPS = THREADS / 32 / WPR, COLS = 32 * WPR * PER * VEC;
-    constexpr bool AHEAD = PER * VEC <= 8;  // room in the registers for the next row
+    constexpr bool AHEAD = PER * VEC <= 16;  // room in the registers for the next row
     typedef typename ln_vec<T, VEC>::type V;
     __shared__ float2 red[2][GROUPS][WPR];
     __shared__ float comb[GROUPS > 1 ? GROUPS * COLS : 1];
@@ -375,10 +375,10 @@ static void ln_launch_vec(rg_ctx* ctx, const ln_args& a, int* nparts) {
     constexpr int P = 8 / VEC;
     if constexpr (BWD) {
         if (a.n <= 256) ln_launch_one<true, T, VEC, P, 1, 256>(ctx, a, nparts);
-        else if (a.n <= 512) ln_launch_one<true, T, VEC, P, 2, 256>(ctx, a, nparts);
-        else if (a.n <= 1024) ln_launch_one<true, T, VEC, P, 4, 256>(ctx, a, nparts);
-        else if (a.n <= 2048) ln_launch_one<true, T, VEC, P, 8, 256>(ctx, a, nparts);
-        else if (a.n <= 4096) ln_launch_one<true, T, VEC, P, 16, 512>(ctx, a, nparts);
+        else if (a.n <= 512) ln_launch_one<true, T, VEC, 2 * P, 1, 256>(ctx, a, nparts);
+        else if (a.n <= 1024) ln_launch_one<true, T, VEC, 2 * P, 2, 256>(ctx, a, nparts);
+        else if (a.n <= 2048) ln_launch_one<true, T, VEC, 2 * P, 4, 256>(ctx, a, nparts);
+        else if (a.n <= 4096) ln_launch_one<true, T, VEC, 2 * P, 8, 256>(ctx, a, nparts);
         else if (a.n <= 8192) ln_launch_one<true, T, VEC, 2 * P, 16, 512>(ctx, a, nparts);
         else ln_launch_one<true, T, VEC, 4 * P, 16, 512>(ctx, a, nparts);
     } else {
