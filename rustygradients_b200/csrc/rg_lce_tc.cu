@@ -22,20 +22,24 @@
 
 #include <algorithm>
 
-#define LT_BM 128
+#define LT_BM 256  // rows of a tile: 128 in each CTA of a pair
 #define LT_BK 64
 #define LT_THREADS 320  // TMA warp, MMA warp, 8 epilogue warps
 #define LT_SPIN_LIMIT (1u << 22)
 #define LT_STAGE_ALL 196608   // bytes of the operand ring
+#define LT_MAX_STAGES 6
 #define LT_SMEM_BYTES (LT_STAGE_ALL + 8 * 32 * 33 * 4 + 1024 + 256)
 #define LT_SEG 4              // k-blocks per accumulator chain for f32 inputs
 
+// Two CTAs (two SMs) work on one tile of 256 x BN: each holds 128 rows of A, half of the columns of B, and the accumulator
+// of its 128 rows.  A k-block then costs an SM 128 x 64 + BN/2 x 64 values from L2 instead of 128 x 64 + BN x 64, which
+// bounded the one-SM form (12.5 TB/s from L2, 1.09 PFLOP/s in bf16).
 template <int PLANES>
 struct lt_shape {
     static constexpr int BN = PLANES == 1 ? 256 : 128;
-    static constexpr int A_BYTES = LT_BM * LT_BK * 2, B_BYTES = BN * LT_BK * 2;
+    static constexpr int A_BYTES = 128 * LT_BK * 2, B_BYTES = BN / 2 * LT_BK * 2;  // of one CTA
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
-    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 4 or 2
+    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6 or 2
 };
 
 // One contraction of a launch: C[M,N] = sum over K of A[m,k] B[n,k]
@@ -62,7 +66,7 @@ struct lt_args {
     const float* lse;         // LT_DZ
     __nv_bfloat16* dz;        // [plane][R][dz_pitch]
     long long dz_pitch;
-    float* dbparts;           // [4 * tiles_m][V] or NULL
+    float* dbparts;           // [LT_BM / 32 * tiles_m][V] or NULL
     float* dxparts;           // LT_GRAD: [splits][R][D]
     int dx_add;               // add to what the pieces before left there
     void* dw;                 // [D][V]
@@ -77,14 +81,36 @@ __device__ __forceinline__ void lt_bar_init(uint64_t* b, uint32_t n) {
 __device__ __forceinline__ void lt_arrive(uint64_t* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(lt_smem(b)) : "memory");
 }
+// the same place in the shared memory of CTA 0 of the pair
+__device__ __forceinline__ uint32_t lt_leader(const void* p) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(lt_smem(p)));
+    return a;
+}
+__device__ __forceinline__ uint32_t lt_peer(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(lt_smem(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void lt_arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool lt_wait(uint64_t* bar, uint32_t parity, int* err) {
     uint32_t ok = 0, spins = 0;
     while (true) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(lt_smem(bar)), "r"(parity)
-            : "memory");
+        if (CLUSTER)
+            asm volatile(
+                "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok)
+                : "r"(lt_smem(bar)), "r"(parity)
+                : "memory");
+        else
+            asm volatile(
+                "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok)
+                : "r"(lt_smem(bar)), "r"(parity)
+                : "memory");
         if (ok) return true;
         if (++spins > LT_SPIN_LIMIT) {
             atomicExch(err, 1);
@@ -92,10 +118,12 @@ __device__ __forceinline__ bool lt_wait(uint64_t* bar, uint32_t parity, int* err
         }
     }
 }
-__device__ __forceinline__ void lt_tma(const CUtensorMap* map, void* dst, uint64_t* bar, int x, int y, int plane) {
+// into this CTA's shared memory; the bytes are counted on a barrier of CTA 0
+__device__ __forceinline__ void lt_tma(const CUtensorMap* map, void* dst, uint32_t bar, int x, int y, int plane) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(lt_smem(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(plane), "r"(lt_smem(bar))
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            lt_smem(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(plane), "r"(bar)
         : "memory");
 }
 // Shared-memory descriptors, 128-byte swizzle.  K-major: rows of 64 elements (128 bytes), groups of 8 rows 1024 bytes
@@ -111,12 +139,15 @@ __device__ __forceinline__ uint64_t lt_desc(uint32_t addr, int mn) {
 }
 __device__ __forceinline__ void lt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
         "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// arrives on the barrier at this place in both CTAs once the MMAs issued so far are done
 __device__ __forceinline__ void lt_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lt_smem(bar)) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(lt_smem(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
 }
 __device__ __forceinline__ void lt_ld32(uint32_t taddr, float (&v)[32]) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -168,6 +199,7 @@ __device__ __forceinline__ lt_tile lt_decode(const lt_args& e, int t) {
 // What a thread keeps of its row while the columns of a tile pass by.
 struct lt_row {
     int row;        // row of C
+    int group;      // number of the warp's 32 rows
     bool live;      // inside the matrix
     int tgt;
     float lse;
@@ -260,8 +292,7 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                         v[i] = keep + __shfl_xor_sync(RG_FULL_MASK, send, half);
                     }
                 }
-                const int q = (threadIdx.x >> 5) & 3;
-                if (lane < left) e.dbparts[(size_t)(t.m * 4 + q) * e.V + c + lane] = v[0];
+                if (lane < left) e.dbparts[(size_t)w.group * e.V + c + lane] = v[0];
             }
         }
         return;
@@ -302,90 +333,106 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
 }
 
 template <int PLANES, int EPI>
-__global__ void __launch_bounds__(LT_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LT_THREADS, 1)
 lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmA1,
               const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ lt_args e) {
     typedef lt_shape<PLANES> S;
     extern __shared__ unsigned char lt_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~(uintptr_t)1023);
     float* stage_all = reinterpret_cast<float*>(ring + LT_STAGE_ALL);
-    uint64_t* full = reinterpret_cast<uint64_t*>(stage_all + 8 * 32 * 33);
-    uint64_t* empty = full + 4;
-    uint64_t* acc_full = empty + 4;     // [2]
-    uint64_t* acc_empty = acc_full + 2; // [2]
-    uint64_t* sched_full = acc_empty + 2;
-    uint64_t* sched_empty = sched_full + 2;
+    uint64_t* full = reinterpret_cast<uint64_t*>(stage_all + 8 * 32 * 33);  // used in CTA 0
+    uint64_t* empty = full + LT_MAX_STAGES;
+    uint64_t* acc_full = empty + LT_MAX_STAGES;  // [2]
+    uint64_t* acc_empty = acc_full + 2;          // [2], used in CTA 0
+    uint64_t* sched_full = acc_empty + 2;        // [2]
+    uint64_t* sched_empty = sched_full + 2;      // [2], used in CTA 0
     uint64_t* drain = sched_empty + 2;
     volatile int* sched_tile = reinterpret_cast<volatile int*>(drain + 1);  // [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     int total = 0;
     for (int i = 0; i < e.nprobs; i++) total += e.p[i].tiles_m * e.p[i].tiles_n * e.p[i].splits;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 4; s++) lt_bar_init(&full[s], 1), lt_bar_init(&empty[s], 1);
+        for (int s = 0; s < LT_MAX_STAGES; s++) lt_bar_init(&full[s], 1), lt_bar_init(&empty[s], 1);
         for (int b = 0; b < 2; b++) {
-            lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 8);
-            lt_bar_init(&sched_full[b], 1), lt_bar_init(&sched_empty[b], 9);
+            lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 16);
+            lt_bar_init(&sched_full[b], 1), lt_bar_init(&sched_empty[b], 18);  // MMA thread and epilogue warps; copy thread and epilogue warps
         }
         lt_bar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(lt_smem(tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(lt_smem(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    // the barriers of both CTAs exist before either uses the other's
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        // ===== one thread hands out tiles and brings their operands =====
+        // ===== one thread of each CTA brings its operands; that of CTA 0 also hands out the tiles to both =====
         if (lane == 0) {
             uint32_t it = 0, ti = 0;
             bool ok = true;
-            int tile = blockIdx.x;
+            int tile = blockIdx.x >> 1;
             while (true) {
                 const uint32_t slot = ti & 1u;
-                ok = lt_wait(&sched_empty[slot], ((ti >> 1) & 1u) ^ 1u, e.err);
-                if (!ok) break;
-                sched_tile[slot] = tile;
-                lt_arrive(&sched_full[slot]);
+                int next = 0;
+                if (rank == 0) {
+                    ok = lt_wait<true>(&sched_empty[slot], ((ti >> 1) & 1u) ^ 1u, e.err);
+                    if (!ok) break;
+                    sched_tile[slot] = tile;
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(lt_peer(const_cast<int*>(&sched_tile[slot]), 1)), "r"(tile) : "memory");
+                    lt_arrive(&sched_full[slot]);
+                    lt_arrive_at(lt_peer(&sched_full[slot], 1));
+                    if (tile < total) next = (int)(gridDim.x >> 1) + atomicAdd(e.counter, 1);  // arrives while this tile is loaded
+                } else {
+                    ok = lt_wait<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
+                    if (!ok) break;
+                    tile = sched_tile[slot];
+                    lt_arrive_at(lt_leader(&sched_empty[slot]));
+                }
                 ti++;
                 if (tile >= total) break;
-                const int next = (int)gridDim.x + atomicAdd(e.counter, 1);  // arrives while this tile is loaded
                 const lt_tile t = lt_decode<EPI>(e, tile);
                 const lt_prob& p = e.p[t.prob];
                 const CUtensorMap* ma = (EPI == LT_GRAD && t.prob) ? &tmA1 : &tmA0;
                 const CUtensorMap* mb = (EPI == LT_GRAD && t.prob) ? &tmB1 : &tmB0;
-                const int m0 = t.m * LT_BM, n0 = t.n * S::BN;
+                const int m0 = t.m * LT_BM + (int)rank * 128, n0 = t.n * S::BN + (int)rank * (S::BN / 2);
                 const int kb0 = t.split * p.kb_per, kb1 = min(kb0 + p.kb_per, (p.K + LT_BK - 1) / LT_BK);
                 for (int kb = kb0; kb < kb1; kb++, it++) {
                     const int s = it % S::STAGES;
                     ok = lt_wait(&empty[s], ((it / S::STAGES) & 1u) ^ 1u, e.err);
                     if (!ok) break;
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lt_smem(&full[s])),
-                                 "r"((uint32_t)S::STAGE_BYTES)
-                                 : "memory");
+                    const uint32_t bar = lt_leader(&full[s]);
+                    if (rank == 0)  // for the bytes of both CTAs (those of CTA 1 may already be arriving: the phase waits for this)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lt_smem(&full[s])),
+                                     "r"((uint32_t)(2 * S::STAGE_BYTES))
+                                     : "memory");
                     unsigned char* a = ring + s * S::STAGE_BYTES;
                     unsigned char* b = a + PLANES * S::A_BYTES;
                     const int k = kb * LT_BK;
 #pragma unroll
                     for (int pl = 0; pl < PLANES; pl++) {
                         if (p.a_mn) {
-                            lt_tma(ma, a + pl * S::A_BYTES, &full[s], m0, k, pl);
-                            lt_tma(ma, a + pl * S::A_BYTES + 8192, &full[s], m0 + 64, k, pl);
+                            lt_tma(ma, a + pl * S::A_BYTES, bar, m0, k, pl);
+                            lt_tma(ma, a + pl * S::A_BYTES + 8192, bar, m0 + 64, k, pl);
                         } else {
-                            lt_tma(ma, a + pl * S::A_BYTES, &full[s], k, m0, pl);
+                            lt_tma(ma, a + pl * S::A_BYTES, bar, k, m0, pl);
                         }
                         if (p.b_mn) {
 #pragma unroll
-                            for (int j = 0; j < S::BN / 64; j++)
-                                lt_tma(mb, b + pl * S::B_BYTES + j * 8192, &full[s], p.b_n0 + n0 + j * 64, k, pl);
+                            for (int j = 0; j < S::BN / 128; j++)
+                                lt_tma(mb, b + pl * S::B_BYTES + j * 8192, bar, p.b_n0 + n0 + j * 64, k, pl);
                         } else {
-                            lt_tma(mb, b + pl * S::B_BYTES, &full[s], p.b_k0 + k, n0, pl);
+                            lt_tma(mb, b + pl * S::B_BYTES, bar, p.b_k0 + k, n0, pl);
                         }
                     }
                 }
@@ -394,11 +441,11 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             }
             if (!ok)  // a wait gave up: the copies in flight land before the CTA's memory goes away
                 for (uint32_t i = it > (uint32_t)S::STAGES ? it - S::STAGES : 0; i < it; i++)
-                    lt_wait(&full[i % S::STAGES], (i / S::STAGES) & 1u, e.err);
+                    lt_wait(&empty[i % S::STAGES], (i / S::STAGES) & 1u, e.err);
         }
     } else if (warp == 1) {
-        // ===== one thread issues the MMAs =====
-        if (lane == 0) {
+        // ===== one thread of CTA 0 issues the MMAs of the pair =====
+        if (lane == 0 && rank == 0) {
             uint32_t it = 0, ti = 0, seg = 0;
             bool ok = true;
             while (true) {
@@ -419,7 +466,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
                     const uint32_t buf = seg & 1u;
-                    ok = lt_wait(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, e.err);
+                    ok = lt_wait<true>(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d0 = tmem + buf * 256, d1 = d0 + 128;
@@ -465,17 +512,18 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
         bool ok = true;
         while (true) {
             const uint32_t slot = ti & 1u;
-            ok = lt_wait(&sched_full[slot], (ti >> 1) & 1u, e.err);
+            ok = lt_wait<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
             if (!ok) break;
             const int tile = sched_tile[slot];
             __syncwarp();
-            if (lane == 0) lt_arrive(&sched_empty[slot]);
+            if (lane == 0) lt_arrive_at(lt_leader(&sched_empty[slot]));
             ti++;
             if (tile >= total) break;
             const lt_tile t = lt_decode<EPI>(e, tile);
             const lt_prob& p = e.p[t.prob];
             lt_row w;
-            w.row = t.m * LT_BM + q * 32 + lane;
+            w.group = t.m * (LT_BM / 32) + (int)rank * 4 + q;
+            w.row = w.group * 32 + lane;
             w.live = w.row < p.M;
             w.ms = {-INFINITY, 0.f};
             w.tgt = (EPI != LT_GRAD && w.live) ? e.tgt[w.row] : -1;
@@ -498,7 +546,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                         if (c == HALF / 32 - 1) {  // the accumulator has been read: hand it back before the last columns are worked on
                             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                             __syncwarp();
-                            if (lane == 0) lt_arrive(&acc_empty[buf]);
+                            if (lane == 0) lt_arrive_at(lt_leader(&acc_empty[buf]));
                         }
                         lt_columns<PLANES, EPI>(e, t, w, acc[0], c0 + c * 32, stage);
                     }
@@ -514,7 +562,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) lt_arrive(&acc_empty[buf]);
+                    if (lane == 0) lt_arrive_at(lt_leader(&acc_empty[buf]));
                 }
             }
             if (!ok) break;
@@ -527,7 +575,9 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    // neither CTA leaves (or gives back its tensor memory) while the other may still reach into it
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -639,7 +689,7 @@ static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
     for (int i = 0; i < e.nprobs; i++) total += (long long)e.p[i].tiles_m * e.p[i].tiles_n * e.p[i].splits;
     if (total > 0x3fffffff) return rg_fail(RG_ERR_SHAPE, "linear_cross_entropy: too many tiles");
     RG_CUDA(cudaMemsetAsync(e.counter, 0, sizeof(int), ctx->stream));
-    const int grid = (int)std::min<long long>(total, ctx->sm_count);
+    const int grid = 2 * (int)std::min<long long>(total, ctx->sm_count / 2);
     lce_tc_kernel<PLANES, EPI><<<grid, LT_THREADS, LT_SMEM_BYTES, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], e);
     RG_CUDA(cudaGetLastError());
     RG_LAUNCHED(ctx);
@@ -666,7 +716,7 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     RG_TRY(lt_operand_of(ctx, c.x, c.R, c.D, c.dtype, &o[0], &x));
     RG_TRY(lt_operand_of(ctx, c.w, c.D, c.V, c.dtype, &o[1], &w));
     CUtensorMap maps[4];
-    RG_TRY(lt_map(&maps[0], x, LT_BM));
+    RG_TRY(lt_map(&maps[0], x, 128));
     RG_TRY(lt_map(&maps[1], w, LT_BK));
     maps[2] = maps[0], maps[3] = maps[1];
     lt_args e;
@@ -699,12 +749,12 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
     lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(c.D, piece, c.R, bn, 1, 1);
     const long long load = (long long)pdx.tiles_m * pdx.tiles_n * pdx.kb_per + (long long)pdw.tiles_m * pdw.tiles_n * pdw.kb_per;
-    const int fair = (int)std::max<long long>(LT_SEG, load / ctx->sm_count / 2);
+    const int fair = (int)std::max<long long>(LT_SEG, load / (ctx->sm_count / 2) / 2);
     // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
     const int run = rg_cdiv(pdx.kb_per, std::min(16, rg_cdiv(pdx.kb_per, fair))), splits = rg_cdiv(pdx.kb_per, run);
     const size_t plen = (size_t)splits * c.R * c.D;
     RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[4]));
-    const int dbrows = 4 * rg_cdiv(c.R, LT_BM);
+    const int dbrows = LT_BM / 32 * rg_cdiv(c.R, LT_BM);
     if (c.dbias) {
         const size_t blen = (size_t)dbrows * c.V;
         RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[5]));
@@ -712,11 +762,11 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
 
     CUtensorMap mz[4], mg[4];
     lt_operand z = {o[3]->raw(), c.R, width, planes, width};
-    RG_TRY(lt_map(&mz[0], x, LT_BM));
+    RG_TRY(lt_map(&mz[0], x, 128));
     RG_TRY(lt_map(&mz[1], w, LT_BK));
     mz[2] = mz[0], mz[3] = mz[1];
-    RG_TRY(lt_map(&mg[0], z, LT_BM));
-    RG_TRY(lt_map(&mg[1], w, bn));
+    RG_TRY(lt_map(&mg[0], z, 128));
+    RG_TRY(lt_map(&mg[1], w, bn / 2));
     RG_TRY(lt_map(&mg[2], x, LT_BK));
     RG_TRY(lt_map(&mg[3], z, LT_BK));
 
