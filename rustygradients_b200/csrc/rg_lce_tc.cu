@@ -92,8 +92,20 @@ __device__ __forceinline__ uint32_t lt_peer(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(lt_smem(p)), "r"(rank));
     return a;
 }
+// Tensor memory has been read, a tile number taken over: nothing in memory is published, so no cluster-wide release (it
+// would wait for every store of this thread that is still on its way).
 __device__ __forceinline__ void lt_arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// with what this thread has written before
+__device__ __forceinline__ void lt_publish_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// e^(v - ref): two roundings of the argument (2^-24 of |v - ref| each) and the 2 steps of the exponential instruction
+__device__ __forceinline__ float lt_exp(float d) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.44269504088896341f));
+    return r;
 }
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool lt_wait(uint64_t* bar, uint32_t parity, int* err) {
@@ -240,19 +252,20 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                 for (int j = 0; j < 32; j++)
                     if (w.tgt == c + j) e.tz[w.row] = v[j];
             }
-            float m = v[0];
+            float mx[4] = {w.ms.m, v[1], v[2], v[3]};
+            mx[0] = fmaxf(mx[0], v[0]);
 #pragma unroll
-            for (int j = 1; j < 32; j++) m = fmaxf(m, v[j]);
-            m = fmaxf(m, w.ms.m);
+            for (int j = 4; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+            const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const float ref = m == -INFINITY ? 0.f : m;
-            float s = w.ms.s * expf(w.ms.m - ref);
+            float s[4] = {w.ms.s * lt_exp(w.ms.m - ref), 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 32; j++) s += expf(v[j] - ref);
-            w.ms = {m, s};
+            for (int j = 0; j < 32; j++) s[j & 3] += lt_exp(v[j] - ref);
+            w.ms = {m, (s[0] + s[1]) + (s[2] + s[3])};
         } else {
             const bool dead = !w.live || w.tgt < 0;
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = (dead || j >= left) ? 0.f : expf(v[j] - w.lse);
+            for (int j = 0; j < 32; j++) v[j] = (dead || j >= left) ? 0.f : lt_exp(v[j] - w.lse);
             if (any && here) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
@@ -270,10 +283,15 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                             const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * k], v[j + 2 * k + 1]);
                             h[0][k] = *reinterpret_cast<const uint32_t*>(&b);
                         } else {
-                            uint32_t a0, a1, a2, b0, b1, b2;
-                            lt_split3(v[j + 2 * k], a0, a1, a2);
-                            lt_split3(v[j + 2 * k + 1], b0, b1, b2);
-                            h[0][k] = a0 | (b0 << 16), h[1][k] = a1 | (b1 << 16), h[2][k] = a2 | (b2 << 16);
+                            // finite but for what was not finite before; each plane truncates, what is left is exact
+                            const float a = v[j + 2 * k], b = v[j + 2 * k + 1];
+                            const float a1 = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                            const float b1 = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+                            const float a2 = a1 - __uint_as_float(__float_as_uint(a1) & 0xffff0000u);
+                            const float b2 = b1 - __uint_as_float(__float_as_uint(b1) & 0xffff0000u);
+                            h[0][k] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+                            h[1][k] = __byte_perm(__float_as_uint(a1), __float_as_uint(b1), 0x7632);
+                            h[2][k] = __byte_perm(__float_as_uint(a2), __float_as_uint(b2), 0x7632);
                         }
                     }
 #pragma unroll
@@ -386,12 +404,12 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t slot = ti & 1u;
                 int next = 0;
                 if (rank == 0) {
-                    ok = lt_wait<true>(&sched_empty[slot], ((ti >> 1) & 1u) ^ 1u, e.err);
+                    ok = lt_wait(&sched_empty[slot], ((ti >> 1) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     sched_tile[slot] = tile;
                     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(lt_peer(const_cast<int*>(&sched_tile[slot]), 1)), "r"(tile) : "memory");
                     lt_arrive(&sched_full[slot]);
-                    lt_arrive_at(lt_peer(&sched_full[slot], 1));
+                    lt_publish_at(lt_peer(&sched_full[slot], 1));
                     if (tile < total) next = (int)(gridDim.x >> 1) + atomicAdd(e.counter, 1);  // arrives while this tile is loaded
                 } else {
                     ok = lt_wait<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
@@ -466,7 +484,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
                     const uint32_t buf = seg & 1u;
-                    ok = lt_wait<true>(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, e.err);
+                    ok = lt_wait(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d0 = tmem + buf * 256, d1 = d0 + 128;
@@ -531,7 +549,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
             const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
-            float acc[PLANES == 1 ? 1 : HALF / 32][32];
+            float acc[2][32];
+            static_assert(PLANES == 1 || HALF == 64, "two groups of 32 columns a thread");
             for (int sg = 0; sg < segs; sg++, seg++) {
                 const uint32_t buf = seg & 1u;
                 ok = lt_wait(&acc_full[buf], (seg >> 1) & 1u, e.err);
@@ -539,16 +558,22 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ta = taddr + buf * 256;
                 if (PLANES == 1) {
+                    // the next 32 columns are on their way while these are worked on
+                    lt_ld32(ta, acc[0]);
 #pragma unroll 1
-                    for (int c = 0; c < HALF / 32; c++) {
-                        lt_ld32(ta + c * 32, acc[0]);
+                    for (int c = 0; c < HALF / 32; c += 2) {
                         lt_ld_wait();
-                        if (c == HALF / 32 - 1) {  // the accumulator has been read: hand it back before the last columns are worked on
+                        lt_ld32(ta + (c + 1) * 32, acc[PLANES == 1 ? 1 : 0]);
+                        lt_columns<PLANES, EPI>(e, t, w, acc[0], c0 + c * 32, stage);
+                        lt_ld_wait();
+                        if (c + 2 < HALF / 32) {
+                            lt_ld32(ta + (c + 2) * 32, acc[0]);
+                        } else {  // the accumulator has been read: hand it back before the last columns are worked on
                             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                             __syncwarp();
                             if (lane == 0) lt_arrive_at(lt_leader(&acc_empty[buf]));
                         }
-                        lt_columns<PLANES, EPI>(e, t, w, acc[0], c0 + c * 32, stage);
+                        lt_columns<PLANES, EPI>(e, t, w, acc[PLANES == 1 ? 1 : 0], c0 + (c + 1) * 32, stage);
                     }
                 } else {
 #pragma unroll
