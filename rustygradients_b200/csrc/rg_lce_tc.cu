@@ -2,7 +2,8 @@
 //
 //   logits  z[R,V]  = x[R,D] w[D,V]      -> (maximum, sum) per row and tile, or dz of a piece of the vocabulary
 //   dx      [R,D]   = dz[R,V] w[D,V]^T
-//   dw      [D,V]   = x[R,D]^T dz[R,V]
+//   dw      [D,V]   = x[R,D]^T dz[R,V], computed as its transpose dz^T x: V fills whole row tiles of 256, and the column
+//                     tiles of D can be narrow
 //
 // Every operand is used as it lies in memory: tcgen05 takes a shared-memory tile either with the contraction axis
 // contiguous ("K-major") or with the other axis contiguous ("MN-major"), so no transposed copy of x, w or dz exists.  TMA
@@ -201,11 +202,20 @@ __device__ __forceinline__ lt_tile lt_decode(const lt_args& e, int t) {
         r.m = t % e.p[0].tiles_m, r.split = t / e.p[0].tiles_m;
         return r;
     }
-    // logits and dw: the row tiles of one column tile together (they share w, dz)
-    r.prob = EPI == LT_GRAD ? 1 : 0;
-    if (EPI == LT_GRAD) t -= n0;
-    r.m = t % e.p[r.prob].tiles_m, r.n = t / e.p[r.prob].tiles_m, r.split = 0;
+    if (EPI == LT_GRAD) {  // dw: the column tiles of one row tile together (they share dz)
+        r.prob = 1, r.split = 0, t -= n0;
+        r.n = t % e.p[1].tiles_n, r.m = t / e.p[1].tiles_n;
+        return r;
+    }
+    // logits: the row tiles of one column tile together (they share w)
+    r.prob = 0, r.split = 0;
+    r.m = t % e.p[0].tiles_m, r.n = t / e.p[0].tiles_m;
     return r;
+}
+// Columns of a tile that are multiplied: the last tile of a row is as narrow as the matrix allows.
+template <int PLANES>
+__device__ __forceinline__ int lt_width(const lt_prob& p, int n) {
+    return min(lt_shape<PLANES>::BN, (p.N - n * lt_shape<PLANES>::BN + 31) & ~31);
 }
 
 // What a thread keeps of its row while the columns of a tile pass by.
@@ -315,36 +325,40 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
         }
         return;
     }
-    // gradients: through shared memory, so that a warp stores 32 consecutive columns of one row at a time whatever the
-    // alignment of the rows (the GPT-2 vocabulary is odd)
+    const lt_prob& p = e.p[t.prob];
+    const int cols = min(32, p.N - col);
+    if (t.prob == 1) {
+        // dw^T: the lanes are neighbouring columns of dw, a register is a row of it, so a warp's store is contiguous
+        if (!w.live) return;
+        const float scale = e.scal[1];
+        const size_t at = (size_t)col * e.V + e.v0 + w.row;
+        if (e.dw_bf16) {
+            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(e.dw) + at;
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (j < cols) o[(size_t)j * e.V] = __float2bfloat16_rn(v[j] * scale);
+        } else {
+            float* o = static_cast<float*>(e.dw) + at;
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (j < cols) o[(size_t)j * e.V] = v[j] * scale;
+        }
+        return;
+    }
+    // partial dx: through shared memory, so that a warp stores 32 consecutive columns of one row at a time
+    if (cols <= 0) return;
 #pragma unroll
     for (int j = 0; j < 32; j++) stage[lane * 33 + j] = v[j];
     __syncwarp();
     const int row0 = w.row - lane;
-    const int n = col + lane;
-    const lt_prob& p = e.p[t.prob];
     const int rows = min(32, p.M - row0);
-    if (n < p.N) {
-        if (t.prob == 0) {
-            float* o = e.dxparts + ((size_t)t.split * e.R + row0) * e.D + n;
+    if (lane < cols) {
+        float* o = e.dxparts + ((size_t)t.split * e.R + row0) * e.D + col + lane;
 #pragma unroll 8
-            for (int r = 0; r < rows; r++) {
-                float s = stage[r * 33 + lane];
-                if (e.dx_add) s += o[(size_t)r * e.D];
-                o[(size_t)r * e.D] = s;
-            }
-        } else {
-            const float scale = e.scal[1];
-            const size_t at = (size_t)row0 * e.V + e.v0 + n;
-            if (e.dw_bf16) {
-                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(e.dw) + at;
-#pragma unroll 8
-                for (int r = 0; r < rows; r++) o[(size_t)r * e.V] = __float2bfloat16_rn(stage[r * 33 + lane] * scale);
-            } else {
-                float* o = static_cast<float*>(e.dw) + at;
-#pragma unroll 8
-                for (int r = 0; r < rows; r++) o[(size_t)r * e.V] = stage[r * 33 + lane] * scale;
-            }
+        for (int r = 0; r < rows; r++) {
+            float s = stage[r * 33 + lane];
+            if (e.dx_add) s += o[(size_t)r * e.D];
+            o[(size_t)r * e.D] = s;
         }
     }
     __syncwarp();
@@ -423,7 +437,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const lt_prob& p = e.p[t.prob];
                 const CUtensorMap* ma = (EPI == LT_GRAD && t.prob) ? &tmA1 : &tmA0;
                 const CUtensorMap* mb = (EPI == LT_GRAD && t.prob) ? &tmB1 : &tmB0;
-                const int m0 = t.m * LT_BM + (int)rank * 128, n0 = t.n * S::BN + (int)rank * (S::BN / 2);
+                const int m0 = t.m * LT_BM + (int)rank * 128, n0 = t.n * S::BN + (int)rank * (lt_width<PLANES>(p, t.n) / 2);
                 const int kb0 = t.split * p.kb_per, kb1 = min(kb0 + p.kb_per, (p.K + LT_BK - 1) / LT_BK);
                 for (int kb = kb0; kb < kb1; kb++, it++) {
                     const int s = it % S::STAGES;
@@ -479,7 +493,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
                 // D f32, A and B bf16, their majors, N, M
                 const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
-                                       ((uint32_t)(S::BN >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
+                                       ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
                 const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
@@ -772,7 +786,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[3], RG_DTYPE_BF16));
 
     // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
-    lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(c.D, piece, c.R, bn, 1, 1);
+    lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
     const long long load = (long long)pdx.tiles_m * pdx.tiles_n * pdx.kb_per + (long long)pdw.tiles_m * pdw.tiles_n * pdw.kb_per;
     const int fair = (int)std::max<long long>(LT_SEG, load / (ctx->sm_count / 2) / 2);
     // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
@@ -792,8 +806,8 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     mz[2] = mz[0], mz[3] = mz[1];
     RG_TRY(lt_map(&mg[0], z, 128));
     RG_TRY(lt_map(&mg[1], w, bn / 2));
-    RG_TRY(lt_map(&mg[2], x, LT_BK));
-    RG_TRY(lt_map(&mg[3], z, LT_BK));
+    RG_TRY(lt_map(&mg[2], z, LT_BK));
+    RG_TRY(lt_map(&mg[3], x, LT_BK));
 
     for (int i = 0; i < pieces; i++) {
         lt_args e;
@@ -811,7 +825,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.p[0] = lt_problem(c.R, c.D, e.vn, bn, 0, 0);
         e.p[0].splits = rg_cdiv(e.p[0].kb_per, run), e.p[0].kb_per = run;
         e.p[0].b_k0 = e.v0;
-        e.p[1] = lt_problem(c.D, e.vn, c.R, bn, 1, 1);
+        e.p[1] = lt_problem(e.vn, c.D, c.R, bn, 1, 1);
         RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
     }
     lce_dx_finish_launch(ctx, o[4]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
