@@ -10,16 +10,22 @@
 // brings 64-element wide boxes (128-byte swizzle) of three-dimensional arrays [plane][row][column]; what lies outside is
 // filled with zeros, which handles every ragged edge of R, D and V.
 //
-// bf16 inputs are one plane and are multiplied as they are.  f32 inputs are split into three bf16 planes that hold all 24
-// bits (x = x0 + x1 + x2 exactly, each the leading 8 bits of what the planes before leave), and six of the nine products
-// are accumulated; the three left out are below 2^-23 of the product of magnitudes.  The tensor core truncates when it adds
-// to its f32 accumulator, so a long chain loses about 2^-25 of the running sum per step (measured: a relative error of
-// 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32 inputs the chain is therefore cut every 256 elements
-// of K: x0 w0 and the five small products have an accumulator each, and the epilogue warps add both to f32 registers with
-// rounding.
+// bf16 inputs are one plane and are multiplied as they are.  f32 inputs are split into planes of 16 bits whose products are
+// accumulated in f32:
+//  * logits: two f16 planes, x = 2^-a (x0 + x1) with one power of two per row of x (column of w) that brings the largest
+//    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits and everything down to 2^-40 of that largest magnitude; three of the four
+//    products are taken, the fourth is below 2^-22 of the magnitudes.  The scales leave in the epilogue.
+//  * dx, dw: the sums run over the vocabulary and over the rows, where dz spans many orders of magnitude (a rare word's
+//    gradient is a sum of tiny ones), so f16's range is not enough: three bf16 planes hold all 24 bits (each the leading 8 bits
+//    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
+// The tensor core truncates when it adds to its f32 accumulator, so a long chain loses about 2^-25 of the running sum per
+// step (measured: a relative error of 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32 inputs the chain is
+// therefore cut every 256 elements of K: the product of the first planes and the small ones have an accumulator each, and
+// the epilogue warps add both to f32 registers with rounding.
 #include "rg_lce.cuh"
 
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -35,12 +41,13 @@
 // Two CTAs (two SMs) work on one tile of 256 x BN: each holds 128 rows of A, half of the columns of B, and the accumulator
 // of its 128 rows.  A k-block then costs an SM 128 x 64 + BN/2 x 64 values from L2 instead of 128 x 64 + BN x 64, which
 // bounded the one-SM form (12.5 TB/s from L2, 1.09 PFLOP/s in bf16).
+// PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.
 template <int PLANES>
 struct lt_shape {
     static constexpr int BN = PLANES == 1 ? 256 : 128;
     static constexpr int A_BYTES = 128 * LT_BK * 2, B_BYTES = BN / 2 * LT_BK * 2;  // of one CTA
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
-    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6 or 2
+    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6, 4 or 2
 };
 
 // One contraction of a launch: C[M,N] = sum over K of A[m,k] B[n,k]
@@ -61,11 +68,12 @@ struct lt_args {
     int R, D, V;
     int v0, vn;    // piece of the vocabulary: first column, number of columns
     const float* bias;
+    const float *xscale, *wscale;  // PLANES 2: what a row (a column) of the accumulated logits is multiplied with
     const int* tgt;
     float2* parts;            // LT_FWD
     float* tz;
     const float* lse;         // LT_DZ
-    __nv_bfloat16* dz;        // [plane][R][dz_pitch]
+    __nv_bfloat16* dz;        // [plane][R][dz_pitch]: 1 plane for bf16, 3 for f32 inputs
     long long dz_pitch;
     float* dbparts;           // [LT_BM / 32 * tiles_m][V] or NULL
     float* dxparts;           // LT_GRAD: [splits][R][D]
@@ -93,12 +101,12 @@ __device__ __forceinline__ uint32_t lt_peer(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(lt_smem(p)), "r"(rank));
     return a;
 }
-// Tensor memory has been read, a tile number taken over: nothing in memory is published, so no cluster-wide release (it
-// would wait for every store of this thread that is still on its way).
+// For what has been read into registers already (tensor memory after its wait, a tile number that has been used): nothing in
+// memory is published, so no cluster-wide release - it would wait for every store of this thread that is still on its way.
 __device__ __forceinline__ void lt_arrive_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// with what this thread has written before
+// ordered after what this thread has read and written before
 __device__ __forceinline__ void lt_publish_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -224,7 +232,7 @@ struct lt_row {
     int group;      // number of the warp's 32 rows
     bool live;      // inside the matrix
     int tgt;
-    float lse;
+    float lse, scale;
     lce_ms ms;
 };
 
@@ -235,6 +243,20 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
     if (EPI == LT_FWD || EPI == LT_DZ) {
         const int c = e.v0 + col, left = e.v0 + e.vn - c;  // vocabulary column of v[0]; columns inside the piece
         if (left <= 0 && EPI == LT_FWD) return;
+        if (PLANES == 2) {  // exact powers of two
+            if (left >= 32) {
+                const float4* b = reinterpret_cast<const float4*>(e.wscale + c);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float4 q = __ldg(b + j);
+                    v[4 * j] *= q.x * w.scale, v[4 * j + 1] *= q.y * w.scale, v[4 * j + 2] *= q.z * w.scale, v[4 * j + 3] *= q.w * w.scale;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (j < left) v[j] *= e.wscale[c + j] * w.scale;
+            }
+        }
         if (e.bias) {
             if (left >= 32) {
                 const float4* b = reinterpret_cast<const float4*>(e.bias + c);
@@ -286,6 +308,7 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                 const long long plane = (long long)e.R * e.dz_pitch;
 #pragma unroll
                 for (int j = 0; j < 32; j += 8) {
+                    constexpr int ZP = PLANES == 1 ? 1 : 3;
                     uint32_t h[3][4];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
@@ -305,7 +328,7 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                         }
                     }
 #pragma unroll
-                    for (int p = 0; p < PLANES; p++)
+                    for (int p = 0; p < ZP; p++)
                         *reinterpret_cast<uint4*>(o + p * plane + j) = make_uint4(h[p][0], h[p][1], h[p][2], h[p][3]);
                 }
             }
@@ -429,7 +452,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                     ok = lt_wait<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
                     if (!ok) break;
                     tile = sched_tile[slot];
-                    lt_arrive_at(lt_leader(&sched_empty[slot]));
+                    lt_publish_at(lt_leader(&sched_empty[slot]));  // after the read
                 }
                 ti++;
                 if (tile >= total) break;
@@ -491,8 +514,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const lt_tile t = lt_decode<EPI>(e, tile);
                 const lt_prob& p = e.p[t.prob];
                 const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
-                // D f32, A and B bf16, their majors, N, M
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
+                // D f32, A and B bf16 (f16), their majors, N, M
+                const uint32_t idesc = (1u << 4) | (PLANES == 2 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
                                        ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
                 const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
@@ -515,7 +538,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                                 lt_mma(d0, lt_desc(a + k * astep, p.a_mn), lt_desc(b + k * bstep, p.b_mn), idesc, kb > 0 || k > 0);
                         } else {
 #pragma unroll
-                            for (int pr = 0; pr < 6; pr++) {
+                            for (int pr = 0; pr < (PLANES == 2 ? 3 : 6); pr++) {
                                 constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
 #pragma unroll
                                 for (int k = 0; k < LT_BK / 16; k++)
@@ -546,8 +569,9 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             const uint32_t slot = ti & 1u;
             ok = lt_wait<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
             if (!ok) break;
-            const int tile = sched_tile[slot];
-            __syncwarp();
+            // lane 0's value goes to all lanes, so its read is complete before it hands the slot back (the arrival alone would not
+            // wait for a read that is queued behind this warp's stores)
+            const int tile = __shfl_sync(RG_FULL_MASK, lane == 0 ? sched_tile[slot] : 0, 0);
             if (lane == 0) lt_arrive_at(lt_leader(&sched_empty[slot]));
             ti++;
             if (tile >= total) break;
@@ -560,6 +584,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.ms = {-INFINITY, 0.f};
             w.tgt = (EPI != LT_GRAD && w.live) ? e.tgt[w.row] : -1;
             w.lse = (EPI == LT_DZ && w.live) ? e.lse[w.row] : 0.f;
+            w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
             const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
@@ -569,6 +594,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t buf = seg & 1u;
                 ok = lt_wait(&acc_full[buf], (seg >> 1) & 1u, e.err);
                 if (!ok) break;
+                __syncwarp();  // the loads below are executed by whole warps
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ta = taddr + buf * 256;
                 if (PLANES == 1) {
@@ -622,34 +648,112 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 // ---------------------------------------------------------------------------
 // operands
 // ---------------------------------------------------------------------------
-// bf16 planes [plane][rows][pitch] of a matrix whose rows TMA cannot address (f32 values, or rows that do not start on
-// 16-byte boundaries).  A thread writes 16 bytes of each plane.
-template <int PLANES, typename T>
-__global__ void __launch_bounds__(256) lt_pack_kernel(const T* __restrict__ src, long long rows, int cols, int pitch,
-                                                      __nv_bfloat16* __restrict__ dst) {
+// A bf16 matrix whose rows TMA cannot address (they do not start on 16-byte boundaries), copied to such rows.
+__global__ void __launch_bounds__(256) lt_align_kernel(const __nv_bfloat16* __restrict__ src, long long rows, int cols, int pitch,
+                                                       __nv_bfloat16* __restrict__ dst) {
     const int groups = pitch / 8;
     const long long n = rows * groups, stride = (long long)gridDim.x * 256;
+    const unsigned short* in = reinterpret_cast<const unsigned short*>(src);
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
         const long long r = i / groups;
         const int c = (int)(i - r * groups) * 8;
-        uint32_t h[3][4];
+        uint32_t h[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const float a = c + 2 * k < cols ? rg_to_float(src[r * cols + c + 2 * k]) : 0.f;
-            const float b = c + 2 * k + 1 < cols ? rg_to_float(src[r * cols + c + 2 * k + 1]) : 0.f;
-            if (PLANES == 1) {
-                const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);  // exact: the values are bf16
-                h[0][k] = *reinterpret_cast<const uint32_t*>(&q);
-            } else {
-                uint32_t a0, a1, a2, b0, b1, b2;
-                lt_split3(a, a0, a1, a2);
-                lt_split3(b, b0, b1, b2);
-                h[0][k] = a0 | (b0 << 16), h[1][k] = a1 | (b1 << 16), h[2][k] = a2 | (b2 << 16);
-            }
+            const uint32_t a = c + 2 * k < cols ? in[r * cols + c + 2 * k] : 0u, b = c + 2 * k + 1 < cols ? in[r * cols + c + 2 * k + 1] : 0u;
+            h[k] = a | (b << 16);
         }
+        *reinterpret_cast<uint4*>(dst + r * pitch + c) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+}
+
+// The scale of a group of values with the largest finite magnitude m: 2^a with m 2^a in [2^14, 2^15), and 2^-a.  The exponent
+// stays where both are normal numbers.
+__device__ __forceinline__ float2 lt_scale(float m) {
+    const int e = m > 0.f ? (int)(__float_as_uint(m) >> 23) - 127 : 14;  // subnormal: -127
+    const int a = min(14 - e, 126);
+    return make_float2(__int_as_float((a + 127) << 23), __int_as_float((127 - a) << 23));
+}
+__device__ __forceinline__ float lt_finite_abs(float v) {
+    const float a = fabsf(v);
+    return a <= 3.4028235e38f ? a : 0.f;  // infinity and NaN do not take part in the scale
+}
+// v 2^a as two f16: nearest, and nearest to what is left.  Infinity and NaN leave nothing.
+__device__ __forceinline__ void lt_split2(float v, float scale, uint32_t& h0, uint32_t& h1) {
+    const float s = v * scale;
+    const __half a = __float2half_rn(s);
+    const float r = s - __half2float(a);
+    const __half b = __float2half_rn(fabsf(s) <= 65504.f ? r : 0.f);
+    h0 = __half_as_ushort(a), h1 = __half_as_ushort(b);
+}
+
+// f32 values as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row (x), and triples of bf16 (NULL: not
+// wanted).  A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
+__global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
+                                                           uint16_t* __restrict__ pair, uint16_t* __restrict__ triple,
+                                                           float* __restrict__ scale_out) {
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= rows) return;
+    const float* p = src + (size_t)r * cols;
+    float m = 0.f;
+#pragma unroll 8
+    for (int c = lane; c < cols; c += 32) m = fmaxf(m, lt_finite_abs(p[c]));
+    const float2 sc = lt_scale(rg_warp_max(m));
+    if (lane == 0) scale_out[r] = sc.y;
+    const size_t plane = (size_t)rows * pitch;
+#pragma unroll 4
+    for (int c = lane; c < cols; c += 32) {
+        const size_t at = (size_t)r * pitch + c;
+        uint32_t h0, h1, h2;
+        lt_split2(p[c], sc.x, h0, h1);
+        pair[at] = (uint16_t)h0, pair[at + plane] = (uint16_t)h1;
+        if (triple) {
+            lt_split3(p[c], h0, h1, h2);
+            triple[at] = (uint16_t)h0, triple[at + plane] = (uint16_t)h1, triple[at + 2 * plane] = (uint16_t)h2;
+        }
+    }
+}
+
+// The same with a scale per column (w).  A CTA owns 64 columns: its 16 warps read all rows for the largest magnitudes, then
+// once more (64 columns of two CTAs per SM stay in L2) to write them; a lane holds two neighbouring columns, so that a warp
+// stores 128 contiguous bytes of each plane.  Memory bound: 4 bytes in, 4 (10 with the triples) out per value.
+__global__ void __launch_bounds__(512) lt_pack_cols_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
+                                                           uint32_t* __restrict__ pair, uint32_t* __restrict__ triple,
+                                                           float* __restrict__ scale_out) {
+    extern __shared__ float lt_red[];  // [16][64]; the launch asks for more to keep the number of resident CTAs at two
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int c = blockIdx.x * 64 + 2 * lane;
+    const bool in0 = c < cols, in1 = c + 1 < cols;
+    float m0 = 0.f, m1 = 0.f;
+#pragma unroll 8
+    for (int r = w; r < rows; r += 16) {
+        const float* p = src + (size_t)r * cols + c;
+        m0 = fmaxf(m0, in0 ? lt_finite_abs(p[0]) : 0.f);
+        m1 = fmaxf(m1, in1 ? lt_finite_abs(p[1]) : 0.f);
+    }
+    lt_red[w * 64 + 2 * lane] = m0, lt_red[w * 64 + 2 * lane + 1] = m1;
+    __syncthreads();
 #pragma unroll
-        for (int p = 0; p < PLANES; p++)
-            *reinterpret_cast<uint4*>(dst + (p * rows + r) * pitch + c) = make_uint4(h[p][0], h[p][1], h[p][2], h[p][3]);
+    for (int k = 0; k < 16; k++) m0 = fmaxf(m0, lt_red[k * 64 + 2 * lane]), m1 = fmaxf(m1, lt_red[k * 64 + 2 * lane + 1]);
+    const float2 s0 = lt_scale(m0), s1 = lt_scale(m1);
+    if (w == 0 && in0) scale_out[c] = s0.y;
+    if (w == 0 && in1) scale_out[c + 1] = s1.y;
+    if (c >= pitch) return;
+    const size_t plane = (size_t)rows * pitch / 2;  // pitch is even
+#pragma unroll 4
+    for (int r = w; r < rows; r += 16) {
+        const float* p = src + (size_t)r * cols + c;
+        const float a = in0 ? p[0] : 0.f, b = in1 ? p[1] : 0.f;
+        const size_t at = ((size_t)r * pitch + c) / 2;
+        uint32_t a0, a1, a2, b0, b1, b2;
+        lt_split2(a, s0.x, a0, a1);
+        lt_split2(b, s1.x, b0, b1);
+        pair[at] = a0 | (b0 << 16), pair[at + plane] = a1 | (b1 << 16);
+        if (triple) {
+            lt_split3(a, a0, a1, a2);
+            lt_split3(b, b0, b1, b2);
+            triple[at] = a0 | (b0 << 16), triple[at + plane] = a1 | (b1 << 16), triple[at + 2 * plane] = a2 | (b2 << 16);
+        }
     }
 }
 
@@ -692,24 +796,55 @@ static rg_status lt_map(CUtensorMap* map, const lt_operand& o, int box_rows) {
     return RG_OK;
 }
 
-// The operand as TMA reads it: the caller's matrix itself, or packed planes in `scratch`.
-static rg_status lt_operand_of(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, rg_storage** scratch, lt_operand* o) {
-    const int planes = dtype == RG_DTYPE_F32 ? 3 : 1;
-    *o = {src, rows, cols, planes, cols};
-    if (planes == 1 && cols % 8 == 0) return RG_OK;
+// x or w as TMA reads it.  bf16: the caller's matrix itself, or a copy with aligned rows; `logits` and `grads` are the same.
+// f32: packed pairs for the logits and, where the call needs them, triples for the gradients.
+struct lt_packed {
+    lt_operand logits, grads;
+    const float* scale;
+    rg_outputs<3> mem;
+};
+static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, bool by_column, bool want_grads, lt_packed* o) {
+    o->scale = nullptr;
+    if (dtype == RG_DTYPE_BF16 && cols % 8 == 0) {
+        o->logits = o->grads = {src, rows, cols, 1, cols};
+        return RG_OK;
+    }
     const int pitch = (cols + 7) / 8 * 8;
-    const size_t halves = (size_t)planes * rows * pitch;
-    RG_TRY(rg_alloc_storage(ctx, &halves, 1, scratch, RG_DTYPE_BF16));
-    o->base = (*scratch)->raw(), o->pitch = pitch;
-    const int grid = (int)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>((*scratch)->raw());
-    if (planes == 3) lt_pack_kernel<3, float><<<grid, 256, 0, ctx->stream>>>((const float*)src, rows, cols, pitch, dst);
-    else lt_pack_kernel<1, __nv_bfloat16><<<grid, 256, 0, ctx->stream>>>((const __nv_bfloat16*)src, rows, cols, pitch, dst);
+    const size_t plane = (size_t)rows * pitch, pair = 2 * plane, triple = 3 * plane, scales = by_column ? cols : rows;
+    if (dtype == RG_DTYPE_BF16) {
+        RG_TRY(rg_alloc_storage(ctx, &plane, 1, &o->mem[0], RG_DTYPE_BF16));
+        const int grid = (int)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
+        lt_align_kernel<<<grid, 256, 0, ctx->stream>>>(static_cast<const __nv_bfloat16*>(src), rows, cols, pitch,
+                                                       static_cast<__nv_bfloat16*>(o->mem[0]->raw()));
+        RG_LAUNCHED(ctx);
+        o->logits = o->grads = {o->mem[0]->raw(), rows, cols, 1, pitch};
+        return RG_OK;
+    }
+    RG_TRY(rg_alloc_storage(ctx, &pair, 1, &o->mem[0], RG_DTYPE_BF16));
+    RG_TRY(rg_alloc_storage(ctx, &scales, 1, &o->mem[1]));
+    if (want_grads) RG_TRY(rg_alloc_storage(ctx, &triple, 1, &o->mem[2], RG_DTYPE_BF16));
+    void* three = want_grads ? o->mem[2]->raw() : nullptr;
+    o->scale = o->mem[1]->data();
+    if (by_column) {
+        const int smem = 80 * 1024;
+        RG_CUDA(cudaFuncSetAttribute(lt_pack_cols_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        lt_pack_cols_kernel<<<rg_cdiv(cols, 64), 512, smem, ctx->stream>>>(static_cast<const float*>(src), rows, cols, pitch,
+                                                                          static_cast<uint32_t*>(o->mem[0]->raw()),
+                                                                          static_cast<uint32_t*>(three), o->mem[1]->data());
+    } else {
+        lt_pack_rows_kernel<<<rg_cdiv(rows, 8), 256, 0, ctx->stream>>>(static_cast<const float*>(src), rows, cols, pitch,
+                                                                      static_cast<uint16_t*>(o->mem[0]->raw()),
+                                                                      static_cast<uint16_t*>(three), o->mem[1]->data());
+    }
+    RG_CUDA(cudaGetLastError());
     RG_LAUNCHED(ctx);
+    o->logits = {o->mem[0]->raw(), rows, cols, 2, pitch};
+    o->grads = {three, rows, cols, 3, pitch};
     return RG_OK;
 }
 
-static int lt_bn(int dtype) { return dtype == RG_DTYPE_F32 ? lt_shape<3>::BN : lt_shape<1>::BN; }
+static int lt_bn(int dtype) { return dtype == RG_DTYPE_F32 ? lt_shape<2>::BN : lt_shape<1>::BN; }
+static_assert(lt_shape<2>::BN == lt_shape<3>::BN, "f32 inputs: one width of column tiles");
 int lce_tc_nparts(int V, int dtype) { return 2 * rg_cdiv(V, lt_bn(dtype)); }
 
 static lt_prob lt_problem(int M, int N, int K, int bn, int a_mn, int b_mn) {
@@ -736,7 +871,7 @@ static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
 }
 template <int EPI>
 static rg_status lt_run(rg_ctx* ctx, const lce_call& c, const CUtensorMap* maps, lt_args& e) {
-    return c.dtype == RG_DTYPE_F32 ? lt_launch<3, EPI>(ctx, maps, e) : lt_launch<1, EPI>(ctx, maps, e);
+    return c.dtype == RG_DTYPE_F32 ? lt_launch<EPI == LT_GRAD ? 3 : 2, EPI>(ctx, maps, e) : lt_launch<1, EPI>(ctx, maps, e);
 }
 
 static void lt_common(rg_ctx* ctx, const lce_call& c, rg_storage* counter, lt_args* e) {
@@ -748,18 +883,19 @@ static void lt_common(rg_ctx* ctx, const lce_call& c, rg_storage* counter, lt_ar
 }
 
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
-    rg_outputs<3> o;  // packed x, packed w, counter
-    lt_operand x, w;
+    rg_outputs<1> o;  // counter
+    lt_packed x, w;
     const size_t one = 1;
-    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[2]));
-    RG_TRY(lt_operand_of(ctx, c.x, c.R, c.D, c.dtype, &o[0], &x));
-    RG_TRY(lt_operand_of(ctx, c.w, c.D, c.V, c.dtype, &o[1], &w));
+    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, false, false, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, true, false, &w));
     CUtensorMap maps[4];
-    RG_TRY(lt_map(&maps[0], x, 128));
-    RG_TRY(lt_map(&maps[1], w, LT_BK));
+    RG_TRY(lt_map(&maps[0], x.logits, 128));
+    RG_TRY(lt_map(&maps[1], w.logits, LT_BK));
     maps[2] = maps[0], maps[3] = maps[1];
     lt_args e;
-    lt_common(ctx, c, o[2], &e);
+    lt_common(ctx, c, o[0], &e);
+    e.xscale = x.scale, e.wscale = w.scale;
     e.nprobs = 1;
     e.p[0] = lt_problem(c.R, c.V, c.D, lt_bn(c.dtype), 0, 1);
     return lt_run<LT_FWD>(ctx, c, maps, e);
@@ -770,20 +906,20 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
 #define LT_DZ_BYTES ((size_t)512 << 20)
 
 rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
-    rg_outputs<6> o;  // packed x, packed w, counter, dz, partial dx, partial dbias
-    lt_operand x, w;
+    rg_outputs<4> o;  // counter, dz, partial dx, partial dbias
+    lt_packed x, w;
     const size_t one = 1;
     const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = lt_bn(c.dtype);
-    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[2]));
-    RG_TRY(lt_operand_of(ctx, c.x, c.R, c.D, c.dtype, &o[0], &x));
-    RG_TRY(lt_operand_of(ctx, c.w, c.D, c.V, c.dtype, &o[1], &w));
+    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, false, true, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, true, true, &w));
 
     const long long most = std::max<long long>(1, (long long)(LT_DZ_BYTES / ((size_t)planes * 2 * c.R)) / 256) * 256;
     const int pieces = (int)((c.V + most - 1) / most);
     const int piece = (int)std::min<long long>(most, (rg_cdiv(c.V, pieces) + 255) / 256 * 256);
     const int width = std::min(piece, (c.V + 63) / 64 * 64);  // columns of dz that are stored
     const size_t zlen = (size_t)planes * c.R * width;
-    RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[3], RG_DTYPE_BF16));
+    RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[1], RG_DTYPE_BF16));
 
     // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
     lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
@@ -792,30 +928,31 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
     const int run = rg_cdiv(pdx.kb_per, std::min(16, rg_cdiv(pdx.kb_per, fair))), splits = rg_cdiv(pdx.kb_per, run);
     const size_t plen = (size_t)splits * c.R * c.D;
-    RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[4]));
+    RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[2]));
     const int dbrows = LT_BM / 32 * rg_cdiv(c.R, LT_BM);
     if (c.dbias) {
         const size_t blen = (size_t)dbrows * c.V;
-        RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[5]));
+        RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[3]));
     }
 
     CUtensorMap mz[4], mg[4];
-    lt_operand z = {o[3]->raw(), c.R, width, planes, width};
-    RG_TRY(lt_map(&mz[0], x, 128));
-    RG_TRY(lt_map(&mz[1], w, LT_BK));
+    lt_operand z = {o[1]->raw(), c.R, width, planes, width};
+    RG_TRY(lt_map(&mz[0], x.logits, 128));
+    RG_TRY(lt_map(&mz[1], w.logits, LT_BK));
     mz[2] = mz[0], mz[3] = mz[1];
     RG_TRY(lt_map(&mg[0], z, 128));
-    RG_TRY(lt_map(&mg[1], w, bn / 2));
+    RG_TRY(lt_map(&mg[1], w.grads, bn / 2));
     RG_TRY(lt_map(&mg[2], z, LT_BK));
-    RG_TRY(lt_map(&mg[3], x, LT_BK));
+    RG_TRY(lt_map(&mg[3], x.grads, LT_BK));
 
     for (int i = 0; i < pieces; i++) {
         lt_args e;
-        lt_common(ctx, c, o[2], &e);
+        lt_common(ctx, c, o[0], &e);
+        e.xscale = x.scale, e.wscale = w.scale;
         e.v0 = i * piece, e.vn = std::min(piece, c.V - e.v0);
-        e.dz = static_cast<__nv_bfloat16*>(o[3]->raw()), e.dz_pitch = width;
-        e.dbparts = c.dbias ? o[5]->data() : nullptr;
-        e.dxparts = o[4]->data(), e.dx_add = i > 0;
+        e.dz = static_cast<__nv_bfloat16*>(o[1]->raw()), e.dz_pitch = width;
+        e.dbparts = c.dbias ? o[3]->data() : nullptr;
+        e.dxparts = o[2]->data(), e.dx_add = i > 0;
         e.dw = c.dw, e.dw_bf16 = c.dtype == RG_DTYPE_BF16;
         e.nprobs = 1;
         e.p[0] = lt_problem(c.R, e.vn, c.D, bn, 0, 1);
@@ -828,7 +965,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.p[1] = lt_problem(e.vn, c.D, c.R, bn, 1, 1);
         RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
     }
-    lce_dx_finish_launch(ctx, o[4]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
-    if (c.dbias) lce_dbias_finish_launch(ctx, o[5]->data(), dbrows, c.V, c.scal, c.dbias);
+    lce_dx_finish_launch(ctx, o[2]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
+    if (c.dbias) lce_dbias_finish_launch(ctx, o[3]->data(), dbrows, c.V, c.scal, c.dbias);
     return RG_OK;
 }

@@ -444,3 +444,173 @@ def test_clip_grad_norm_extremes(backend):
     for m in (0.0, -1.0, float("nan")):
         with pytest.raises(rg.InvalidInput):
             be.clip_grad_norm([g], m)
+
+
+def test_linear_cross_entropy_scales_of_rows_and_columns(backend):
+    """f32 rows and columns of very different magnitudes, large channels, columns of zeros: the result depends on the products."""
+    be = backend
+    R, D, V = 150, 200, 300
+    x, w, b, t = ce_inputs(R, D, V, "f32", True, 0.1, 77)
+    x *= 1e-15 * 2.0 ** np.random.default_rng(1).integers(-6, 7, (R, 1))
+    x[:, 3] *= 1000
+    w *= 1e15 * 2.0 ** np.random.default_rng(2).integers(-6, 1, (1, V))
+    w[3] *= 1e-3
+    w[:, 17], x[5] = 0, 0
+    x, w = x.astype(np.float32), w.astype(np.float32)
+    w *= np.float32(20 / np.abs(x.astype(np.float64) @ w).max())
+    ex, live = ce_exact(x, w, b, t), t != IGNORE
+    tlse, tloss, tdx, tdw, tdb = ce_bounds(x, w, b, "f32", ex, live)
+    X, W, B, T = put(be, x), put(be, w), put(be, b), put(be, t)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    within(get(be, lse), ex["lse"], tlse, "lse")
+    within(get(be, loss), np.array([ex["loss"]]), tloss, "loss")
+    dx, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, put(be, ex["lse"].astype(np.float32)))
+    within(get(be, dx), ex["dx"], tdx + 1e-45, "dx")
+    within(get(be, dw), ex["dw"], tdw + 1e-45, "dw")
+    within(get(be, db), ex["db"], tdb, "dbias")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R", [5, 40])
+def test_linear_cross_entropy_masked_and_empty_rows(backend, R, dtype):
+    """Vocabulary entries masked by a bias of -inf or the lowest value, no row with a target, non-finite rows."""
+    be = backend
+    D, V = 48, 205
+    x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.0, 3)
+    b[10:40], b[100:204] = -np.inf, np.finfo(np.float32).min
+    t[:] = np.where((t >= 10) & (t < 40) | (t >= 100), 3, t)
+    with np.errstate(all="ignore"):
+        ex, live = ce_exact(x, w, b, t), t != IGNORE
+    z = ex["z"].copy()
+    keep = np.isfinite(b) & (b > -1e30)
+    sub = ce_exact(x, w[:, keep], b[keep], np.searchsorted(np.flatnonzero(keep), t).astype(np.float32))
+    tl, tloss, tdx, _, _ = ce_bounds(x, w[:, keep], b[keep], dtype, sub, live)
+    X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    within(get(be, lse), sub["lse"], tl, "lse")
+    within(get(be, loss), np.array([sub["loss"]]), tloss, "loss")
+    dx, dw, db = (get(be, s) for s in be.linear_cross_entropy_bwd(X, W, B, T, lse))
+    within(dx, sub["dx"], tdx + 2e-5 * np.abs(sub["dx"]).max(), "dx")   # lse of the forward pass instead of the exact one
+    assert not dw[:, 10:40].any() and not dw[:, 100:204].any() and not db[10:40].any() and np.isfinite(dw).all()
+    # no row has a target: loss 0, all gradients 0
+    T0 = put(be, np.full(R, IGNORE, np.float32))
+    loss, lse0 = be.linear_cross_entropy(X, W, B, T0)
+    assert be.to_vec(loss)[0] == 0 and np.array_equal(be.to_vec(lse0), be.to_vec(lse))
+    assert not any(be.to_vec(s).any() for s in be.linear_cross_entropy_bwd(X, W, B, T0, lse0))
+    # every entry masked: no distribution, the loss says so; the other rows of lse are untouched by a row of NaN
+    allm = put(be, np.full(V, -np.inf, np.float32))
+    loss, lsem = be.linear_cross_entropy(X, W, allm, T)
+    assert np.isnan(be.to_vec(loss)[0]) and np.all(be.to_vec(lsem) == -np.inf)
+    xn = x.copy()
+    xn[1, 7] = np.nan
+    tn = t.copy()
+    tn[1] = IGNORE
+    loss, lsen = be.linear_cross_entropy(put(be, xn, dtype), W, B, put(be, tn))
+    got = be.to_vec(lsen)
+    assert np.isnan(got[1]) and np.array_equal(np.delete(got, 1), np.delete(be.to_vec(lse), 1)) and np.isfinite(be.to_vec(loss)[0])
+    dxn, _, _ = be.linear_cross_entropy_bwd(put(be, xn, dtype), W, B, put(be, tn), lsen)
+    assert np.isfinite(np.delete(get(be, dxn), 1, 0)).all() and not get(be, dxn)[1].any()
+
+
+@pytest.mark.parametrize("R", [6, 70])
+def test_linear_cross_entropy_targets_and_refusals(backend, R):
+    be = backend
+    D, V = 24, 50
+    x, w, b, t = ce_inputs(R, D, V, "f32", True, 0.0, 8)
+    X, W, B, T = put(be, x), put(be, w), put(be, b), put(be, t)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    # an ignore_index that is a class, and ids that are not whole are truncated like other index inputs
+    t0 = t.copy()
+    t0[: R // 2] = 7
+    ex = ce_exact(x, w, b, t0, ignore=7)
+    assert abs(be.to_vec(be.linear_cross_entropy(X, W, B, put(be, t0), ignore_index=7)[0])[0] - ex["loss"]) < 1e-4
+    assert np.array_equal(be.to_vec(be.linear_cross_entropy(X, W, B, put(be, t + 0.5))[0]), be.to_vec(loss))
+    for bad in (-1.0, float(V), np.nan, np.inf, -np.inf, 1e30, -0.5):
+        tb = t.copy()
+        tb[R - 1] = bad
+        TB = put(be, tb)
+        with pytest.raises(rg.ShapeError):
+            be.linear_cross_entropy(X, W, B, TB)
+        with pytest.raises(rg.ShapeError):
+            be.linear_cross_entropy_bwd(X, W, B, TB, lse)
+    # the context works on
+    assert np.array_equal(be.to_vec(be.linear_cross_entropy(X, W, B, T)[0]), be.to_vec(loss))
+    # siblings agree: the loss over materialised logits
+    z = be.add(be.matmul(X, W), be.reshape(B, [1, V]))
+    assert abs(be.to_vec(be.sparse_cross_entropy(z, T))[0] - be.to_vec(loss)[0]) < 1e-4
+    H = be.cast(X, "bf16")
+    for call, err in ((lambda: be.linear_cross_entropy(H, W, B, T), rg.Unsupported),
+                      (lambda: be.linear_cross_entropy(X, W, be.cast(B, "bf16"), T), rg.Unsupported),
+                      (lambda: be.linear_cross_entropy(X, W, be.ones([V + 1]), T), rg.ShapeError),
+                      (lambda: be.linear_cross_entropy(X, W, B, be.zeros([R + 1])), rg.ShapeError),
+                      (lambda: be.linear_cross_entropy(X, be.zeros([D + 1, V]), B, T), rg.ShapeError),
+                      (lambda: be.linear_cross_entropy(X, be.zeros([D, 0]), None, T), rg.ShapeError),
+                      (lambda: be.linear_cross_entropy(be.zeros([2, 3, 4]), W, B, T), rg.DimensionError),
+                      (lambda: be.linear_cross_entropy_bwd(X, W, B, T, be.zeros([R + 1])), rg.ShapeError),
+                      (lambda: be.linear_cross_entropy_bwd(X, W, B, T, lse, be.zeros([2])), rg.ShapeError),
+                      (lambda: be.linear_cross_entropy_bwd(X, W, B, T, be.cast(lse, "bf16")), rg.Unsupported)):
+        with pytest.raises(err):
+            call()
+    loss0, lse0 = be.linear_cross_entropy(be.zeros([0, D]), W, B, be.zeros([0]))
+    assert be.to_vec(loss0)[0] == 0 and lse0.shape == [0]
+    dx, dw, db = be.linear_cross_entropy_bwd(be.zeros([0, D]), W, B, be.zeros([0]), lse0)
+    assert dx.shape == [0, D] and not be.to_vec(dw).any() and not be.to_vec(db).any()
+
+
+@pytest.mark.parametrize("R", [7, 33])
+def test_linear_cross_entropy_gradient_against_differences(backend, R):
+    be = backend
+    D, V = 20, 31
+    x, w, b, t = ce_inputs(R, D, V, "f32", True, 0.2, 21)
+    X, W, B, T = put(be, x), put(be, w), put(be, b), put(be, t)
+    _, lse = be.linear_cross_entropy(X, W, B, T)
+    dx, dw, db = (get(be, s) for s in be.linear_cross_entropy_bwd(X, W, B, T, lse))
+    rng = np.random.default_rng(2)
+    for _ in range(3):
+        vx, vw, vb = rng.standard_normal(x.shape), rng.standard_normal(w.shape), rng.standard_normal(b.shape)
+        e = 1e-5
+        num = (ce_exact(x + e * vx, w + e * vw, b + e * vb, t)["loss"] - ce_exact(x - e * vx, w - e * vw, b - e * vb, t)["loss"]) / (2 * e)
+        ana = (dx * vx).sum() + (dw * vw).sum() + (db * vb).sum()
+        # third derivatives O(1e2) e^2 = 1e-8, cancellation 2^-52 * 5 / e = 1e-10, f32 gradient relative 1e-5
+        assert abs(num - ana) <= 1e-4 * (1 + abs(num))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear_cross_entropy_over_pieces_of_the_vocabulary(backend, dtype):
+    """Enough rows that the gradient goes over the vocabulary in pieces (512 MiB of dz): rows of zeros keep the oracle small."""
+    be = backend
+    D, V = 8, 2100
+    R = 200000 if dtype == "bf16" else 70000
+    live = 600
+    x, w, b, t = ce_inputs(live, D, V, dtype, True, 0.1, 4)
+    xf, tf = np.zeros((R, D), np.float32), np.full(R, IGNORE, np.float32)
+    at = np.sort(np.random.default_rng(0).permutation(R)[:live])
+    xf[at], tf[at] = x, t
+    X, W, B, T = put(be, xf, dtype), put(be, w, dtype), put(be, b), put(be, tf)
+    ex = ce_exact(x, w, b, t)
+    tlse, tloss, tdx, tdw, tdb = ce_bounds(x, w, b, dtype, ex, t != IGNORE)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    within(get(be, lse)[at], ex["lse"], tlse, "lse")
+    within(get(be, loss), np.array([ex["loss"]]), tloss, "loss")
+    dx, dw, db = (get(be, s) for s in be.linear_cross_entropy_bwd(X, W, B, T, lse))
+    slack = 1e-5          # lse of the forward pass instead of the exact one: |p| (tlse) <= 1e-5 of each term
+    within(dx[at], ex["dx"], tdx + slack * ex["scale"] * (ex["p"] @ np.abs(w.astype(np.float64)).T), "dx")
+    within(dw, ex["dw"], tdw + slack * ex["scale"] * (np.abs(x.astype(np.float64)).T @ ex["p"]), "dw")
+    # 200000 rows: their dz is 0, the chains of the column sums are longer than the live rows' only by exact additions of 0
+    within(db, ex["db"], tdb + slack * ex["scale"] * ex["p"].sum(0), "dbias")
+    gone = np.ones(R, bool)
+    gone[at] = False
+    assert not dx[gone].any()
+
+
+def test_linear_cross_entropy_gives_the_same_bits_again(backend):
+    be = backend
+    for R in (9, 500):
+        x, w, b, t = ce_inputs(R, 100, 3001, "f32", True, 0.1)
+        X, W, B, T = put(be, x), put(be, w), put(be, b), put(be, t)
+        loss, lse = be.linear_cross_entropy(X, W, B, T)
+        first = [be.to_vec(s) for s in (loss, lse, *be.linear_cross_entropy_bwd(X, W, B, T, lse))]
+        for _ in range(3):
+            loss, lse2 = be.linear_cross_entropy(X, W, B, T)
+            again = [be.to_vec(s) for s in (loss, lse2, *be.linear_cross_entropy_bwd(X, W, B, T, lse))]
+            assert all(np.array_equal(p, q) for p, q in zip(first, again))
