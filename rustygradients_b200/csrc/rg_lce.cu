@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(1024) lce_check_kernel(const float* __restrict
         scal[1] = live_s ? (dloss ? dloss[0] : 1.f) / (float)live_s : 0.f;
         status[0] = bad_s;
         status[1] = 0;  // ticket of lce_loss_kernel
+        status[2] = 0;  // largest magnitude of w
     }
 }
 
@@ -404,11 +405,12 @@ static rg_status lce_args(const char* op, rg_ctx* ctx, const rg_storage* x, cons
 // Enqueues the check of the targets; lce_checked waits for it (not for what was enqueued after it).
 static rg_status lce_check_launch(rg_ctx* ctx, lce_call& c, const rg_storage* targets, long long ignore, const rg_storage* dloss,
                                   rg_storage** scratch) {
-    // tgt [R] | tz [R] | scal, status [4]
-    const size_t words = 2 * (size_t)c.R + 4;
+    // tgt [R] | tz [R] | scal [2] | status [3]
+    const size_t words = 2 * (size_t)c.R + 5;
     RG_TRY(rg_alloc_storage(ctx, &words, 1, scratch));
     float* base = (*scratch)->data();
     c.tgt = reinterpret_cast<int*>(base), c.tz = base + c.R, c.scal = base + 2 * (size_t)c.R;
+    c.wmax = reinterpret_cast<unsigned*>(base + 2 * (size_t)c.R + 4);
     lce_check_kernel<<<1, 1024, 0, ctx->stream>>>(targets->data(), c.R, c.V, ignore, dloss ? dloss->data() : nullptr,
                                                   const_cast<int*>(c.tgt), c.tz, const_cast<float*>(c.scal),
                                                   reinterpret_cast<int*>(const_cast<float*>(c.scal)) + 2);

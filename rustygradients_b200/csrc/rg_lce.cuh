@@ -12,6 +12,7 @@ struct lce_call {
     const int* tgt;        // R: target column, -1 for a row that is left out
     const float* lse;      // backward: R
     const float* scal;     // device: [0] rows with a target, [1] dloss / rows (0 when there is none)
+    unsigned* wmax;        // a word that is 0
     float2* parts;         // forward: (maximum, sum of exponentials) of row r over slice p at [p * R + r]
     float* tz;             // forward: logit of the target
     int nparts;

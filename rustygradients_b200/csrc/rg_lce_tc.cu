@@ -12,9 +12,10 @@
 //
 // bf16 inputs are one plane and are multiplied as they are.  f32 inputs are split into planes of 16 bits whose products are
 // accumulated in f32:
-//  * logits: two f16 planes, x = 2^-a (x0 + x1) with one power of two per row of x (column of w) that brings the largest
-//    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits and everything down to 2^-40 of that largest magnitude; three of the four
-//    products are taken, the fourth is below 2^-22 of the magnitudes.  The scales leave in the epilogue.
+//  * logits: two f16 planes, x = 2^-a (x0 + x1) with a power of two per row of x and one for w that bring the largest
+//    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits and everything down to 2^-40 of that largest magnitude (a logit is off by
+//    2^-40 of the largest product of magnitudes, and only its absolute error counts in a softmax); three of the four products
+//    are taken, the fourth is below 2^-22 of the magnitudes.  The scales leave in the epilogue.
 //  * dx, dw: the sums run over the vocabulary and over the rows, where dz spans many orders of magnitude (a rare word's
 //    gradient is a sum of tiny ones), so f16's range is not enough: three bf16 planes hold all 24 bits (each the leading 8 bits
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
@@ -68,7 +69,7 @@ struct lt_args {
     int R, D, V;
     int v0, vn;    // piece of the vocabulary: first column, number of columns
     const float* bias;
-    const float *xscale, *wscale;  // PLANES 2: what a row (a column) of the accumulated logits is multiplied with
+    const float *xscale, *wscale;  // PLANES 2: the scale of each row of x and of w, to be taken out of the logits
     const int* tgt;
     float2* parts;            // LT_FWD
     float* tz;
@@ -243,19 +244,9 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
     if (EPI == LT_FWD || EPI == LT_DZ) {
         const int c = e.v0 + col, left = e.v0 + e.vn - c;  // vocabulary column of v[0]; columns inside the piece
         if (left <= 0 && EPI == LT_FWD) return;
-        if (PLANES == 2) {  // exact powers of two
-            if (left >= 32) {
-                const float4* b = reinterpret_cast<const float4*>(e.wscale + c);
+        if (PLANES == 2) {  // an exact power of two
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float4 q = __ldg(b + j);
-                    v[4 * j] *= q.x * w.scale, v[4 * j + 1] *= q.y * w.scale, v[4 * j + 2] *= q.z * w.scale, v[4 * j + 3] *= q.w * w.scale;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; j++)
-                    if (j < left) v[j] *= e.wscale[c + j] * w.scale;
-            }
+            for (int j = 0; j < 32; j++) v[j] *= w.scale;
         }
         if (e.bias) {
             if (left >= 32) {
@@ -584,7 +575,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.ms = {-INFINITY, 0.f};
             w.tgt = (EPI != LT_GRAD && w.live) ? e.tgt[w.row] : -1;
             w.lse = (EPI == LT_DZ && w.live) ? e.lse[w.row] : 0.f;
-            w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] : 0.f;
+            w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] * e.wscale[0] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
             const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
@@ -687,8 +678,7 @@ __device__ __forceinline__ void lt_split2(float v, float scale, uint32_t& h0, ui
     h0 = __half_as_ushort(a), h1 = __half_as_ushort(b);
 }
 
-// f32 values as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row (x), and triples of bf16 (NULL: not
-// wanted).  A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
+// x as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row, and triples of bf16 (NULL: not wanted).  A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
 __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                            uint16_t* __restrict__ pair, uint16_t* __restrict__ triple,
                                                            float* __restrict__ scale_out) {
@@ -714,45 +704,61 @@ __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restri
     }
 }
 
-// The same with a scale per column (w).  A CTA owns 64 columns: its 16 warps read all rows for the largest magnitudes, then
-// once more (64 columns of two CTAs per SM stay in L2) to write them; a lane holds two neighbouring columns, so that a warp
-// stores 128 contiguous bytes of each plane.  Memory bound: 4 bytes in, 4 (10 with the triples) out per value.
-__global__ void __launch_bounds__(512) lt_pack_cols_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
-                                                           uint32_t* __restrict__ pair, uint32_t* __restrict__ triple,
-                                                           float* __restrict__ scale_out) {
-    extern __shared__ float lt_red[];  // [16][64]; the launch asks for more to keep the number of resident CTAs at two
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int c = blockIdx.x * 64 + 2 * lane;
-    const bool in0 = c < cols, in1 = c + 1 < cols;
-    float m0 = 0.f, m1 = 0.f;
-#pragma unroll 8
-    for (int r = w; r < rows; r += 16) {
-        const float* p = src + (size_t)r * cols + c;
-        m0 = fmaxf(m0, in0 ? lt_finite_abs(p[0]) : 0.f);
-        m1 = fmaxf(m1, in1 ? lt_finite_abs(p[1]) : 0.f);
-    }
-    lt_red[w * 64 + 2 * lane] = m0, lt_red[w * 64 + 2 * lane + 1] = m1;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; k++) m0 = fmaxf(m0, lt_red[k * 64 + 2 * lane]), m1 = fmaxf(m1, lt_red[k * 64 + 2 * lane + 1]);
-    const float2 s0 = lt_scale(m0), s1 = lt_scale(m1);
-    if (w == 0 && in0) scale_out[c] = s0.y;
-    if (w == 0 && in1) scale_out[c + 1] = s1.y;
-    if (c >= pitch) return;
-    const size_t plane = (size_t)rows * pitch / 2;  // pitch is even
+// Largest finite magnitude of w (as bits: they order like the values), into a word that lce_check_kernel has set to 0.
+__global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ src, size_t n, unsigned* __restrict__ out) {
+    const size_t stride = (size_t)gridDim.x * 256;
+    const float4* v4 = reinterpret_cast<const float4*>(src);
+    float m = 0.f;
 #pragma unroll 4
-    for (int r = w; r < rows; r += 16) {
-        const float* p = src + (size_t)r * cols + c;
-        const float a = in0 ? p[0] : 0.f, b = in1 ? p[1] : 0.f;
-        const size_t at = ((size_t)r * pitch + c) / 2;
-        uint32_t a0, a1, a2, b0, b1, b2;
-        lt_split2(a, s0.x, a0, a1);
-        lt_split2(b, s1.x, b0, b1);
-        pair[at] = a0 | (b0 << 16), pair[at + plane] = a1 | (b1 << 16);
-        if (triple) {
-            lt_split3(a, a0, a1, a2);
-            lt_split3(b, b0, b1, b2);
-            triple[at] = a0 | (b0 << 16), triple[at + plane] = a1 | (b1 << 16), triple[at + 2 * plane] = a2 | (b2 << 16);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n / 4; i += stride) {
+        const float4 q = v4[i];
+        m = fmaxf(m, fmaxf(fmaxf(lt_finite_abs(q.x), lt_finite_abs(q.y)), fmaxf(lt_finite_abs(q.z), lt_finite_abs(q.w))));
+    }
+    if (blockIdx.x == 0 && threadIdx.x < n % 4) m = fmaxf(m, lt_finite_abs(src[n - 1 - threadIdx.x]));
+    m = rg_warp_max(m);
+    if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));  // a maximum: the order does not matter
+}
+
+// w as pairs of f16 with one scale for the whole matrix, and (NULL: not wanted) triples of bf16.  A thread takes 8
+// neighbouring values of a row and writes 16 bytes of each plane.  The values are walked from the end: what the last-level
+// cache still holds of lt_max_kernel's pass is read from there.  Memory bound: 4 bytes in, 4 (10 with the triples) out.
+template <bool TRIPLE>
+__global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
+                                                      const unsigned* __restrict__ largest, uint16_t* __restrict__ pair,
+                                                      uint16_t* __restrict__ triple, float* __restrict__ scale_out) {
+    const float2 sc = lt_scale(__uint_as_float(*largest));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *scale_out = sc.y;
+    const int groups = pitch / 8;
+    const long long n = (long long)rows * groups, stride = (long long)gridDim.x * 256;
+    const size_t plane = (size_t)rows * pitch;
+    for (long long i = n - 1 - ((long long)blockIdx.x * 256 + threadIdx.x); i >= 0; i -= stride) {
+        const long long r = i / groups;
+        const int c = (int)(i - r * groups) * 8;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = c + k < cols ? src[r * cols + c + k] : 0.f;
+        const size_t at = (size_t)r * pitch + c;
+        uint32_t h0[4], h1[4], h2[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint32_t a0, a1, b0, b1;
+            lt_split2(v[2 * k], sc.x, a0, a1);
+            lt_split2(v[2 * k + 1], sc.x, b0, b1);
+            h0[k] = a0 | (b0 << 16), h1[k] = a1 | (b1 << 16);
+        }
+        *reinterpret_cast<uint4*>(pair + at) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
+        *reinterpret_cast<uint4*>(pair + plane + at) = make_uint4(h1[0], h1[1], h1[2], h1[3]);
+        if (TRIPLE) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                uint32_t a0, a1, a2, b0, b1, b2;
+                lt_split3(v[2 * k], a0, a1, a2);
+                lt_split3(v[2 * k + 1], b0, b1, b2);
+                h0[k] = a0 | (b0 << 16), h1[k] = a1 | (b1 << 16), h2[k] = a2 | (b2 << 16);
+            }
+            *reinterpret_cast<uint4*>(triple + at) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
+            *reinterpret_cast<uint4*>(triple + plane + at) = make_uint4(h1[0], h1[1], h1[2], h1[3]);
+            *reinterpret_cast<uint4*>(triple + 2 * plane + at) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
         }
     }
 }
@@ -803,14 +809,15 @@ struct lt_packed {
     const float* scale;
     rg_outputs<3> mem;
 };
-static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, bool by_column, bool want_grads, lt_packed* o) {
+// `largest` (w): a word that is 0, for one scale over the matrix; NULL (x): a scale per row.
+static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, unsigned* largest, bool want_grads, lt_packed* o) {
     o->scale = nullptr;
     if (dtype == RG_DTYPE_BF16 && cols % 8 == 0) {
         o->logits = o->grads = {src, rows, cols, 1, cols};
         return RG_OK;
     }
     const int pitch = (cols + 7) / 8 * 8;
-    const size_t plane = (size_t)rows * pitch, pair = 2 * plane, triple = 3 * plane, scales = by_column ? cols : rows;
+    const size_t plane = (size_t)rows * pitch, pair = 2 * plane, triple = 3 * plane, scales = largest ? 1 : rows;
     if (dtype == RG_DTYPE_BF16) {
         RG_TRY(rg_alloc_storage(ctx, &plane, 1, &o->mem[0], RG_DTYPE_BF16));
         const int grid = (int)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
@@ -825,12 +832,19 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
     if (want_grads) RG_TRY(rg_alloc_storage(ctx, &triple, 1, &o->mem[2], RG_DTYPE_BF16));
     void* three = want_grads ? o->mem[2]->raw() : nullptr;
     o->scale = o->mem[1]->data();
-    if (by_column) {
-        const int smem = 80 * 1024;
-        RG_CUDA(cudaFuncSetAttribute(lt_pack_cols_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        lt_pack_cols_kernel<<<rg_cdiv(cols, 64), 512, smem, ctx->stream>>>(static_cast<const float*>(src), rows, cols, pitch,
-                                                                          static_cast<uint32_t*>(o->mem[0]->raw()),
-                                                                          static_cast<uint32_t*>(three), o->mem[1]->data());
+    if (largest) {
+        const float* w = static_cast<const float*>(src);
+        const size_t n = (size_t)rows * cols;
+        const int most = ctx->sm_count * 16;
+        lt_max_kernel<<<(unsigned)std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, ctx->sm_count * 8)), 256, 0, ctx->stream>>>(w, n, largest);
+        const unsigned grid = (unsigned)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, most);
+        if (want_grads)
+            lt_pack_kernel<true><<<grid, 256, 0, ctx->stream>>>(w, rows, cols, pitch, largest, static_cast<uint16_t*>(o->mem[0]->raw()),
+                                                                static_cast<uint16_t*>(three), o->mem[1]->data());
+        else
+            lt_pack_kernel<false><<<grid, 256, 0, ctx->stream>>>(w, rows, cols, pitch, largest, static_cast<uint16_t*>(o->mem[0]->raw()),
+                                                                 nullptr, o->mem[1]->data());
+        RG_LAUNCHED(ctx);
     } else {
         lt_pack_rows_kernel<<<rg_cdiv(rows, 8), 256, 0, ctx->stream>>>(static_cast<const float*>(src), rows, cols, pitch,
                                                                       static_cast<uint16_t*>(o->mem[0]->raw()),
@@ -887,8 +901,8 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     lt_packed x, w;
     const size_t one = 1;
     RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, false, false, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, true, false, &w));
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, false, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, false, &w));
     CUtensorMap maps[4];
     RG_TRY(lt_map(&maps[0], x.logits, 128));
     RG_TRY(lt_map(&maps[1], w.logits, LT_BK));
@@ -911,8 +925,8 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     const size_t one = 1;
     const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = lt_bn(c.dtype);
     RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, false, true, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, true, true, &w));
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, &w));
 
     const long long most = std::max<long long>(1, (long long)(LT_DZ_BYTES / ((size_t)planes * 2 * c.R)) / 256) * 256;
     const int pieces = (int)((c.V + most - 1) / most);
