@@ -445,7 +445,7 @@ extern "C" rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, c
     }
     RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, nullptr, &o[2]));
     const bool few = c.R <= LCE_FEW_ROWS;
-    c.nparts = few ? rg_cdiv(c.V, 128) : lce_tc_nparts(c.V, c.dtype);
+    c.nparts = few ? rg_cdiv(c.V, 128) : lce_tc_nparts(c.V);
     const size_t pwords = 2 * (size_t)c.nparts * rows, blocks = (size_t)rg_cdiv(c.R, 8), swords = 2 * blocks;
     RG_TRY(rg_alloc_storage(ctx, &pwords, 1, &o[3]));
     RG_TRY(rg_alloc_storage(ctx, &swords, 1, &o[4]));

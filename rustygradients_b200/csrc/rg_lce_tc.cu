@@ -21,8 +21,9 @@
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
 // The tensor core truncates when it adds to its f32 accumulator, so a long chain loses about 2^-25 of the running sum per
 // step (measured: a relative error of 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32 inputs the chain is
-// therefore cut every 256 elements of K: the product of the first planes and the small ones have an accumulator each, and
-// the epilogue warps add both to f32 registers with rounding.
+// therefore cut after every k-block of 64: its small products come first and that of the leading planes last, and the
+// epilogue warps add the block to their f32 registers with rounding (64 or 128 additions a thread in the 1536 cycles that a
+// block's products take).
 #include "rg_lce.cuh"
 
 #include <cuda.h>
@@ -32,12 +33,10 @@
 
 #define LT_BM 256  // rows of a tile: 128 in each CTA of a pair
 #define LT_BK 64
-#define LT_THREADS 320  // TMA warp, MMA warp, 8 epilogue warps
 #define LT_SPIN_LIMIT (1u << 22)
 #define LT_STAGE_ALL 196608   // bytes of the operand ring
 #define LT_MAX_STAGES 6
 #define LT_SMEM_BYTES (LT_STAGE_ALL + 8 * 32 * 33 * 4 + 1024 + 256)
-#define LT_SEG 4              // k-blocks per accumulator chain for f32 inputs
 
 // Two CTAs (two SMs) work on one tile of 256 x BN: each holds 128 rows of A, half of the columns of B, and the accumulator
 // of its 128 rows.  A k-block then costs an SM 128 x 64 + BN/2 x 64 values from L2 instead of 128 x 64 + BN x 64, which
@@ -45,10 +44,16 @@
 // PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.
 template <int PLANES>
 struct lt_shape {
-    static constexpr int BN = PLANES == 1 ? 256 : 128;
+    static constexpr int BN = PLANES == 3 ? 128 : 256;
     static constexpr int A_BYTES = 128 * LT_BK * 2, B_BYTES = BN / 2 * LT_BK * 2;  // of one CTA
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
-    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6, 4 or 2
+    static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6, 3 or 2
+    static constexpr int BUFFERS = 512 / BN;  // accumulators in tensor memory
+    // Warp 0 copies, warp 1 multiplies, FIRST.. the eight epilogue warps.  Pairs: a thread holds 128 columns in registers,
+    // more than 12 warps get at launch, so registers move between whole groups of four warps: 384 threads x 168 at launch
+    // = 128 x (56 + 224 + 224).
+    static constexpr bool MOVE_REGS = PLANES == 2;
+    static constexpr int FIRST = MOVE_REGS ? 4 : 2, THREADS = 32 * (FIRST + 8);
 };
 
 // One contraction of a launch: C[M,N] = sum over K of A[m,k] B[n,k]
@@ -379,7 +384,7 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
 }
 
 template <int PLANES, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LT_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lt_shape<PLANES>::THREADS, 1)
 lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmA1,
               const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ lt_args e) {
     typedef lt_shape<PLANES> S;
@@ -388,9 +393,9 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     float* stage_all = reinterpret_cast<float*>(ring + LT_STAGE_ALL);
     uint64_t* full = reinterpret_cast<uint64_t*>(stage_all + 8 * 32 * 33);  // used in CTA 0
     uint64_t* empty = full + LT_MAX_STAGES;
-    uint64_t* acc_full = empty + LT_MAX_STAGES;  // [2]
-    uint64_t* acc_empty = acc_full + 2;          // [2], used in CTA 0
-    uint64_t* sched_full = acc_empty + 2;        // [2]
+    uint64_t* acc_full = empty + LT_MAX_STAGES;  // [4]
+    uint64_t* acc_empty = acc_full + 4;          // [4], used in CTA 0
+    uint64_t* sched_full = acc_empty + 4;        // [2]
     uint64_t* sched_empty = sched_full + 2;      // [2], used in CTA 0
     uint64_t* drain = sched_empty + 2;
     volatile int* sched_tile = reinterpret_cast<volatile int*>(drain + 1);  // [2]
@@ -404,8 +409,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < LT_MAX_STAGES; s++) lt_bar_init(&full[s], 1), lt_bar_init(&empty[s], 1);
+        for (int b = 0; b < S::BUFFERS; b++) lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 16);
         for (int b = 0; b < 2; b++) {
-            lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 16);
             lt_bar_init(&sched_full[b], 1), lt_bar_init(&sched_empty[b], 18);  // MMA thread and epilogue warps; copy thread and epilogue warps
         }
         lt_bar_init(drain, 1);
@@ -422,6 +427,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
+    if (warp < S::FIRST) {
+    if (S::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
         // ===== one thread of each CTA brings its operands; that of CTA 0 also hands out the tiles to both =====
         if (lane == 0) {
@@ -509,34 +516,29 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t idesc = (1u << 4) | (PLANES == 2 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
                                        ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
-                const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
+                // bf16: one accumulator for all of K; f32: one per k-block
+                const int segs = PLANES == 1 ? 1 : nkb;
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
-                    const uint32_t buf = seg & 1u;
-                    ok = lt_wait(&acc_empty[buf], ((seg >> 1) & 1u) ^ 1u, e.err);
+                    const uint32_t buf = seg % S::BUFFERS;
+                    ok = lt_wait(&acc_empty[buf], ((seg / S::BUFFERS) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d0 = tmem + buf * 256, d1 = d0 + 128;
-                    const int kn = PLANES == 1 ? nkb : min(LT_SEG, nkb - sg * LT_SEG);
-                    for (int kb = 0; kb < kn; kb++, it++) {
+                    const uint32_t d = tmem + buf * S::BN;
+                    for (int kb = 0; kb < (PLANES == 1 ? nkb : 1); kb++, it++) {
                         const int s = it % S::STAGES;
                         ok = lt_wait(&full[s], (it / S::STAGES) & 1u, e.err);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t a = lt_smem(ring + s * S::STAGE_BYTES), b = a + PLANES * S::A_BYTES;
-                        if (PLANES == 1) {
+                        // pairs of planes, the smallest products first
+                        constexpr int PRODUCTS = PLANES == 1 ? 1 : PLANES == 2 ? 3 : 6;
+                        constexpr int pa[3][6] = {{0}, {0, 1, 0}, {0, 2, 1, 0, 1, 0}}, pb[3][6] = {{0}, {1, 0, 0}, {2, 0, 1, 1, 0, 0}};
+#pragma unroll
+                        for (int pr = 0; pr < PRODUCTS; pr++)
 #pragma unroll
                             for (int k = 0; k < LT_BK / 16; k++)
-                                lt_mma(d0, lt_desc(a + k * astep, p.a_mn), lt_desc(b + k * bstep, p.b_mn), idesc, kb > 0 || k > 0);
-                        } else {
-#pragma unroll
-                            for (int pr = 0; pr < (PLANES == 2 ? 3 : 6); pr++) {
-                                constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
-#pragma unroll
-                                for (int k = 0; k < LT_BK / 16; k++)
-                                    lt_mma(pr == 0 ? d0 : d1, lt_desc(a + pa[pr] * S::A_BYTES + k * astep, p.a_mn),
-                                           lt_desc(b + pb[pr] * S::B_BYTES + k * bstep, p.b_mn), idesc, kb > 0 || k > 0 || pr > 1);
-                            }
-                        }
+                                lt_mma(d, lt_desc(a + pa[PLANES - 1][pr] * S::A_BYTES + k * astep, p.a_mn),
+                                       lt_desc(b + pb[PLANES - 1][pr] * S::B_BYTES + k * bstep, p.b_mn), idesc, kb > 0 || pr > 0 || k > 0);
                         lt_commit(&empty[s]);
                     }
                     if (ok) lt_commit(&acc_full[buf]);
@@ -548,11 +550,13 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 lt_wait(drain, 0, e.err);
             }
         }
+    }
     } else {
-        // ===== epilogue warps: TMEM lane quarter = warp % 4, warps 2..5 the left half of the columns, 6..9 the right =====
+        if (S::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ===== epilogue warps: TMEM lane quarter = warp % 4, four for the left half of the columns, four for the right =====
         constexpr int HALF = S::BN / 2;
-        const int q = warp & 3, half = warp < 6 ? 0 : 1;
-        float* stage = stage_all + (warp - 2) * 32 * 33;
+        const int q = warp & 3, half = warp < S::FIRST + 4 ? 0 : 1;
+        float* stage = stage_all + (warp - S::FIRST) * 32 * 33;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + half * HALF;
         uint32_t ti = 0, seg = 0;
         bool ok = true;
@@ -578,23 +582,22 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] * e.wscale[0] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
-            const int segs = PLANES == 1 ? 1 : (nkb + LT_SEG - 1) / LT_SEG;
-            float acc[2][32];
-            static_assert(PLANES == 1 || HALF == 64, "two groups of 32 columns a thread");
+            const int segs = PLANES == 1 ? 1 : nkb;
+            float acc[PLANES == 1 ? 2 : HALF / 32][32];
             for (int sg = 0; sg < segs; sg++, seg++) {
-                const uint32_t buf = seg & 1u;
-                ok = lt_wait(&acc_full[buf], (seg >> 1) & 1u, e.err);
+                const uint32_t buf = seg % S::BUFFERS;
+                ok = lt_wait(&acc_full[buf], (seg / S::BUFFERS) & 1u, e.err);
                 if (!ok) break;
                 __syncwarp();  // the loads below are executed by whole warps
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t ta = taddr + buf * 256;
+                const uint32_t ta = taddr + buf * S::BN;
                 if (PLANES == 1) {
                     // the next 32 columns are on their way while these are worked on
                     lt_ld32(ta, acc[0]);
 #pragma unroll 1
                     for (int c = 0; c < HALF / 32; c += 2) {
                         lt_ld_wait();
-                        lt_ld32(ta + (c + 1) * 32, acc[PLANES == 1 ? 1 : 0]);
+                        lt_ld32(ta + (c + 1) * 32, acc[1]);
                         lt_columns<PLANES, EPI>(e, t, w, acc[0], c0 + c * 32, stage);
                         lt_ld_wait();
                         if (c + 2 < HALF / 32) {
@@ -604,17 +607,19 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                             __syncwarp();
                             if (lane == 0) lt_arrive_at(lt_leader(&acc_empty[buf]));
                         }
-                        lt_columns<PLANES, EPI>(e, t, w, acc[PLANES == 1 ? 1 : 0], c0 + (c + 1) * 32, stage);
+                        lt_columns<PLANES, EPI>(e, t, w, acc[1], c0 + (c + 1) * 32, stage);
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < HALF / 32; c++) {
-                        float big[32], small[32];
-                        lt_ld32(ta + c * 32, big);
-                        lt_ld32(ta + 128 + c * 32, small);
+                    for (int c = 0; c < HALF / 32; c += 2) {
+                        float block[2][32];
+                        lt_ld32(ta + c * 32, block[0]);
+                        lt_ld32(ta + c * 32 + 32, block[1]);
                         lt_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; j++) acc[c][j] = (sg ? acc[c][j] : 0.f) + (big[j] + small[j]);
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int j = 0; j < 32; j++) acc[c + h][j] = sg ? acc[c + h][j] + block[h][j] : block[h][j];
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
@@ -857,9 +862,9 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
     return RG_OK;
 }
 
-static int lt_bn(int dtype) { return dtype == RG_DTYPE_F32 ? lt_shape<2>::BN : lt_shape<1>::BN; }
-static_assert(lt_shape<2>::BN == lt_shape<3>::BN, "f32 inputs: one width of column tiles");
-int lce_tc_nparts(int V, int dtype) { return 2 * rg_cdiv(V, lt_bn(dtype)); }
+static_assert(lt_shape<1>::BN == lt_shape<2>::BN, "the logits have one width of column tiles");
+#define LT_BN lt_shape<1>::BN
+int lce_tc_nparts(int V) { return 2 * rg_cdiv(V, LT_BN); }
 
 static lt_prob lt_problem(int M, int N, int K, int bn, int a_mn, int b_mn) {
     lt_prob p;
@@ -878,7 +883,7 @@ static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
     if (total > 0x3fffffff) return rg_fail(RG_ERR_SHAPE, "linear_cross_entropy: too many tiles");
     RG_CUDA(cudaMemsetAsync(e.counter, 0, sizeof(int), ctx->stream));
     const int grid = 2 * (int)std::min<long long>(total, ctx->sm_count / 2);
-    lce_tc_kernel<PLANES, EPI><<<grid, LT_THREADS, LT_SMEM_BYTES, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], e);
+    lce_tc_kernel<PLANES, EPI><<<grid, lt_shape<PLANES>::THREADS, LT_SMEM_BYTES, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], e);
     RG_CUDA(cudaGetLastError());
     RG_LAUNCHED(ctx);
     return RG_OK;
@@ -911,7 +916,7 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     lt_common(ctx, c, o[0], &e);
     e.xscale = x.scale, e.wscale = w.scale;
     e.nprobs = 1;
-    e.p[0] = lt_problem(c.R, c.V, c.D, lt_bn(c.dtype), 0, 1);
+    e.p[0] = lt_problem(c.R, c.V, c.D, LT_BN, 0, 1);
     return lt_run<LT_FWD>(ctx, c, maps, e);
 }
 
@@ -923,7 +928,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     rg_outputs<4> o;  // counter, dz, partial dx, partial dbias
     lt_packed x, w;
     const size_t one = 1;
-    const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = lt_bn(c.dtype);
+    const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = planes == 3 ? lt_shape<3>::BN : lt_shape<1>::BN;  // of the gradients
     RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
     RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, &x));
     RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, &w));
@@ -938,7 +943,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
     lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
     const long long load = (long long)pdx.tiles_m * pdx.tiles_n * pdx.kb_per + (long long)pdw.tiles_m * pdw.tiles_n * pdw.kb_per;
-    const int fair = (int)std::max<long long>(LT_SEG, load / (ctx->sm_count / 2) / 2);
+    const int fair = (int)std::max<long long>(4, load / (ctx->sm_count / 2) / 2);
     // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
     const int run = rg_cdiv(pdx.kb_per, std::min(16, rg_cdiv(pdx.kb_per, fair))), splits = rg_cdiv(pdx.kb_per, run);
     const size_t plen = (size_t)splits * c.R * c.D;
@@ -969,7 +974,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.dxparts = o[2]->data(), e.dx_add = i > 0;
         e.dw = c.dw, e.dw_bf16 = c.dtype == RG_DTYPE_BF16;
         e.nprobs = 1;
-        e.p[0] = lt_problem(c.R, e.vn, c.D, bn, 0, 1);
+        e.p[0] = lt_problem(c.R, e.vn, c.D, LT_BN, 0, 1);
         e.p[0].b_n0 = e.v0;
         RG_TRY(lt_run<LT_DZ>(ctx, c, mz, e));
         e.nprobs = 2;
