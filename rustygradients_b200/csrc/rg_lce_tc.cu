@@ -299,33 +299,43 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                 for (int j = 0; j < 32; j++)
                     if (w.tgt == c + j) v[j] -= 1.f;
             }
-            if (w.live && col < e.dz_pitch) {
-                __nv_bfloat16* o = e.dz + (long long)w.row * e.dz_pitch + col;
-                const long long plane = (long long)e.R * e.dz_pitch;
+            if (col < e.dz_pitch) {
+                // A thread holds 64 bytes of a row of each plane.  Stored from here, a warp's instruction would touch 32 lines
+                // with 16 bytes each; through shared memory four lanes store the 64 bytes of a row together.
+                constexpr int ZP = PLANES == 1 ? 1 : 3;
+                unsigned char* rows_s = reinterpret_cast<unsigned char*>(stage);  // 32 rows of 64 bytes, 80 apart
+                const int row0 = w.row - lane, rows = e.R - row0;
+                float rest[32];
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    constexpr int ZP = PLANES == 1 ? 1 : 3;
-                    uint32_t h[3][4];
+                for (int j = 0; j < 32; j++) rest[j] = v[j];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (PLANES == 1) {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * k], v[j + 2 * k + 1]);
-                            h[0][k] = *reinterpret_cast<const uint32_t*>(&b);
-                        } else {
-                            // finite but for what was not finite before; each plane truncates, what is left is exact
-                            const float a = v[j + 2 * k], b = v[j + 2 * k + 1];
-                            const float a1 = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-                            const float b1 = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-                            const float a2 = a1 - __uint_as_float(__float_as_uint(a1) & 0xffff0000u);
-                            const float b2 = b1 - __uint_as_float(__float_as_uint(b1) & 0xffff0000u);
-                            h[0][k] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-                            h[1][k] = __byte_perm(__float_as_uint(a1), __float_as_uint(b1), 0x7632);
-                            h[2][k] = __byte_perm(__float_as_uint(a2), __float_as_uint(b2), 0x7632);
+                for (int p = 0; p < ZP; p++) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float a = rest[j + 2 * k], b = rest[j + 2 * k + 1];
+                            if (PLANES == 1) {
+                                const __nv_bfloat162 q = __floats2bfloat162_rn(a, b);
+                                h[k] = *reinterpret_cast<const uint32_t*>(&q);
+                            } else {  // the leading 16 bits; what they leave is exact and goes to the next plane
+                                h[k] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+                                rest[j + 2 * k] = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                                rest[j + 2 * k + 1] = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+                            }
                         }
+                        *reinterpret_cast<uint4*>(rows_s + lane * 80 + j * 2) = make_uint4(h[0], h[1], h[2], h[3]);
                     }
+                    __syncwarp();
+                    __nv_bfloat16* o = e.dz + ((long long)p * e.R + row0) * e.dz_pitch + col + (lane & 3) * 8;
 #pragma unroll
-                    for (int p = 0; p < ZP; p++)
-                        *reinterpret_cast<uint4*>(o + p * plane + j) = make_uint4(h[p][0], h[p][1], h[p][2], h[p][3]);
+                    for (int i = 0; i < 4; i++) {
+                        const int r = i * 8 + (lane >> 2);
+                        if (r < rows)
+                            *reinterpret_cast<uint4*>(o + r * e.dz_pitch) = *reinterpret_cast<const uint4*>(rows_s + r * 80 + (lane & 3) * 16);
+                    }
+                    __syncwarp();
                 }
             }
             if (e.dbparts) {
