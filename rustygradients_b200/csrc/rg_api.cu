@@ -102,10 +102,12 @@ static rg_status ctx_create(int device, bool own_stream, cudaStream_t stream, rg
     if (e == cudaSuccess) e = cudaMalloc(&c->d_flag, sizeof(int) * 4);
     if (e == cudaSuccess) e = cudaMemsetAsync(c->d_flag, 0, sizeof(int) * 4, c->stream);
     if (e == cudaSuccess) e = cudaMallocHost(&c->h_flag, sizeof(int) * 4);
-    if (e == cudaSuccess) e = cudaEventCreateWithFlags(&c->check_ev, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaMallocHost((void**)&c->h_check, sizeof(unsigned long long));
+    if (e == cudaSuccess) *c->h_check = 0;
     if (e != cudaSuccess) {
         cudaFree(c->d_flag);
         cudaFreeHost(c->h_flag);
+        cudaFreeHost((void*)c->h_check);
         if (own_stream && c->stream) cudaStreamDestroy(c->stream);
         delete c;
         return rg_fail(RG_ERR_BACKEND, "rg_ctx_create: %s", cudaGetErrorString(e));
@@ -133,10 +135,10 @@ extern "C" rg_status rg_ctx_destroy(rg_ctx* ctx) {
             v.clear();
         }
         if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
-        cudaEventDestroy(ctx->check_ev);
         cudaFree(ctx->d_flag);
         cudaFree(ctx->tc_ws);
         cudaFreeHost(ctx->h_flag);
+        cudaFreeHost((void*)ctx->h_check);
     }
     delete ctx;
     return RG_OK;

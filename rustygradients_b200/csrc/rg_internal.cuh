@@ -68,7 +68,9 @@ struct rg_ctx {
     bool pdl = false;        // launch with programmatic stream serialization (inside a chain of rg_pdl_sync kernels)
     float* tc_ws = nullptr;  // split-k workspace of the tensor-core GEMM (this context's stream only)
     size_t tc_ws_bytes = 0;
-    cudaEvent_t check_ev = nullptr;  // the host waits for an op's argument check here, not for the op itself
+    // An op's argument check writes its number and result here (pinned), and the host waits for it, not for the op itself
+    volatile unsigned long long* h_check = nullptr;
+    unsigned check_no = 0;
     // storages outlive nothing they need: a buffer frees itself on `stream` only while the context is alive
     std::shared_ptr<rg_ctx_life> life = std::make_shared<rg_ctx_life>();
 };

@@ -13,13 +13,16 @@
 // ---------------------------------------------------------------------------
 // targets
 // ---------------------------------------------------------------------------
-// Ids are carried as f32 and truncated like the other index inputs.  One CTA: the rows with a target are counted, the bad
-// ones reported in status[0], and what the later kernels of the call need is set up.
+// Ids are carried as f32 and truncated like the other index inputs.  One CTA: the rows with a target are counted, the number
+// of bad ones goes to the host with the number of the call, and what the later kernels of the call need is set up.
 __global__ void __launch_bounds__(1024) lce_check_kernel(const float* __restrict__ targets, int R, int V, long long ignore,
                                                          const float* __restrict__ dloss, int* __restrict__ tgt, float* __restrict__ tz,
-                                                         float* __restrict__ scal, int* __restrict__ status) {
+                                                         float* __restrict__ scal, int* __restrict__ zero, int nzero,
+                                                         volatile unsigned long long* host, unsigned call) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ int live_s, bad_s;
     if (threadIdx.x == 0) live_s = bad_s = 0;
+    for (int i = threadIdx.x; i < nzero; i += 1024) zero[i] = 0;
     __syncthreads();
     int live = 0, bad = 0;
 #pragma unroll 4
@@ -40,9 +43,7 @@ __global__ void __launch_bounds__(1024) lce_check_kernel(const float* __restrict
     if (threadIdx.x == 0) {
         scal[0] = (float)live_s;
         scal[1] = live_s ? (dloss ? dloss[0] : 1.f) / (float)live_s : 0.f;
-        status[0] = bad_s;
-        status[1] = 0;  // ticket of lce_loss_kernel
-        status[2] = 0;  // largest magnitude of w
+        *host = (unsigned long long)call << 32 | (unsigned)bad_s;
     }
 }
 
@@ -56,23 +57,32 @@ __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict_
     __shared__ float red[32][9];
     __shared__ double rows_s[8];
     __shared__ bool last;
+    rg_pdl_sync();
     const int row = threadIdx.x & 7, slice = threadIdx.x >> 3;
     const int r = blockIdx.x * 8 + row;
-    const float2* mine = parts + (size_t)slice * R + r;
+    // the first 16 slices of a thread stay in registers (all of them up to a vocabulary of 65536)
+    float2 v[16];
     float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int p = slice + 32 * k;
+        v[k] = (r < R && p < nparts) ? parts[(size_t)p * R + r] : make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k++) m = fmaxf(m, v[k].x);
     if (r < R)
-#pragma unroll 8
-        for (int p = slice; p < nparts; p += 32) m = fmaxf(m, parts[(size_t)p * R + r].x);
+        for (int p = slice + 512; p < nparts; p += 32) m = fmaxf(m, parts[(size_t)p * R + r].x);
     red[slice][row] = m;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 32; k++) m = fmaxf(m, red[k][row]);
     const float ref = m == -INFINITY ? 0.f : m;  // a row of -inf only: every term below is 0
+#pragma unroll
+    for (int k = 0; k < 16; k++) s += v[k].y * expf(v[k].x - ref);
     if (r < R)
-#pragma unroll 8
-        for (int p = slice; p < nparts; p += 32, mine += (size_t)32 * R) {
-            const float2 v = *mine;
-            s += v.y * expf(v.x - ref);
+        for (int p = slice + 512; p < nparts; p += 32) {
+            const float2 q = parts[(size_t)p * R + r];
+            s += q.y * expf(q.x - ref);
         }
     __syncthreads();
     red[slice][row] = s;
@@ -112,89 +122,207 @@ __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict_
     if (threadIdx.x == 0) loss[0] = scal[0] > 0.f ? (float)(tot[0] / (double)scal[0]) : 0.f;
 }
 
-template <typename T>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) lce_dx_finish_kernel(const float* __restrict__ parts, int nparts, size_t count,
                                                             const float* __restrict__ scal, T* __restrict__ dx) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= count) return;
-    dx[i] = rg_from_float<T>(rg_sum_parts(parts + i, nparts, count) * scal[1]);
+    rg_pdl_sync();
+    const float scale = scal[1];
+    const size_t stride = (size_t)gridDim.x * 256 * VEC;
+    for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * VEC; i < count; i += stride) {
+        if constexpr (VEC == 4) {
+            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int z = 0; z < nparts; z++) {
+                const float4 q = *reinterpret_cast<const float4*>(parts + (size_t)z * count + i);
+                t.x += q.x, t.y += q.y, t.z += q.z, t.w += q.w;
+            }
+            const float v[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) dx[i + k] = rg_from_float<T>(v[k] * scale);
+        } else {
+            dx[i] = rg_from_float<T>(rg_sum_parts(parts + i, nparts, count) * scale);
+        }
+    }
 }
-void lce_dx_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* dx, int dtype) {
-    const unsigned grid = (unsigned)((count + 255) / 256);
-    if (dtype == RG_DTYPE_F32) lce_dx_finish_kernel<float><<<grid, 256, 0, ctx->stream>>>(parts, nparts, count, scal, (float*)dx);
-    else lce_dx_finish_kernel<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(parts, nparts, count, scal, (__nv_bfloat16*)dx);
+template <typename T>
+static void lce_dx_finish_typed(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, T* dx) {
+    // four values a thread where every partial starts on a 16-byte boundary and there are threads enough (768 values and 50
+    // partials: 15 us against 6; 6.5 million values and one partial: 9 us against 26)
+    const bool vec = count % 4 == 0 && count >= ((size_t)1 << 19);
+    const unsigned grid = (unsigned)std::min<size_t>((count + (vec ? 1023 : 255)) / (vec ? 1024 : 256), (size_t)ctx->sm_count * 16);
+    if (vec) rg_launch(true, lce_dx_finish_kernel<T, 4>, dim3(grid), dim3(256), 0, ctx->stream, parts, nparts, count, scal, dx);
+    else rg_launch(true, lce_dx_finish_kernel<T, 1>, dim3(grid), dim3(256), 0, ctx->stream, parts, nparts, count, scal, dx);
     RG_LAUNCHED(ctx);
 }
+void lce_dx_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* dx, int dtype) {
+    if (dtype == RG_DTYPE_F32) lce_dx_finish_typed(ctx, parts, nparts, count, scal, (float*)dx);
+    else lce_dx_finish_typed(ctx, parts, nparts, count, scal, (__nv_bfloat16*)dx);
+}
 
-__global__ void __launch_bounds__(1024) lce_dbias_finish_kernel(const float* __restrict__ parts, int nparts, int V,
-                                                                const float* __restrict__ scal, float* __restrict__ out) {
-    __shared__ float red[32][33];
+__global__ void __launch_bounds__(256) lce_dbias_finish_kernel(const float* __restrict__ parts, int nparts, int V,
+                                                               const float* __restrict__ scal, float* __restrict__ out) {
+    __shared__ float red[8][32];
+    rg_pdl_sync();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.f;
     if (c < V)
-        for (int p = w; p < nparts; p += 32) s += parts[(size_t)p * V + c];
+#pragma unroll 8
+        for (int p = w; p < nparts; p += 8) s += parts[(size_t)p * V + c];
     red[w][lane] = s;
     __syncthreads();
-    s = rg_warp_sum(red[lane][w]);
-    const int o = blockIdx.x * 32 + w;
-    if (lane == 0 && o < V) out[o] = s * scal[1];
+    if (w || c >= V) return;
+#pragma unroll
+    for (int k = 1; k < 8; k++) s += red[k][lane];
+    out[c] = s * scal[1];
 }
 void lce_dbias_finish_launch(rg_ctx* ctx, const float* parts, int nparts, int V, const float* scal, float* dbias) {
-    lce_dbias_finish_kernel<<<rg_cdiv(V, 32), 1024, 0, ctx->stream>>>(parts, nparts, V, scal, dbias);
+    rg_launch(true, lce_dbias_finish_kernel, dim3((unsigned)rg_cdiv(V, 32)), dim3(256), 0, ctx->stream, parts, nparts, V, scal, dbias);
     RG_LAUNCHED(ctx);
 }
 
 // ---------------------------------------------------------------------------
 // few rows: w is read once (twice in the gradient) by coalesced loads, the products are f32 FMAs
 // ---------------------------------------------------------------------------
-// A CTA owns 128 columns, a lane the columns lane + 32 j: no alignment of the rows of w is needed.  Its 8 warps share the D
-// axis and add their sums through shared memory.  x lies in shared memory as [d][row], so the RB values of one d are one or
-// a few broadcast loads.
-#define LCE_DC 1024  // rows of w between two refills of x
-template <int RB>
-constexpr size_t lce_few_smem() {
-    return sizeof(float) * (LCE_DC * RB > 8 * RB * 128 ? LCE_DC * RB : 8 * RB * 128);
+// Four values of a row of w are one load, although rows of an odd vocabulary start anywhere: warp q takes rows q, q + 8, ...,
+// all of which start at the same offset from an aligned address, and shifts its columns by it.  A tile is 124 columns, so
+// that the 128 a warp reads cover it for every shift; what it reads outside belongs to columns whose sums are not used.
+template <typename T>
+struct lce_four;
+template <>
+struct lce_four<float> { typedef float4 type; };
+template <>
+struct lce_four<__nv_bfloat16> { typedef uint2 type; };
+
+// w[at .. at + 3], at a multiple of 4; zeros beyond the matrix
+template <typename T>
+__device__ __forceinline__ void lce_load4(const T* __restrict__ w, size_t at, size_t total, float (&v)[4]) {
+    typedef typename lce_four<T>::type F;
+    if (at + 4 <= total) {
+        const F raw = *reinterpret_cast<const F*>(w + at);
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = rg_to_float(e[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = at + k < total ? rg_to_float(w[at + k]) : 0.f;
+    }
 }
 
+// RB values from shared memory, as wide as they are aligned
+template <int RB>
+__device__ __forceinline__ void lce_rows(const float* p, float (&v)[RB]) {
+    if constexpr (RB >= 4) {
+#pragma unroll
+        for (int r = 0; r < RB; r += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p + r);
+            v[r] = q.x, v[r + 1] = q.y, v[r + 2] = q.z, v[r + 3] = q.w;
+        }
+    } else if constexpr (RB == 2) {
+        const float2 q = *reinterpret_cast<const float2*>(p);
+        v[0] = q.x, v[1] = q.y;
+    } else {
+        v[0] = *p;
+    }
+}
+
+// Two f32 products and additions in one instruction.
+__device__ __forceinline__ float2 lce_fma2(float2 a, float2 b, float2 c) {
+    union U { float2 f; unsigned long long u; } x, y, z;
+    x.f = a, y.f = b, z.f = c;
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(z.u) : "l"(x.u), "l"(y.u));
+    return z.f;
+}
+
+#define LCE_COLS 124
 template <typename T, int RB>
-__device__ __forceinline__ void lce_few_logits(const lce_call& c, float* sm, float (&z)[RB / 8 > 0 ? RB / 8 : 1][4]) {
+struct lce_few {
+    static constexpr int PAIRS = (RB + 1) / 2;
+    static constexpr int DC = RB == 16 ? 512 : 1024;     // rows of w between two refills of x
+    static constexpr int AHEAD = 32 / (int)sizeof(T);     // rows of w a warp has on their way: 4 KB
+    static constexpr int RING = 8 * AHEAD * 128 * (int)sizeof(T), X = DC * RB * 4, SUMS = 8 * RB * 128 * 4;
+    static constexpr size_t SMEM = RING + X > SUMS ? RING + X : SUMS;
+};
+
+// z[k][j]: logit of row warp + 8 k and column lane + 32 j of the tile (-inf outside).  The 8 warps share the D axis.  Each lane
+// copies its four values of the warp's next rows of w asynchronously into a ring of its own in shared memory (kept in
+// registers they left too few warps: 3.5 TB/s), and multiplies them with the RB values of x, which lie in shared memory as
+// [d][row]: one or a few broadcast loads.  Rows of x are multiplied two at a time.
+template <typename T, int RB>
+__device__ __forceinline__ void lce_few_logits(const lce_call& c, unsigned char* sm, float (&z)[RB / 8 > 0 ? RB / 8 : 1][4]) {
+    typedef lce_few<T, RB> F;
+    typedef typename lce_four<T>::type V4;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int c0 = blockIdx.x * 128 + lane;
+    const int c0 = blockIdx.x * LCE_COLS, shift = (int)(((long long)w * c.V) & 3);
+    // lanes beyond the row read its last aligned place again: their sums are not used
+    const int col0 = min(c0 - shift + 4 * lane, ((c.V - 1 + shift) & ~3) - shift);
+    const size_t total = (size_t)c.D * c.V, step = (size_t)8 * c.V;
     const T* x = static_cast<const T*>(c.x);
     const T* wt = static_cast<const T*>(c.w);
-    float acc[RB][4];
+    V4* ring = reinterpret_cast<V4*>(sm) + w * F::AHEAD * 32 + lane;
+    float* xs = reinterpret_cast<float*>(sm + F::RING);
+    float2 acc[F::PAIRS][4];  // rows 2 i and 2 i + 1 of column j
 #pragma unroll
-    for (int r = 0; r < RB; r++)
+    for (int i = 0; i < F::PAIRS; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[r][j] = 0.f;
-    for (int d0 = 0; d0 < c.D; d0 += LCE_DC) {
-        const int dn = min(LCE_DC, c.D - d0);
-        __syncthreads();
-        for (int i = threadIdx.x; i < LCE_DC * RB; i += 256) {
-            const int r = i / LCE_DC, d = i % LCE_DC;
-            sm[d * RB + r] = (r < c.R && d < dn) ? rg_to_float(x[(size_t)r * c.D + d0 + d]) : 0.f;
+        for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
+    // this warp's rows of w: w, w + 8, ...; the last row of all ends the matrix, its read is guarded
+    const int rows = (c.D - w + 7) / 8, safe = (c.D - 1 - w + 7) / 8;
+    const T* from = wt + (size_t)w * c.V + col0;
+    auto copy = [&](int k) {
+        if (k < safe) {
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + (k % F::AHEAD) * 32);
+            if constexpr (sizeof(V4) == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from + (size_t)k * step) : "memory");
+            else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from + (size_t)k * step) : "memory");
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int k = 0; k < F::AHEAD - 1; k++) copy(k);
+    for (int d0 = 0; d0 < c.D; d0 += F::DC) {
+        const int dn = min(F::DC, c.D - d0), k1 = min(rows, (d0 + F::DC) / 8);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll 2
+            for (int d = threadIdx.x; d < dn; d += 256) xs[d * RB + r] = r < c.R ? rg_to_float(x[(size_t)r * c.D + d0 + d]) : 0.f;
         __syncthreads();
 #pragma unroll 4
-        for (int d = w; d < dn; d += 8) {
-            const T* wr = wt + (size_t)(d0 + d) * c.V;
+        for (int k = d0 / 8; k < k1; k++) {
+            copy(k + F::AHEAD - 1);  // into the slot that was read in the turn before
+            asm volatile("cp.async.wait_group %0;" ::"n"(F::AHEAD - 1) : "memory");
             float wv[4];
+            if (k < safe) {
+                const V4 raw = ring[(k % F::AHEAD) * 32];
+                const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-            for (int j = 0; j < 4; j++) wv[j] = c0 + 32 * j < c.V ? rg_to_float(wr[c0 + 32 * j]) : 0.f;
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                const float xv = sm[d * RB + r];
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[r][j] = fmaf(xv, wv[j], acc[r][j]);
+                for (int j = 0; j < 4; j++) wv[j] = rg_to_float(e[j]);
+            } else {
+                lce_load4(wt, (size_t)(w + 8 * k) * c.V + col0, total, wv);
             }
+            float xv[RB];
+            lce_rows<RB>(xs + (w + 8 * k - d0) * RB, xv);
+#pragma unroll
+            for (int i = 0; i < F::PAIRS; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (RB == 1) acc[0][j].x = fmaf(xv[0], wv[j], acc[0][j].x);
+                    else acc[i][j] = lce_fma2(make_float2(xv[2 * i], xv[2 * i + 1]), make_float2(wv[j], wv[j]), acc[i][j]);
+                }
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float* sums = reinterpret_cast<float*>(sm);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) sm[(w * RB + r) * 128 + lane + 32 * j] = acc[r][j];
+        for (int j = 0; j < 4; j++) {
+            const int col = 4 * lane + j - shift;
+            if (col >= 0 && c0 + col < c.V) sums[(w * RB + r) * 128 + col] = r % 2 ? acc[r / 2][j].y : acc[r / 2][j].x;
+        }
     __syncthreads();
     // warp w takes rows w, w + 8, ...: the sum over the 8 slices of D, then the bias
 #pragma unroll
@@ -202,27 +330,30 @@ __device__ __forceinline__ void lce_few_logits(const lce_call& c, float* sm, flo
         const int r = w + 8 * k;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            float s = 0.f;
-            if (r < RB)
+            const int col = lane + 32 * j;
+            const bool in = col < LCE_COLS && c0 + col < c.V;
+            float t = 0.f;
+            if (r < RB && in)
 #pragma unroll
-                for (int q = 0; q < 8; q++) s += sm[(q * RB + r) * 128 + lane + 32 * j];
-            const int col = c0 + 32 * j;
-            z[k][j] = col < c.V ? s + (c.bias ? c.bias[col] : 0.f) : -INFINITY;
+                for (int q = 0; q < 8; q++) t += sums[(q * RB + r) * 128 + col];
+            z[k][j] = in ? t + (c.bias ? c.bias[c0 + col] : 0.f) : -INFINITY;
         }
     }
 }
 
 template <typename T, int RB>
-__global__ void __launch_bounds__(256) lce_few_fwd_kernel(const lce_call c) {
-    extern __shared__ float sm[];
+__global__ void __launch_bounds__(256, RB <= 4 ? 4 : RB <= 8 ? 3 : 2) lce_few_fwd_kernel(const lce_call c) {
+    extern __shared__ __align__(16) unsigned char lce_sm[];
     float z[RB / 8 > 0 ? RB / 8 : 1][4];
-    lce_few_logits<T, RB>(c, sm, z);
+    lce_few_logits<T, RB>(c, lce_sm, z);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the targets; x and w were there before
 #pragma unroll
     for (int k = 0; k < (RB / 8 > 0 ? RB / 8 : 1); k++) {
         const int r = w + 8 * k;
         if (r >= c.R || r >= RB) continue;  // whole warps
-        const int t = c.tgt[r];
+        const int t = c.tgt[r] - (int)blockIdx.x * LCE_COLS;
         float m = fmaxf(fmaxf(z[k][0], z[k][1]), fmaxf(z[k][2], z[k][3]));
         m = rg_warp_max(m);
         const float ref = m == -INFINITY ? 0.f : m;
@@ -230,7 +361,7 @@ __global__ void __launch_bounds__(256) lce_few_fwd_kernel(const lce_call c) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             s += expf(z[k][j] - ref);
-            if (t == (int)blockIdx.x * 128 + lane + 32 * j) c.tz[r] = z[k][j];
+            if (t == lane + 32 * j && t < LCE_COLS) c.tz[r] = z[k][j];
         }
         s = rg_warp_sum(s);
         if (lane == 0) c.parts[(size_t)blockIdx.x * c.R + r] = make_float2(m, s);
@@ -239,25 +370,30 @@ __global__ void __launch_bounds__(256) lce_few_fwd_kernel(const lce_call c) {
 
 // dz (without the common factor dloss / n) of all rows, f32 [R][V], and the bias gradient
 template <typename T, int RB>
-__global__ void __launch_bounds__(256) lce_few_dz_kernel(const lce_call c, float* __restrict__ dz) {
-    extern __shared__ float sm[];
+__global__ void __launch_bounds__(256, RB <= 4 ? 4 : RB <= 8 ? 3 : 2) lce_few_dz_kernel(const lce_call c, float* __restrict__ dz) {
+    extern __shared__ __align__(16) unsigned char lce_sm[];
     float z[RB / 8 > 0 ? RB / 8 : 1][4];
-    lce_few_logits<T, RB>(c, sm, z);
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    lce_few_logits<T, RB>(c, lce_sm, z);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c0 = (int)blockIdx.x * LCE_COLS;
+    float* sm = reinterpret_cast<float*>(lce_sm);
     float col[4] = {0.f, 0.f, 0.f, 0.f};
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the targets; x and w were there before
+    {
 #pragma unroll
-    for (int k = 0; k < (RB / 8 > 0 ? RB / 8 : 1); k++) {
-        const int r = w + 8 * k;
-        if (r >= c.R || r >= RB) continue;
-        const int t = c.tgt[r];
-        const float lse = c.lse[r];
+        for (int k = 0; k < (RB / 8 > 0 ? RB / 8 : 1); k++) {
+            const int r = w + 8 * k;
+            if (r >= c.R || r >= RB) continue;
+            const int t = c.tgt[r];
+            const float lse = c.lse[r];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int v = (int)blockIdx.x * 128 + lane + 32 * j;
-            if (v < c.V) {
-                const float p = t < 0 ? 0.f : expf(z[k][j] - lse) - (v == t ? 1.f : 0.f);
-                dz[(size_t)r * c.V + v] = p;
-                col[j] += p;
+            for (int j = 0; j < 4; j++) {
+                const int v = c0 + lane + 32 * j;
+                if (lane + 32 * j < LCE_COLS && v < c.V) {
+                    const float p = t < 0 ? 0.f : expf(z[k][j] - lse) - (v == t ? 1.f : 0.f);
+                    dz[(size_t)r * c.V + v] = p;
+                    col[j] += p;
+                }
             }
         }
     }
@@ -266,61 +402,78 @@ __global__ void __launch_bounds__(256) lce_few_dz_kernel(const lce_call c, float
 #pragma unroll
     for (int j = 0; j < 4; j++) sm[w * 128 + lane + 32 * j] = col[j];
     __syncthreads();
-    if (threadIdx.x < 128) {
-        const int v = (int)blockIdx.x * 128 + threadIdx.x;
+    if (threadIdx.x < LCE_COLS && c0 + (int)threadIdx.x < c.V) {
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < 8; q++) s += sm[q * 128 + threadIdx.x];
-        if (v < c.V) c.dbias[v] = s * c.scal[1];
+        c.dbias[c0 + threadIdx.x] = s * c.scal[1];
     }
 }
 
-// dw and partial dx.  A thread holds dz of RB rows and 4 columns in registers and walks LCE_DG rows of w: one load of w
-// and one store of dw per element; the RB products with dz are summed over the warp by halving exchanges (each exchange
-// adds two rows at once, so RB rows cost RB shuffles plus the steps left), over the 8 warps in shared memory.
+// dw and partial dx.  A warp has 128 columns (lane + 32 j), a CTA 1024, and walks LCE_DG rows of w: a thread holds dz of RB
+// rows and 4 columns in registers, each value of w is one load, each of dw one store.  The RB products with dz are summed
+// over the warp by halving exchanges (each adds two rows at once, so RB rows cost RB shuffles plus the steps left), over the
+// 8 warps in shared memory.  (Four-value loads with shifted columns, as above, need their own dz per shift: slower.)
 #define LCE_DG 32
 template <typename T, int RB>
 __global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, const float* __restrict__ dz, float* __restrict__ dxparts) {
-    __shared__ float xs[LCE_DG][RB];
+    constexpr int PAIRS = (RB + 1) / 2;
+    __shared__ __align__(16) float xs[LCE_DG][RB];
     __shared__ float dxs[8][LCE_DG][RB];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int c0 = (int)blockIdx.x * 1024 + w * 128 + lane;
     const int d0 = (int)blockIdx.y * LCE_DG, dn = min(LCE_DG, c.D - d0);
     const T* x = static_cast<const T*>(c.x);
-    const T* wt = static_cast<const T*>(c.w);
-    T* dw = static_cast<T*>(c.dw);
+    const T* wt = static_cast<const T*>(c.w) + (size_t)d0 * c.V + c0;
+    T* dw = static_cast<T*>(c.dw) + (size_t)d0 * c.V + c0;
+    rg_pdl_sync();
     const float scale = c.scal[1];
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) in[j] = c0 + 32 * j < c.V;
     for (int i = threadIdx.x; i < LCE_DG * RB; i += 256) {
         const int r = i / LCE_DG, d = i % LCE_DG;
         xs[d][r] = (r < c.R && d < dn) ? rg_to_float(x[(size_t)r * c.D + d0 + d]) : 0.f;
     }
-    float g[RB][4];
+    float2 g[PAIRS][4];
 #pragma unroll
-    for (int r = 0; r < RB; r++)
+    for (int i = 0; i < PAIRS; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) g[r][j] = (r < c.R && c0 + 32 * j < c.V) ? dz[(size_t)r * c.V + c0 + 32 * j] : 0.f;
+        for (int j = 0; j < 4; j++) {
+            g[i][j].x = (2 * i < c.R && in[j]) ? dz[(size_t)(2 * i) * c.V + c0 + 32 * j] : 0.f;
+            g[i][j].y = (2 * i + 1 < c.R && in[j]) ? dz[(size_t)(2 * i + 1) * c.V + c0 + 32 * j] : 0.f;
+        }
+    T next[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) next[j] = in[j] ? wt[32 * j] : rg_from_float<T>(0.f);
     __syncthreads();
 #pragma unroll 2
-    for (int d = 0; d < dn; d++) {
-        const size_t at = (size_t)(d0 + d) * c.V + c0;
-        float wv[4], o[4];
+    for (int d = 0; d < dn; d++, wt += c.V, dw += c.V) {
+        float wv[4];
+        float2 o[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) wv[j] = c0 + 32 * j < c.V ? rg_to_float(wt[at + 32 * j]) : 0.f, o[j] = 0.f;
-        float q[RB];
+        for (int j = 0; j < 4; j++) wv[j] = rg_to_float(next[j]), o[j] = make_float2(0.f, 0.f);
+        if (d + 1 < dn)
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            const float xv = xs[d][r];
-            q[r] = 0.f;
+            for (int j = 0; j < 4; j++)
+                if (in[j]) next[j] = wt[c.V + 32 * j];
+        float xv[RB], q[2 * PAIRS];
+        lce_rows<RB>(xs[d], xv);
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) {
+            const float2 xp = make_float2(xv[2 * i], RB > 1 ? xv[RB > 1 ? 2 * i + 1 : 0] : 0.f);
+            float2 s = make_float2(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                o[j] = fmaf(xv, g[r][j], o[j]);
-                q[r] = fmaf(g[r][j], wv[j], q[r]);
+                o[j] = lce_fma2(xp, g[i][j], o[j]);
+                s = lce_fma2(g[i][j], make_float2(wv[j], wv[j]), s);
             }
+            q[2 * i] = s.x, q[2 * i + 1] = s.y;
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (c0 + 32 * j < c.V) dw[at + 32 * j] = rg_from_float<T>(o[j] * scale);
-        // halving exchange: after it, lane l holds row (l / (32 / RB)) summed over the lanes that share it
+            if (in[j]) dw[32 * j] = rg_from_float<T>((o[j].x + o[j].y) * scale);
+        // after the exchanges lane l holds row l / (32 / RB), summed over the lanes that share it
         int half = 16;
 #pragma unroll
         for (int n = RB / 2; n >= 1; n >>= 1, half >>= 1) {
@@ -347,21 +500,29 @@ __global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, con
     }
 }
 
-#define LCE_FEW_ROWS 16
+// The form for few rows, by what was measured at [R,768] x [768,50257] (us, forward + gradient): f32 16 rows 73 + 201, the
+// tensor cores 158 + 375 for 17; bf16 with an aligned vocabulary 4 rows 40 + 100, the tensor cores 40 + 117; with an odd one
+// (whose rows have to be copied first) 8 rows 50 + 125, the tensor cores 72 + 147.
+static bool lce_is_few(const lce_call& c) { return c.R <= (c.dtype == RG_DTYPE_F32 ? 16 : c.V % 8 == 0 ? 4 : 8); }
+
+static int lce_few_tiles(int V) { return rg_cdiv(V, LCE_COLS); }
+static int lce_few_parts(int V) { return rg_cdiv(V, 1024); }
 
 template <typename T, int RB>
 static void lce_few_launch(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
-    const unsigned tiles = (unsigned)rg_cdiv(c.V, 128);
-    const size_t smem = lce_few_smem<RB>();
+    const dim3 tiles((unsigned)lce_few_tiles(c.V));
+    const size_t smem = lce_few<T, RB>::SMEM;
+    // these start while the check of the targets runs and wait for it before they use them
     if (!dz) {
         if (smem > 48 * 1024) cudaFuncSetAttribute(lce_few_fwd_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        lce_few_fwd_kernel<T, RB><<<tiles, 256, smem, ctx->stream>>>(c);
+        rg_launch(true, lce_few_fwd_kernel<T, RB>, tiles, dim3(256), smem, ctx->stream, c);
         RG_LAUNCHED(ctx);
         return;
     }
     if (smem > 48 * 1024) cudaFuncSetAttribute(lce_few_dz_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    lce_few_dz_kernel<T, RB><<<tiles, 256, smem, ctx->stream>>>(c, dz);
-    lce_few_grad_kernel<T, RB><<<dim3((unsigned)rg_cdiv(c.V, 1024), (unsigned)rg_cdiv(c.D, LCE_DG)), 256, 0, ctx->stream>>>(c, dz, dxparts);
+    rg_launch(true, lce_few_dz_kernel<T, RB>, tiles, dim3(256), smem, ctx->stream, c, dz);
+    rg_launch(true, lce_few_grad_kernel<T, RB>, dim3((unsigned)lce_few_parts(c.V), (unsigned)rg_cdiv(c.D, LCE_DG)), dim3(256), 0, ctx->stream, c,
+              (const float*)dz, dxparts);
     ctx->launches += 2;
 }
 template <typename T>
@@ -372,7 +533,7 @@ static void lce_few_rows(rg_ctx* ctx, const lce_call& c, float* dz, float* dxpar
     else if (c.R <= 8) lce_few_launch<T, 8>(ctx, c, dz, dxparts);
     else lce_few_launch<T, 16>(ctx, c, dz, dxparts);
 }
-static void lce_few(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
+static void lce_few_run(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
     if (c.dtype == RG_DTYPE_F32) lce_few_rows<float>(ctx, c, dz, dxparts);
     else lce_few_rows<__nv_bfloat16>(ctx, c, dz, dxparts);
 }
@@ -397,32 +558,41 @@ static rg_status lce_args(const char* op, rg_ctx* ctx, const rg_storage* x, cons
     if (bias && bias->len != V) return rg_fail(RG_ERR_SHAPE, "bias holds %zu elements for %zu classes", bias->len, V);
     RG_TRY(rg_not_capturing(ctx, op));
     memset(c, 0, sizeof(*c));
+    c->err = ctx->d_flag + 1;
     c->R = (int)R, c->D = (int)D, c->V = (int)V, c->dtype = x->dtype;
     c->x = x->raw(), c->w = w->raw(), c->bias = bias ? bias->data() : nullptr;
     return RG_OK;
 }
 
-// Enqueues the check of the targets; lce_checked waits for it (not for what was enqueued after it).
+// Enqueues the check of the targets; lce_checked waits for its answer (not for what was enqueued after it).
 static rg_status lce_check_launch(rg_ctx* ctx, lce_call& c, const rg_storage* targets, long long ignore, const rg_storage* dloss,
                                   rg_storage** scratch) {
-    // tgt [R] | tz [R] | scal [2] | status [3]
-    const size_t words = 2 * (size_t)c.R + 5;
+    // tgt [R] | tz [R] | scal [2] | words that start at 0
+    const int nzero = 2 + c.ncounters;
+    const size_t words = 2 * (size_t)c.R + 2 + nzero;
     RG_TRY(rg_alloc_storage(ctx, &words, 1, scratch));
     float* base = (*scratch)->data();
     c.tgt = reinterpret_cast<int*>(base), c.tz = base + c.R, c.scal = base + 2 * (size_t)c.R;
-    c.wmax = reinterpret_cast<unsigned*>(base + 2 * (size_t)c.R + 4);
+    c.ticket = reinterpret_cast<int*>(base + 2 * (size_t)c.R + 2);
+    c.wmax = reinterpret_cast<unsigned*>(base + 2 * (size_t)c.R + 3);
+    c.counters = reinterpret_cast<int*>(base + 2 * (size_t)c.R + 4);
     lce_check_kernel<<<1, 1024, 0, ctx->stream>>>(targets->data(), c.R, c.V, ignore, dloss ? dloss->data() : nullptr,
-                                                  const_cast<int*>(c.tgt), c.tz, const_cast<float*>(c.scal),
-                                                  reinterpret_cast<int*>(const_cast<float*>(c.scal)) + 2);
+                                                  const_cast<int*>(c.tgt), c.tz, const_cast<float*>(c.scal), c.ticket, nzero, ctx->h_check,
+                                                  ++ctx->check_no);
     RG_LAUNCHED(ctx);
     RG_CUDA(cudaGetLastError());
-    RG_CUDA(cudaMemcpyAsync(ctx->h_flag, c.scal + 2, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
-    RG_CUDA(cudaEventRecord(ctx->check_ev, ctx->stream));
     return RG_OK;
 }
 static rg_status lce_checked(rg_ctx* ctx, const lce_call& c) {
-    RG_CUDA(cudaEventSynchronize(ctx->check_ev));
-    if (ctx->h_flag[0]) return rg_fail(RG_ERR_SHAPE, "Target index out of bounds for %d classes", c.V);
+    unsigned long long v;
+    for (unsigned spins = 1; (unsigned)((v = *ctx->h_check) >> 32) != ctx->check_no; spins++) {
+        if (spins % 65536) continue;
+        const cudaError_t e = cudaStreamQuery(ctx->stream);  // a stream that failed never answers
+        if (e == cudaErrorNotReady) continue;
+        if (e == cudaSuccess && (unsigned)(*ctx->h_check >> 32) == ctx->check_no) continue;
+        return rg_fail(RG_ERR_BACKEND, "linear_cross_entropy: %s", cudaGetErrorString(e));
+    }
+    if ((unsigned)v) return rg_fail(RG_ERR_SHAPE, "Target index out of bounds for %d classes", c.V);
     return RG_OK;
 }
 
@@ -443,18 +613,18 @@ extern "C" rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, c
         o.give({loss, lse});
         return RG_OK;
     }
+    const bool few = lce_is_few(c);
+    c.ncounters = few ? 0 : 1;
     RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, nullptr, &o[2]));
-    const bool few = c.R <= LCE_FEW_ROWS;
-    c.nparts = few ? rg_cdiv(c.V, 128) : lce_tc_nparts(c.V);
+    c.nparts = few ? lce_few_tiles(c.V) : lce_tc_nparts(c.V);
     const size_t pwords = 2 * (size_t)c.nparts * rows, blocks = (size_t)rg_cdiv(c.R, 8), swords = 2 * blocks;
     RG_TRY(rg_alloc_storage(ctx, &pwords, 1, &o[3]));
     RG_TRY(rg_alloc_storage(ctx, &swords, 1, &o[4]));
     c.parts = static_cast<float2*>(o[3]->raw());
-    if (few) lce_few(ctx, c, nullptr, nullptr);
+    if (few) lce_few_run(ctx, c, nullptr, nullptr);
     else RG_TRY(lce_tc_forward(ctx, c));
-    lce_loss_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(c.parts, c.nparts, c.R, c.tgt, c.tz, c.scal,
-                                                               reinterpret_cast<int*>(const_cast<float*>(c.scal)) + 3,
-                                                               static_cast<double*>(o[4]->raw()), o[1]->data(), o[0]->data());
+    rg_launch(true, lce_loss_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, (const float2*)c.parts, c.nparts, c.R, c.tgt,
+              (const float*)c.tz, c.scal, c.ticket, static_cast<double*>(o[4]->raw()), o[1]->data(), o[0]->data());
     RG_LAUNCHED(ctx);
     RG_CUDA(cudaGetLastError());
     RG_TRY(lce_checked(ctx, c));
@@ -484,12 +654,14 @@ extern "C" rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* 
         RG_CUDA(cudaMemsetAsync(o[1]->raw(), 0, o[1]->len * rg_dtype_size(o[1]->dtype), ctx->stream));
         if (bias) RG_CUDA(cudaMemsetAsync(o[2]->raw(), 0, o[2]->len * 4, ctx->stream));
     } else {
+        const bool few = lce_is_few(c);
+        c.ncounters = few ? 0 : lce_tc_backward_launches(c);
         RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, dloss, &o[3]));
-        if (c.R <= LCE_FEW_ROWS) {
-            const size_t zlen = (size_t)c.R * c.V, nparts = (size_t)rg_cdiv(c.V, 1024), plen = nparts * c.R * c.D;
+        if (few) {
+            const size_t zlen = (size_t)c.R * c.V, nparts = (size_t)lce_few_parts(c.V), plen = nparts * c.R * c.D;
             RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[4]));
             RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[5]));
-            lce_few(ctx, c, o[4]->data(), o[5]->data());
+            lce_few_run(ctx, c, o[4]->data(), o[5]->data());
             lce_dx_finish_launch(ctx, o[5]->data(), (int)nparts, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
         } else {
             RG_TRY(lce_tc_backward(ctx, c));

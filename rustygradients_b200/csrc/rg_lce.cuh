@@ -12,7 +12,11 @@ struct lce_call {
     const int* tgt;        // R: target column, -1 for a row that is left out
     const float* lse;      // backward: R
     const float* scal;     // device: [0] rows with a target, [1] dloss / rows (0 when there is none)
-    unsigned* wmax;        // a word that is 0
+    int* err;              // raised by a wait that gives up
+    int ncounters;         // tile counters that the call needs
+    int* ticket;           // words that start at 0
+    unsigned* wmax;
+    int* counters;
     float2* parts;         // forward: (maximum, sum of exponentials) of row r over slice p at [p * R + r]
     float* tz;             // forward: logit of the target
     int nparts;
@@ -40,3 +44,4 @@ void lce_dbias_finish_launch(rg_ctx* ctx, const float* parts, int nparts, int V,
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c);
 rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c);
 int lce_tc_nparts(int V);
+int lce_tc_backward_launches(const lce_call& c);

@@ -412,6 +412,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     int total = 0;
@@ -436,6 +437,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    // everything above needs nothing from the kernels before; from here on they are complete
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp < S::FIRST) {
     if (S::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -638,8 +641,16 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             }
             if (!ok) break;
             if (PLANES != 1) {
+                // one copy of the epilogue's code: the next 32 columns move into its registers (four copies, 130 KB of
+                // instructions, took a single tile from 14 to 26 us)
+#pragma unroll 1
+                for (int c = 0; c < HALF / 32; c++) {
+                    lt_columns<PLANES, EPI>(e, t, w, acc[0], c0 + c * 32, stage);
 #pragma unroll
-                for (int c = 0; c < HALF / 32; c++) lt_columns<PLANES, EPI>(e, t, w, acc[c], c0 + c * 32, stage);
+                    for (int k = 1; k < HALF / 32; k++)
+#pragma unroll
+                        for (int j = 0; j < 32; j++) acc[k - 1][j] = acc[k][j];
+                }
             }
             if (EPI == LT_FWD && w.live) e.parts[(size_t)(t.n * 2 + half) * e.R + w.row] = make_float2(w.ms.m, w.ms.s);
         }
@@ -657,17 +668,33 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 // A bf16 matrix whose rows TMA cannot address (they do not start on 16-byte boundaries), copied to such rows.
 __global__ void __launch_bounds__(256) lt_align_kernel(const __nv_bfloat16* __restrict__ src, long long rows, int cols, int pitch,
                                                        __nv_bfloat16* __restrict__ dst) {
+    rg_pdl_sync();
     const int groups = pitch / 8;
-    const long long n = rows * groups, stride = (long long)gridDim.x * 256;
+    const long long n = rows * groups, stride = (long long)gridDim.x * 256, total = rows * cols;
     const unsigned short* in = reinterpret_cast<const unsigned short*>(src);
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
         const long long r = i / groups;
         const int c = (int)(i - r * groups) * 8;
+        // eight values from two aligned loads (the second is a neighbour's first); what lies beyond the row is never read
+        const long long at = r * cols + c, base = at & ~7ll;
+        const int shift = (int)(at & 7);
         uint32_t h[4];
+        if (base + 16 <= total) {
+            const uint4 p = *reinterpret_cast<const uint4*>(in + base), q = *reinterpret_cast<const uint4*>(in + base + 8);
+            const uint32_t w[9] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w, 0u};
+            const int words = shift >> 1, bits = (shift & 1) * 16;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t a = c + 2 * k < cols ? in[r * cols + c + 2 * k] : 0u, b = c + 2 * k + 1 < cols ? in[r * cols + c + 2 * k + 1] : 0u;
-            h[k] = a | (b << 16);
+            for (int k = 0; k < 4; k++) {
+                const uint32_t lo = words == 0 ? w[k] : words == 1 ? w[k + 1] : words == 2 ? w[k + 2] : w[k + 3];
+                const uint32_t hi = words == 0 ? w[k + 1] : words == 1 ? w[k + 2] : words == 2 ? w[k + 3] : w[k + 4];
+                h[k] = __funnelshift_r(lo, hi, bits);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t a = at + 2 * k < total ? in[at + 2 * k] : 0u, b = at + 2 * k + 1 < total ? in[at + 2 * k + 1] : 0u;
+                h[k] = a | (b << 16);
+            }
         }
         *reinterpret_cast<uint4*>(dst + r * pitch + c) = make_uint4(h[0], h[1], h[2], h[3]);
     }
@@ -697,6 +724,7 @@ __device__ __forceinline__ void lt_split2(float v, float scale, uint32_t& h0, ui
 __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                            uint16_t* __restrict__ pair, uint16_t* __restrict__ triple,
                                                            float* __restrict__ scale_out) {
+    rg_pdl_sync();
     const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (r >= rows) return;
     const float* p = src + (size_t)r * cols;
@@ -721,6 +749,7 @@ __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restri
 
 // Largest finite magnitude of w (as bits: they order like the values), into a word that lce_check_kernel has set to 0.
 __global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ src, size_t n, unsigned* __restrict__ out) {
+    rg_pdl_sync();
     const size_t stride = (size_t)gridDim.x * 256;
     const float4* v4 = reinterpret_cast<const float4*>(src);
     float m = 0.f;
@@ -741,6 +770,7 @@ template <bool TRIPLE>
 __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                       const unsigned* __restrict__ largest, uint16_t* __restrict__ pair,
                                                       uint16_t* __restrict__ triple, float* __restrict__ scale_out) {
+    rg_pdl_sync();
     const float2 sc = lt_scale(__uint_as_float(*largest));
     if (blockIdx.x == 0 && threadIdx.x == 0) *scale_out = sc.y;
     const int groups = pitch / 8;
@@ -836,8 +866,8 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
     if (dtype == RG_DTYPE_BF16) {
         RG_TRY(rg_alloc_storage(ctx, &plane, 1, &o->mem[0], RG_DTYPE_BF16));
         const int grid = (int)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
-        lt_align_kernel<<<grid, 256, 0, ctx->stream>>>(static_cast<const __nv_bfloat16*>(src), rows, cols, pitch,
-                                                       static_cast<__nv_bfloat16*>(o->mem[0]->raw()));
+        RG_CUDA(rg_launch(true, lt_align_kernel, dim3(grid), dim3(256), 0, ctx->stream, static_cast<const __nv_bfloat16*>(src),
+                          (long long)rows, cols, pitch, static_cast<__nv_bfloat16*>(o->mem[0]->raw())));
         RG_LAUNCHED(ctx);
         o->logits = o->grads = {o->mem[0]->raw(), rows, cols, 1, pitch};
         return RG_OK;
@@ -851,19 +881,16 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
         const float* w = static_cast<const float*>(src);
         const size_t n = (size_t)rows * cols;
         const int most = ctx->sm_count * 16;
-        lt_max_kernel<<<(unsigned)std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, ctx->sm_count * 8)), 256, 0, ctx->stream>>>(w, n, largest);
+        RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, ctx->sm_count * 8))),
+                          dim3(256), 0, ctx->stream, w, n, largest));
         const unsigned grid = (unsigned)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, most);
-        if (want_grads)
-            lt_pack_kernel<true><<<grid, 256, 0, ctx->stream>>>(w, rows, cols, pitch, largest, static_cast<uint16_t*>(o->mem[0]->raw()),
-                                                                static_cast<uint16_t*>(three), o->mem[1]->data());
-        else
-            lt_pack_kernel<false><<<grid, 256, 0, ctx->stream>>>(w, rows, cols, pitch, largest, static_cast<uint16_t*>(o->mem[0]->raw()),
-                                                                 nullptr, o->mem[1]->data());
+        RG_CUDA(rg_launch(true, want_grads ? lt_pack_kernel<true> : lt_pack_kernel<false>, dim3(grid), dim3(256), 0, ctx->stream, w, rows, cols,
+                          pitch, (const unsigned*)largest, static_cast<uint16_t*>(o->mem[0]->raw()), static_cast<uint16_t*>(three),
+                          o->mem[1]->data()));
         RG_LAUNCHED(ctx);
     } else {
-        lt_pack_rows_kernel<<<rg_cdiv(rows, 8), 256, 0, ctx->stream>>>(static_cast<const float*>(src), rows, cols, pitch,
-                                                                      static_cast<uint16_t*>(o->mem[0]->raw()),
-                                                                      static_cast<uint16_t*>(three), o->mem[1]->data());
+        RG_CUDA(rg_launch(true, lt_pack_rows_kernel, dim3((unsigned)rg_cdiv(rows, 8)), dim3(256), 0, ctx->stream, static_cast<const float*>(src), rows,
+                          cols, pitch, static_cast<uint16_t*>(o->mem[0]->raw()), static_cast<uint16_t*>(three), o->mem[1]->data()));
     }
     RG_CUDA(cudaGetLastError());
     RG_LAUNCHED(ctx);
@@ -891,11 +918,11 @@ static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
     long long total = 0;
     for (int i = 0; i < e.nprobs; i++) total += (long long)e.p[i].tiles_m * e.p[i].tiles_n * e.p[i].splits;
     if (total > 0x3fffffff) return rg_fail(RG_ERR_SHAPE, "linear_cross_entropy: too many tiles");
-    RG_CUDA(cudaMemsetAsync(e.counter, 0, sizeof(int), ctx->stream));
     const int grid = 2 * (int)std::min<long long>(total, ctx->sm_count / 2);
-    lce_tc_kernel<PLANES, EPI><<<grid, lt_shape<PLANES>::THREADS, LT_SMEM_BYTES, ctx->stream>>>(maps[0], maps[1], maps[2], maps[3], e);
-    RG_CUDA(cudaGetLastError());
+    RG_CUDA(rg_launch(true, lce_tc_kernel<PLANES, EPI>, dim3(grid), dim3(lt_shape<PLANES>::THREADS), LT_SMEM_BYTES, ctx->stream, maps[0], maps[1],
+                      maps[2], maps[3], e));
     RG_LAUNCHED(ctx);
+    e.counter++;  // each launch hands out its tiles from a counter of its own
     return RG_OK;
 }
 template <int EPI>
@@ -903,19 +930,16 @@ static rg_status lt_run(rg_ctx* ctx, const lce_call& c, const CUtensorMap* maps,
     return c.dtype == RG_DTYPE_F32 ? lt_launch<EPI == LT_GRAD ? 3 : 2, EPI>(ctx, maps, e) : lt_launch<1, EPI>(ctx, maps, e);
 }
 
-static void lt_common(rg_ctx* ctx, const lce_call& c, rg_storage* counter, lt_args* e) {
+static void lt_common(rg_ctx* ctx, const lce_call& c, int* counter, lt_args* e) {
     memset(e, 0, sizeof(*e));
-    e->counter = reinterpret_cast<int*>(counter->raw()), e->err = ctx->d_flag + 1;
+    e->counter = counter, e->err = ctx->d_flag + 1;
     e->R = c.R, e->D = c.D, e->V = c.V, e->v0 = 0, e->vn = c.V;
     e->bias = c.bias, e->tgt = c.tgt, e->lse = c.lse, e->scal = c.scal;
     e->parts = c.parts, e->tz = c.tz;
 }
 
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
-    rg_outputs<1> o;  // counter
     lt_packed x, w;
-    const size_t one = 1;
-    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
     RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, false, &x));
     RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, false, &w));
     CUtensorMap maps[4];
@@ -923,7 +947,7 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     RG_TRY(lt_map(&maps[1], w.logits, LT_BK));
     maps[2] = maps[0], maps[3] = maps[1];
     lt_args e;
-    lt_common(ctx, c, o[0], &e);
+    lt_common(ctx, c, c.counters, &e);
     e.xscale = x.scale, e.wscale = w.scale;
     e.nprobs = 1;
     e.p[0] = lt_problem(c.R, c.V, c.D, LT_BN, 0, 1);
@@ -934,21 +958,25 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
 // bf16 planes, then one launch multiplies it with w and with x.
 #define LT_DZ_BYTES ((size_t)512 << 20)
 
+static int lt_piece(const lce_call& c) {
+    const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1;
+    const long long most = std::max<long long>(1, (long long)(LT_DZ_BYTES / ((size_t)planes * 2 * c.R)) / 256) * 256;
+    const int pieces = (int)((c.V + most - 1) / most);
+    return (int)std::min<long long>(most, (rg_cdiv(c.V, pieces) + 255) / 256 * 256);
+}
+int lce_tc_backward_launches(const lce_call& c) { return 2 * rg_cdiv(c.V, lt_piece(c)); }
+
 rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
-    rg_outputs<4> o;  // counter, dz, partial dx, partial dbias
+    rg_outputs<3> o;  // dz, partial dx, partial dbias
     lt_packed x, w;
-    const size_t one = 1;
     const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = planes == 3 ? lt_shape<3>::BN : lt_shape<1>::BN;  // of the gradients
-    RG_TRY(rg_alloc_storage(ctx, &one, 1, &o[0]));
     RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, &x));
     RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, &w));
 
-    const long long most = std::max<long long>(1, (long long)(LT_DZ_BYTES / ((size_t)planes * 2 * c.R)) / 256) * 256;
-    const int pieces = (int)((c.V + most - 1) / most);
-    const int piece = (int)std::min<long long>(most, (rg_cdiv(c.V, pieces) + 255) / 256 * 256);
+    const int piece = lt_piece(c), pieces = rg_cdiv(c.V, piece);
     const int width = std::min(piece, (c.V + 63) / 64 * 64);  // columns of dz that are stored
     const size_t zlen = (size_t)planes * c.R * width;
-    RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[1], RG_DTYPE_BF16));
+    RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[0], RG_DTYPE_BF16));
 
     // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
     lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
@@ -957,15 +985,15 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
     const int run = rg_cdiv(pdx.kb_per, std::min(16, rg_cdiv(pdx.kb_per, fair))), splits = rg_cdiv(pdx.kb_per, run);
     const size_t plen = (size_t)splits * c.R * c.D;
-    RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[2]));
+    RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[1]));
     const int dbrows = LT_BM / 32 * rg_cdiv(c.R, LT_BM);
     if (c.dbias) {
         const size_t blen = (size_t)dbrows * c.V;
-        RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[3]));
+        RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[2]));
     }
 
     CUtensorMap mz[4], mg[4];
-    lt_operand z = {o[1]->raw(), c.R, width, planes, width};
+    lt_operand z = {o[0]->raw(), c.R, width, planes, width};
     RG_TRY(lt_map(&mz[0], x.logits, 128));
     RG_TRY(lt_map(&mz[1], w.logits, LT_BK));
     mz[2] = mz[0], mz[3] = mz[1];
@@ -976,12 +1004,12 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
 
     for (int i = 0; i < pieces; i++) {
         lt_args e;
-        lt_common(ctx, c, o[0], &e);
+        lt_common(ctx, c, c.counters + 2 * i, &e);
         e.xscale = x.scale, e.wscale = w.scale;
         e.v0 = i * piece, e.vn = std::min(piece, c.V - e.v0);
-        e.dz = static_cast<__nv_bfloat16*>(o[1]->raw()), e.dz_pitch = width;
-        e.dbparts = c.dbias ? o[3]->data() : nullptr;
-        e.dxparts = o[2]->data(), e.dx_add = i > 0;
+        e.dz = static_cast<__nv_bfloat16*>(o[0]->raw()), e.dz_pitch = width;
+        e.dbparts = c.dbias ? o[2]->data() : nullptr;
+        e.dxparts = o[1]->data(), e.dx_add = i > 0;
         e.dw = c.dw, e.dw_bf16 = c.dtype == RG_DTYPE_BF16;
         e.nprobs = 1;
         e.p[0] = lt_problem(c.R, e.vn, c.D, LT_BN, 0, 1);
@@ -994,7 +1022,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.p[1] = lt_problem(e.vn, c.D, c.R, bn, 1, 1);
         RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
     }
-    lce_dx_finish_launch(ctx, o[2]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
-    if (c.dbias) lce_dbias_finish_launch(ctx, o[3]->data(), dbrows, c.V, c.scal, c.dbias);
+    lce_dx_finish_launch(ctx, o[1]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
+    if (c.dbias) lce_dbias_finish_launch(ctx, o[2]->data(), dbrows, c.V, c.scal, c.dbias);
     return RG_OK;
 }

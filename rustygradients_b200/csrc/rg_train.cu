@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kerne
     for (int j = 0; j < PER; j++)
 #pragma unroll
         for (int i = 0; i < VEC; i++) dg[j][i] = db[j][i] = 0.f;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over the CTAs waits for all of this kernel
     const float inv_n = 1.f / (float)n;
     long long row = (long long)blockIdx.x * GROUPS + group;
     V nx[PER], ng[PER];
@@ -307,6 +308,7 @@ __global__ void __launch_bounds__(256) rg_ln_bwd_long_cols_kernel(const T* __res
 __global__ void __launch_bounds__(1024) rg_colsum_kernel(const float* __restrict__ parts, int nparts, long long cols,
                                                          float* __restrict__ out0, float* __restrict__ out1, long long split) {
     __shared__ float red[32][33];
+    rg_pdl_sync();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const long long c = (long long)blockIdx.x * 32 + lane;
     float s = 0.f;
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(1024) rg_colsum_kernel(const float* __restrict
 }
 
 void rg_colsum_launch(rg_ctx* ctx, const float* parts, int nparts, long long cols, float* out0, float* out1, long long split) {
-    rg_colsum_kernel<<<rg_cdiv(cols, 32), 1024, 0, ctx->stream>>>(parts, nparts, cols, out0, out1, split);
+    rg_launch(true, rg_colsum_kernel, dim3((unsigned)rg_cdiv(cols, 32)), dim3(1024), 0, ctx->stream, parts, nparts, cols, out0, out1, split);
     RG_LAUNCHED(ctx);
 }
 
@@ -577,6 +579,7 @@ __device__ __forceinline__ void clip_add8(double& acc, const float (&v)[8]) {
 
 __global__ void __launch_bounds__(256) rg_clip_sumsq_kernel(const __grid_constant__ clip_table t, double* __restrict__ parts) {
     __shared__ double red[8];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     double acc = 0.0;
     for (int p = blockIdx.x; p < t.pieces; p += gridDim.x) {
         const clip_entry& e = t.e[clip_find(t, p)];
@@ -628,6 +631,7 @@ __global__ void __launch_bounds__(256) rg_clip_sumsq_kernel(const __grid_constan
 __global__ void __launch_bounds__(256) rg_clip_scale_kernel(const __grid_constant__ clip_table t, const double* __restrict__ parts,
                                                             int nparts, float max_norm, float* __restrict__ norm_out) {
     __shared__ double red[8];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     double s = 0.0;
     for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
     s = clip_block_sum(s, red);
@@ -721,8 +725,9 @@ extern "C" rg_status rg_clip_grad_norm(rg_ctx* ctx, const rg_storage* const* gra
             rg_clip_sumsq_kernel<<<ctas[k], 256, 0, ctx->stream>>>(tables[k], parts + at);
             at += ctas[k];
         }
-        for (size_t k = tables.size(); k-- > 0;)
-            rg_clip_scale_kernel<<<ctas[k], 256, 0, ctx->stream>>>(tables[k], parts, nparts, max_norm, k ? nullptr : o[0]->data());
+        for (size_t k = tables.size(); k-- > 0;)  // the first one follows the sums directly and may start early
+            rg_launch(k + 1 == tables.size(), rg_clip_scale_kernel, dim3(ctas[k]), dim3(256), 0, ctx->stream, tables[k], (const double*)parts, nparts,
+                      max_norm, k ? nullptr : o[0]->data());
         ctx->launches += 2 * tables.size();
         RG_CUDA(cudaGetLastError());
         for (size_t i = 0; i < n; i++) out[i] = made[i].release();
