@@ -274,6 +274,30 @@ __device__ __forceinline__ void rg_pdl_sync() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Two f32 operations in one instruction.
+union rg_pair {
+    float2 f;
+    unsigned long long u;
+};
+__device__ __forceinline__ float2 rg_fma2(float2 a, float2 b, float2 c) {
+    rg_pair x, y, z;
+    x.f = a, y.f = b, z.f = c;
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(z.u) : "l"(x.u), "l"(y.u));
+    return z.f;
+}
+__device__ __forceinline__ float2 rg_mul2(float2 a, float2 b) {
+    rg_pair x, y, z;
+    x.f = a, y.f = b;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(z.u) : "l"(x.u), "l"(y.u));
+    return z.f;
+}
+__device__ __forceinline__ float2 rg_add2(float2 a, float2 b) {
+    rg_pair x, y, z;
+    x.f = a, y.f = b;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(z.u) : "l"(x.u), "l"(y.u));
+    return z.f;
+}
+
 __device__ __forceinline__ float rg_to_float(float v) { return v; }
 __device__ __forceinline__ float rg_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T>

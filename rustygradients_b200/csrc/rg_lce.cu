@@ -226,14 +226,6 @@ __device__ __forceinline__ void lce_rows(const float* p, float (&v)[RB]) {
     }
 }
 
-// Two f32 products and additions in one instruction.
-__device__ __forceinline__ float2 lce_fma2(float2 a, float2 b, float2 c) {
-    union U { float2 f; unsigned long long u; } x, y, z;
-    x.f = a, y.f = b, z.f = c;
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(z.u) : "l"(x.u), "l"(y.u));
-    return z.f;
-}
-
 #define LCE_COLS 124
 template <typename T, int RB>
 struct lce_few {
@@ -309,7 +301,7 @@ __device__ __forceinline__ void lce_few_logits(const lce_call& c, unsigned char*
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if constexpr (RB == 1) acc[0][j].x = fmaf(xv[0], wv[j], acc[0][j].x);
-                    else acc[i][j] = lce_fma2(make_float2(xv[2 * i], xv[2 * i + 1]), make_float2(wv[j], wv[j]), acc[i][j]);
+                    else acc[i][j] = rg_fma2(make_float2(xv[2 * i], xv[2 * i + 1]), make_float2(wv[j], wv[j]), acc[i][j]);
                 }
         }
     }
@@ -465,8 +457,8 @@ __global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, con
             float2 s = make_float2(0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                o[j] = lce_fma2(xp, g[i][j], o[j]);
-                s = lce_fma2(g[i][j], make_float2(wv[j], wv[j]), s);
+                o[j] = rg_fma2(xp, g[i][j], o[j]);
+                s = rg_fma2(g[i][j], make_float2(wv[j], wv[j]), s);
             }
             q[2 * i] = s.x, q[2 * i + 1] = s.y;
         }

@@ -159,30 +159,31 @@ __global__ void __launch_bounds__(512) rg_ln_fwd_long_kernel(const T* __restrict
         y[(long long)blockIdx.x * n + c] = rg_from_float<T>((rg_to_float(xr[c]) - mean) * rstd * gamma[c] + beta[c]);
 }
 
-// Resident CTAs per SM of the gradient: registers for 8 values a thread (two column sums, this row and the next one)
-#define LN_BWD_CTAS(threads) ((threads) == 256 ? 2 : 1)
+__device__ __forceinline__ float ln_half(float2 v, int i) { return i & 1 ? v.y : v.x; }
+
+// Resident CTAs per SM of the gradient: registers for 8 or 16 values a thread (two column sums, this row and the next one)
+#define LN_BWD_CTAS(threads, values) ((threads) == 256 ? ((values) == 8 ? 3 : 2) : 1)
 
 // dx = rstd (a - mean(a) - xh mean(a xh)), and the two column sums dgamma = sum dy xh, dbeta = sum dy.  One read of dy and
 // x serves all three: a group walks rows, every thread always on the same columns, so the column sums stay in its registers
 // until the end; then the CTA's groups are added and the CTA leaves one partial row of sums, which rg_colsum_kernel adds over
 // the CTAs.  Memory bound: dy and x in, dx out; the next row's loads are in flight behind the sums of this one.
 template <typename T, int VEC, int PER, int WPR, int THREADS>
-__global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+__global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS, PER * VEC)) rg_ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                             const float* __restrict__ gamma, const float* __restrict__ mean,
                                                             const float* __restrict__ rstd, T* __restrict__ dx,
                                                             float* __restrict__ parts, long long rows, int n) {
     constexpr int GROUPS = THREADS / 32 / WPR, COLS = 32 * WPR * PER * VEC;
+    constexpr int PAIRS = PER * VEC / 2;     // value e of a thread (vector e / VEC) is half e % 2 of pair e / 2
     constexpr bool AHEAD = PER * VEC <= 16;  // room in the registers for the next row
     typedef typename ln_vec<T, VEC>::type V;
     __shared__ float2 red[2][GROUPS][WPR];
     __shared__ float comb[GROUPS > 1 ? GROUPS * COLS : 1];
     const int group = threadIdx.x / (32 * WPR), t = threadIdx.x % (32 * WPR), gwarp = t >> 5;
     const long long step = (long long)gridDim.x * GROUPS;
-    float dg[PER][VEC], db[PER][VEC];
+    float2 dg[PAIRS], db[PAIRS];
 #pragma unroll
-    for (int j = 0; j < PER; j++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) dg[j][i] = db[j][i] = 0.f;
+    for (int i = 0; i < PAIRS; i++) dg[i] = db[i] = make_float2(0.f, 0.f);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over the CTAs waits for all of this kernel
     const float inv_n = 1.f / (float)n;
     long long row = (long long)blockIdx.x * GROUPS + group;
@@ -203,41 +204,46 @@ __global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kerne
     if (AHEAD) fetch(row);
     for (int turn = 0; row < rows; row += step, turn ^= 1) {
         if (!AHEAD) fetch(row);
-        float xv[PER][VEC], gv[PER][VEC];
+        float2 xv[PAIRS], gv[PAIRS];
         const float m = nm, r = nr;
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int c = (t + j * 32 * WPR) * VEC;
-            const T *ex = reinterpret_cast<const T*>(&nx[j]), *eg = reinterpret_cast<const T*>(&ng[j]);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) xv[j][i] = c < n ? rg_to_float(ex[i]) : m, gv[j][i] = c < n ? rg_to_float(eg[i]) : 0.f;
+        for (int e = 0; e < PER * VEC; e++) {
+            const bool in = (t + e / VEC * 32 * WPR) * VEC < n;
+            const float a = in ? rg_to_float(reinterpret_cast<const T*>(&nx[e / VEC])[e % VEC]) : m;
+            const float b = in ? rg_to_float(reinterpret_cast<const T*>(&ng[e / VEC])[e % VEC]) : 0.f;
+            if (e % 2) xv[e / 2].y = a, gv[e / 2].y = b;
+            else xv[e / 2].x = a, gv[e / 2].x = b;
         }
         if (AHEAD) fetch(row + step);
-        float s1 = 0.f, s2 = 0.f;
+        float gm[PER][VEC];
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int c = (t + j * 32 * WPR) * VEC;
-            float gm[VEC];
-            ln_param<VEC>(gamma + (c < n ? c : 0), gm);  // dy is 0 beyond the row
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float xh = (xv[j][i] - m) * r;
-                db[j][i] += gv[j][i];
-                dg[j][i] += gv[j][i] * xh;
-                const float a = gv[j][i] * gm[i];
-                s1 += a, s2 += a * xh;
-                xv[j][i] = xh, gv[j][i] = a;
-            }
+            ln_param<VEC>(gamma + (c < n ? c : 0), gm[j]);  // dy is 0 beyond the row
         }
-        const float2 s = ln_group_sum<WPR>(s1, s2, red[turn][group], group, gwarp);
-        s1 = s.x * inv_n, s2 = s.y * inv_n;
+        const float2 m2 = make_float2(-m, -m), r2 = make_float2(r, r);
+        float2 s1 = make_float2(0.f, 0.f), s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) {
+            const float2 xh = rg_mul2(rg_add2(xv[i], m2), r2), g = gv[i];
+            db[i] = rg_add2(db[i], g);
+            dg[i] = rg_fma2(g, xh, dg[i]);
+            const float2 a = rg_mul2(g, make_float2(gm[2 * i / VEC][2 * i % VEC], gm[(2 * i + 1) / VEC][(2 * i + 1) % VEC]));
+            s1 = rg_add2(s1, a), s2 = rg_fma2(a, xh, s2);
+            xv[i] = xh, gv[i] = a;
+        }
+        const float2 s = ln_group_sum<WPR>(s1.x + s1.y, s2.x + s2.y, red[turn][group], group, gwarp);
+        const float2 k1 = make_float2(-s.x * inv_n, -s.x * inv_n), k2 = make_float2(-s.y * inv_n, -s.y * inv_n);
+#pragma unroll
+        for (int i = 0; i < PAIRS; i++) gv[i] = rg_mul2(r2, rg_fma2(xv[i], k2, rg_add2(gv[i], k1)));
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int c = (t + j * 32 * WPR) * VEC;
             if (c < n) {
+                float o[VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; i++) gv[j][i] = r * (gv[j][i] - s1 - xv[j][i] * s2);
-                ln_store<T, VEC>(dx + row * n + c, gv[j]);
+                for (int i = 0; i < VEC; i++) o[i] = ln_half(gv[(j * VEC + i) / 2], j * VEC + i);
+                ln_store<T, VEC>(dx + row * n + c, o);
             }
         }
     }
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kerne
 #pragma unroll
             for (int j = 0; j < PER; j++)
 #pragma unroll
-                for (int i = 0; i < VEC; i++) comb[group * COLS + (t + j * 32 * WPR) * VEC + i] = which ? db[j][i] : dg[j][i];
+                for (int i = 0; i < VEC; i++) comb[group * COLS + (t + j * 32 * WPR) * VEC + i] = ln_half(which ? db[(j * VEC + i) / 2] : dg[(j * VEC + i) / 2], j * VEC + i);
             __syncthreads();
             for (int c = threadIdx.x; c < n; c += THREADS) {
                 float s = 0.f;
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS)) rg_ln_bwd_kerne
                 const int c = (t + j * 32 * WPR) * VEC;
                 if (c < n)
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) out[which * n + c + i] = which ? db[j][i] : dg[j][i];
+                    for (int i = 0; i < VEC; i++) out[which * n + c + i] = ln_half(which ? db[(j * VEC + i) / 2] : dg[(j * VEC + i) / 2], j * VEC + i);
             }
         }
     }
@@ -362,7 +368,7 @@ static void ln_launch_one(rg_ctx* ctx, const ln_args& a, int* nparts) {
         rg_ln_fwd_kernel<T, VEC, PER, WPR, THREADS><<<grid, THREADS, 0, ctx->stream>>>(
             (const T*)a.x, a.gamma, a.beta, (T*)a.out, a.mean_out, a.rstd_out, a.rows, a.n, a.eps);
     } else {
-        *nparts = (int)std::min<long long>(groups, (long long)ctx->sm_count * LN_BWD_CTAS(THREADS));
+        *nparts = (int)std::min<long long>(groups, (long long)ctx->sm_count * LN_BWD_CTAS(THREADS, PER * VEC));
         if (!a.parts) return;  // the caller asks for the number of partial rows first
         rg_ln_bwd_kernel<T, VEC, PER, WPR, THREADS><<<*nparts, THREADS, 0, ctx->stream>>>((const T*)a.dy, (const T*)a.x, a.gamma, a.mean,
                                                                                          a.rstd, (T*)a.out, a.parts, a.rows, a.n);
@@ -370,16 +376,17 @@ static void ln_launch_one(rg_ctx* ctx, const ln_args& a, int* nparts) {
     RG_LAUNCHED(ctx);
 }
 
-// Values per thread: 8 in the gradient (two column sums each stay in registers), up to 32 forward; more only where a group
-// is the whole CTA.
+// Values per thread of the gradient (16384 x 1600, us with the column sums): f32 8 64, 16 67; bf16 8 46, 16 40; rows that
+// allow only single-value loads 8 (32000 x 767: 54 against 81).  Forward up to 32.  More only where a group is the whole CTA.
 template <bool BWD, typename T, int VEC>
 static void ln_launch_vec(rg_ctx* ctx, const ln_args& a, int* nparts) {
     constexpr int P = 8 / VEC;
     if constexpr (BWD) {
+        constexpr int Q = sizeof(T) == 2 && VEC > 1 ? 2 : 1;  // 8 Q values, 256 Q columns a warp
         if (a.n <= 256) ln_launch_one<true, T, VEC, P, 1, 256>(ctx, a, nparts);
-        else if (a.n <= 512) ln_launch_one<true, T, VEC, 2 * P, 1, 256>(ctx, a, nparts);
-        else if (a.n <= 1024) ln_launch_one<true, T, VEC, 2 * P, 2, 256>(ctx, a, nparts);
-        else if (a.n <= 2048) ln_launch_one<true, T, VEC, 2 * P, 4, 256>(ctx, a, nparts);
+        else if (a.n <= 512) ln_launch_one<true, T, VEC, Q * P, 2 / Q, 256>(ctx, a, nparts);
+        else if (a.n <= 1024) ln_launch_one<true, T, VEC, Q * P, 4 / Q, 256>(ctx, a, nparts);
+        else if (a.n <= 2048) ln_launch_one<true, T, VEC, Q * P, 8 / Q, 256>(ctx, a, nparts);
         else if (a.n <= 4096) ln_launch_one<true, T, VEC, 2 * P, 8, 256>(ctx, a, nparts);
         else if (a.n <= 8192) ln_launch_one<true, T, VEC, 2 * P, 16, 512>(ctx, a, nparts);
         else ln_launch_one<true, T, VEC, 4 * P, 16, 512>(ctx, a, nparts);
