@@ -21,9 +21,9 @@
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
 // The tensor core truncates when it adds to its f32 accumulator, so a long chain loses about 2^-25 of the running sum per
 // step (measured: a relative error of 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32 inputs the chain is
-// therefore cut after every k-block of 64: its small products come first and that of the leading planes last, and the
-// epilogue warps add the block to their f32 registers with rounding (64 or 128 additions a thread in the 1536 cycles that a
-// block's products take).
+// therefore cut after every two k-blocks of 64: in each the small products come first and that of the leading planes last, and
+// the epilogue warps add the result to their f32 registers with rounding.  (A cut after every block: 907 instead of 852 us for
+// the loss of 4096x768x50257.)
 #include "rg_lce.cuh"
 
 #include <cuda.h>
@@ -33,6 +33,7 @@
 
 #define LT_BM 256  // rows of a tile: 128 in each CTA of a pair
 #define LT_BK 64
+#define LT_CHAIN 2  // k-blocks per accumulator for f32 inputs
 #define LT_SPIN_LIMIT (1u << 22)
 #define LT_STAGE_ALL 196608   // bytes of the operand ring
 #define LT_MAX_STAGES 6
@@ -116,10 +117,12 @@ __device__ __forceinline__ void lt_arrive_at(uint32_t cluster_addr) {
 __device__ __forceinline__ void lt_publish_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// e^(v - ref): two roundings of the argument (2^-24 of |v - ref| each) and the 2 steps of the exponential instruction
-__device__ __forceinline__ float lt_exp(float d) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.44269504088896341f));
+// e^(v + less) of two values: two roundings of the argument (2^-24 of it each) and the 2 steps of the exponential instruction
+__device__ __forceinline__ float2 lt_exp2(float2 v, float2 less) {
+    const float2 t = rg_mul2(rg_add2(v, less), make_float2(1.44269504088896341f, 1.44269504088896341f));
+    float2 r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(t.y));
     return r;
 }
 template <bool CLUSTER = false>
@@ -286,14 +289,18 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
             for (int j = 4; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
             const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const float ref = m == -INFINITY ? 0.f : m;
-            float s[4] = {w.ms.s * lt_exp(w.ms.m - ref), 0.f, 0.f, 0.f};
+            const float2 less = make_float2(-ref, -ref);
+            float2 s[2] = {make_float2(w.ms.s * lt_exp2(make_float2(w.ms.m, w.ms.m), less).x, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 32; j++) s[j & 3] += lt_exp(v[j] - ref);
-            w.ms = {m, (s[0] + s[1]) + (s[2] + s[3])};
+            for (int j = 0; j < 32; j += 2) s[(j >> 1) & 1] = rg_add2(s[(j >> 1) & 1], lt_exp2(make_float2(v[j], v[j + 1]), less));
+            w.ms = {m, (s[0].x + s[0].y) + (s[1].x + s[1].y)};
         } else {
             const bool dead = !w.live || w.tgt < 0;
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = (dead || j >= left) ? 0.f : lt_exp(v[j] - w.lse);
+            for (int j = 0; j < 32; j += 2) {
+                const float2 p = lt_exp2(make_float2(v[j], v[j + 1]), make_float2(-w.lse, -w.lse));
+                v[j] = (dead || j >= left) ? 0.f : p.x, v[j + 1] = (dead || j + 1 >= left) ? 0.f : p.y;
+            }
             if (any && here) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
@@ -529,15 +536,15 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t idesc = (1u << 4) | (PLANES == 2 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
                                        ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
-                // bf16: one accumulator for all of K; f32: one per k-block
-                const int segs = PLANES == 1 ? 1 : nkb;
+                // bf16: one accumulator for all of K; f32: one per LT_CHAIN k-blocks
+                const int segs = PLANES == 1 ? 1 : (nkb + LT_CHAIN - 1) / LT_CHAIN;
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
                     const uint32_t buf = seg % S::BUFFERS;
                     ok = lt_wait(&acc_empty[buf], ((seg / S::BUFFERS) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d = tmem + buf * S::BN;
-                    for (int kb = 0; kb < (PLANES == 1 ? nkb : 1); kb++, it++) {
+                    for (int kb = 0; kb < (PLANES == 1 ? nkb : min(LT_CHAIN, nkb - sg * LT_CHAIN)); kb++, it++) {
                         const int s = it % S::STAGES;
                         ok = lt_wait(&full[s], (it / S::STAGES) & 1u, e.err);
                         if (!ok) break;
@@ -595,8 +602,13 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] * e.wscale[0] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
-            const int segs = PLANES == 1 ? 1 : nkb;
+            const int segs = PLANES == 1 ? 1 : (nkb + LT_CHAIN - 1) / LT_CHAIN;
             float acc[PLANES == 1 ? 2 : HALF / 32][32];
+            if (PLANES != 1)
+#pragma unroll
+                for (int c = 0; c < HALF / 32; c++)
+#pragma unroll
+                    for (int j = 0; j < 32; j++) acc[c][j] = 0.f;
             for (int sg = 0; sg < segs; sg++, seg++) {
                 const uint32_t buf = seg % S::BUFFERS;
                 ok = lt_wait(&acc_full[buf], (seg / S::BUFFERS) & 1u, e.err);
@@ -632,7 +644,10 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 #pragma unroll
                         for (int h = 0; h < 2; h++)
 #pragma unroll
-                            for (int j = 0; j < 32; j++) acc[c + h][j] = sg ? acc[c + h][j] + block[h][j] : block[h][j];
+                            for (int j = 0; j < 32; j += 2) {
+                                const float2 t = rg_add2(make_float2(acc[c + h][j], acc[c + h][j + 1]), make_float2(block[h][j], block[h][j + 1]));
+                                acc[c + h][j] = t.x, acc[c + h][j + 1] = t.y;
+                            }
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
