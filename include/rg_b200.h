@@ -59,7 +59,7 @@ RG_API rg_status rg_ctx_create(int device, rg_ctx** out);
 /* The same on a stream of the caller (a cudaStream_t of that device, NULL for its default stream), for the ops of this
  * header next to another owner of the GPU: every call enqueues on it, so arrays of that owner that are ordered on the
  * stream need no further synchronisation in either direction.  The stream must outlive the context and its storages.
- * rg_gpt_create refuses such a context (RG_ERR_UNSUPPORTED). */
+ * Ops are not captured into a graph there, and rg_gpt_create refuses such a context (RG_ERR_UNSUPPORTED both). */
 RG_API rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** out);
 RG_API rg_status rg_ctx_destroy(rg_ctx* ctx);
 /* Backend::synchronize, src/backend/mod.rs:137-138 */
@@ -140,7 +140,8 @@ RG_API rg_status rg_sparse_cross_entropy(rg_ctx* ctx, const rg_storage* logits, 
  * clipping.  Activations and matrices are f32 or bf16 (one type per call where not said otherwise); LayerNorm parameters,
  * biases, targets, statistics, losses and their gradients are f32, as in bf16-weight mode of the model below.  Every sum and
  * statistic is held in 32 bits or more; results do not depend on timing (no atomics on values).  These calls are not
- * enqueued into a stream capture (RG_ERR_UNSUPPORTED). ------------------------------------------------------------- */
+ * enqueued into a stream capture (RG_ERR_UNSUPPORTED).  A device-side wait that gives up is reported by the next
+ * synchronising call (rg_synchronize, rg_to_vec: RG_ERR_TIMEOUT). -------------------------------------------------- */
 /* layer_norm that keeps its statistics for the gradient: y as rg_layer_norm (type of x), mean and rstd = 1/sqrt(var + eps)
  * f32, one per row (the leading axes of x).  No row is not an error; an empty last axis is RG_ERR_SHAPE. */
 RG_API rg_status rg_layer_norm_fwd(rg_ctx* ctx, const rg_storage* x, const rg_storage* gamma, const rg_storage* beta, float epsilon,

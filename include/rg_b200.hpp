@@ -65,6 +65,7 @@ class Storage {
         return std::vector<size_t>(buf, buf + nd);
     }
     size_t len() const { return rg_storage_len(h_.get()); }
+    bool is_bf16() const { return rg_storage_dtype(h_.get()) == RG_DTYPE_BF16; }
 
   private:
     std::shared_ptr<rg_storage> h_;
@@ -76,6 +77,12 @@ class B200Backend {
     explicit B200Backend(int device_index = 0) : index_(device_index) {
         rg_ctx* c = nullptr;
         check(rg_ctx_create(device_index, &c));
+        ctx_.reset(c, [](rg_ctx* p) { rg_ctx_destroy(p); });
+    }
+    // on a cudaStream_t of the caller (nullptr: the default stream) instead of a stream of its own
+    B200Backend(int device_index, void* stream) : index_(device_index) {
+        rg_ctx* c = nullptr;
+        check(rg_ctx_create_on_stream(device_index, stream, &c));
         ctx_.reset(c, [](rg_ctx* p) { rg_ctx_destroy(p); });
     }
     static int device_count() { return rg_device_count(); }
@@ -115,6 +122,52 @@ class B200Backend {
     Storage transpose(const Storage& a, size_t ax1, size_t ax2) const { return make([&](rg_storage** o) { return rg_transpose(ctx_.get(), a.get(), ax1, ax2, o); }); }
     Storage layer_norm(const Storage& x, const Storage& gamma, const Storage& beta, float eps) const {
         return make([&](rg_storage** o) { return rg_layer_norm(ctx_.get(), x.get(), gamma.get(), beta.get(), eps, o); });
+    }
+
+    // values as RG_DTYPE_F32 or RG_DTYPE_BF16; a storage over device memory of the caller
+    Storage cast(const Storage& a, int dtype) const { return make([&](rg_storage** o) { return rg_cast(ctx_.get(), a.get(), dtype, o); }); }
+    Storage from_device(void* data, int dtype, const std::vector<size_t>& shape) const {
+        return make([&](rg_storage** o) { return rg_from_device(ctx_.get(), data, dtype, shape.data(), (int)shape.size(), o); });
+    }
+
+    // training ops (the steps of train_step, src/wasm_api.rs:62-94, behind the last block)
+    struct LayerNorm { Storage y, mean, rstd; };
+    struct LayerNormGrad { Storage dx, dgamma, dbeta; };
+    struct Loss { Storage loss, lse; };
+    struct LossGrad { Storage dx, dw, dbias; };  // dbias is empty without a bias
+    LayerNorm layer_norm_fwd(const Storage& x, const Storage& gamma, const Storage& beta, float eps) const {
+        rg_storage *y = nullptr, *m = nullptr, *r = nullptr;
+        check(rg_layer_norm_fwd(ctx_.get(), x.get(), gamma.get(), beta.get(), eps, &y, &m, &r));
+        return {Storage(y), Storage(m), Storage(r)};
+    }
+    LayerNormGrad layer_norm_bwd(const Storage& dy, const Storage& x, const Storage& gamma, const Storage& mean, const Storage& rstd) const {
+        rg_storage *dx = nullptr, *dg = nullptr, *db = nullptr;
+        check(rg_layer_norm_bwd(ctx_.get(), dy.get(), x.get(), gamma.get(), mean.get(), rstd.get(), &dx, &dg, &db));
+        return {Storage(dx), Storage(dg), Storage(db)};
+    }
+    // bias: nullptr for none
+    Loss linear_cross_entropy(const Storage& x, const Storage& w, const Storage* bias, const Storage& targets, int64_t ignore_index = -100) const {
+        rg_storage *loss = nullptr, *lse = nullptr;
+        check(rg_linear_cross_entropy(ctx_.get(), x.get(), w.get(), bias ? bias->get() : nullptr, targets.get(), ignore_index, &loss, &lse));
+        return {Storage(loss), Storage(lse)};
+    }
+    LossGrad linear_cross_entropy_bwd(const Storage& x, const Storage& w, const Storage* bias, const Storage& targets, const Storage& lse,
+                                      const Storage* dloss = nullptr, int64_t ignore_index = -100) const {
+        rg_storage *dx = nullptr, *dw = nullptr, *db = nullptr;
+        check(rg_linear_cross_entropy_bwd(ctx_.get(), x.get(), w.get(), bias ? bias->get() : nullptr, targets.get(), ignore_index, lse.get(),
+                                          dloss ? dloss->get() : nullptr, &dx, &dw, bias ? &db : nullptr));
+        return {Storage(dx), Storage(dw), db ? Storage(db) : Storage()};
+    }
+    // {clipped gradients, norm}
+    std::pair<std::vector<Storage>, Storage> clip_grad_norm(const std::vector<Storage>& grads, float max_norm) const {
+        std::vector<const rg_storage*> in;
+        for (const Storage& g : grads) in.push_back(g.get());
+        std::vector<rg_storage*> out(grads.size(), nullptr);
+        rg_storage* norm = nullptr;
+        check(rg_clip_grad_norm(ctx_.get(), in.data(), in.size(), max_norm, out.data(), &norm));
+        std::vector<Storage> clipped;
+        for (rg_storage* p : out) clipped.emplace_back(p);
+        return {std::move(clipped), Storage(norm)};
     }
 
   private:

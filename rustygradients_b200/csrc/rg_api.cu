@@ -41,7 +41,7 @@ rg_devbuf::~rg_devbuf() {
     bool done = false;
     if (life && life->alive) {
         cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
+        if (!captured && (cudaStreamIsCapturing(stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)) {
             cudaGetLastError();
             life->parked.push_back(ptr);
             done = true;
@@ -184,6 +184,12 @@ rg_status rg_need_f32(const char* op, const rg_storage* a, const rg_storage* b, 
 
 rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storage** out, int dtype) {
     if (ndim < 0 || ndim > 8) return rg_fail(RG_ERR_DIMENSION, "storage rank %d not in 0..8", ndim);
+    // A buffer that a graph writes at every replay cannot be one that is handed out again: on a caller's stream nothing of this
+    // library is captured.
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    const bool capturing = cudaStreamIsCapturing(ctx->stream, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone;
+    if (capturing) cudaGetLastError();
+    if (capturing && !ctx->own_stream) return rg_fail(RG_ERR_UNSUPPORTED, "ops are not enqueued into a capture of the caller's stream");
     return rg_no_throw([&] {
         std::unique_ptr<rg_storage> s(new rg_storage());
         s->ctx = ctx;
@@ -195,7 +201,8 @@ rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storag
         s->buf->bytes = (s->len ? s->len : 1) * rg_dtype_size(dtype);
         s->buf->stream = ctx->stream;
         s->buf->life = ctx->life;
-        if (s->buf->bytes <= RG_SMALL_MAX) {
+        s->buf->captured = capturing;
+        if (s->buf->bytes <= RG_SMALL_MAX && !capturing) {
             int k = 0;
             while (((size_t)1 << (RG_SMALL_MIN_LOG2 + k)) < s->buf->bytes) k++;
             s->buf->small = k;

@@ -84,6 +84,7 @@ struct rg_devbuf {
     int device = 0;
     cudaStream_t stream = nullptr;
     int small = -1;         // size class of a small buffer
+    bool captured = false;  // allocated inside a stream capture: its free belongs there too
     bool borrowed = false;  // the caller's memory (rg_from_device): never freed here
     std::shared_ptr<rg_ctx_life> life;
     ~rg_devbuf();  // the caller holds life->mu

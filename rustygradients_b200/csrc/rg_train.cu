@@ -492,7 +492,8 @@ extern "C" rg_status rg_layer_norm_bwd(rg_ctx* ctx, const rg_storage* dy, const 
         memset(&a, 0, sizeof(a));
         a.x = x->raw(), a.dy = dy->raw(), a.gamma = gamma->data(), a.mean = mean->data(), a.rstd = rstd->data(), a.out = o[0]->raw();
         a.rows = (long long)rows, a.n = (int)n;
-        int nparts = (int)std::min<size_t>(rows, 64);
+        // long rows: slices of the rows until the blocks of 256 columns fill the GPU
+        int nparts = (int)std::min<size_t>({rows, 64, std::max<size_t>(1, (size_t)ctx->sm_count * 8 * 256 / n)});
         if (n <= LN_MAX_N) ln_launch<true>(ctx, a, x->dtype, &nparts);  // a.parts is NULL: only counts
         const size_t pshape[2] = {(size_t)nparts, 2 * n};
         RG_TRY(rg_alloc_storage(ctx, pshape, 2, &o[3]));

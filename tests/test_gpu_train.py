@@ -132,7 +132,7 @@ def test_calls_inside_a_capture_are_refused():
             a.add_(1)
             for call in (lambda: be.layer_norm_fwd(x, g, g, EPS), lambda: be.layer_norm_bwd(y, x, g, m, r),
                          lambda: be.linear_cross_entropy(x, w, None, t), lambda: be.linear_cross_entropy_bwd(x, w, None, t, t),
-                         lambda: be.clip_grad_norm([x], 1.0)):
+                         lambda: be.clip_grad_norm([x], 1.0), lambda: be.add(x, x), lambda: be.cast(x, "bf16"), lambda: be.ones([3])):
                 with pytest.raises(rg.Unsupported):
                     call()
             del dead      # its memory is given back after the capture
@@ -614,3 +614,50 @@ def test_linear_cross_entropy_gives_the_same_bits_again(backend):
             loss, lse2 = be.linear_cross_entropy(X, W, B, T)
             again = [be.to_vec(s) for s in (loss, lse2, *be.linear_cross_entropy_bwd(X, W, B, T, lse))]
             assert all(np.array_equal(p, q) for p, q in zip(first, again))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [12, 96])
+def test_training_step_behind_the_last_block(backend, rows, dtype):
+    """Final LayerNorm -> LM head with its loss -> gradients -> clipping of all of them, as WasmGptTrainer::train_step runs them,
+    against the formulas in 64 bits, and against differences of the whole loss."""
+    be = backend
+    D, V, max_norm = 64, 333, 0.05
+    h, _, g, b = ln_inputs(rows, D, dtype, 40)
+    _, w, bias, t = ce_inputs(rows, D, V, dtype, True, 0.25, 41)
+    H, W, G, B, BI, T = put(be, h, dtype), put(be, w, dtype), put(be, g), put(be, b), put(be, bias), put(be, t)
+    y, mean, rstd = be.layer_norm_fwd(H, G, B, EPS)
+    loss, lse = be.linear_cross_entropy(y, W, BI, T)
+    dy, dw, dbias = be.linear_cross_entropy_bwd(y, W, BI, T, lse)
+    dh, dg, db = be.layer_norm_bwd(dy, H, G, mean, rstd)
+    clipped, norm = be.clip_grad_norm([dh, dg, db, dw, dbias], max_norm)
+
+    def total(h_, g_, b_, w_, bi_):
+        return ce_exact(ln_exact(h_, g_, b_)[0], w_, bi_, t)["loss"]
+
+    wy, wm, wr = ln_exact(h, g, b)
+    ex = ce_exact(wy, w, bias, t)
+    xh = (h - wm) * wr
+    a = ex["dx"] * g
+    want = [wr * (a - a.mean(-1, keepdims=True) - xh * (a * xh).mean(-1, keepdims=True)), (ex["dx"] * xh).sum(0, keepdims=True),
+            ex["dx"].sum(0, keepdims=True), ex["dw"], ex["db"]]
+    # every step rounds its matrices to dtype: y, dz, dx, dw by half a step each, and each of them reaches the gradients once
+    tol = 8 * U[dtype] + 2e-5
+    assert abs(get(be, loss)[0] - ex["loss"]) <= tol * (1 + np.abs(ex["z"]).max())
+    for got, exact, name in zip((dh, dg, db, dw, dbias), want, ("dh", "dgamma", "dbeta", "dw", "dbias")):
+        e = np.linalg.norm(get(be, got).reshape(exact.shape) - exact) / np.linalg.norm(exact)
+        assert e <= tol * (1 + np.abs(ex["z"]).max()), (name, e)
+    n = np.sqrt(sum((e ** 2).sum() for e in want))
+    assert n > max_norm and abs(get(be, norm)[0] / n - 1) <= tol * (1 + np.abs(ex["z"]).max())
+    sq = sum((get(be, c) ** 2).sum() for c in clipped)
+    assert abs(np.sqrt(sq) / max_norm - 1) <= 2 * U[dtype] + 1e-6
+    rng = np.random.default_rng(5)
+    v = [rng.standard_normal(p.shape) for p in (h, g, b, w, bias)]
+    e = 1e-5
+    num = (total(*[p + e * q for p, q in zip((h, g, b, w, bias), v)]) - total(*[p - e * q for p, q in zip((h, g, b, w, bias), v)])) / (2 * e)
+    ana = sum((get(be, got).reshape(q.shape) * q).sum() for got, q in zip((dh, dg, db, dw, dbias), v))
+    size = sum(np.abs(x * q).sum() for x, q in zip(want, v))
+    assert abs(num - ana) <= tol * (1 + np.abs(ex["z"]).max()) * size / 10 + 1e-6

@@ -1,0 +1,98 @@
+"""Host side of the training ops without a GPU: refusals of the C entries, and the number forms the tensor cores get."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from rustygradients_b200 import _lib, build
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+EXE = os.path.join(ROOT, "tests", "cpp", "train_mirror_test")
+
+
+def test_null_arguments_are_refused_before_any_device_call():
+    lib = _lib.load()
+    p = C.c_void_p()
+    ref = C.byref(p)
+    calls = [lambda: lib.rg_cast(None, None, 0, ref), lambda: lib.rg_from_device(None, None, 0, None, 0, ref),
+             lambda: lib.rg_to_dlpack(None, ref), lambda: lib.rg_layer_norm_fwd(None, None, None, None, 1e-5, ref, ref, ref),
+             lambda: lib.rg_layer_norm_bwd(None, None, None, None, None, None, ref, ref, ref),
+             lambda: lib.rg_linear_cross_entropy(None, None, None, None, None, -100, ref, ref),
+             lambda: lib.rg_linear_cross_entropy_bwd(None, None, None, None, None, -100, None, None, ref, ref, ref),
+             lambda: lib.rg_clip_grad_norm(None, None, 0, 1.0, None, ref), lambda: lib.rg_ctx_create_on_stream(0, None, None)]
+    for call in calls:
+        assert call() == _lib.RG_ERR_INVALID_INPUT and lib.rg_last_error()
+    assert lib.rg_storage_dtype(None) == _lib.RG_DTYPE_F32 and lib.rg_storage_free(None) == _lib.RG_OK
+
+
+def test_no_gpu_is_an_error_on_a_caller_stream_too():
+    import rustygradients_b200 as rg
+    if rg.B200Backend.device_count() > 0:
+        pytest.skip("a GPU is present")
+    with pytest.raises(rg.BackendError):
+        rg.B200Backend(0, stream=0)
+
+
+def _bits(a):
+    return np.ascontiguousarray(a, np.float32).view(np.uint32)
+
+
+def test_three_truncated_bf16_planes_hold_an_f32():
+    """What the gradients' products rest on: each plane takes the leading 8 bits of what the planes before leave, exactly."""
+    rng = np.random.default_rng(0)
+    x = np.concatenate([rng.standard_normal(20000) * 10.0 ** rng.integers(-20, 20, 20000), [0.0, 1.0, 3.4028235e38, -3.4028235e38]]).astype(np.float32)
+    rest, planes = x.copy(), []
+    for _ in range(3):
+        hi = (_bits(rest) & 0xFFFF0000).view(np.float32)
+        planes.append(hi)
+        rest = rest - hi
+    assert not rest.any() and np.isfinite(planes).all()
+    assert np.array_equal(sum(p.astype(np.float64) for p in planes), x.astype(np.float64))
+    a, b = rng.permutation(x[:20000]).astype(np.float64), x[:20000].astype(np.float64)
+    pa, pb = [], []
+    for v, out in ((a, pa), (b, pb)):
+        r = v.astype(np.float32)
+        for _ in range(3):
+            hi = (_bits(r) & 0xFFFF0000).view(np.float32)
+            out.append(hi.astype(np.float64))
+            r = r - hi
+    taken = sum(pa[i] * pb[j] for i, j in ((0, 0), (0, 1), (1, 0), (1, 1), (0, 2), (2, 0)))
+    live = np.abs(a * b) > 0
+    assert (np.abs(taken - a * b)[live] <= 2.0 ** -21 * np.abs(a * b)[live]).all()
+
+
+def test_two_scaled_f16_planes_hold_22_bits():
+    """What the logits' products rest on: with the largest magnitude of a group at 2^14..2^15, two f16 are within 2^-22 of a
+    value, or within 2^-40 of the largest one."""
+    rng = np.random.default_rng(1)
+    for scale in (1e-30, 1.0, 1e25):
+        x = (rng.standard_normal(5000) * 10.0 ** rng.uniform(-12, 0, 5000) * scale).astype(np.float32)
+        m = np.abs(x).max()
+        a = 14 - (int(_bits(m)[()] >> 23) - 127) if np.ndim(m) == 0 else None
+        s = x.astype(np.float64) * 2.0 ** a
+        assert 2 ** 14 <= np.abs(s).max() < 2 ** 15
+        hi = s.astype(np.float16)
+        lo = (s - hi.astype(np.float64)).astype(np.float16)
+        err = np.abs(hi.astype(np.float64) + lo.astype(np.float64) - s)
+        assert (err <= np.maximum(2.0 ** -22 * np.abs(s), 2.0 ** -40 * 2 ** 15)).all()
+
+
+def _compile():
+    lib = build.build()
+    cmd = ["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "cpp", "train_mirror_test.cpp"),
+           "-o", EXE, "-L", os.path.dirname(lib), "-lrg_b200", "-Wl,-rpath," + os.path.dirname(lib)]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    return EXE
+
+
+def test_cpp_mirror_of_the_training_ops_compiles():
+    assert os.path.exists(_compile())
+
+
+@pytest.mark.gpu
+def test_cpp_mirror_of_the_training_ops_runs():
+    r = subprocess.run([_compile()], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "OK" in r.stdout, r.stdout + r.stderr
