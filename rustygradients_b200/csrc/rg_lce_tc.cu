@@ -62,7 +62,7 @@ struct lt_prob {
     int M, N, K;
     int tiles_m, tiles_n, splits, kb_per;  // the K axis is cut into `splits` runs of kb_per 64-wide blocks
     int a_mn, b_mn;                        // 1: the M (N) axis is the contiguous one
-    int b_k0, b_n0;                        // where the piece of the vocabulary starts in B
+    int a_k0, b_k0, b_n0;                  // where the piece of the vocabulary starts in A or B
 };
 
 enum { LT_FWD = 0, LT_DZ = 1, LT_GRAD = 2 };
@@ -85,7 +85,9 @@ struct lt_args {
     float* dbparts;           // [LT_BM / 32 * tiles_m][V] or NULL
     float* dxparts;           // LT_GRAD: [splits][R][D]
     int dx_add;               // add to what the pieces before left there
+    int dx_t;                 // the first problem computes dx^T
     void* dw;                 // [D][V]
+    float* dwparts;           // [splits][D][V], or NULL: the second problem's K axis is not cut
     int dw_bf16;
     const float* scal;
 };
@@ -220,8 +222,9 @@ __device__ __forceinline__ lt_tile lt_decode(const lt_args& e, int t) {
         return r;
     }
     if (EPI == LT_GRAD) {  // dw: the column tiles of one row tile together (they share dz)
-        r.prob = 1, r.split = 0, t -= n0;
-        r.n = t % e.p[1].tiles_n, r.m = t / e.p[1].tiles_n;
+        r.prob = 1, t -= n0;
+        r.n = t % e.p[1].tiles_n, t /= e.p[1].tiles_n;
+        r.m = t % e.p[1].tiles_m, r.split = t / e.p[1].tiles_m;
         return r;
     }
     // logits: the row tiles of one column tile together (they share w)
@@ -366,9 +369,14 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
     if (t.prob == 1) {
         // dw^T: the lanes are neighbouring columns of dw, a register is a row of it, so a warp's store is contiguous
         if (!w.live) return;
-        const float scale = e.scal[1];
+        const float scale = e.dwparts ? 1.f : e.scal[1];
         const size_t at = (size_t)col * e.V + e.v0 + w.row;
-        if (e.dw_bf16) {
+        if (e.dwparts) {
+            float* o = e.dwparts + (size_t)t.split * e.D * e.V + at;
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (j < cols) o[(size_t)j * e.V] = v[j];
+        } else if (e.dw_bf16) {
             __nv_bfloat16* o = static_cast<__nv_bfloat16*>(e.dw) + at;
 #pragma unroll
             for (int j = 0; j < 32; j++)
@@ -381,8 +389,16 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
         }
         return;
     }
-    // partial dx: through shared memory, so that a warp stores 32 consecutive columns of one row at a time
     if (cols <= 0) return;
+    if (e.dx_t) {  // the lanes are neighbouring columns of dx
+        if (!w.live) return;
+        float* o = e.dxparts + ((size_t)t.split * e.R + col) * e.D + w.row;
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (j < cols) o[(size_t)j * e.D] = e.dx_add ? o[(size_t)j * e.D] + v[j] : v[j];
+        return;
+    }
+    // partial dx: through shared memory, so that a warp stores 32 consecutive columns of one row at a time
 #pragma unroll
     for (int j = 0; j < 32; j++) stage[lane * 33 + j] = v[j];
     __syncwarp();
@@ -498,7 +514,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                             lt_tma(ma, a + pl * S::A_BYTES, bar, m0, k, pl);
                             lt_tma(ma, a + pl * S::A_BYTES + 8192, bar, m0 + 64, k, pl);
                         } else {
-                            lt_tma(ma, a + pl * S::A_BYTES, bar, k, m0, pl);
+                            lt_tma(ma, a + pl * S::A_BYTES, bar, p.a_k0 + k, m0, pl);
                         }
                         if (p.b_mn) {
 #pragma unroll
@@ -735,7 +751,8 @@ __device__ __forceinline__ void lt_split2(float v, float scale, uint32_t& h0, ui
     h0 = __half_as_ushort(a), h1 = __half_as_ushort(b);
 }
 
-// x as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row, and triples of bf16 (NULL: not wanted).  A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
+// x as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row, and triples of bf16 (either NULL: not wanted).
+// A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
 __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                            uint16_t* __restrict__ pair, uint16_t* __restrict__ triple,
                                                            float* __restrict__ scale_out) {
@@ -744,17 +761,20 @@ __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restri
     if (r >= rows) return;
     const float* p = src + (size_t)r * cols;
     float m = 0.f;
+    if (pair)
 #pragma unroll 8
-    for (int c = lane; c < cols; c += 32) m = fmaxf(m, lt_finite_abs(p[c]));
+        for (int c = lane; c < cols; c += 32) m = fmaxf(m, lt_finite_abs(p[c]));
     const float2 sc = lt_scale(rg_warp_max(m));
-    if (lane == 0) scale_out[r] = sc.y;
+    if (pair && lane == 0) scale_out[r] = sc.y;
     const size_t plane = (size_t)rows * pitch;
 #pragma unroll 4
     for (int c = lane; c < cols; c += 32) {
         const size_t at = (size_t)r * pitch + c;
         uint32_t h0, h1, h2;
-        lt_split2(p[c], sc.x, h0, h1);
-        pair[at] = (uint16_t)h0, pair[at + plane] = (uint16_t)h1;
+        if (pair) {
+            lt_split2(p[c], sc.x, h0, h1);
+            pair[at] = (uint16_t)h0, pair[at + plane] = (uint16_t)h1;
+        }
         if (triple) {
             lt_split3(p[c], h0, h1, h2);
             triple[at] = (uint16_t)h0, triple[at + plane] = (uint16_t)h1, triple[at + 2 * plane] = (uint16_t)h2;
@@ -778,16 +798,16 @@ __global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ s
     if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));  // a maximum: the order does not matter
 }
 
-// w as pairs of f16 with one scale for the whole matrix, and (NULL: not wanted) triples of bf16.  A thread takes 8
+// w as pairs of f16 with one scale for the whole matrix, and triples of bf16, or one of them.  A thread takes 8
 // neighbouring values of a row and writes 16 bytes of each plane.  The values are walked from the end: what the last-level
 // cache still holds of lt_max_kernel's pass is read from there.  Memory bound: 4 bytes in, 4 (10 with the triples) out.
-template <bool TRIPLE>
+template <bool PAIR, bool TRIPLE>
 __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                       const unsigned* __restrict__ largest, uint16_t* __restrict__ pair,
                                                       uint16_t* __restrict__ triple, float* __restrict__ scale_out) {
     rg_pdl_sync();
-    const float2 sc = lt_scale(__uint_as_float(*largest));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *scale_out = sc.y;
+    const float2 sc = PAIR ? lt_scale(__uint_as_float(*largest)) : make_float2(1.f, 1.f);
+    if (PAIR && blockIdx.x == 0 && threadIdx.x == 0) *scale_out = sc.y;
     const int groups = pitch / 8;
     const long long n = (long long)rows * groups, stride = (long long)gridDim.x * 256;
     const size_t plane = (size_t)rows * pitch;
@@ -799,15 +819,17 @@ __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ 
         for (int k = 0; k < 8; k++) v[k] = c + k < cols ? src[r * cols + c + k] : 0.f;
         const size_t at = (size_t)r * pitch + c;
         uint32_t h0[4], h1[4], h2[4];
+        if (PAIR) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            uint32_t a0, a1, b0, b1;
-            lt_split2(v[2 * k], sc.x, a0, a1);
-            lt_split2(v[2 * k + 1], sc.x, b0, b1);
-            h0[k] = a0 | (b0 << 16), h1[k] = a1 | (b1 << 16);
+            for (int k = 0; k < 4; k++) {
+                uint32_t a0, a1, b0, b1;
+                lt_split2(v[2 * k], sc.x, a0, a1);
+                lt_split2(v[2 * k + 1], sc.x, b0, b1);
+                h0[k] = a0 | (b0 << 16), h1[k] = a1 | (b1 << 16);
+            }
+            *reinterpret_cast<uint4*>(pair + at) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
+            *reinterpret_cast<uint4*>(pair + plane + at) = make_uint4(h1[0], h1[1], h1[2], h1[3]);
         }
-        *reinterpret_cast<uint4*>(pair + at) = make_uint4(h0[0], h0[1], h0[2], h0[3]);
-        *reinterpret_cast<uint4*>(pair + plane + at) = make_uint4(h1[0], h1[1], h1[2], h1[3]);
         if (TRIPLE) {
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -870,7 +892,8 @@ struct lt_packed {
     rg_outputs<3> mem;
 };
 // `largest` (w): a word that is 0, for one scale over the matrix; NULL (x): a scale per row.
-static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, unsigned* largest, bool want_grads, lt_packed* o) {
+static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, unsigned* largest, bool want_logits, bool want_grads,
+                         lt_packed* o) {
     o->scale = nullptr;
     if (dtype == RG_DTYPE_BF16 && cols % 8 == 0) {
         o->logits = o->grads = {src, rows, cols, 1, cols};
@@ -887,29 +910,31 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
         o->logits = o->grads = {o->mem[0]->raw(), rows, cols, 1, pitch};
         return RG_OK;
     }
-    RG_TRY(rg_alloc_storage(ctx, &pair, 1, &o->mem[0], RG_DTYPE_BF16));
+    if (want_logits) RG_TRY(rg_alloc_storage(ctx, &pair, 1, &o->mem[0], RG_DTYPE_BF16));
     RG_TRY(rg_alloc_storage(ctx, &scales, 1, &o->mem[1]));
     if (want_grads) RG_TRY(rg_alloc_storage(ctx, &triple, 1, &o->mem[2], RG_DTYPE_BF16));
-    void* three = want_grads ? o->mem[2]->raw() : nullptr;
+    uint16_t* two = want_logits ? static_cast<uint16_t*>(o->mem[0]->raw()) : nullptr;
+    uint16_t* three = want_grads ? static_cast<uint16_t*>(o->mem[2]->raw()) : nullptr;
     o->scale = o->mem[1]->data();
     if (largest) {
         const float* w = static_cast<const float*>(src);
         const size_t n = (size_t)rows * cols;
         const int most = ctx->sm_count * 16;
-        RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, ctx->sm_count * 8))),
-                          dim3(256), 0, ctx->stream, w, n, largest));
+        if (want_logits) {
+            RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, ctx->sm_count * 8))),
+                              dim3(256), 0, ctx->stream, w, n, largest));
+            RG_LAUNCHED(ctx);
+        }
         const unsigned grid = (unsigned)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, most);
-        RG_CUDA(rg_launch(true, want_grads ? lt_pack_kernel<true> : lt_pack_kernel<false>, dim3(grid), dim3(256), 0, ctx->stream, w, rows, cols,
-                          pitch, (const unsigned*)largest, static_cast<uint16_t*>(o->mem[0]->raw()), static_cast<uint16_t*>(three),
-                          o->mem[1]->data()));
-        RG_LAUNCHED(ctx);
+        RG_CUDA(rg_launch(true, !want_grads ? lt_pack_kernel<true, false> : want_logits ? lt_pack_kernel<true, true> : lt_pack_kernel<false, true>,
+                          dim3(grid), dim3(256), 0, ctx->stream, w, rows, cols, pitch, (const unsigned*)largest, two, three, o->mem[1]->data()));
     } else {
         RG_CUDA(rg_launch(true, lt_pack_rows_kernel, dim3((unsigned)rg_cdiv(rows, 8)), dim3(256), 0, ctx->stream, static_cast<const float*>(src), rows,
-                          cols, pitch, static_cast<uint16_t*>(o->mem[0]->raw()), static_cast<uint16_t*>(three), o->mem[1]->data()));
+                          cols, pitch, two, three, o->mem[1]->data()));
     }
     RG_CUDA(cudaGetLastError());
     RG_LAUNCHED(ctx);
-    o->logits = {o->mem[0]->raw(), rows, cols, 2, pitch};
+    o->logits = {two, rows, cols, 2, pitch};
     o->grads = {three, rows, cols, 3, pitch};
     return RG_OK;
 }
@@ -955,8 +980,8 @@ static void lt_common(rg_ctx* ctx, const lce_call& c, int* counter, lt_args* e) 
 
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     lt_packed x, w;
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, false, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, false, &w));
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, false, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, false, &w));
     CUtensorMap maps[4];
     RG_TRY(lt_map(&maps[0], x.logits, 128));
     RG_TRY(lt_map(&maps[1], w.logits, LT_BK));
@@ -982,25 +1007,37 @@ static int lt_piece(const lce_call& c) {
 int lce_tc_backward_launches(const lce_call& c) { return 2 * rg_cdiv(c.V, lt_piece(c)); }
 
 rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
-    rg_outputs<3> o;  // dz, partial dx, partial dbias
+    rg_outputs<4> o;  // dz, partial dx, partial dbias, partial dw
     lt_packed x, w;
     const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = planes == 3 ? lt_shape<3>::BN : lt_shape<1>::BN;  // of the gradients
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, &w));
+    const int clusters = ctx->sm_count / 2;
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, true, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, true, &w));
 
     const int piece = lt_piece(c), pieces = rg_cdiv(c.V, piece);
     const int width = std::min(piece, (c.V + 63) / 64 * 64);  // columns of dz that are stored
     const size_t zlen = (size_t)planes * c.R * width;
     RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[0], RG_DTYPE_BF16));
 
-    // the K axis of dx is the vocabulary: cut it when its few tiles would otherwise outlast the many short ones of dw
-    lt_prob pdx = lt_problem(c.R, c.D, piece, bn, 0, 0), pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
+    // dx or its transpose: whichever pads less (a row tile is 256, a column tile as narrow as 32)
+    auto pad = [](long long m, long long n) { return (m + 255) / 256 * 256 * ((n + 31) / 32 * 32); };
+    const bool dx_t = pad(c.D, c.R) < pad(c.R, c.D);
+    lt_prob pdx = dx_t ? lt_problem(c.D, c.R, piece, bn, 0, 0) : lt_problem(c.R, c.D, piece, bn, 0, 0);
+    lt_prob pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
+    // The K axes are cut where tiles are fewer or longer than makes an even load: runs of `run` k-blocks, none of them empty.  A
+    // smaller last piece has fewer runs of dx and leaves the other sums alone; dw is only cut when there is one piece.
     const long long load = (long long)pdx.tiles_m * pdx.tiles_n * pdx.kb_per + (long long)pdw.tiles_m * pdw.tiles_n * pdw.kb_per;
-    const int fair = (int)std::max<long long>(4, load / (ctx->sm_count / 2) / 2);
-    // runs of `run` k-blocks, none of them empty; a smaller last piece has fewer runs and leaves the other sums alone
-    const int run = rg_cdiv(pdx.kb_per, std::min(16, rg_cdiv(pdx.kb_per, fair))), splits = rg_cdiv(pdx.kb_per, run);
-    const size_t plen = (size_t)splits * c.R * c.D;
+    const int fair = (int)std::max<long long>(8, load / clusters / 2);
+    auto cut = [&](lt_prob& p) {
+        p.kb_per = rg_cdiv(p.kb_per, std::min(16, rg_cdiv(p.kb_per, fair)));
+        return p.kb_per;
+    };
+    const int run = cut(pdx), splits = rg_cdiv(rg_cdiv(piece, LT_BK), run);
+    const bool cut_dw = pieces == 1 && pdw.tiles_m * pdw.tiles_n < clusters && pdw.kb_per > fair;
+    const int run_w = cut_dw ? cut(pdw) : pdw.kb_per, splits_w = rg_cdiv(rg_cdiv(c.R, LT_BK), run_w);
+    const size_t plen = (size_t)splits * c.R * c.D, wlen = (size_t)splits_w * c.D * c.V;
     RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[1]));
+    if (cut_dw) RG_TRY(rg_alloc_storage(ctx, &wlen, 1, &o[3]));
     const int dbrows = LT_BM / 32 * rg_cdiv(c.R, LT_BM);
     if (c.dbias) {
         const size_t blen = (size_t)dbrows * c.V;
@@ -1012,8 +1049,8 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     RG_TRY(lt_map(&mz[0], x.logits, 128));
     RG_TRY(lt_map(&mz[1], w.logits, LT_BK));
     mz[2] = mz[0], mz[3] = mz[1];
-    RG_TRY(lt_map(&mg[0], z, 128));
-    RG_TRY(lt_map(&mg[1], w.grads, bn / 2));
+    RG_TRY(lt_map(&mg[0], dx_t ? w.grads : z, 128));
+    RG_TRY(lt_map(&mg[1], dx_t ? z : w.grads, bn / 2));
     RG_TRY(lt_map(&mg[2], z, LT_BK));
     RG_TRY(lt_map(&mg[3], x.grads, LT_BK));
 
@@ -1024,20 +1061,23 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.v0 = i * piece, e.vn = std::min(piece, c.V - e.v0);
         e.dz = static_cast<__nv_bfloat16*>(o[0]->raw()), e.dz_pitch = width;
         e.dbparts = c.dbias ? o[2]->data() : nullptr;
-        e.dxparts = o[1]->data(), e.dx_add = i > 0;
+        e.dxparts = o[1]->data(), e.dx_add = i > 0, e.dx_t = dx_t;
         e.dw = c.dw, e.dw_bf16 = c.dtype == RG_DTYPE_BF16;
+        e.dwparts = cut_dw ? o[3]->data() : nullptr;
         e.nprobs = 1;
         e.p[0] = lt_problem(c.R, e.vn, c.D, LT_BN, 0, 1);
         e.p[0].b_n0 = e.v0;
         RG_TRY(lt_run<LT_DZ>(ctx, c, mz, e));
         e.nprobs = 2;
-        e.p[0] = lt_problem(c.R, c.D, e.vn, bn, 0, 0);
+        e.p[0] = dx_t ? lt_problem(c.D, c.R, e.vn, bn, 0, 0) : lt_problem(c.R, c.D, e.vn, bn, 0, 0);
         e.p[0].splits = rg_cdiv(e.p[0].kb_per, run), e.p[0].kb_per = run;
-        e.p[0].b_k0 = e.v0;
+        (dx_t ? e.p[0].a_k0 : e.p[0].b_k0) = e.v0;
         e.p[1] = lt_problem(e.vn, c.D, c.R, bn, 1, 1);
+        e.p[1].splits = splits_w, e.p[1].kb_per = run_w;
         RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
     }
     lce_dx_finish_launch(ctx, o[1]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
+    if (cut_dw) lce_dx_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, c.dw, c.dtype);
     if (c.dbias) lce_dbias_finish_launch(ctx, o[2]->data(), dbrows, c.V, c.scal, c.dbias);
     return RG_OK;
 }

@@ -374,7 +374,8 @@ def ce_check(be, R, D, V, dtype, bias=True, ignored=0.2, dloss=None, seed=0):
 FEW = [(1, 1, 1), (1, 8, 2), (1, 64, 1000), (2, 13, 97), (3, 768, 257), (4, 32, 128), (5, 300, 1025), (8, 128, 129), (9, 31, 63),
        (16, 257, 2047), (13, 520, 333)]
 MANY = [(17, 1, 1), (17, 8, 2), (33, 13, 97), (64, 64, 64), (64, 192, 97), (127, 65, 255), (128, 128, 256), (129, 72, 257), (200, 100, 1000),
-        (300, 320, 513), (511, 257, 775), (640, 768, 1024), (1025, 40, 2049), (260, 520, 5003)]
+        (300, 320, 513), (511, 257, 775), (640, 768, 1024), (1025, 40, 2049), (260, 520, 5003), (30, 700, 2000), (200, 768, 1500),
+        (2500, 40, 300), (8000, 128, 97)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -601,6 +602,39 @@ def test_linear_cross_entropy_over_pieces_of_the_vocabulary(backend, dtype):
     gone = np.ones(R, bool)
     gone[at] = False
     assert not dx[gone].any()
+
+
+def test_linear_cross_entropy_of_few_rows_over_pieces_of_the_vocabulary(backend):
+    """So wide a vocabulary that a few hundred rows go over it in pieces: dx is summed over both."""
+    torch = pytest.importorskip("torch")
+    be = backend
+    R, D, V = 200, 256, 450000
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(R, D, device="cuda", generator=gen)
+    w = torch.randn(D, V, device="cuda", generator=gen) * 2.5 / D ** 0.5
+    t = torch.randint(0, V, (R,), device="cuda", generator=gen).float()
+    z = x.double() @ w.double()
+    exact = torch.logsumexp(z, -1)
+    p = torch.exp(z - exact[:, None])
+    dz = p.clone()
+    dz[torch.arange(R), t.long()] -= 1
+    torch.cuda.synchronize()
+    X, W, T = be.from_device(x), be.from_device(w), be.from_device(t)
+    L = put(be, exact.cpu().numpy().astype(np.float32))
+    dx, dw, _ = be.linear_cross_entropy_bwd(X, W, None, T, L)
+    # as ce_bounds has it: a logit's error is max(D / 8 + 8, 2 * 18 + 4 + D / 256) half steps of the magnitudes, the chain over
+    # the vocabulary 2 * 18 + 4 + V / 256
+    mags = x.double().abs() @ w.double().abs()
+    edz = p * ((41 * mags + 3 * (z.abs() + exact.abs()[:, None])) * E32 + 4 * E32) * 1.01 + E32 * dz.abs()
+    ez = edz + 2.0 ** -21 * dz.abs()
+    tdx = (ez + (40 + V / 256) * E32 * dz.abs()) @ w.double().abs().T / R
+    ex = dz @ w.double().T / R
+    got = torch.from_numpy(get(be, dx)).cuda()
+    assert bool(((got - ex).abs() <= tdx + 4 * E32 * ex.abs() + 1e-45).all())
+    tdw = x.double().abs().T @ (ez + 41 * E32 * dz.abs()) / R
+    exw = x.double().T @ dz / R
+    got = torch.from_numpy(be.to_vec(dw).reshape(D, V)).cuda().double()
+    assert bool(((got - exw).abs() <= tdw + 4 * E32 * exw.abs() + 1e-45).all())
 
 
 def test_linear_cross_entropy_gives_the_same_bits_again(backend):
