@@ -608,7 +608,7 @@ extern "C" rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, c
     const bool few = lce_is_few(c);
     c.ncounters = few ? 0 : 1;
     RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, nullptr, &o[2]));
-    c.nparts = few ? lce_few_tiles(c.V) : lce_tc_nparts(c.V);
+    c.nparts = few ? lce_few_tiles(c.V) : lce_tc_nparts(ctx, c);
     const size_t pwords = 2 * (size_t)c.nparts * rows, blocks = (size_t)rg_cdiv(c.R, 8), swords = 2 * blocks;
     RG_TRY(rg_alloc_storage(ctx, &pwords, 1, &o[3]));
     RG_TRY(rg_alloc_storage(ctx, &swords, 1, &o[4]));

@@ -43,5 +43,5 @@ void lce_dbias_finish_launch(rg_ctx* ctx, const float* parts, int nparts, int V,
 // The tensor-core form.
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c);
 rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c);
-int lce_tc_nparts(int V);
+int lce_tc_nparts(rg_ctx* ctx, const lce_call& c);
 int lce_tc_backward_launches(const lce_call& c);

@@ -150,6 +150,11 @@ __device__ __forceinline__ bool lt_wait(uint64_t* bar, uint32_t parity, int* err
         }
     }
 }
+// by a whole warp: all of its lanes go on, or none does
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool lt_wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+    return __all_sync(RG_FULL_MASK, lt_wait<CLUSTER>(bar, parity, err));
+}
 // into this CTA's shared memory; the bytes are counted on a barrier of CTA 0
 __device__ __forceinline__ void lt_tma(const CUtensorMap* map, void* dst, uint32_t bar, int x, int y, int plane) {
     asm volatile(
@@ -598,7 +603,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
         bool ok = true;
         while (true) {
             const uint32_t slot = ti & 1u;
-            ok = lt_wait<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
+            ok = lt_wait_warp<true>(&sched_full[slot], (ti >> 1) & 1u, e.err);
             if (!ok) break;
             // lane 0's value goes to all lanes, so its read is complete before it hands the slot back (the arrival alone would not
             // wait for a read that is queued behind this warp's stores)
@@ -627,9 +632,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                     for (int j = 0; j < 32; j++) acc[c][j] = 0.f;
             for (int sg = 0; sg < segs; sg++, seg++) {
                 const uint32_t buf = seg % S::BUFFERS;
-                ok = lt_wait(&acc_full[buf], (seg / S::BUFFERS) & 1u, e.err);
+                ok = lt_wait_warp(&acc_full[buf], (seg / S::BUFFERS) & 1u, e.err);
                 if (!ok) break;
-                __syncwarp();  // the loads below are executed by whole warps
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ta = taddr + buf * S::BN;
                 if (PLANES == 1) {
@@ -691,6 +695,388 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     // neither CTA leaves (or gives back its tensor memory) while the other may still reach into it
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// some rows: logits from w as it lies in memory
+// ---------------------------------------------------------------------------
+// With up to LM_MOST_ROWS rows the kernel above spends its time on the planes of w: a pass for the scale, one that writes 4
+// bytes for every 4 it reads, and reading those.  Here eight warps read w once, with plain loads (a row of an odd vocabulary
+// starts on any 2 or 4 bytes), split it in registers and write the planes to shared memory, where the tensor core takes them;
+// only x, which is small, is packed before.  The sides are swapped: z^T = w^T x^T, 128 columns of the vocabulary are the rows
+// of a tile and 64 (32) rows of x its columns, so a thread of the epilogue holds one column of the vocabulary.  f32 is split
+// into bf16 triples (six products; no scale is needed), each k-block has an accumulator of its own and the sum is taken in
+// registers with rounding.
+// Bound by the bytes of w: 4 (2) D V, and by the instructions of the split (about 12 per value).
+#define LM_MOST_ROWS 192
+// Four epilogue warps, sixteen that convert (eight, two to a scheduler, were bound by the latency of their instructions: 62
+// instead of XX us for 17x768x50257), one that copies x, one that multiplies, two that only give their registers away:
+// 768 threads x 80 at launch = 128 x 152 + 512 x 64 + 128 x 72.
+#define LM_THREADS 768
+
+template <typename T>
+struct lm_shape {
+    static constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+    static constexpr int X_BYTES = 64 * LT_BK * 2, STAGE_BYTES = PLANES * X_BYTES;  // shared memory: x
+    static constexpr int W_COLS = LT_BK / 2, STAGE_COLS = PLANES * W_COLS;  // tensor memory: w, two values to a column's word
+    static constexpr int STAGES = PLANES == 3 ? 3 : 6;
+    // accumulators of 64 columns: the tensor core goes on while the epilogue works on a tile's sums
+    static constexpr int BUFFERS = (512 - STAGES * STAGE_COLS) / 64;
+    static constexpr int CHAIN = PLANES == 3 ? LT_CHAIN : 1 << 20;  // k-blocks per accumulator
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 2 * 4 * 64 * 8 + 1024 + 256;
+};
+
+struct lm_args {
+    const void* w;   // [D][V]
+    int R, D, V;
+    int tile;        // columns of the vocabulary per tile, at most 128
+    int tiles, groups;  // of columns; of 64 rows
+    int cols;        // columns that are covered: V, or those of dz
+    int* err;
+    const float* bias;
+    const int* tgt;
+    float2* parts;   // LT_FWD
+    float* tz;
+    const float* lse;  // LT_DZ
+    __nv_bfloat16* dz;  // [3][R][cols]
+    float* dbparts;  // [groups][V] or NULL
+};
+
+// A from tensor memory
+__device__ __forceinline__ void lm_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+        "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void lm_st8(uint32_t taddr, const uint32_t (&h)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(h[0]), "r"(h[1]), "r"(h[2]),
+                 "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7])
+                 : "memory");
+}
+__device__ __forceinline__ void lm_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lt_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void lm_tma(const CUtensorMap* map, void* dst, uint64_t* bar, int x, int y, int plane) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     lt_smem(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(plane), "r"(lt_smem(bar))
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t lm_bits(const float* p) { return __float_as_uint(__ldg(p)); }
+__device__ __forceinline__ uint32_t lm_bits(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const unsigned short*>(p)); }
+
+// sums over the warp of 32 values per lane: 31 halving exchanges leave that of value `lane` in each lane
+__device__ __forceinline__ float lm_across(float (&v)[32], int lane) {
+#pragma unroll
+    for (int half = 16; half >= 1; half >>= 1) {
+        const bool up = lane & half;
+#pragma unroll
+        for (int i = 0; i < half; i++) {
+            const float keep = up ? v[i + half] : v[i], send = up ? v[i] : v[i + half];
+            v[i] = keep + __shfl_xor_sync(RG_FULL_MASK, send, half);
+        }
+    }
+    return v[0];
+}
+__device__ __forceinline__ float lm_max(float v) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+
+template <typename T, int EPI>
+__global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ lm_args e) {
+    typedef lm_shape<T> S;
+    extern __shared__ unsigned char lm_raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lm_raw) + 1023) & ~(uintptr_t)1023);
+    float2* sums = reinterpret_cast<float2*>(ring + S::STAGES * S::STAGE_BYTES);  // [2][4][64]
+    uint64_t* full_w = reinterpret_cast<uint64_t*>(sums + 2 * 4 * 64);
+    uint64_t* full_x = full_w + S::STAGES;
+    uint64_t* empty = full_x + S::STAGES;
+    uint64_t* acc_full = empty + S::STAGES;  // [S::BUFFERS]
+    uint64_t* acc_empty = acc_full + S::BUFFERS;
+    uint64_t* merge = acc_empty + S::BUFFERS;
+    uint64_t* drain = merge + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+    // the same in all lanes, and known to be: what follows from it is computed once per warp
+    const int warp = __shfl_sync(RG_FULL_MASK, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int total = e.tiles * e.groups, nkb = (e.D + LT_BK - 1) / LT_BK;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; s++) lt_bar_init(&full_w[s], 16), lt_bar_init(&full_x[s], 1), lt_bar_init(&empty[s], 1);
+        for (int b = 0; b < S::BUFFERS; b++) lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 4);
+        lt_bar_init(merge, 4);
+        lt_bar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 21) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(lt_smem(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp >= 4 && warp < 20) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        // ===== w: a thread takes one column of the vocabulary (its lane of tensor memory) and 16 of the 64 rows of a k-block, so
+        // 32 lanes read side by side.  The values of the k-block after the next are loaded into the registers that the
+        // conversion of this one frees. =====
+        const int row = ((warp - 4) >> 2) * 16;
+        const T *w = static_cast<const T*>(e.w), *p = nullptr;
+        int t = blockIdx.x, kb = 0;  // of the loads, two k-blocks ahead
+        const uint32_t blocks = (uint32_t)((total - t + (int)gridDim.x - 1) / (int)gridDim.x) * nkb;
+        auto place = [&]() {
+            const int v0 = (t / e.groups) * e.tile;
+            p = w + (size_t)row * e.V + min(v0 + (warp & 3) * 32 + lane, min(e.V, v0 + e.tile) - 1);
+        };
+        auto load = [&](uint32_t* r) {
+            const T* q = p + (size_t)(kb * LT_BK) * e.V;
+            const int rows = t < total ? e.D - kb * LT_BK - row : 0;
+            if (rows >= 16) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) r[j] = lm_bits(q + (size_t)j * e.V);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) r[j] = j < rows ? lm_bits(q + (size_t)j * e.V) : 0u;
+            }
+        };
+        auto next = [&]() {
+            if (++kb == nkb) {
+                kb = 0, t += gridDim.x;
+                if (t < total) place();
+            }
+        };
+        uint32_t it = 0;
+        auto convert = [&](uint32_t (&raw)[16]) {
+            const int s = it % S::STAGES;
+            if (!lt_wait_warp(&empty[s], ((it / S::STAGES) & 1u) ^ 1u, e.err)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + s * S::STAGE_COLS + row / 2;
+#pragma unroll
+            for (int p2 = 0; p2 < S::PLANES; p2++) {
+                // f32: the leading 16 bits, and what they leave, which is exact (infinity leaves a NaN, NaN stays one)
+                uint32_t h[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    uint32_t &a = raw[2 * j], &b = raw[2 * j + 1];
+                    h[j] = S::PLANES == 1 ? __byte_perm(a, b, 0x5410) : __byte_perm(a, b, 0x7632);
+                    a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
+                    b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+                }
+                lm_st8(to + p2 * S::W_COLS, h);
+            }
+            load(raw);
+            next();
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) lt_arrive(&full_w[s]);
+            it++;
+            return true;
+        };
+        uint32_t raw[2][16];
+        place();
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            load(raw[k]);
+            next();
+        }
+        while (it < blocks) {
+            if (!convert(raw[0]) || it == blocks) break;
+            if (!convert(raw[1])) break;
+        }
+    } else if (warp >= 20) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 20 && lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < total; t += gridDim.x)
+                for (int kb = 0; kb < nkb; kb++, it++) {
+                    const int s = it % S::STAGES;
+                    ok = lt_wait(&empty[s], ((it / S::STAGES) & 1u) ^ 1u, e.err);
+                    if (!ok) break;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(lt_smem(&full_x[s])),
+                                 "r"((uint32_t)(S::PLANES * S::X_BYTES))
+                                 : "memory");
+                    unsigned char* x = ring + s * S::STAGE_BYTES;
+#pragma unroll
+                    for (int p = 0; p < S::PLANES; p++) lm_tma(&tmX, x + p * S::X_BYTES, &full_x[s], kb * LT_BK, (t % e.groups) * 64, p);
+                }
+            // the copies have landed before the CTA's memory goes away, also where a wait gave up
+            for (uint32_t i = it > (uint32_t)S::STAGES ? it - S::STAGES : 0; i < it; i++)
+                lt_wait(&full_x[i % S::STAGES], (i / S::STAGES) & 1u, e.err);
+        }
+        if (warp == 21) {
+            // The whole warp walks the loops and one lane issues: an MMA's operands then are uniform values.  (One thread in the
+            // loops alone took 14 instructions, 30 ns, for each MMA to bring them there.)
+            uint32_t it = 0, seg = 0, one;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+                const int rows = min(64, e.R - (t % e.groups) * 64);
+                // D f32, A and B bf16, N, M = 128
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(rows > 32 ? 8 : 4) << 17) | (8u << 24);
+                for (int kb0 = 0; ok && kb0 < nkb; kb0 += S::CHAIN, seg++) {
+                    const uint32_t buf = seg % S::BUFFERS;
+                    ok = lt_wait_warp(&acc_empty[buf], ((seg / S::BUFFERS) & 1u) ^ 1u, e.err);
+                    const uint32_t d = tmem + S::STAGES * S::STAGE_COLS + buf * 64;
+                    const int end = min(S::CHAIN, nkb - kb0);
+                    for (int kb = 0; ok && kb < end; kb++, it++) {
+                        const int s = it % S::STAGES;
+                        ok = lt_wait_warp(&full_x[s], (it / S::STAGES) & 1u, e.err) && lt_wait_warp(&full_w[s], (it / S::STAGES) & 1u, e.err);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t a = tmem + s * S::STAGE_COLS;
+                        const uint64_t b = lt_desc(lt_smem(ring + s * S::STAGE_BYTES), 0);
+                        constexpr int PRODUCTS = S::PLANES == 1 ? 1 : 6;
+                        constexpr int pa[6] = {0, 2, 1, 0, 1, 0}, pb[6] = {2, 0, 1, 1, 0, 0};  // the smallest products first
+                        if (one) {
+#pragma unroll
+                            for (int pr = 0; pr < PRODUCTS; pr++)
+#pragma unroll
+                                for (int k = 0; k < LT_BK / 16; k++)
+                                    lm_mma(d, a + (S::PLANES == 1 ? 0 : pa[pr]) * S::W_COLS + k * 8,
+                                               b + ((S::PLANES == 1 ? 0 : pb[pr]) * S::X_BYTES + k * 32) / 16, idesc, kb > 0 || pr > 0 || k > 0);
+                            lm_commit(&empty[s]);
+                            if (kb + 1 == end) lm_commit(&acc_full[buf]);
+                        }
+                    }
+                }
+            }
+            if (one) lm_commit(drain);  // MMAs in flight finish before the tensor memory is given back
+            lt_wait(drain, 0, e.err);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        // ===== epilogue: a thread holds one column of the vocabulary, 64 rows in two halves =====
+        const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16) + S::STAGES * S::STAGE_COLS;
+        const int place = warp * 32 + lane;
+        uint32_t it = 0, nt = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < total; t += gridDim.x, nt++) {
+            const int row0 = (t % e.groups) * 64, rows = min(64, e.R - row0), v0 = (t / e.groups) * e.tile;
+            const int c = v0 + place;
+            const bool mine = place < e.tile && c < e.cols, live = mine && c < e.V;
+            const float bias = e.bias && live ? e.bias[c] : 0.f;
+            float acc[2][32];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < 32; j++) acc[h][j] = 0.f;
+            for (int kb = 0; kb < nkb; kb += S::CHAIN, it++) {
+                const uint32_t buf = it % S::BUFFERS;
+                ok = lt_wait_warp(&acc_full[buf], (it / S::BUFFERS) & 1u, e.err);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (h && rows <= 32) break;
+                    float block[32];
+                    lt_ld32(taddr + buf * 64 + h * 32, block);
+                    lt_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 q = rg_add2(make_float2(acc[h][j], acc[h][j + 1]), make_float2(block[j], block[j + 1]));
+                        acc[h][j] = q.x, acc[h][j + 1] = q.y;
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) lt_arrive(&acc_empty[buf]);
+            }
+            if (!ok) break;
+            float db = 0.f;
+            float2* mine_s = sums + ((nt & 1) * 4 + warp) * 64;
+#pragma unroll 1
+            for (int h = 0; h * 32 < rows; h++) {
+                const int r0 = row0 + h * 32, left = min(32, e.R - r0);
+                float(&v)[32] = acc[0];
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] += bias;
+                const int tgt = lane < left ? __ldg(e.tgt + r0 + lane) : -1;  // of row `lane`
+                unsigned hits = __ballot_sync(RG_FULL_MASK, tgt >= v0 && tgt < v0 + e.tile);  // rows whose target is in the tile
+                if (EPI == LT_FWD) {
+                    for (; hits; hits &= hits - 1) {
+                        const int r = __ffs(hits) - 1;
+                        const bool here = __shfl_sync(RG_FULL_MASK, tgt, r) == c && live;
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (here && j == r) e.tz[r0 + j] = v[j];
+                    }
+                    __syncwarp();
+                    float m = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        v[j] = live ? v[j] : -INFINITY, v[j + 1] = live ? v[j + 1] : -INFINITY;
+                        const float m0 = lm_max(v[j]), m1 = lm_max(v[j + 1]);
+                        const float2 q = lt_exp2(make_float2(v[j], v[j + 1]), make_float2(m0 == -INFINITY ? 0.f : -m0, m1 == -INFINITY ? 0.f : -m1));
+                        v[j] = q.x, v[j + 1] = q.y;
+                        m = lane == j ? m0 : lane == j + 1 ? m1 : m;
+                    }
+                    mine_s[h * 32 + lane] = make_float2(m, lm_across(v, lane));
+                } else {
+                    const float lse = lane < left ? __ldg(e.lse + r0 + lane) : 0.f;
+                    const unsigned dead = __ballot_sync(RG_FULL_MASK, tgt < 0);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 less = make_float2(-__shfl_sync(RG_FULL_MASK, lse, j), -__shfl_sync(RG_FULL_MASK, lse, j + 1));
+                        const float2 q = lt_exp2(make_float2(v[j], v[j + 1]), less);
+                        v[j] = (dead >> j & 1) || !live ? 0.f : q.x, v[j + 1] = (dead >> (j + 1) & 1) || !live ? 0.f : q.y;
+                    }
+                    for (; hits; hits &= hits - 1) {
+                        const int r = __ffs(hits) - 1;
+                        const bool here = __shfl_sync(RG_FULL_MASK, tgt, r) == c && live;
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (here && j == r) v[j] -= 1.f;
+                    }
+                    __syncwarp();
+                    unsigned short* z = reinterpret_cast<unsigned short*>(e.dz + (size_t)r0 * e.cols + c);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        float d = v[j];
+                        db += d;
+                        if (!mine || j >= left) continue;
+                        unsigned short* o = z + (size_t)j * e.cols;
+#pragma unroll
+                        for (int p = 0; p < 3; p++) {
+                            o[(size_t)p * e.R * e.cols] = (unsigned short)(__float_as_uint(d) >> 16);
+                            d -= __uint_as_float(__float_as_uint(d) & 0xffff0000u);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j++) acc[0][j] = acc[1][j];
+            }
+            if (EPI == LT_FWD) {  // the four warps' columns; the other half of `sums` is still being read for the tile before
+                __syncwarp();
+                if (lane == 0) lt_arrive(merge);
+                ok = lt_wait_warp(merge, nt & 1u, e.err);
+                if (!ok) break;
+                const int r = threadIdx.x;
+                if (r < rows) {
+                    lce_ms a = {-INFINITY, 0.f};
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const float2 b = sums[((nt & 1) * 4 + q) * 64 + r];
+                        a = lce_merge(a, {b.x, b.y});
+                    }
+                    e.parts[(size_t)(t / e.groups) * e.R + row0 + r] = make_float2(a.m, a.s);
+                }
+            } else if (e.dbparts && live) {
+                e.dbparts[(size_t)(t % e.groups) * e.V + c] = db;
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -941,7 +1327,32 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
 
 static_assert(lt_shape<1>::BN == lt_shape<2>::BN, "the logits have one width of column tiles");
 #define LT_BN lt_shape<1>::BN
-int lce_tc_nparts(int V) { return 2 * rg_cdiv(V, LT_BN); }
+
+// The form of lce_mid_kernel.
+static bool lm_takes(const lce_call& c) { return c.R <= LM_MOST_ROWS && (c.dtype == RG_DTYPE_F32 || c.V % 8); }
+
+// Columns of a tile: as many tiles as whole rounds of the SMs hold.
+static int lm_tile(rg_ctx* ctx, const lce_call& c, int cols) {
+    const long long groups = rg_cdiv(c.R, 64), rounds = rg_cdiv(rg_cdiv(cols, 128) * groups, ctx->sm_count);
+    const int tiles = (int)std::max<long long>(1, rounds * ctx->sm_count / groups);
+    return std::min(128, std::max(64, (rg_cdiv(cols, tiles) + 3) / 4 * 4));
+}
+int lce_tc_nparts(rg_ctx* ctx, const lce_call& c) { return lm_takes(c) ? rg_cdiv(c.V, lm_tile(ctx, c, c.V)) : 2 * rg_cdiv(c.V, LT_BN); }
+
+template <typename T, int EPI>
+static rg_status lm_launch(rg_ctx* ctx, const lce_call& c, const lt_packed& x, lm_args& e) {
+    CUtensorMap map;
+    RG_TRY(lt_map(&map, x.grads, 64));
+    e.w = c.w, e.R = c.R, e.D = c.D, e.V = c.V;
+    e.groups = rg_cdiv(c.R, 64), e.tile = lm_tile(ctx, c, e.cols), e.tiles = rg_cdiv(e.cols, e.tile);
+    e.err = ctx->d_flag + 1;
+    e.bias = c.bias, e.tgt = c.tgt, e.parts = c.parts, e.tz = c.tz, e.lse = c.lse;
+    const int grid = (int)std::min<long long>((long long)e.tiles * e.groups, ctx->sm_count);
+    RG_CUDA(cudaFuncSetAttribute(lce_mid_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, lm_shape<T>::SMEM));
+    RG_CUDA(rg_launch(true, lce_mid_kernel<T, EPI>, dim3(grid), dim3(LM_THREADS), lm_shape<T>::SMEM, ctx->stream, map, e));
+    RG_LAUNCHED(ctx);
+    return RG_OK;
+}
 
 static lt_prob lt_problem(int M, int N, int K, int bn, int a_mn, int b_mn) {
     lt_prob p;
@@ -980,6 +1391,13 @@ static void lt_common(rg_ctx* ctx, const lce_call& c, int* counter, lt_args* e) 
 
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     lt_packed x, w;
+    if (lm_takes(c)) {
+        RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, false, true, &x));
+        lm_args e;
+        memset(&e, 0, sizeof(e));
+        e.cols = c.V;
+        return c.dtype == RG_DTYPE_F32 ? lm_launch<float, LT_FWD>(ctx, c, x, e) : lm_launch<__nv_bfloat16, LT_FWD>(ctx, c, x, e);
+    }
     RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, false, &x));
     RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, false, &w));
     CUtensorMap maps[4];
@@ -1011,10 +1429,11 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     lt_packed x, w;
     const int planes = c.dtype == RG_DTYPE_F32 ? 3 : 1, bn = planes == 3 ? lt_shape<3>::BN : lt_shape<1>::BN;  // of the gradients
     const int clusters = ctx->sm_count / 2;
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, true, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, true, &w));
-
     const int piece = lt_piece(c), pieces = rg_cdiv(c.V, piece);
+    const bool mid = c.dtype == RG_DTYPE_F32 && lm_takes(c) && pieces == 1;  // bf16: w is copied for dx all the same
+    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, !mid, true, &x));
+    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, !mid, true, &w));
+
     const int width = std::min(piece, (c.V + 63) / 64 * 64);  // columns of dz that are stored
     const size_t zlen = (size_t)planes * c.R * width;
     RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[0], RG_DTYPE_BF16));
@@ -1038,7 +1457,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     const size_t plen = (size_t)splits * c.R * c.D, wlen = (size_t)splits_w * c.D * c.V;
     RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[1]));
     if (cut_dw) RG_TRY(rg_alloc_storage(ctx, &wlen, 1, &o[3]));
-    const int dbrows = LT_BM / 32 * rg_cdiv(c.R, LT_BM);
+    const int dbrows = mid ? rg_cdiv(c.R, 64) : LT_BM / 32 * rg_cdiv(c.R, LT_BM);
     if (c.dbias) {
         const size_t blen = (size_t)dbrows * c.V;
         RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[2]));
@@ -1046,8 +1465,8 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
 
     CUtensorMap mz[4], mg[4];
     lt_operand z = {o[0]->raw(), c.R, width, planes, width};
-    RG_TRY(lt_map(&mz[0], x.logits, 128));
-    RG_TRY(lt_map(&mz[1], w.logits, LT_BK));
+    if (!mid) RG_TRY(lt_map(&mz[0], x.logits, 128));
+    if (!mid) RG_TRY(lt_map(&mz[1], w.logits, LT_BK));
     mz[2] = mz[0], mz[3] = mz[1];
     RG_TRY(lt_map(&mg[0], dx_t ? w.grads : z, 128));
     RG_TRY(lt_map(&mg[1], dx_t ? z : w.grads, bn / 2));
@@ -1067,7 +1486,14 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.nprobs = 1;
         e.p[0] = lt_problem(c.R, e.vn, c.D, LT_BN, 0, 1);
         e.p[0].b_n0 = e.v0;
-        RG_TRY(lt_run<LT_DZ>(ctx, c, mz, e));
+        if (mid) {
+            lm_args m;
+            memset(&m, 0, sizeof(m));
+            m.cols = width, m.dz = e.dz, m.dbparts = e.dbparts;
+            RG_TRY((lm_launch<float, LT_DZ>(ctx, c, x, m)));
+        } else {
+            RG_TRY(lt_run<LT_DZ>(ctx, c, mz, e));
+        }
         e.nprobs = 2;
         e.p[0] = dx_t ? lt_problem(c.D, c.R, e.vn, bn, 0, 0) : lt_problem(c.R, c.D, e.vn, bn, 0, 0);
         e.p[0].splits = rg_cdiv(e.p[0].kb_per, run), e.p[0].kb_per = run;
