@@ -492,42 +492,64 @@ __global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, con
     }
 }
 
-// The form for few rows, by what was measured at [R,768] x [768,50257] (us, forward + gradient): f32 16 rows 73 + 201, the
-// tensor cores 158 + 375 for 17; bf16 with an aligned vocabulary 4 rows 40 + 100, the tensor cores 40 + 117; with an odd one
-// (whose rows have to be copied first) 8 rows 50 + 125, the tensor cores 72 + 147.
-static bool lce_is_few(const lce_call& c) { return c.R <= (c.dtype == RG_DTYPE_F32 ? 16 : c.V % 8 == 0 ? 4 : 8); }
+// The form for few rows, by what was measured at [R,768] x [768,50257] (us for the call; the other side for the same rows):
+//   forward   f32  8 rows 46, the tensor cores 57;  9 rows 67 and 55
+//             bf16 V aligned: 2 rows 34, the tensor cores 38; 3 rows 37 and 37
+//             bf16 V odd: the tensor cores, 34 for 1 to 16 rows (34 for 1, 38 for 4, 47 for 8 rows here)
+//   gradient  f32  16 rows 203, the tensor cores 227
+//             bf16 V aligned: 4 rows 98, the tensor cores 107; 8 rows 121
+//             bf16 V odd: 8 rows 120, the tensor cores 135; 9 rows 184
+static bool lce_is_few(const lce_call& c, bool grad) {
+    if (c.dtype == RG_DTYPE_F32) return c.R <= (grad ? 16 : 8);
+    if (c.V % 8 == 0) return c.R <= (grad ? 4 : 2);
+    return grad && c.R <= 8;
+}
 
 static int lce_few_tiles(int V) { return rg_cdiv(V, LCE_COLS); }
 static int lce_few_parts(int V) { return rg_cdiv(V, 1024); }
 
 template <typename T, int RB>
-static void lce_few_launch(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
-    const dim3 tiles((unsigned)lce_few_tiles(c.V));
+static void lce_few_fwd_launch(rg_ctx* ctx, const lce_call& c) {
     const size_t smem = lce_few<T, RB>::SMEM;
-    // these start while the check of the targets runs and wait for it before they use them
-    if (!dz) {
-        if (smem > 48 * 1024) cudaFuncSetAttribute(lce_few_fwd_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        rg_launch(true, lce_few_fwd_kernel<T, RB>, tiles, dim3(256), smem, ctx->stream, c);
-        RG_LAUNCHED(ctx);
-        return;
-    }
+    if (smem > 48 * 1024) cudaFuncSetAttribute(lce_few_fwd_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // starts while the check of the targets runs and waits for it before it uses them
+    rg_launch(true, lce_few_fwd_kernel<T, RB>, dim3((unsigned)lce_few_tiles(c.V)), dim3(256), smem, ctx->stream, c);
+    RG_LAUNCHED(ctx);
+}
+template <typename T, int RB>
+static void lce_few_bwd_launch(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
+    const size_t smem = lce_few<T, RB>::SMEM;
     if (smem > 48 * 1024) cudaFuncSetAttribute(lce_few_dz_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    rg_launch(true, lce_few_dz_kernel<T, RB>, tiles, dim3(256), smem, ctx->stream, c, dz);
+    rg_launch(true, lce_few_dz_kernel<T, RB>, dim3((unsigned)lce_few_tiles(c.V)), dim3(256), smem, ctx->stream, c, dz);
     rg_launch(true, lce_few_grad_kernel<T, RB>, dim3((unsigned)lce_few_parts(c.V), (unsigned)rg_cdiv(c.D, LCE_DG)), dim3(256), 0, ctx->stream, c,
               (const float*)dz, dxparts);
     ctx->launches += 2;
 }
-template <typename T>
-static void lce_few_rows(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
-    if (c.R <= 1) lce_few_launch<T, 1>(ctx, c, dz, dxparts);
-    else if (c.R <= 2) lce_few_launch<T, 2>(ctx, c, dz, dxparts);
-    else if (c.R <= 4) lce_few_launch<T, 4>(ctx, c, dz, dxparts);
-    else if (c.R <= 8) lce_few_launch<T, 8>(ctx, c, dz, dxparts);
-    else lce_few_launch<T, 16>(ctx, c, dz, dxparts);
+// the rows of lce_is_few
+static void lce_few_forward(rg_ctx* ctx, const lce_call& c) {
+    if (c.dtype == RG_DTYPE_F32) {
+        if (c.R <= 1) lce_few_fwd_launch<float, 1>(ctx, c);
+        else if (c.R <= 2) lce_few_fwd_launch<float, 2>(ctx, c);
+        else if (c.R <= 4) lce_few_fwd_launch<float, 4>(ctx, c);
+        else lce_few_fwd_launch<float, 8>(ctx, c);
+    } else {
+        if (c.R <= 1) lce_few_fwd_launch<__nv_bfloat16, 1>(ctx, c);
+        else lce_few_fwd_launch<__nv_bfloat16, 2>(ctx, c);
+    }
 }
-static void lce_few_run(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
-    if (c.dtype == RG_DTYPE_F32) lce_few_rows<float>(ctx, c, dz, dxparts);
-    else lce_few_rows<__nv_bfloat16>(ctx, c, dz, dxparts);
+static void lce_few_backward(rg_ctx* ctx, const lce_call& c, float* dz, float* dxparts) {
+    if (c.dtype == RG_DTYPE_F32) {
+        if (c.R <= 1) lce_few_bwd_launch<float, 1>(ctx, c, dz, dxparts);
+        else if (c.R <= 2) lce_few_bwd_launch<float, 2>(ctx, c, dz, dxparts);
+        else if (c.R <= 4) lce_few_bwd_launch<float, 4>(ctx, c, dz, dxparts);
+        else if (c.R <= 8) lce_few_bwd_launch<float, 8>(ctx, c, dz, dxparts);
+        else lce_few_bwd_launch<float, 16>(ctx, c, dz, dxparts);
+    } else {
+        if (c.R <= 1) lce_few_bwd_launch<__nv_bfloat16, 1>(ctx, c, dz, dxparts);
+        else if (c.R <= 2) lce_few_bwd_launch<__nv_bfloat16, 2>(ctx, c, dz, dxparts);
+        else if (c.R <= 4) lce_few_bwd_launch<__nv_bfloat16, 4>(ctx, c, dz, dxparts);
+        else lce_few_bwd_launch<__nv_bfloat16, 8>(ctx, c, dz, dxparts);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -605,7 +627,7 @@ extern "C" rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, c
         o.give({loss, lse});
         return RG_OK;
     }
-    const bool few = lce_is_few(c);
+    const bool few = lce_is_few(c, false);
     c.ncounters = few ? 0 : 1;
     RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, nullptr, &o[2]));
     c.nparts = few ? lce_few_tiles(c.V) : lce_tc_nparts(ctx, c);
@@ -613,7 +635,7 @@ extern "C" rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, c
     RG_TRY(rg_alloc_storage(ctx, &pwords, 1, &o[3]));
     RG_TRY(rg_alloc_storage(ctx, &swords, 1, &o[4]));
     c.parts = static_cast<float2*>(o[3]->raw());
-    if (few) lce_few_run(ctx, c, nullptr, nullptr);
+    if (few) lce_few_forward(ctx, c);
     else RG_TRY(lce_tc_forward(ctx, c));
     rg_launch(true, lce_loss_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, (const float2*)c.parts, c.nparts, c.R, c.tgt,
               (const float*)c.tz, c.scal, c.ticket, static_cast<double*>(o[4]->raw()), o[1]->data(), o[0]->data());
@@ -646,14 +668,14 @@ extern "C" rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* 
         RG_CUDA(cudaMemsetAsync(o[1]->raw(), 0, o[1]->len * rg_dtype_size(o[1]->dtype), ctx->stream));
         if (bias) RG_CUDA(cudaMemsetAsync(o[2]->raw(), 0, o[2]->len * 4, ctx->stream));
     } else {
-        const bool few = lce_is_few(c);
+        const bool few = lce_is_few(c, true);
         c.ncounters = few ? 0 : lce_tc_backward_launches(c);
         RG_TRY(lce_check_launch(ctx, c, targets, ignore_index, dloss, &o[3]));
         if (few) {
             const size_t zlen = (size_t)c.R * c.V, nparts = (size_t)lce_few_parts(c.V), plen = nparts * c.R * c.D;
             RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[4]));
             RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[5]));
-            lce_few_run(ctx, c, o[4]->data(), o[5]->data());
+            lce_few_backward(ctx, c, o[4]->data(), o[5]->data());
             lce_dx_finish_launch(ctx, o[5]->data(), (int)nparts, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
         } else {
             RG_TRY(lce_tc_backward(ctx, c));

@@ -700,29 +700,30 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 // ---------------------------------------------------------------------------
 // some rows: logits from w as it lies in memory
 // ---------------------------------------------------------------------------
-// With up to LM_MOST_ROWS rows the kernel above spends its time on the planes of w: a pass for the scale, one that writes 4
-// bytes for every 4 it reads, and reading those.  Here eight warps read w once, with plain loads (a row of an odd vocabulary
-// starts on any 2 or 4 bytes), split it in registers and write the planes to shared memory, where the tensor core takes them;
-// only x, which is small, is packed before.  The sides are swapped: z^T = w^T x^T, 128 columns of the vocabulary are the rows
-// of a tile and 64 (32) rows of x its columns, so a thread of the epilogue holds one column of the vocabulary.  f32 is split
-// into bf16 triples (six products; no scale is needed), each k-block has an accumulator of its own and the sum is taken in
-// registers with rounding.
-// Bound by the bytes of w: 4 (2) D V, and by the instructions of the split (about 12 per value).
-#define LM_MOST_ROWS 192
-// Four epilogue warps, sixteen that convert (eight, two to a scheduler, were bound by the latency of their instructions: 62
-// instead of XX us for 17x768x50257), one that copies x, one that multiplies, two that only give their registers away:
+// With few row tiles the kernel above waits for the planes of w: a pass for their scale, one that writes 4 bytes for every 4 it
+// reads, and reading those.  Here sixteen warps read w once, with plain loads (a row of an odd vocabulary starts on any 2 or
+// 4 bytes), split it in registers and store the planes to tensor memory, where it is the A operand; only x, which is small,
+// is packed before.  The sides are swapped: z^T = w^T x^T, 128 columns of the vocabulary are the lanes of a tile and 64 (32)
+// rows of x its columns, so a thread of the epilogue holds one column of the vocabulary.  f32 is split into bf16 triples (six
+// products, no scale), the accumulator is cut every 128 of K and the sum taken in registers with rounding.
+// Bound by the instructions of the split and by what one k-block ahead leaves in flight: 41 us for [17,768]x[768,50257], 3.8
+// TB/s of w (bf16 26 us, 2.9 TB/s).  Steps, us for f32 and bf16: w through shared memory 62, 40 (A was read from there for
+// each product); through tensor memory 61, 37; the MMA warp's loops walked by all lanes, so that an MMA's operands are
+// uniform values instead of 14 instructions each, 44, 36; k-blocks of 128 instead of 64, 41, 26.
+// Four epilogue warps, sixteen that convert, one that copies x, one that multiplies, two that only give their registers away:
 // 768 threads x 80 at launch = 128 x 152 + 512 x 64 + 128 x 72.
 #define LM_THREADS 768
+#define LM_BK 128
 
 template <typename T>
 struct lm_shape {
     static constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
-    static constexpr int X_BYTES = 64 * LT_BK * 2, STAGE_BYTES = PLANES * X_BYTES;  // shared memory: x
-    static constexpr int W_COLS = LT_BK / 2, STAGE_COLS = PLANES * W_COLS;  // tensor memory: w, two values to a column's word
-    static constexpr int STAGES = PLANES == 3 ? 3 : 6;
+    static constexpr int X_BYTES = 64 * LM_BK * 2, STAGE_BYTES = PLANES * X_BYTES;  // shared memory: x
+    static constexpr int W_COLS = LM_BK / 2, STAGE_COLS = PLANES * W_COLS;  // tensor memory: w, two values to a column's word
+    static constexpr int STAGES = PLANES == 3 ? 2 : 4;
     // accumulators of 64 columns: the tensor core goes on while the epilogue works on a tile's sums
     static constexpr int BUFFERS = (512 - STAGES * STAGE_COLS) / 64;
-    static constexpr int CHAIN = PLANES == 3 ? LT_CHAIN : 1 << 20;  // k-blocks per accumulator
+    static constexpr int CHAIN = PLANES == 3 ? LT_CHAIN * LT_BK / LM_BK : 1 << 20;  // k-blocks per accumulator
     static constexpr int SMEM = STAGES * STAGE_BYTES + 2 * 4 * 64 * 8 + 1024 + 256;
 };
 
@@ -749,10 +750,12 @@ __device__ __forceinline__ void lm_mma(uint32_t d, uint32_t a, uint64_t b, uint3
         "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void lm_st8(uint32_t taddr, const uint32_t (&h)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(h[0]), "r"(h[1]), "r"(h[2]),
-                 "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7])
-                 : "memory");
+__device__ __forceinline__ void lm_st16(uint32_t taddr, const uint32_t (&h)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]), "r"(h[8]), "r"(h[9]), "r"(h[10]), "r"(h[11]),
+        "r"(h[12]), "r"(h[13]), "r"(h[14]), "r"(h[15])
+        : "memory");
 }
 __device__ __forceinline__ void lm_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(lt_smem(bar)) : "memory");
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
     // the same in all lanes, and known to be: what follows from it is computed once per warp
     const int warp = __shfl_sync(RG_FULL_MASK, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int total = e.tiles * e.groups, nkb = (e.D + LT_BK - 1) / LT_BK;
+    const int total = e.tiles * e.groups, nkb = (e.D + LM_BK - 1) / LM_BK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) lt_bar_init(&full_w[s], 16), lt_bar_init(&full_x[s], 1), lt_bar_init(&empty[s], 1);
         for (int b = 0; b < S::BUFFERS; b++) lt_bar_init(&acc_full[b], 1), lt_bar_init(&acc_empty[b], 4);
@@ -823,72 +826,58 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
 
     if (warp >= 4 && warp < 20) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        // ===== w: a thread takes one column of the vocabulary (its lane of tensor memory) and 16 of the 64 rows of a k-block, so
-        // 32 lanes read side by side.  The values of the k-block after the next are loaded into the registers that the
-        // conversion of this one frees. =====
-        const int row = ((warp - 4) >> 2) * 16;
+        // ===== w: a thread takes one column of the vocabulary (its lane of tensor memory) and 32 of the 128 rows of a k-block, so
+        // 32 lanes read side by side.  The values of the next k-block are loaded into the registers that the conversion of this one
+        // frees. =====
+        const int row = ((warp - 4) >> 2) * 32;
         const T *w = static_cast<const T*>(e.w), *p = nullptr;
-        int t = blockIdx.x, kb = 0;  // of the loads, two k-blocks ahead
+        int t = blockIdx.x, kb = 0;  // of the loads, a k-block ahead
         const uint32_t blocks = (uint32_t)((total - t + (int)gridDim.x - 1) / (int)gridDim.x) * nkb;
         auto place = [&]() {
             const int v0 = (t / e.groups) * e.tile;
             p = w + (size_t)row * e.V + min(v0 + (warp & 3) * 32 + lane, min(e.V, v0 + e.tile) - 1);
         };
-        auto load = [&](uint32_t* r) {
-            const T* q = p + (size_t)(kb * LT_BK) * e.V;
-            const int rows = t < total ? e.D - kb * LT_BK - row : 0;
-            if (rows >= 16) {
+        uint32_t raw[32];
+        auto load = [&]() {
+            const T* q = p + (size_t)(kb * LM_BK) * e.V;
+            const int rows = t < total ? e.D - kb * LM_BK - row : 0;
+            if (rows >= 32) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) r[j] = lm_bits(q + (size_t)j * e.V);
+                for (int j = 0; j < 32; j++) raw[j] = lm_bits(q + (size_t)j * e.V);
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; j++) r[j] = j < rows ? lm_bits(q + (size_t)j * e.V) : 0u;
+                for (int j = 0; j < 32; j++) raw[j] = j < rows ? lm_bits(q + (size_t)j * e.V) : 0u;
             }
         };
-        auto next = [&]() {
+        place();
+        load();
+        for (uint32_t it = 0; it < blocks; it++) {
+            const int s = it % S::STAGES;
             if (++kb == nkb) {
                 kb = 0, t += gridDim.x;
                 if (t < total) place();
             }
-        };
-        uint32_t it = 0;
-        auto convert = [&](uint32_t (&raw)[16]) {
-            const int s = it % S::STAGES;
-            if (!lt_wait_warp(&empty[s], ((it / S::STAGES) & 1u) ^ 1u, e.err)) return false;
+            if (!lt_wait_warp(&empty[s], ((it / S::STAGES) & 1u) ^ 1u, e.err)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + s * S::STAGE_COLS + row / 2;
 #pragma unroll
-            for (int p2 = 0; p2 < S::PLANES; p2++) {
+            for (int q = 0; q < S::PLANES; q++) {
                 // f32: the leading 16 bits, and what they leave, which is exact (infinity leaves a NaN, NaN stays one)
-                uint32_t h[8];
+                uint32_t h[16];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (int j = 0; j < 16; j++) {
                     uint32_t &a = raw[2 * j], &b = raw[2 * j + 1];
-                    h[j] = S::PLANES == 1 ? __byte_perm(a, b, 0x5410) : __byte_perm(a, b, 0x7632);
+                    h[j] = __byte_perm(a, b, S::PLANES == 1 ? 0x5410 : 0x7632);
                     a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
                     b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
                 }
-                lm_st8(to + p2 * S::W_COLS, h);
+                lm_st16(to + q * S::W_COLS, h);
             }
-            load(raw);
-            next();
+            load();
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) lt_arrive(&full_w[s]);
-            it++;
-            return true;
-        };
-        uint32_t raw[2][16];
-        place();
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            load(raw[k]);
-            next();
-        }
-        while (it < blocks) {
-            if (!convert(raw[0]) || it == blocks) break;
-            if (!convert(raw[1])) break;
         }
     } else if (warp >= 20) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -905,7 +894,8 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
                                  : "memory");
                     unsigned char* x = ring + s * S::STAGE_BYTES;
 #pragma unroll
-                    for (int p = 0; p < S::PLANES; p++) lm_tma(&tmX, x + p * S::X_BYTES, &full_x[s], kb * LT_BK, (t % e.groups) * 64, p);
+                    for (int p = 0; p < 2 * S::PLANES; p++)  // 64 columns of a plane each; what lies outside x is filled with zeros
+                        lm_tma(&tmX, x + p * (S::X_BYTES / 2), &full_x[s], kb * LM_BK + (p & 1) * 64, (t % e.groups) * 64, p >> 1);
                 }
             // the copies have landed before the CTA's memory goes away, also where a wait gave up
             for (uint32_t i = it > (uint32_t)S::STAGES ? it - S::STAGES : 0; i < it; i++)
@@ -939,9 +929,9 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
 #pragma unroll
                             for (int pr = 0; pr < PRODUCTS; pr++)
 #pragma unroll
-                                for (int k = 0; k < LT_BK / 16; k++)
+                                for (int k = 0; k < LM_BK / 16; k++)
                                     lm_mma(d, a + (S::PLANES == 1 ? 0 : pa[pr]) * S::W_COLS + k * 8,
-                                               b + ((S::PLANES == 1 ? 0 : pb[pr]) * S::X_BYTES + k * 32) / 16, idesc, kb > 0 || pr > 0 || k > 0);
+                                               b + ((S::PLANES == 1 ? 0 : pb[pr]) * S::X_BYTES + (k >> 2) * (S::X_BYTES / 2) + (k & 3) * 32) / 16, idesc, kb > 0 || pr > 0 || k > 0);
                             lm_commit(&empty[s]);
                             if (kb + 1 == end) lm_commit(&acc_full[buf]);
                         }
@@ -1328,8 +1318,11 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
 static_assert(lt_shape<1>::BN == lt_shape<2>::BN, "the logits have one width of column tiles");
 #define LT_BN lt_shape<1>::BN
 
-// The form of lce_mid_kernel.
-static bool lm_takes(const lce_call& c) { return c.R <= LM_MOST_ROWS && (c.dtype == RG_DTYPE_F32 || c.V % 8); }
+// The form of lce_mid_kernel, by what was measured at [R,768] x [768,50257] (us for the call, and with packed or copied operands):
+// f32 forward 17 rows 53 (153), 128 rows 86 (152), 256 rows 139 (154); gradient 17 rows 229 (309), 192 rows 385 (402), 256
+// rows 462 (434); bf16 with an odd vocabulary forward 17 rows 39 (65), 128 rows 56 (65), 192 rows 67 (66).  With an aligned
+// one bf16 is read as it lies by TMA.
+static bool lm_takes(const lce_call& c) { return c.dtype == RG_DTYPE_F32 ? c.R <= 192 : c.R <= 128 && c.V % 8; }
 
 // Columns of a tile: as many tiles as whole rounds of the SMs hold.
 static int lm_tile(rg_ctx* ctx, const lce_call& c, int cols) {
