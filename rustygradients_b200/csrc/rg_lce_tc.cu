@@ -705,7 +705,8 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 // 4 bytes), split it in registers and store the planes to tensor memory, where it is the A operand; only x, which is small,
 // is packed before.  The sides are swapped: z^T = w^T x^T, 128 columns of the vocabulary are the lanes of a tile and 64 (32)
 // rows of x its columns, so a thread of the epilogue holds one column of the vocabulary.  f32 is split into bf16 triples (six
-// products, no scale), the accumulator is cut every 128 of K and the sum taken in registers with rounding.
+// products; no scale: what a value below 2^-117 has in its last bits is lost, bf16 has nothing smaller), the accumulator is
+// cut every 128 of K and the sum taken in registers with rounding.
 // Bound by the instructions of the split and by what one k-block ahead leaves in flight: 41 us for [17,768]x[768,50257], 3.8
 // TB/s of w (bf16 26 us, 2.9 TB/s).  Steps, us for f32 and bf16: w through shared memory 62, 40 (A was read from there for
 // each product); through tensor memory 61, 37; the MMA warp's loops walked by all lanes, so that an MMA's operands are
@@ -989,16 +990,13 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += bias;
                 const int tgt = lane < left ? __ldg(e.tgt + r0 + lane) : -1;  // of row `lane`
-                unsigned hits = __ballot_sync(RG_FULL_MASK, tgt >= v0 && tgt < v0 + e.tile);  // rows whose target is in the tile
+                const bool hits = __any_sync(RG_FULL_MASK, tgt >= v0 && tgt < v0 + e.tile);  // a row has its target in the tile
                 if (EPI == LT_FWD) {
-                    for (; hits; hits &= hits - 1) {
-                        const int r = __ffs(hits) - 1;
-                        const bool here = __shfl_sync(RG_FULL_MASK, tgt, r) == c && live;
+                    if (hits) {
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if (here && j == r) e.tz[r0 + j] = v[j];
+                            if (__shfl_sync(RG_FULL_MASK, tgt, j) == c && live) e.tz[r0 + j] = v[j];
                     }
-                    __syncwarp();
                     float m = 0.f;
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
@@ -1018,25 +1016,28 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
                         const float2 q = lt_exp2(make_float2(v[j], v[j + 1]), less);
                         v[j] = (dead >> j & 1) || !live ? 0.f : q.x, v[j + 1] = (dead >> (j + 1) & 1) || !live ? 0.f : q.y;
                     }
-                    for (; hits; hits &= hits - 1) {
-                        const int r = __ffs(hits) - 1;
-                        const bool here = __shfl_sync(RG_FULL_MASK, tgt, r) == c && live;
+                    if (hits) {
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if (here && j == r) v[j] -= 1.f;
+                            if (__shfl_sync(RG_FULL_MASK, tgt, j) == c && live) v[j] -= 1.f;
                     }
-                    __syncwarp();
-                    unsigned short* z = reinterpret_cast<unsigned short*>(e.dz + (size_t)r0 * e.cols + c);
+                    // Neighbouring lanes hold neighbouring columns: for each two rows they exchange halves, so an even lane stores
+                    // two columns of the first row and an odd lane of the second (e.cols, e.tile and v0 are even).
+                    const bool odd = lane & 1;
+                    const size_t plane = (size_t)e.R * e.cols;
+                    unsigned short* z = reinterpret_cast<unsigned short*>(e.dz + (size_t)(r0 + odd) * e.cols + (c - odd));
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        float d = v[j];
-                        db += d;
-                        if (!mine || j >= left) continue;
-                        unsigned short* o = z + (size_t)j * e.cols;
+                    for (int j = 0; j < 32; j += 2, z += 2 * (size_t)e.cols) {
+                        float d0 = v[j], d1 = v[j + 1];
+                        db += d0, db += d1;
 #pragma unroll
                         for (int p = 0; p < 3; p++) {
-                            o[(size_t)p * e.R * e.cols] = (unsigned short)(__float_as_uint(d) >> 16);
-                            d -= __uint_as_float(__float_as_uint(d) & 0xffff0000u);
+                            const uint32_t h = __byte_perm(__float_as_uint(d0), __float_as_uint(d1), 0x7632);  // rows j | j + 1
+                            const uint32_t other = __shfl_xor_sync(RG_FULL_MASK, h, 1);
+                            if (mine && j + odd < left)
+                                *reinterpret_cast<uint32_t*>(z + p * plane) = odd ? __byte_perm(other, h, 0x7632) : __byte_perm(h, other, 0x5410);
+                            d0 -= __uint_as_float(__float_as_uint(d0) & 0xffff0000u);
+                            d1 -= __uint_as_float(__float_as_uint(d1) & 0xffff0000u);
                         }
                     }
                 }
@@ -1456,7 +1457,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[2]));
     }
 
-    CUtensorMap mz[4], mg[4];
+    CUtensorMap mz[4] = {}, mg[4];
     lt_operand z = {o[0]->raw(), c.R, width, planes, width};
     if (!mid) RG_TRY(lt_map(&mz[0], x.logits, 128));
     if (!mid) RG_TRY(lt_map(&mz[1], w.logits, LT_BK));
