@@ -1,4 +1,5 @@
-// Linear cross entropy on the tensor cores (sm_100a): the three contractions of rg_lce.cuh for many rows.
+// Linear cross entropy on the tensor cores (sm_100a): the three contractions of rg_lce.cuh for many rows (lce_tc_kernel), and
+// the logits of a few row tiles straight from w (lce_mid_kernel).
 //
 //   logits  z[R,V]  = x[R,D] w[D,V]      -> (maximum, sum) per row and tile, or dz of a piece of the vocabulary
 //   dx      [R,D]   = dz[R,V] w[D,V]^T
@@ -42,6 +43,10 @@
 // Two CTAs (two SMs) work on one tile of 256 x BN: each holds 128 rows of A, half of the columns of B, and the accumulator
 // of its 128 rows.  A k-block then costs an SM 128 x 64 + BN/2 x 64 values from L2 instead of 128 x 64 + BN x 64, which
 // bounded the one-SM form (12.5 TB/s from L2, 1.09 PFLOP/s in bf16).
+// Measured (PFLOP/s of the products that are multiplied; a library product of bf16 reaches 1.6, 1.37 for seconds on end):
+// logits of 4096x768x50257 f32 1.49 (640 us, tensor pipe active 80 %), of 8192x768x50257 bf16 1.26 (504 us, 63 %: one product
+// for each operand brought from L2, 64 bytes a clock and SM at full rate); gradient of 2048x768x50257 f32: dz 0.95 (47 %, its
+// three planes are stored), dx and dw 1.32 (68 %); of 4096x1600x50257 bf16: dz 1.28, dx and dw 1.21.
 // PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.
 template <int PLANES>
 struct lt_shape {
@@ -708,7 +713,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
 // products; no scale: what a value below 2^-117 has in its last bits is lost, bf16 has nothing smaller), the accumulator is
 // cut every 128 of K and the sum taken in registers with rounding.
 // Bound by the instructions of the split and by what one k-block ahead leaves in flight: 41 us for [17,768]x[768,50257], 3.8
-// TB/s of w (bf16 26 us, 2.9 TB/s).  Steps, us for f32 and bf16: w through shared memory 62, 40 (A was read from there for
+// TB/s of w (bf16 26 us, 2.9 TB/s); dz of 64 rows 53 us.  Steps, us for f32 and bf16: w through shared memory 62, 40 (A was read from there for
 // each product); through tensor memory 61, 37; the MMA warp's loops walked by all lanes, so that an MMA's operands are
 // uniform values instead of 14 instructions each, 44, 36; k-blocks of 128 instead of 64, 41, 26.
 // Four epilogue warps, sixteen that convert, one that copies x, one that multiplies, two that only give their registers away:
@@ -1073,7 +1078,8 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // operands
 // ---------------------------------------------------------------------------
-// A bf16 matrix whose rows TMA cannot address (they do not start on 16-byte boundaries), copied to such rows.
+// A bf16 matrix whose rows TMA cannot address (they do not start on 16-byte boundaries), copied to such rows (768 x 50257: 26
+// us, 5.9 TB/s).
 __global__ void __launch_bounds__(256) lt_align_kernel(const __nv_bfloat16* __restrict__ src, long long rows, int cols, int pitch,
                                                        __nv_bfloat16* __restrict__ dst) {
     rg_pdl_sync();
@@ -1177,7 +1183,8 @@ __global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ s
 
 // w as pairs of f16 with one scale for the whole matrix, and triples of bf16, or one of them.  A thread takes 8
 // neighbouring values of a row and writes 16 bytes of each plane.  The values are walked from the end: what the last-level
-// cache still holds of lt_max_kernel's pass is read from there.  Memory bound: 4 bytes in, 4 (10 with the triples) out.
+// cache still holds of lt_max_kernel's pass is read from there.  Memory bound: 4 bytes in, 4 (6, 10) out for pairs (triples,
+// both); 768 x 50257: 52 (62, 89) us, 5.9 to 6.2 TB/s, and 30 us for the pass before.
 template <bool PAIR, bool TRIPLE>
 __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                       const unsigned* __restrict__ largest, uint16_t* __restrict__ pair,
