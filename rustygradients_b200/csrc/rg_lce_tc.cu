@@ -44,9 +44,9 @@
 // of its 128 rows.  A k-block then costs an SM 128 x 64 + BN/2 x 64 values from L2 instead of 128 x 64 + BN x 64, which
 // bounded the one-SM form (12.5 TB/s from L2, 1.09 PFLOP/s in bf16).
 // Measured (PFLOP/s of the products that are multiplied; a library product of bf16 reaches 1.6, 1.37 for seconds on end):
-// logits of 4096x768x50257 f32 1.49 (640 us, tensor pipe active 80 %), of 8192x768x50257 bf16 1.26 (504 us, 63 %: one product
-// for each operand brought from L2, 64 bytes a clock and SM at full rate); gradient of 2048x768x50257 f32: dz 0.95 (47 %, its
-// three planes are stored), dx and dw 1.32 (68 %); of 4096x1600x50257 bf16: dz 1.28, dx and dw 1.21.
+// logits of 4096x768x50257 f32 1.49 (640 us, tensor pipe active 80 %), of 8192x768x50257 bf16 1.26 (504 us, 63 %; 447 us when
+// nothing is brought from L2, 487 when the epilogue does nothing); gradient of 2048x768x50257 f32: dz 0.95 (502 us, 47 %; 340
+// without its planes and column sums), dx and dw 1.32 (68 %); of 4096x1600x50257 bf16: dz 1.28, dx and dw 1.21.
 // PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.
 template <int PLANES>
 struct lt_shape {
@@ -937,7 +937,8 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
 #pragma unroll
                                 for (int k = 0; k < LM_BK / 16; k++)
                                     lm_mma(d, a + (S::PLANES == 1 ? 0 : pa[pr]) * S::W_COLS + k * 8,
-                                               b + ((S::PLANES == 1 ? 0 : pb[pr]) * S::X_BYTES + (k >> 2) * (S::X_BYTES / 2) + (k & 3) * 32) / 16, idesc, kb > 0 || pr > 0 || k > 0);
+                                           b + ((S::PLANES == 1 ? 0 : pb[pr]) * S::X_BYTES + (k >> 2) * (S::X_BYTES / 2) + (k & 3) * 32) / 16,
+                                           idesc, kb > 0 || pr > 0 || k > 0);
                             lm_commit(&empty[s]);
                             if (kb + 1 == end) lm_commit(&acc_full[buf]);
                         }
@@ -1313,8 +1314,8 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
         RG_CUDA(rg_launch(true, !want_grads ? lt_pack_kernel<true, false> : want_logits ? lt_pack_kernel<true, true> : lt_pack_kernel<false, true>,
                           dim3(grid), dim3(256), 0, ctx->stream, w, rows, cols, pitch, (const unsigned*)largest, two, three, o->mem[1]->data()));
     } else {
-        RG_CUDA(rg_launch(true, lt_pack_rows_kernel, dim3((unsigned)rg_cdiv(rows, 8)), dim3(256), 0, ctx->stream, static_cast<const float*>(src), rows,
-                          cols, pitch, two, three, o->mem[1]->data()));
+        RG_CUDA(rg_launch(true, lt_pack_rows_kernel, dim3((unsigned)rg_cdiv(rows, 8)), dim3(256), 0, ctx->stream,
+                          static_cast<const float*>(src), rows, cols, pitch, two, three, o->mem[1]->data()));
     }
     RG_CUDA(cudaGetLastError());
     RG_LAUNCHED(ctx);
