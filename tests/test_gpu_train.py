@@ -695,3 +695,130 @@ def test_training_step_behind_the_last_block(backend, rows, dtype):
     ana = sum((get(be, got).reshape(q.shape) * q).sum() for got, q in zip((dh, dg, db, dw, dbias), v))
     size = sum(np.abs(x * q).sum() for x, q in zip(want, v))
     assert abs(num - ana) <= tol * (1 + np.abs(ex["z"]).max()) * size / 10 + 1e-6
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_calls_from_several_threads(backend, shared):
+    """Three threads with the forms of all sizes, on one context (its calls take turns) and on one each (their kernels share
+    the GPU): every result has the bits of the call alone."""
+    import threading
+    shapes = [(3, 130, 2001, "f32"), (40, 130, 2001, "f32"), (40, 130, 2001, "bf16"), (300, 130, 2001, "f32"), (300, 136, 2000, "bf16")]
+
+    def run(be, order):
+        out = {}
+        for k in order:
+            R, D, V, dtype = shapes[k]
+            x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.1, k)
+            X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t)
+            loss, lse = be.linear_cross_entropy(X, W, B, T)
+            dx, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, lse)
+            y, m, r = be.layer_norm_fwd(dx, be.ones([D]), be.zeros([D]), EPS)
+            clipped, norm = be.clip_grad_norm([dw, db, y], 1e-3)
+            out[k] = [be.to_vec(s) for s in (loss, lse, dx, dw, db, y, m, r, norm, *clipped)]
+        return out
+
+    alone = run(backend, range(len(shapes)))
+    got, backends = [None] * 3, [backend if shared else rg.B200Backend(0) for _ in range(3)]
+
+    def work(i):
+        got[i] = [run(backends[i], [(k + 2 * i) % len(shapes) for k in range(len(shapes))]) for _ in range(4)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for rounds in got:
+        for out in rounds:
+            for k, want in alone.items():
+                assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(out[k], want)), shapes[k]
+
+
+@pytest.mark.parametrize("R,dtype", [(3, "f32"), (20, "f32"), (200, "f32"), (3, "bf16"), (20, "bf16"), (200, "bf16")])
+def test_linear_cross_entropy_beyond_32_bits(R, dtype):
+    """A matrix of more than 2^31 values: the logits, dz and gradients of its last columns."""
+    import torch
+    torch.cuda.set_device(0)
+    stream = torch.cuda.current_stream()
+    be = rg.B200Backend(0, stream=stream.cuda_stream)
+    D, V, step = 180, 12000001, 1 << 20
+    assert D * V > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(R)
+    kind = torch.float32 if dtype == "f32" else torch.bfloat16
+    w = torch.empty(D, V, device="cuda", dtype=kind)
+    for v in range(0, V, step):
+        w[:, v:v + step] = torch.randn(D, min(step, V - v), device="cuda", generator=gen) * (2.5 / D ** 0.5)
+    x = torch.randn(R, D, device="cuda", generator=gen).to(kind)
+    t = (V - 1 - torch.randint(0, 1000, (R,), device="cuda", generator=gen)).float()
+    pieces, xd = [], x.double()
+    mags = torch.zeros(R, device="cuda", dtype=torch.float64)
+    for v in range(0, V, step):
+        wd = w[:, v:v + step].double()
+        pieces.append(torch.logsumexp(xd @ wd, -1))
+        mags = torch.maximum(mags, (xd.abs() @ wd.abs()).amax(-1))
+    exact = torch.logsumexp(torch.stack(pieces), 0)
+    X, W, T = be.from_device(x), be.from_device(w), be.from_device(t)
+    loss, lse = be.linear_cross_entropy(X, W, None, T)
+    # as ce_bounds has it, with the partial sums of the slices (at least 64 columns) in 32 chains
+    steps = max(2 * (D / 16 + 2) if dtype == "bf16" else 40 + D / 256, D / 8 + 8)
+    tol = steps * E32 * mags + (300 + V / 64 / 32) * E32 + 4 * E32 * (exact.abs() + 1)
+    got = torch.from_dlpack(lse).double()
+    assert bool(((got - exact).abs() <= tol).all())
+    wt = w[:, t.long()].double()
+    assert abs(torch.from_dlpack(loss).item() - (exact - (xd * wt.T).sum(-1)).mean().item()) <= 2 * tol.max().item()
+    dx, dw, _ = be.linear_cross_entropy_bwd(X, W, None, T, be.from_device(exact.float()))
+    tail = 5000
+    wd = w[:, V - tail:].double()
+    z = xd @ wd
+    p = torch.exp(z - exact[:, None])
+    dz = p.clone()
+    dz[torch.arange(R), (t.long() - (V - tail))] -= 1
+    edz = p * (steps * E32 * (xd.abs() @ wd.abs()) + 3 * E32 * (z.abs() + exact.abs()[:, None]) + 4 * E32) * 1.01 + E32 * dz.abs()
+    ez = edz + (2.0 ** -21 if dtype == "f32" else U["bf16"] * 1.01) * dz.abs()
+    want = xd.T @ dz / R
+    tol = xd.abs().T @ (ez + (40 + R / 8) * E32 * dz.abs()) / R
+    got = torch.from_dlpack(dw)[:, V - tail:].double()
+    assert bool(((got - want).abs() <= tol + (U[dtype] + 3 * E32) * (want.abs() + tol) + 1e-45).all())
+    # dx: the targets' columns, all of them at the end, carry nearly all of it; the rest are 12 million tiny terms
+    want, bound = dz @ wd.T, (ez + (40 + V / 16) * E32 * dz.abs()) @ wd.abs().T
+    for v in range(0, V - tail, step):
+        wd = w[:, v:min(v + step, V - tail)].double()
+        p = torch.exp(xd @ wd - exact[:, None])
+        e = (steps + 40 + V / 16) * E32 * p * (1 + mags[:, None] + exact.abs()[:, None]) + (2.0 ** -21 if dtype == "f32" else U["bf16"] * 1.01) * p
+        want, bound = want + p @ wd.T, bound + e @ wd.abs().T
+    got, want, bound = torch.from_dlpack(dx).double(), want / R, bound / R
+    assert bool(((got - want).abs() <= bound + (U[dtype] + 3 * E32) * (want.abs() + bound) + 1e-45).all())
+    # and the same call gives the first columns too: bf16 rounds dz and dw by 2^-8 each, the exponentials are off by less than 1 %
+    z = xd @ w[:, :64].double()
+    want = xd.T @ torch.exp(z - exact[:, None]) / R
+    assert bool((torch.from_dlpack(dw)[:, :64].double() - want).abs().max() <= 0.02 * want.abs().max())
+
+
+def test_rows_and_tensors_beyond_32_bits():
+    import torch
+    torch.cuda.set_device(0)
+    be = rg.B200Backend(0, stream=torch.cuda.current_stream().cuda_stream)
+    rows, n, last = 140000, 16000, 4
+    assert rows * n > 2 ** 31
+    x = torch.zeros(rows, n, device="cuda", dtype=torch.bfloat16)
+    dy = torch.zeros(rows, n, device="cuda", dtype=torch.bfloat16)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x[-last:] = torch.randn(last, n, device="cuda", generator=gen).bfloat16()
+    dy[-last:] = torch.randn(last, n, device="cuda", generator=gen).bfloat16()
+    g = torch.randn(n, device="cuda", generator=gen)
+    G, B = be.from_device(g), be.from_device(torch.zeros(n, device="cuda"))
+
+    def step(x, dy):
+        X, DY = be.from_device(x), be.from_device(dy)
+        y, m, r = be.layer_norm_fwd(X, G, B, EPS)
+        return [torch.from_dlpack(s) for s in (y, m, r, *be.layer_norm_bwd(DY, X, G, m, r))]
+
+    big, small = step(x, dy), step(x[-last:], dy[-last:])
+    assert all(torch.equal(a[-last:], b) for a, b in zip(big[:4], small[:4]))
+    # rows of zeros add nothing to the column sums; the order of the others' additions may differ
+    assert all(torch.allclose(a, b, rtol=0, atol=8 * E32 * float(dy.abs().max() * 6 * last)) for a, b in zip(big[4:], small[4:]))
+    clipped, norm = be.clip_grad_norm([be.from_device(x)], 1.0)
+    exact = x[-last:].double().norm().item()
+    assert abs(torch.from_dlpack(norm).item() / exact - 1) <= 2 * E32
+    got, want = torch.from_dlpack(clipped[0]), x[-last:].double() / exact
+    assert bool(((got[-last:].double() - want).abs() <= (U["bf16"] + 3 * E32) * want.abs() + 1e-40).all()) and not bool(got[:last].any())
