@@ -169,7 +169,8 @@ __device__ __forceinline__ float ln_half(float2 v, int i) { return i & 1 ? v.y :
 // x serves all three: a group walks rows, every thread always on the same columns, so the column sums stay in its registers
 // until the end; then the CTA's groups are added and the CTA leaves one partial row of sums, which rg_colsum_kernel adds over
 // the CTAs.  Memory bound: dy and x in, dx out; the next row's loads are in flight behind the sums of this one.  16384 x 1600
-// bf16: 33 us, 4.8 TB/s (the 32 column sums of a thread leave registers for one row ahead only), and 5.6 us for the sums.
+// bf16: 33 us, 4.8 TB/s, and 5.6 us for the sums; bound by the two sums of every row, which 16 warps an SM (their 32 column
+// sums a thread fill the registers) do not hide: rows further ahead, through shared memory, gained nothing.
 template <typename T, int VEC, int PER, int WPR, int THREADS>
 __global__ void __launch_bounds__(THREADS, LN_BWD_CTAS(THREADS, PER * VEC)) rg_ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                             const float* __restrict__ gamma, const float* __restrict__ mean,
