@@ -122,12 +122,31 @@ __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict_
     if (threadIdx.x == 0) loss[0] = scal[0] > 0.f ? (float)(tot[0] / (double)scal[0]) : 0.f;
 }
 
+// The final sums of the gradient: the first `xblocks` blocks those of dx (or dw), the others 32 columns of dbias each, eight
+// warps sharing the partials.  (A launch of its own for dbias cost 3 us.)
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) lce_dx_finish_kernel(const float* __restrict__ parts, int nparts, size_t count,
-                                                            const float* __restrict__ scal, T* __restrict__ dx) {
+__global__ void __launch_bounds__(256) lce_finish_kernel(const float* __restrict__ parts, int nparts, size_t count, const float* __restrict__ scal,
+                                                         T* __restrict__ dx, int xblocks, const float* __restrict__ dbparts, int dbrows, int V,
+                                                         float* __restrict__ dbias) {
+    __shared__ float red[8][32];
     rg_pdl_sync();
     const float scale = scal[1];
-    const size_t stride = (size_t)gridDim.x * 256 * VEC;
+    if ((int)blockIdx.x >= xblocks) {
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+        const int c = ((int)blockIdx.x - xblocks) * 32 + lane;
+        float s = 0.f;
+        if (c < V)
+#pragma unroll 8
+            for (int p = w; p < dbrows; p += 8) s += dbparts[(size_t)p * V + c];
+        red[w][lane] = s;
+        __syncthreads();
+        if (w || c >= V) return;
+#pragma unroll
+        for (int k = 1; k < 8; k++) s += red[k][lane];
+        dbias[c] = s * scale;
+        return;
+    }
+    const size_t stride = (size_t)xblocks * 256 * VEC;
     for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * VEC; i < count; i += stride) {
         if constexpr (VEC == 4) {
             float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -145,40 +164,20 @@ __global__ void __launch_bounds__(256) lce_dx_finish_kernel(const float* __restr
     }
 }
 template <typename T>
-static void lce_dx_finish_typed(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, T* dx) {
+static void lce_finish_typed(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, T* dx, const float* dbparts,
+                             int dbrows, int V, float* dbias) {
     // four values a thread where every partial starts on a 16-byte boundary and there are threads enough (768 values and 50
     // partials: 15 us against 6; 6.5 million values and one partial: 9 us against 26)
     const bool vec = count % 4 == 0 && count >= ((size_t)1 << 19);
-    const unsigned grid = (unsigned)std::min<size_t>((count + (vec ? 1023 : 255)) / (vec ? 1024 : 256), (size_t)ctx->sm_count * 16);
-    if (vec) rg_launch(true, lce_dx_finish_kernel<T, 4>, dim3(grid), dim3(256), 0, ctx->stream, parts, nparts, count, scal, dx);
-    else rg_launch(true, lce_dx_finish_kernel<T, 1>, dim3(grid), dim3(256), 0, ctx->stream, parts, nparts, count, scal, dx);
+    const int xblocks = (int)std::min<size_t>((count + (vec ? 1023 : 255)) / (vec ? 1024 : 256), (size_t)ctx->sm_count * 16);
+    rg_launch(true, vec ? lce_finish_kernel<T, 4> : lce_finish_kernel<T, 1>, dim3((unsigned)(xblocks + (dbias ? rg_cdiv(V, 32) : 0))), dim3(256),
+              0, ctx->stream, parts, nparts, count, scal, dx, xblocks, dbparts, dbrows, V, dbias);
     RG_LAUNCHED(ctx);
 }
-void lce_dx_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* dx, int dtype) {
-    if (dtype == RG_DTYPE_F32) lce_dx_finish_typed(ctx, parts, nparts, count, scal, (float*)dx);
-    else lce_dx_finish_typed(ctx, parts, nparts, count, scal, (__nv_bfloat16*)dx);
-}
-
-__global__ void __launch_bounds__(256) lce_dbias_finish_kernel(const float* __restrict__ parts, int nparts, int V,
-                                                               const float* __restrict__ scal, float* __restrict__ out) {
-    __shared__ float red[8][32];
-    rg_pdl_sync();
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
-    float s = 0.f;
-    if (c < V)
-#pragma unroll 8
-        for (int p = w; p < nparts; p += 8) s += parts[(size_t)p * V + c];
-    red[w][lane] = s;
-    __syncthreads();
-    if (w || c >= V) return;
-#pragma unroll
-    for (int k = 1; k < 8; k++) s += red[k][lane];
-    out[c] = s * scal[1];
-}
-void lce_dbias_finish_launch(rg_ctx* ctx, const float* parts, int nparts, int V, const float* scal, float* dbias) {
-    rg_launch(true, lce_dbias_finish_kernel, dim3((unsigned)rg_cdiv(V, 32)), dim3(256), 0, ctx->stream, parts, nparts, V, scal, dbias);
-    RG_LAUNCHED(ctx);
+void lce_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* out, int dtype,
+                          const float* dbparts, int dbrows, int V, float* dbias) {
+    if (dtype == RG_DTYPE_F32) lce_finish_typed(ctx, parts, nparts, count, scal, (float*)out, dbparts, dbrows, V, dbias);
+    else lce_finish_typed(ctx, parts, nparts, count, scal, (__nv_bfloat16*)out, dbparts, dbrows, V, dbias);
 }
 
 // ---------------------------------------------------------------------------
@@ -678,7 +677,7 @@ extern "C" rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* 
             RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[4]));
             RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[5]));
             lce_few_backward(ctx, c, o[4]->data(), o[5]->data());
-            lce_dx_finish_launch(ctx, o[5]->data(), (int)nparts, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
+            lce_finish_launch(ctx, o[5]->data(), (int)nparts, (size_t)c.R * c.D, c.scal, c.dx, c.dtype, nullptr, 0, 0, nullptr);
         } else {
             RG_TRY(lce_tc_backward(ctx, c));
         }

@@ -1137,33 +1137,48 @@ __device__ __forceinline__ void lt_split2(float v, float scale, uint32_t& h0, ui
 
 // x as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row, and triples of bf16 (either NULL: not wanted).
 // A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
-__global__ void __launch_bounds__(256) lt_pack_rows_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
-                                                           uint16_t* __restrict__ pair, uint16_t* __restrict__ triple,
-                                                           float* __restrict__ scale_out) {
-    rg_pdl_sync();
-    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= rows) return;
-    const float* p = src + (size_t)r * cols;
+struct lt_rows {
+    const float* src;
+    int rows, cols, pitch;
+    uint16_t *pair, *triple;
+    float* scale;
+};
+__device__ __forceinline__ void lt_pack_row(const lt_rows& x, int r) {
+    const int lane = threadIdx.x & 31;
+    if (r >= x.rows) return;
+    const float* __restrict__ p = x.src + (size_t)r * x.cols;
+    uint16_t* __restrict__ pair = x.pair ? x.pair + (size_t)r * x.pitch : nullptr;
+    uint16_t* __restrict__ triple = x.triple ? x.triple + (size_t)r * x.pitch : nullptr;
     float m = 0.f;
     if (pair)
 #pragma unroll 8
-        for (int c = lane; c < cols; c += 32) m = fmaxf(m, lt_finite_abs(p[c]));
+        for (int c = lane; c < x.cols; c += 32) m = fmaxf(m, lt_finite_abs(__ldg(p + c)));
     const float2 sc = lt_scale(rg_warp_max(m));
-    if (pair && lane == 0) scale_out[r] = sc.y;
-    const size_t plane = (size_t)rows * pitch;
-#pragma unroll 4
-    for (int c = lane; c < cols; c += 32) {
-        const size_t at = (size_t)r * pitch + c;
-        uint32_t h0, h1, h2;
-        if (pair) {
-            lt_split2(p[c], sc.x, h0, h1);
-            pair[at] = (uint16_t)h0, pair[at + plane] = (uint16_t)h1;
-        }
-        if (triple) {
-            lt_split3(p[c], h0, h1, h2);
-            triple[at] = (uint16_t)h0, triple[at + plane] = (uint16_t)h1, triple[at + 2 * plane] = (uint16_t)h2;
+    if (pair && lane == 0) x.scale[r] = sc.y;
+    const size_t plane = (size_t)x.rows * x.pitch;
+    for (int c0 = lane; c0 < x.cols; c0 += 128) {
+        float v[4];  // loads first
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = c0 + 32 * k < x.cols ? __ldg(p + c0 + 32 * k) : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int c = c0 + 32 * k;
+            if (c >= x.cols) break;
+            uint32_t h0, h1, h2;
+            if (pair) {
+                lt_split2(v[k], sc.x, h0, h1);
+                pair[c] = (uint16_t)h0, pair[c + plane] = (uint16_t)h1;
+            }
+            if (triple) {
+                lt_split3(v[k], h0, h1, h2);
+                triple[c] = (uint16_t)h0, triple[c + plane] = (uint16_t)h1, triple[c + 2 * plane] = (uint16_t)h2;
+            }
         }
     }
+}
+__global__ void __launch_bounds__(256) lt_pack_rows_kernel(const lt_rows x) {
+    rg_pdl_sync();
+    lt_pack_row(x, blockIdx.x * 8 + (threadIdx.x >> 5));
 }
 
 // Largest finite magnitude of w (as bits: they order like the values), into a word that lce_check_kernel has set to 0.
@@ -1185,18 +1200,24 @@ __global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ s
 // w as pairs of f16 with one scale for the whole matrix, and triples of bf16, or one of them.  A thread takes 8
 // neighbouring values of a row and writes 16 bytes of each plane.  The values are walked from the end: what the last-level
 // cache still holds of lt_max_kernel's pass is read from there.  Memory bound: 4 bytes in, 4 (6, 10) out for pairs (triples,
-// both); 768 x 50257: 52 (62, 89) us, 5.9 to 6.2 TB/s, and 30 us for the pass before.
+// both); 768 x 50257: 52 (62, 89) us, 5.9 to 6.2 TB/s, and 30 us for the pass before.  The first blocks pack x, which took a
+// launch of 4 to 8 us of its own.
 template <bool PAIR, bool TRIPLE>
 __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
                                                       const unsigned* __restrict__ largest, uint16_t* __restrict__ pair,
-                                                      uint16_t* __restrict__ triple, float* __restrict__ scale_out) {
+                                                      uint16_t* __restrict__ triple, float* __restrict__ scale_out, const lt_rows x) {
     rg_pdl_sync();
+    const int xblocks = (x.rows + 7) / 8, block = (int)blockIdx.x - xblocks;
+    if (block < 0) {
+        lt_pack_row(x, blockIdx.x * 8 + (threadIdx.x >> 5));
+        return;
+    }
     const float2 sc = PAIR ? lt_scale(__uint_as_float(*largest)) : make_float2(1.f, 1.f);
-    if (PAIR && blockIdx.x == 0 && threadIdx.x == 0) *scale_out = sc.y;
+    if (PAIR && block == 0 && threadIdx.x == 0) *scale_out = sc.y;
     const int groups = pitch / 8;
-    const long long n = (long long)rows * groups, stride = (long long)gridDim.x * 256;
+    const long long n = (long long)rows * groups, stride = (long long)(gridDim.x - xblocks) * 256;
     const size_t plane = (size_t)rows * pitch;
-    for (long long i = n - 1 - ((long long)blockIdx.x * 256 + threadIdx.x); i >= 0; i -= stride) {
+    for (long long i = n - 1 - ((long long)block * 256 + threadIdx.x); i >= 0; i -= stride) {
         const long long r = i / groups;
         const int c = (int)(i - r * groups) * 8;
         float v[8];
@@ -1274,18 +1295,19 @@ static rg_status lt_map(CUtensorMap* map, const lt_operand& o, int box_rows) {
 struct lt_packed {
     lt_operand logits, grads;
     const float* scale;
+    lt_rows rows;  // f32 x: what is still to be packed
     rg_outputs<3> mem;
 };
-// `largest` (w): a word that is 0, for one scale over the matrix; NULL (x): a scale per row.
-static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, unsigned* largest, bool want_logits, bool want_grads,
-                         lt_packed* o) {
+// Allocates the planes of a matrix, or copies the rows of a bf16 one that TMA cannot address.
+static rg_status lt_planes(rg_ctx* ctx, const void* src, int rows, int cols, int dtype, size_t scales, bool want_logits, bool want_grads,
+                           lt_packed* o) {
     o->scale = nullptr;
     if (dtype == RG_DTYPE_BF16 && cols % 8 == 0) {
         o->logits = o->grads = {src, rows, cols, 1, cols};
         return RG_OK;
     }
     const int pitch = (cols + 7) / 8 * 8;
-    const size_t plane = (size_t)rows * pitch, pair = 2 * plane, triple = 3 * plane, scales = largest ? 1 : rows;
+    const size_t plane = (size_t)rows * pitch, pair = 2 * plane, triple = 3 * plane;
     if (dtype == RG_DTYPE_BF16) {
         RG_TRY(rg_alloc_storage(ctx, &plane, 1, &o->mem[0], RG_DTYPE_BF16));
         const int grid = (int)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
@@ -1296,31 +1318,39 @@ static rg_status lt_pack(rg_ctx* ctx, const void* src, int rows, int cols, int d
         return RG_OK;
     }
     if (want_logits) RG_TRY(rg_alloc_storage(ctx, &pair, 1, &o->mem[0], RG_DTYPE_BF16));
-    RG_TRY(rg_alloc_storage(ctx, &scales, 1, &o->mem[1]));
+    if (want_logits) RG_TRY(rg_alloc_storage(ctx, &scales, 1, &o->mem[1]));
     if (want_grads) RG_TRY(rg_alloc_storage(ctx, &triple, 1, &o->mem[2], RG_DTYPE_BF16));
     uint16_t* two = want_logits ? static_cast<uint16_t*>(o->mem[0]->raw()) : nullptr;
     uint16_t* three = want_grads ? static_cast<uint16_t*>(o->mem[2]->raw()) : nullptr;
-    o->scale = o->mem[1]->data();
-    if (largest) {
-        const float* w = static_cast<const float*>(src);
-        const size_t n = (size_t)rows * cols;
-        const int most = ctx->sm_count * 16;
-        if (want_logits) {
-            RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, ctx->sm_count * 8))),
-                              dim3(256), 0, ctx->stream, w, n, largest));
-            RG_LAUNCHED(ctx);
-        }
-        const unsigned grid = (unsigned)std::min<long long>(((long long)rows * (pitch / 8) + 255) / 256, most);
-        RG_CUDA(rg_launch(true, !want_grads ? lt_pack_kernel<true, false> : want_logits ? lt_pack_kernel<true, true> : lt_pack_kernel<false, true>,
-                          dim3(grid), dim3(256), 0, ctx->stream, w, rows, cols, pitch, (const unsigned*)largest, two, three, o->mem[1]->data()));
-    } else {
-        RG_CUDA(rg_launch(true, lt_pack_rows_kernel, dim3((unsigned)rg_cdiv(rows, 8)), dim3(256), 0, ctx->stream,
-                          static_cast<const float*>(src), rows, cols, pitch, two, three, o->mem[1]->data()));
-    }
-    RG_CUDA(cudaGetLastError());
-    RG_LAUNCHED(ctx);
+    float* scale = want_logits ? o->mem[1]->data() : nullptr;
+    o->scale = scale;
+    o->rows = {static_cast<const float*>(src), rows, cols, pitch, two, three, scale};
     o->logits = {two, rows, cols, 2, pitch};
     o->grads = {three, rows, cols, 3, pitch};
+    return RG_OK;
+}
+// x and (w_too) w as the kernels read them.  A scale per row of x, one for w.
+static rg_status lt_pack(rg_ctx* ctx, const lce_call& c, bool w_too, bool want_logits, bool want_grads, lt_packed* x, lt_packed* w) {
+    RG_TRY(lt_planes(ctx, c.x, c.R, c.D, c.dtype, (size_t)c.R, want_logits, want_grads, x));
+    if (w_too) RG_TRY(lt_planes(ctx, c.w, c.D, c.V, c.dtype, 1, want_logits, want_grads, w));
+    if (c.dtype == RG_DTYPE_BF16) return RG_OK;
+    const int xblocks = rg_cdiv(c.R, 8);
+    if (!w_too) {
+        RG_CUDA(rg_launch(true, lt_pack_rows_kernel, dim3((unsigned)xblocks), dim3(256), 0, ctx->stream, x->rows));
+    } else {
+        const lt_rows& m = w->rows;
+        if (want_logits) {
+            const size_t n = (size_t)m.rows * m.cols;
+            const size_t grid = std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, (size_t)ctx->sm_count * 8));
+            RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, m.src, n, c.wmax));
+            RG_LAUNCHED(ctx);
+        }
+        const unsigned grid = (unsigned)std::min<long long>(((long long)m.rows * (m.pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
+        RG_CUDA(rg_launch(true, !want_grads ? lt_pack_kernel<true, false> : want_logits ? lt_pack_kernel<true, true> : lt_pack_kernel<false, true>,
+                          dim3(xblocks + grid), dim3(256), 0, ctx->stream, m.src, m.rows, m.cols, m.pitch, (const unsigned*)c.wmax, m.pair,
+                          m.triple, m.scale, x->rows));
+    }
+    RG_LAUNCHED(ctx);
     return RG_OK;
 }
 
@@ -1394,14 +1424,13 @@ static void lt_common(rg_ctx* ctx, const lce_call& c, int* counter, lt_args* e) 
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     lt_packed x, w;
     if (lm_takes(c)) {
-        RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, false, true, &x));
+        RG_TRY(lt_pack(ctx, c, false, false, true, &x, nullptr));
         lm_args e;
         memset(&e, 0, sizeof(e));
         e.cols = c.V;
         return c.dtype == RG_DTYPE_F32 ? lm_launch<float, LT_FWD>(ctx, c, x, e) : lm_launch<__nv_bfloat16, LT_FWD>(ctx, c, x, e);
     }
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, true, false, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, true, false, &w));
+    RG_TRY(lt_pack(ctx, c, true, true, false, &x, &w));
     CUtensorMap maps[4];
     RG_TRY(lt_map(&maps[0], x.logits, 128));
     RG_TRY(lt_map(&maps[1], w.logits, LT_BK));
@@ -1433,8 +1462,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     const int clusters = ctx->sm_count / 2;
     const int piece = lt_piece(c), pieces = rg_cdiv(c.V, piece);
     const bool mid = c.dtype == RG_DTYPE_F32 && lm_takes(c) && pieces == 1;  // bf16: w is copied for dx all the same
-    RG_TRY(lt_pack(ctx, c.x, c.R, c.D, c.dtype, nullptr, !mid, true, &x));
-    RG_TRY(lt_pack(ctx, c.w, c.D, c.V, c.dtype, c.wmax, !mid, true, &w));
+    RG_TRY(lt_pack(ctx, c, true, !mid, true, &x, &w));
 
     const int width = std::min(piece, (c.V + 63) / 64 * 64);  // columns of dz that are stored
     const size_t zlen = (size_t)planes * c.R * width;
@@ -1504,8 +1532,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.p[1].splits = splits_w, e.p[1].kb_per = run_w;
         RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
     }
-    lce_dx_finish_launch(ctx, o[1]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype);
-    if (cut_dw) lce_dx_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, c.dw, c.dtype);
-    if (c.dbias) lce_dbias_finish_launch(ctx, o[2]->data(), dbrows, c.V, c.scal, c.dbias);
+    lce_finish_launch(ctx, o[1]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype, c.dbias ? o[2]->data() : nullptr, dbrows, c.V, c.dbias);
+    if (cut_dw) lce_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, c.dw, c.dtype, nullptr, 0, 0, nullptr);
     return RG_OK;
 }
