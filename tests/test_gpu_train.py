@@ -372,10 +372,11 @@ def ce_check(be, R, D, V, dtype, bias=True, ignored=0.2, dloss=None, seed=0):
 
 
 FEW = [(1, 1, 1), (1, 8, 2), (1, 64, 1000), (2, 13, 97), (3, 768, 257), (4, 32, 128), (5, 300, 1025), (8, 128, 129), (9, 31, 63),
-       (16, 257, 2047), (13, 520, 333), (2, 70, 5000), (6, 129, 20011)]
+       (16, 257, 2047), (13, 520, 333), (2, 70, 5000), (6, 129, 20011), (3, 9000, 65), (14, 9000, 65)]
 MANY = [(17, 1, 1), (17, 8, 2), (33, 13, 97), (64, 64, 64), (64, 192, 97), (127, 65, 255), (128, 128, 256), (129, 72, 257), (200, 100, 1000),
         (300, 320, 513), (511, 257, 775), (640, 768, 1024), (1025, 40, 2049), (260, 520, 5003), (30, 700, 2000), (200, 768, 1500),
-        (2500, 40, 300), (8000, 128, 97), (192, 130, 515), (193, 60, 131), (70, 130, 20011), (33, 257, 40001)]
+        (2500, 40, 300), (8000, 128, 97), (192, 130, 515), (193, 60, 131), (70, 130, 20011), (33, 257, 40001), (40, 9000, 65),
+        (300, 9000, 72)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
