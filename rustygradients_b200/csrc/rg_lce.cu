@@ -7,6 +7,7 @@
 // The logits exist a tile at a time: the forward pass keeps (maximum, sum of exponentials) per row and slice of the
 // vocabulary, the backward pass computes them once more from x, w and the saved lse.
 #include "rg_lce.cuh"
+#include "rg_lce_plan.h"
 
 #include <algorithm>
 
@@ -245,9 +246,9 @@ __device__ __forceinline__ void lce_few_logits(const lce_call& c, unsigned char*
     typedef lce_few<T, RB> F;
     typedef typename lce_four<T>::type V4;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int c0 = blockIdx.x * LCE_COLS, shift = (int)(((long long)w * c.V) & 3);
+    const int c0 = blockIdx.x * LCE_COLS, shift = lce_few_shift(c.V, w);
     // lanes beyond the row read its last aligned place again: their sums are not used
-    const int col0 = min(c0 - shift + 4 * lane, ((c.V - 1 + shift) & ~3) - shift);
+    const int col0 = min(c0 - shift + 4 * lane, lce_few_last(c.V, shift));
     const size_t total = (size_t)c.D * c.V, step = (size_t)8 * c.V;
     const T* x = static_cast<const T*>(c.x);
     const T* wt = static_cast<const T*>(c.w);
@@ -258,8 +259,8 @@ __device__ __forceinline__ void lce_few_logits(const lce_call& c, unsigned char*
     for (int i = 0; i < F::PAIRS; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
-    // this warp's rows of w: w, w + 8, ...; the last row of all ends the matrix, its read is guarded
-    const int rows = (c.D - w + 7) / 8, safe = (c.D - 1 - w + 7) / 8;
+    // this warp's rows of w: w, w + 8, ...; those at the end of the matrix are read with a guard
+    const int rows = (c.D - w + 7) / 8, safe = lce_few_safe(c.D, c.V, w);
     const T* from = wt + (size_t)w * c.V + col0;
     auto copy = [&](int k) {
         if (k < safe) {

@@ -823,3 +823,11 @@ def test_rows_and_tensors_beyond_32_bits():
     assert abs(torch.from_dlpack(norm).item() / exact - 1) <= 2 * E32
     got, want = torch.from_dlpack(clipped[0]), x[-last:].double() / exact
     assert bool(((got[-last:].double() - want).abs() <= (U["bf16"] + 3 * E32) * want.abs() + 1e-40).all()) and not bool(got[:last].any())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R", [1, 3, 8])
+@pytest.mark.parametrize("D,V", [(2, 1), (3, 1), (5, 1), (9, 1), (5, 2), (10, 3), (1026, 1), (1025, 2), (1, 3)])
+def test_linear_cross_entropy_of_few_rows_and_classes(backend, R, D, V, dtype):
+    """Vocabularies narrower than a read of w: several of the last rows end past the matrix."""
+    ce_check(backend, R, D, V, dtype, bias=R != 3, dloss=0.5)

@@ -96,3 +96,13 @@ def test_cpp_mirror_of_the_training_ops_compiles():
 def test_cpp_mirror_of_the_training_ops_runs():
     r = subprocess.run([_compile()], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "OK" in r.stdout, r.stdout + r.stderr
+
+
+def test_few_row_reads_stay_inside_the_matrix(tmp_path):
+    """Every 16-byte read that the form for few rows makes without a guard, for matrices down to one column and one row."""
+    exe = str(tmp_path / "lce_plan_test")
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "rustygradients_b200", "csrc"),
+                        os.path.join(ROOT, "tests", "cpp", "lce_plan_test.cpp"), "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "OK" in r.stdout, r.stdout
