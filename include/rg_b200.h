@@ -155,7 +155,8 @@ RG_API rg_status rg_layer_norm_bwd(rg_ctx* ctx, const rg_storage* dy, const rg_s
  * src/nn/linear.rs:14-19; same type as x), bias V values f32 or NULL, targets R values f32 (ids, as rg_sparse_cross_entropy).
  * Rows whose target equals ignore_index are left out of the mean; any other target outside 0..V-1 is RG_ERR_SHAPE.
  * loss [1] = mean over the remaining rows of lse - z[target] (0 when none remains); lse [R] = log sum exp z of every row.
- * A bias of -inf takes a class out; an infinite or NaN value of x or w makes the logits that it enters NaN or infinite.
+ * A bias of -inf takes a class out; an infinite or NaN value of x or w makes the logits that it enters NaN or infinite.  A logit
+ * of f32 inputs is off by at most 2^-16 beside the rounding of its own products, whatever the magnitudes of the other values.
  * The host waits until the targets are checked, not for the result. */
 RG_API rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, const rg_storage* w, const rg_storage* bias,
                                          const rg_storage* targets, int64_t ignore_index, rg_storage** loss, rg_storage** lse);

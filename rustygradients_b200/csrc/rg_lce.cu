@@ -584,14 +584,14 @@ static rg_status lce_args(const char* op, rg_ctx* ctx, const rg_storage* x, cons
 static rg_status lce_check_launch(rg_ctx* ctx, lce_call& c, const rg_storage* targets, long long ignore, const rg_storage* dloss,
                                   rg_storage** scratch) {
     // tgt [R] | tz [R] | scal [2] | words that start at 0
-    const int nzero = 2 + c.ncounters;
+    const int nzero = 3 + c.ncounters;
     const size_t words = 2 * (size_t)c.R + 2 + nzero;
     RG_TRY(rg_alloc_storage(ctx, &words, 1, scratch));
     float* base = (*scratch)->data();
     c.tgt = reinterpret_cast<int*>(base), c.tz = base + c.R, c.scal = base + 2 * (size_t)c.R;
     c.ticket = reinterpret_cast<int*>(base + 2 * (size_t)c.R + 2);
-    c.wmax = reinterpret_cast<unsigned*>(base + 2 * (size_t)c.R + 3);
-    c.counters = reinterpret_cast<int*>(base + 2 * (size_t)c.R + 4);
+    c.largest = reinterpret_cast<unsigned*>(base + 2 * (size_t)c.R + 3);
+    c.counters = reinterpret_cast<int*>(base + 2 * (size_t)c.R + 5);
     lce_check_kernel<<<1, 1024, 0, ctx->stream>>>(targets->data(), c.R, c.V, ignore, dloss ? dloss->data() : nullptr,
                                                   const_cast<int*>(c.tgt), c.tz, const_cast<float*>(c.scal), c.ticket, nzero, ctx->h_check,
                                                   ++ctx->check_no);

@@ -15,7 +15,7 @@ struct lce_call {
     int* err;              // raised by a wait that gives up
     int ncounters;         // tile counters that the call needs
     int* ticket;           // words that start at 0
-    unsigned* wmax;
+    unsigned* largest;     // f32 on the tensor cores: largest finite magnitude of w and of x, as bits
     int* counters;
     float2* parts;         // forward: (maximum, sum of exponentials) of row r over slice p at [p * R + r]
     float* tz;             // forward: logit of the target

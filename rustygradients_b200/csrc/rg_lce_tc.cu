@@ -14,9 +14,13 @@
 // bf16 inputs are one plane and are multiplied as they are.  f32 inputs are split into planes of 16 bits whose products are
 // accumulated in f32:
 //  * logits: two f16 planes, x = 2^-a (x0 + x1) with a power of two per row of x and one for w that bring the largest
-//    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits and everything down to 2^-40 of that largest magnitude (a logit is off by
-//    2^-40 of the largest product of magnitudes, and only its absolute error counts in a softmax); three of the four products
-//    are taken, the fourth is below 2^-22 of the magnitudes.  The scales leave in the epilogue.
+//    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits, or what is above 2^-39 of that largest magnitude, whichever is less exact;
+//    three of the four products are taken, the fourth is below 2^-22 of the magnitudes.  The scales leave in the epilogue.
+//    A logit is then off by up to 2^-38 D max|x| max|w| beside the 2^-21 of its own products, and only its absolute error counts
+//    in a softmax: pairs are used while that stays below 2^-16 (lt_wide; roundings that do not all go the same way leave some 2^-23).  A single
+//    huge value - in a class that a bias of -inf takes out, or a channel that the other side leaves at zero - would cost all
+//    other logits their digits; where the largest magnitudes allow that, lce_mid_kernel multiplies triples of bf16 instead,
+//    which have f32's range.  Both launches are enqueued and the device decides, so the host does not wait for the maxima.
 //  * dx, dw: the sums run over the vocabulary and over the rows, where dz spans many orders of magnitude (a rare word's
 //    gradient is a sum of tiny ones), so f16's range is not enough: three bf16 planes hold all 24 bits (each the leading 8 bits
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
@@ -81,6 +85,7 @@ struct lt_args {
     int v0, vn;    // piece of the vocabulary: first column, number of columns
     const float* bias;
     const float *xscale, *wscale;  // PLANES 2: the scale of each row of x and of w, to be taken out of the logits
+    const unsigned* largest;       // PLANES 2: no tile is worked on where lt_wide() says so
     const int* tgt;
     float2* parts;            // LT_FWD
     float* tz;
@@ -96,6 +101,12 @@ struct lt_args {
     int dw_bf16;
     const float* scal;
 };
+
+// f32 logits: do the largest finite magnitudes of w and x ask for more range than a pair of f16 has?  (A product beyond f32 is
+// infinite here, and wide.)
+__device__ __forceinline__ bool lt_wide(const unsigned* largest, int D) {
+    return __uint_as_float(largest[0]) * __uint_as_float(largest[1]) * (float)D > 0x1p22f;
+}
 
 __device__ __forceinline__ uint32_t lt_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void lt_bar_init(uint64_t* b, uint32_t n) {
@@ -472,6 +483,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
     const uint32_t tmem = *tmem_slot;
     // everything above needs nothing from the kernels before; from here on they are complete
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (PLANES == 2 && lt_wide(e.largest, e.D)) total = 0;  // lce_mid_kernel does all of it
 
     if (warp < S::FIRST) {
     if (S::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -738,7 +750,8 @@ struct lm_args {
     int R, D, V;
     int tile;        // columns of the vocabulary per tile, at most 128
     int tiles, groups;  // of columns; of 64 rows
-    int cols;        // columns that are covered: V, or those of dz
+    int v0, cols;    // columns that are covered: from v0, those of dz or of the partial sums
+    const unsigned* largest;  // not NULL: only where lt_wide() says so, in place of lce_tc_kernel
     int* err;
     const float* bias;
     const int* tgt;
@@ -746,7 +759,8 @@ struct lm_args {
     float* tz;
     const float* lse;  // LT_DZ
     __nv_bfloat16* dz;  // [3][R][cols]
-    float* dbparts;  // [groups][V] or NULL
+    float* dbparts;  // [groups * db_rows][V] or NULL
+    int db_rows;     // rows of dbparts for each group: the sums, then zeros
 };
 
 // A from tensor memory
@@ -812,6 +826,10 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
     // the same in all lanes, and known to be: what follows from it is computed once per warp
     const int warp = __shfl_sync(RG_FULL_MASK, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (e.largest) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!lt_wide(e.largest, e.D)) return;
+    }
     const int total = e.tiles * e.groups, nkb = (e.D + LM_BK - 1) / LM_BK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) lt_bar_init(&full_w[s], 16), lt_bar_init(&full_x[s], 1), lt_bar_init(&empty[s], 1);
@@ -840,7 +858,7 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
         int t = blockIdx.x, kb = 0;  // of the loads, a k-block ahead
         const uint32_t blocks = (uint32_t)((total - t + (int)gridDim.x - 1) / (int)gridDim.x) * nkb;
         auto place = [&]() {
-            const int v0 = (t / e.groups) * e.tile;
+            const int v0 = e.v0 + (t / e.groups) * e.tile;
             p = w + (size_t)row * e.V + min(v0 + (warp & 3) * 32 + lane, min(e.V, v0 + e.tile) - 1);
         };
         uint32_t raw[32];
@@ -956,9 +974,9 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
         uint32_t it = 0, nt = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < total; t += gridDim.x, nt++) {
-            const int row0 = (t % e.groups) * 64, rows = min(64, e.R - row0), v0 = (t / e.groups) * e.tile;
+            const int row0 = (t % e.groups) * 64, rows = min(64, e.R - row0), at = (t / e.groups) * e.tile, v0 = e.v0 + at;
             const int c = v0 + place;
-            const bool mine = place < e.tile && c < e.cols, live = mine && c < e.V;
+            const bool mine = place < e.tile && at + place < e.cols, live = mine && c < e.V;
             const float bias = e.bias && live ? e.bias[c] : 0.f;
             float acc[2][32];
 #pragma unroll
@@ -1028,10 +1046,10 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
                             if (__shfl_sync(RG_FULL_MASK, tgt, j) == c && live) v[j] -= 1.f;
                     }
                     // Neighbouring lanes hold neighbouring columns: for each two rows they exchange halves, so an even lane stores
-                    // two columns of the first row and an odd lane of the second (e.cols, e.tile and v0 are even).
+                    // two columns of the first row and an odd lane of the second (e.cols, e.tile and at are even).
                     const bool odd = lane & 1;
                     const size_t plane = (size_t)e.R * e.cols;
-                    unsigned short* z = reinterpret_cast<unsigned short*>(e.dz + (size_t)(r0 + odd) * e.cols + (c - odd));
+                    unsigned short* z = reinterpret_cast<unsigned short*>(e.dz + (size_t)(r0 + odd) * e.cols + (at + place - odd));
 #pragma unroll
                     for (int j = 0; j < 32; j += 2, z += 2 * (size_t)e.cols) {
                         float d0 = v[j], d1 = v[j + 1];
@@ -1066,7 +1084,9 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
                     e.parts[(size_t)(t / e.groups) * e.R + row0 + r] = make_float2(a.m, a.s);
                 }
             } else if (e.dbparts && live) {
-                e.dbparts[(size_t)(t % e.groups) * e.V + c] = db;
+                float* o = e.dbparts + (size_t)(t % e.groups) * e.db_rows * e.V + c;
+                o[0] = db;
+                for (int k = 1; k < e.db_rows; k++) o[(size_t)k * e.V] = 0.f;
             }
         }
     }
@@ -1135,7 +1155,7 @@ __device__ __forceinline__ void lt_split2(float v, float scale, uint32_t& h0, ui
     h0 = __half_as_ushort(a), h1 = __half_as_ushort(b);
 }
 
-// x as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row, and triples of bf16 (either NULL: not wanted).
+// x as 16-bit planes [plane][rows][pitch]: pairs of f16 with a scale per row, triples of bf16, or both.
 // A warp per row: the row is read for its largest magnitude and once more, from L1 or L2, to be written.
 struct lt_rows {
     const float* src;
@@ -1143,12 +1163,12 @@ struct lt_rows {
     uint16_t *pair, *triple;
     float* scale;
 };
-__device__ __forceinline__ void lt_pack_row(const lt_rows& x, int r) {
+__device__ __forceinline__ void lt_pack_row(const lt_rows& x, int r, bool pairs, bool triples) {
     const int lane = threadIdx.x & 31;
     if (r >= x.rows) return;
     const float* __restrict__ p = x.src + (size_t)r * x.cols;
-    uint16_t* __restrict__ pair = x.pair ? x.pair + (size_t)r * x.pitch : nullptr;
-    uint16_t* __restrict__ triple = x.triple ? x.triple + (size_t)r * x.pitch : nullptr;
+    uint16_t* __restrict__ pair = pairs ? x.pair + (size_t)r * x.pitch : nullptr;
+    uint16_t* __restrict__ triple = triples ? x.triple + (size_t)r * x.pitch : nullptr;
     float m = 0.f;
     if (pair)
 #pragma unroll 8
@@ -1178,26 +1198,32 @@ __device__ __forceinline__ void lt_pack_row(const lt_rows& x, int r) {
 }
 __global__ void __launch_bounds__(256) lt_pack_rows_kernel(const lt_rows x) {
     rg_pdl_sync();
-    lt_pack_row(x, blockIdx.x * 8 + (threadIdx.x >> 5));
+    lt_pack_row(x, blockIdx.x * 8 + (threadIdx.x >> 5), false, true);
 }
 
-// Largest finite magnitude of w (as bits: they order like the values), into a word that lce_check_kernel has set to 0.
-__global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ src, size_t n, unsigned* __restrict__ out) {
+// Largest finite magnitudes of w (all blocks but the last `xblocks`) and of x (those), as bits - they order like the values -,
+// into two words that lce_check_kernel has set to 0.
+__global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ w, size_t wn, const float* __restrict__ x, size_t xn, int xblocks,
+                                                     unsigned* __restrict__ out) {
     rg_pdl_sync();
-    const size_t stride = (size_t)gridDim.x * 256;
+    const int wblocks = (int)gridDim.x - xblocks;
+    const bool of_x = (int)blockIdx.x >= wblocks;
+    const float* __restrict__ src = of_x ? x : w;
+    const size_t n = of_x ? xn : wn, block = of_x ? blockIdx.x - wblocks : blockIdx.x, stride = (size_t)(of_x ? xblocks : wblocks) * 256;
     const float4* v4 = reinterpret_cast<const float4*>(src);
     float m = 0.f;
 #pragma unroll 4
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n / 4; i += stride) {
+    for (size_t i = block * 256 + threadIdx.x; i < n / 4; i += stride) {
         const float4 q = v4[i];
         m = fmaxf(m, fmaxf(fmaxf(lt_finite_abs(q.x), lt_finite_abs(q.y)), fmaxf(lt_finite_abs(q.z), lt_finite_abs(q.w))));
     }
-    if (blockIdx.x == 0 && threadIdx.x < n % 4) m = fmaxf(m, lt_finite_abs(src[n - 1 - threadIdx.x]));
+    if (block == 0 && threadIdx.x < n % 4) m = fmaxf(m, lt_finite_abs(src[n - 1 - threadIdx.x]));
     m = rg_warp_max(m);
-    if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(out, __float_as_uint(m));  // a maximum: the order does not matter
+    if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(out + of_x, __float_as_uint(m));  // a maximum: the order does not matter
 }
 
-// w as pairs of f16 with one scale for the whole matrix, and triples of bf16, or one of them.  A thread takes 8
+// w as pairs of f16 with one scale for the whole matrix (not where lt_wide() says that they are not used), and triples of bf16,
+// or one of them.  A thread takes 8
 // neighbouring values of a row and writes 16 bytes of each plane.  The values are walked from the end: what the last-level
 // cache still holds of lt_max_kernel's pass is read from there.  Memory bound: 4 bytes in, 4 (6, 10) out for pairs (triples,
 // both); 768 x 50257: 52 (62, 89) us, 5.9 to 6.2 TB/s, and 30 us for the pass before.  The first blocks pack x, which took a
@@ -1208,10 +1234,12 @@ __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ 
                                                       uint16_t* __restrict__ triple, float* __restrict__ scale_out, const lt_rows x) {
     rg_pdl_sync();
     const int xblocks = (x.rows + 7) / 8, block = (int)blockIdx.x - xblocks;
+    const bool wide = PAIR && lt_wide(largest, rows);
     if (block < 0) {
-        lt_pack_row(x, blockIdx.x * 8 + (threadIdx.x >> 5));
+        lt_pack_row(x, blockIdx.x * 8 + (threadIdx.x >> 5), PAIR && !wide, TRIPLE || wide);
         return;
     }
+    if (wide && !TRIPLE) return;
     const float2 sc = PAIR ? lt_scale(__uint_as_float(*largest)) : make_float2(1.f, 1.f);
     if (PAIR && block == 0 && threadIdx.x == 0) *scale_out = sc.y;
     const int groups = pitch / 8;
@@ -1225,7 +1253,7 @@ __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ 
         for (int k = 0; k < 8; k++) v[k] = c + k < cols ? src[r * cols + c + k] : 0.f;
         const size_t at = (size_t)r * pitch + c;
         uint32_t h0[4], h1[4], h2[4];
-        if (PAIR) {
+        if (PAIR && !wide) {
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 uint32_t a0, a1, b0, b1;
@@ -1329,9 +1357,10 @@ static rg_status lt_planes(rg_ctx* ctx, const void* src, int rows, int cols, int
     o->grads = {three, rows, cols, 3, pitch};
     return RG_OK;
 }
-// x and (w_too) w as the kernels read them.  A scale per row of x, one for w.
+// x and (w_too) w as the kernels read them.  A scale per row of x, one for w.  Where x has pairs it has room for triples too:
+// lce_mid_kernel may have to take the call.
 static rg_status lt_pack(rg_ctx* ctx, const lce_call& c, bool w_too, bool want_logits, bool want_grads, lt_packed* x, lt_packed* w) {
-    RG_TRY(lt_planes(ctx, c.x, c.R, c.D, c.dtype, (size_t)c.R, want_logits, want_grads, x));
+    RG_TRY(lt_planes(ctx, c.x, c.R, c.D, c.dtype, (size_t)c.R, want_logits, true, x));
     if (w_too) RG_TRY(lt_planes(ctx, c.w, c.D, c.V, c.dtype, 1, want_logits, want_grads, w));
     if (c.dtype == RG_DTYPE_BF16) return RG_OK;
     const int xblocks = rg_cdiv(c.R, 8);
@@ -1340,14 +1369,15 @@ static rg_status lt_pack(rg_ctx* ctx, const lce_call& c, bool w_too, bool want_l
     } else {
         const lt_rows& m = w->rows;
         if (want_logits) {
-            const size_t n = (size_t)m.rows * m.cols;
-            const size_t grid = std::max<size_t>(1, std::min<size_t>((n / 4 + 255) / 256, (size_t)ctx->sm_count * 8));
-            RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, m.src, n, c.wmax));
+            const size_t n = (size_t)m.rows * m.cols, xn = (size_t)c.R * c.D;
+            auto blocks = [&](size_t k) { return (unsigned)std::max<size_t>(1, std::min<size_t>((k / 4 + 255) / 256, (size_t)ctx->sm_count * 8)); };
+            RG_CUDA(rg_launch(true, lt_max_kernel, dim3(blocks(n) + blocks(xn)), dim3(256), 0, ctx->stream, m.src, n, x->rows.src, xn,
+                              (int)blocks(xn), c.largest));
             RG_LAUNCHED(ctx);
         }
         const unsigned grid = (unsigned)std::min<long long>(((long long)m.rows * (m.pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
         RG_CUDA(rg_launch(true, !want_grads ? lt_pack_kernel<true, false> : want_logits ? lt_pack_kernel<true, true> : lt_pack_kernel<false, true>,
-                          dim3(xblocks + grid), dim3(256), 0, ctx->stream, m.src, m.rows, m.cols, m.pitch, (const unsigned*)c.wmax, m.pair,
+                          dim3(xblocks + grid), dim3(256), 0, ctx->stream, m.src, m.rows, m.cols, m.pitch, (const unsigned*)c.largest, m.pair,
                           m.triple, m.scale, x->rows));
     }
     RG_LAUNCHED(ctx);
@@ -1371,19 +1401,39 @@ static int lm_tile(rg_ctx* ctx, const lce_call& c, int cols) {
 }
 int lce_tc_nparts(rg_ctx* ctx, const lce_call& c) { return lm_takes(c) ? rg_cdiv(c.V, lm_tile(ctx, c, c.V)) : 2 * rg_cdiv(c.V, LT_BN); }
 
+// `e` comes with the columns that are covered, and what the gradient stores.
 template <typename T, int EPI>
 static rg_status lm_launch(rg_ctx* ctx, const lce_call& c, const lt_packed& x, lm_args& e) {
     CUtensorMap map;
     RG_TRY(lt_map(&map, x.grads, 64));
     e.w = c.w, e.R = c.R, e.D = c.D, e.V = c.V;
-    e.groups = rg_cdiv(c.R, 64), e.tile = lm_tile(ctx, c, e.cols), e.tiles = rg_cdiv(e.cols, e.tile);
+    if (!e.groups) e.groups = rg_cdiv(c.R, 64);
+    if (!e.tile) e.tile = lm_tile(ctx, c, e.cols);
+    if (!e.db_rows) e.db_rows = 1;
+    e.tiles = rg_cdiv(e.cols, e.tile);
     e.err = ctx->d_flag + 1;
     e.bias = c.bias, e.tgt = c.tgt, e.parts = c.parts, e.tz = c.tz, e.lse = c.lse;
-    const int grid = (int)std::min<long long>((long long)e.tiles * e.groups, ctx->sm_count);
+    const long long total = (long long)e.tiles * e.groups;
+    if (total > 0x7fffffff - 2 * ctx->sm_count) return rg_fail(RG_ERR_SHAPE, "linear_cross_entropy: too many tiles");
+    const int grid = (int)std::min<long long>(total, ctx->sm_count);
     RG_CUDA(cudaFuncSetAttribute(lce_mid_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, lm_shape<T>::SMEM));
     RG_CUDA(rg_launch(true, lce_mid_kernel<T, EPI>, dim3(grid), dim3(LM_THREADS), lm_shape<T>::SMEM, ctx->stream, map, e));
     RG_LAUNCHED(ctx);
     return RG_OK;
+}
+// The same work as a launch of lce_tc_kernel<2, EPI> before it (x packed as triples too), done where that one leaves it: the
+// same partial sums of 128 columns (FWD), the same dz, and rows of dbparts for 32 rows each (DZ).  Calls, us, with one weight of 1e10
+// against ordinary weights: loss of 256 rows x768x50257 192 and 156, of 4096 2,180 and 770 to 850; gradient of 2048 3,020 and 2,210
+// to 2,310.  Where it is not needed it costs 3 us.
+template <int EPI>
+static rg_status lm_launch_wide(rg_ctx* ctx, const lce_call& c, const lt_packed& x, int v0, int cols, __nv_bfloat16* dz, float* dbparts) {
+    lm_args e;
+    memset(&e, 0, sizeof(e));
+    e.largest = c.largest;
+    e.tile = LT_BN / 2, e.v0 = v0, e.cols = cols;
+    if (EPI == LT_DZ) e.groups = LT_BM / 64 * rg_cdiv(c.R, LT_BM), e.db_rows = 2;
+    e.dz = dz, e.dbparts = dbparts;
+    return lm_launch<float, EPI>(ctx, c, x, e);
 }
 
 static lt_prob lt_problem(int M, int N, int K, int bn, int a_mn, int b_mn) {
@@ -1418,7 +1468,7 @@ static void lt_common(rg_ctx* ctx, const lce_call& c, int* counter, lt_args* e) 
     e->counter = counter, e->err = ctx->d_flag + 1;
     e->R = c.R, e->D = c.D, e->V = c.V, e->v0 = 0, e->vn = c.V;
     e->bias = c.bias, e->tgt = c.tgt, e->lse = c.lse, e->scal = c.scal;
-    e->parts = c.parts, e->tz = c.tz;
+    e->parts = c.parts, e->tz = c.tz, e->largest = c.largest;
 }
 
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
@@ -1440,7 +1490,9 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     e.xscale = x.scale, e.wscale = w.scale;
     e.nprobs = 1;
     e.p[0] = lt_problem(c.R, c.V, c.D, LT_BN, 0, 1);
-    return lt_run<LT_FWD>(ctx, c, maps, e);
+    RG_TRY(lt_run<LT_FWD>(ctx, c, maps, e));
+    if (c.dtype == RG_DTYPE_F32) RG_TRY(lm_launch_wide<LT_FWD>(ctx, c, x, 0, c.nparts * (LT_BN / 2), nullptr, nullptr));
+    return RG_OK;
 }
 
 // The gradient goes over pieces of the vocabulary: dz of a piece (at most LT_DZ_BYTES, whatever R and V are) is written as
@@ -1523,6 +1575,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
             RG_TRY((lm_launch<float, LT_DZ>(ctx, c, x, m)));
         } else {
             RG_TRY(lt_run<LT_DZ>(ctx, c, mz, e));
+            if (c.dtype == RG_DTYPE_F32) RG_TRY(lm_launch_wide<LT_DZ>(ctx, c, x, e.v0, width, e.dz, e.dbparts));
         }
         e.nprobs = 2;
         e.p[0] = dx_t ? lt_problem(c.D, c.R, e.vn, bn, 0, 0) : lt_problem(c.R, c.D, e.vn, bn, 0, 0);

@@ -831,3 +831,122 @@ def test_rows_and_tensors_beyond_32_bits():
 def test_linear_cross_entropy_of_few_rows_and_classes(backend, R, D, V, dtype):
     """Vocabularies narrower than a read of w: several of the last rows end past the matrix."""
     ce_check(backend, R, D, V, dtype, bias=R != 3, dloss=0.5)
+
+
+# Inputs that took a form for some rows when their tests were written, for the tiles of many rows too.
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R", [200, 300])
+def test_linear_cross_entropy_masked_and_empty_rows_of_many(backend, R, dtype):
+    test_linear_cross_entropy_masked_and_empty_rows(backend, R, dtype)
+
+
+@pytest.mark.parametrize("R", [200, 300])
+def test_linear_cross_entropy_refusals_and_differences_of_many(backend, R):
+    test_linear_cross_entropy_targets_and_refusals(backend, R)
+    test_linear_cross_entropy_gradient_against_differences(backend, R)
+
+
+def ce_one_large_value(be, R, D, V, dtype, kind, size):
+    """One large weight whose products count for nothing: every other logit keeps its digits.  The oracle leaves out the class
+    that has no probability (a bias of -inf, or a logit of -size: exp of it is 0 in 64 bits too)."""
+    x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.1, 9)
+    d0, v0, r0 = 5, 31 % V, R // 2
+    t[t == v0] = (v0 + 1) % V
+    big = rounded(np.array([size], np.float32), dtype)[0]
+    if kind == "dead channel":
+        x[:, d0], w[d0, v0] = 0, big
+    elif kind == "masked class":
+        x[:, d0], w[d0, v0], b[v0] = 1, big, -np.inf
+    elif kind == "class switched off":
+        x[:, d0], w[d0, v0] = 1, -big
+    else:
+        assert kind == "dead row of w"
+        x[r0, d0], w[d0] = big, 0
+    keep = np.ones(V, bool)
+    keep[v0] = kind not in ("masked class", "class switched off")
+    sub = np.cumsum(keep) - 1
+    ts = np.where(t == IGNORE, IGNORE, sub[np.where(t == IGNORE, 0, t).astype(int)]).astype(np.float32)
+    wk, bk, live = w[:, keep], b[keep], t != IGNORE
+    ex = ce_exact(x, wk, bk, ts)
+    tlse, tloss, tdx, tdw, tdb = ce_bounds(x, wk, bk, dtype, ex, live)
+    X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    within(get(be, lse), ex["lse"], tlse, "lse")
+    within(get(be, loss), np.array([ex["loss"]]), tloss, "loss")
+    dx, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, put(be, ex["lse"].astype(np.float32)))
+    within(get(be, dx), ex["dx"], tdx + 1e-45, "dx")
+    within(get(be, dw)[:, keep], ex["dw"], tdw + 1e-45, "dw")
+    within(get(be, db)[keep], ex["db"], tdb + 1e-45, "dbias")
+    if not keep.all():
+        assert not get(be, dw)[:, ~keep].any() and not get(be, db)[~keep].any()
+
+
+@pytest.mark.parametrize("kind", ["dead channel", "masked class", "class switched off", "dead row of w"])
+@pytest.mark.parametrize("dtype,R", [("f32", 6), ("f32", 70), ("f32", 200), ("f32", 300), ("bf16", 300)])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e8, 1e12, 1e30])
+def test_linear_cross_entropy_with_one_large_value(backend, R, dtype, kind, size):
+    ce_one_large_value(backend, R, 64, 1000, dtype, kind, size)
+
+
+@pytest.mark.parametrize("R,D,V", [(193, 8, 5), (257, 100, 1000), (500, 64, 129), (1000, 40, 2049), (300, 700, 385)])
+def test_linear_cross_entropy_on_both_sides_of_the_range_rule(backend, R, D, V):
+    """Just below and just above D max|x| max|w| = 2^22, where the products of f32 change from pairs to triples."""
+    be = backend
+    x, w, b, t = ce_inputs(R, D, V, "f32", True, 0.1, 12)
+    for factor in (0.98, 1.02):
+        ce_one_large_value(be, R, D, V, "f32", "dead channel", factor * 2.0 ** 22 / D / np.abs(np.delete(x, 5, 1)).max())
+
+
+def test_linear_cross_entropy_scales_of_many_rows_and_columns(backend):
+    """As test_linear_cross_entropy_scales_of_rows_and_columns, at 300 rows, with rows and columns whose scales differ by 2^12, and
+    by 2^40 where only one side of a product is far from 1."""
+    be = backend
+    R, D, V = 300, 200, 300
+    for spread in (6, 20):
+        x, w, b, t = ce_inputs(R, D, V, "f32", True, 0.1, 77)
+        x *= 1e-15 * 2.0 ** np.random.default_rng(1).integers(-spread, spread + 1, (R, 1))
+        x[:, 3] *= 1000
+        w *= 1e15 * 2.0 ** np.random.default_rng(2).integers(-spread, 1, (1, V))
+        w[3] *= 1e-3
+        w[:, 17], x[5] = 0, 0
+        x, w = x.astype(np.float32), w.astype(np.float32)
+        w *= np.float32(20 / np.abs(x.astype(np.float64) @ w).max())
+        ex, live = ce_exact(x, w, b, t), t != IGNORE
+        tlse, tloss, tdx, tdw, tdb = ce_bounds(x, w, b, "f32", ex, live)
+        # pairs add up to 2^-38 D max|x| max|w| to a logit
+        off = 2.0 ** -38 * D * float(np.abs(x).max()) * float(np.abs(w).max())
+        off = off if off <= 2.0 ** -16 else 0.0
+        more = off * ex["scale"] * live[:, None] * ex["p"]
+        X, W, B, T = put(be, x), put(be, w), put(be, b), put(be, t)
+        loss, lse = be.linear_cross_entropy(X, W, B, T)
+        within(get(be, lse), ex["lse"], tlse + off, "lse")
+        within(get(be, loss), np.array([ex["loss"]]), tloss + 2 * off, "loss")
+        dx, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, put(be, ex["lse"].astype(np.float32)))
+        within(get(be, dx), ex["dx"], tdx + 1.01 * more @ np.abs(w.astype(np.float64)).T + 1e-45, "dx")
+        within(get(be, dw), ex["dw"], tdw + 1.01 * np.abs(x.astype(np.float64)).T @ more + 1e-45, "dw")
+        within(get(be, db), ex["db"], tdb + 1.01 * more.sum(0), "dbias")
+
+
+def test_linear_cross_entropy_with_one_large_value_over_pieces(backend):
+    """The triples of f32 where the gradient goes over pieces of the vocabulary (512 MiB of dz)."""
+    be = backend
+    R, D, V = 70000, 8, 2100
+    rng = np.random.default_rng(6)
+    keep = np.sort(rng.permutation(R)[:300])
+    x, w, b, t = ce_inputs(300, D, V, "f32", True, 0.1, 14)
+    x[:, 5], w[5, [3, 1300, 2099]] = 0, 1e10
+    xf, tf = np.zeros((R, D), np.float32), np.full(R, IGNORE, np.float32)
+    xf[keep], tf[keep] = x, t
+    ex = ce_exact(x, w, b, t)
+    tlse, tloss, tdx, tdw, tdb = ce_bounds(x, w, b, "f32", ex, t != IGNORE)
+    X, W, B, T = put(be, xf), put(be, w), put(be, b), put(be, tf)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    within(get(be, lse)[keep], ex["lse"], tlse, "lse")
+    within(get(be, loss), np.array([ex["loss"]]), tloss, "loss")
+    L = np.zeros(R, np.float32)
+    L[keep] = ex["lse"]
+    dx, dw, db = (get(be, s) for s in be.linear_cross_entropy_bwd(X, W, B, T, put(be, L)))
+    within(dx[keep], ex["dx"], tdx + 1e-45, "dx")
+    within(dw, ex["dw"], tdw + 1e-45, "dw")
+    within(db, ex["db"], tdb + 1e-45, "dbias")
+    assert not np.delete(dx, keep, 0).any()

@@ -79,6 +79,33 @@ def test_two_scaled_f16_planes_hold_22_bits():
         assert (err <= np.maximum(2.0 ** -22 * np.abs(s), 2.0 ** -40 * 2 ** 15)).all()
 
 
+def _pair_logits(x, w):
+    """The three products of scaled f16 pairs, summed in 64 bits: a power of two per row of x, one for w."""
+    def split(a, m):
+        up = 2.0 ** (14 - np.floor(np.log2(m)))
+        s = a.astype(np.float64) * up
+        hi = s.astype(np.float16).astype(np.float64)
+        return hi, (s - hi).astype(np.float16).astype(np.float64), up
+    x0, x1, xs = split(x, np.abs(x).max(-1, keepdims=True))
+    w0, w1, ws = split(w, np.abs(w).max())
+    return (x0 @ w0 + x0 @ w1 + x1 @ w0) / xs / ws
+
+
+@pytest.mark.parametrize("D", [8, 64, 768])
+def test_logits_of_pairs_within_the_rule(D):
+    """Up to D max|x| max|w| = 2^22 a logit from f16 pairs is off by at most 2^-16 and 2^-21 of its products' magnitudes, also where
+    all roundings go the same way; far beyond, one large weight costs the other logits their digits."""
+    rng = np.random.default_rng(D)
+    x, w = rng.standard_normal((40, D)).astype(np.float32), (rng.standard_normal((D, 50)) * 0.1).astype(np.float32)
+    x[:, 0] = 0
+    w[1:, 7] = 0.1                      # one rounding for a whole column
+    for size, inside in ((1.0, True), (1.0 / 64, True), (2.0 ** 20, False)):
+        w[0, 3] = size * 2.0 ** 22 / D / np.abs(x).max()
+        exact, mags = x.astype(np.float64) @ w.astype(np.float64), np.abs(x).astype(np.float64) @ np.abs(w).astype(np.float64)
+        err = np.abs(_pair_logits(x, w) - exact)
+        assert (err <= 2.0 ** -16 + 2.0 ** -21 * mags).all() == inside, (size, err.max())
+
+
 def _compile():
     lib = build.build()
     cmd = ["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "cpp", "train_mirror_test.cpp"),
