@@ -168,7 +168,8 @@ RG_API rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* x, c
                                              const rg_storage* dloss, rg_storage** dx, rg_storage** dw, rg_storage** dbias);
 /* clip_gradients (src/wasm_api.rs:202-224): norm [1] = sqrt of the sum of squares over all n gradients (f32 and bf16 may be
  * mixed; sums in f64) and, in out[i], gradient i times min(1, max_norm / norm) in its own type.  max_norm must be positive
- * (infinity only measures); a NaN anywhere makes norm and every output NaN. */
+ * (infinity only measures: the outputs are the inputs, infinite values included); a NaN anywhere makes norm and every output
+ * NaN. */
 RG_API rg_status rg_clip_grad_norm(rg_ctx* ctx, const rg_storage* const* grads, size_t n, float max_norm, rg_storage** out,
                                    rg_storage** norm);
 

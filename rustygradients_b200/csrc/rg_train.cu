@@ -650,11 +650,12 @@ __global__ void __launch_bounds__(256) rg_clip_scale_kernel(const __grid_constan
     for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
     s = clip_block_sum(s, red);
     const double norm = sqrt(s);  // may be beyond f32 where every gradient is inside
-    // min(1, max / norm); a NaN norm fails the comparison and stays.  A factor near the smallest normal f32 would lose digits:
-    // it is applied in two steps, the second one an exact power of two.
-    const double ratio = (double)max_norm / norm;
+    // min(1, max / norm); a NaN norm fails the comparisons and stays, an infinite maximum leaves everything as it is, infinities
+    // too.  A factor near the smallest normal f32 would lose digits: it is applied in two steps, the second one an exact power of
+    // two.
+    const double ratio = norm <= (double)max_norm ? 1.0 : (double)max_norm / norm;
     const bool tiny = ratio < 0x1p-100;
-    const float c = (float)(ratio >= 1.0 ? 1.0 : tiny ? ratio * 0x1p64 : ratio), c2 = tiny ? 0x1p-64f : 1.f;
+    const float c = (float)(tiny ? ratio * 0x1p64 : ratio), c2 = tiny ? 0x1p-64f : 1.f;
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out) *norm_out = (float)norm;
     const int turns = (t.pieces - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     for (int k = turns - 1; k >= 0; k--) {

@@ -950,3 +950,20 @@ def test_linear_cross_entropy_with_one_large_value_over_pieces(backend):
     within(dw, ex["dw"], tdw + 1e-45, "dw")
     within(db, ex["db"], tdb + 1e-45, "dbias")
     assert not np.delete(dx, keep, 0).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_clip_grad_norm_only_measures_with_an_infinite_maximum(backend, dtype):
+    """Overflowed gradients are measured, not destroyed; a NaN still shows everywhere."""
+    be = backend
+    a = rounded(np.random.default_rng(0).standard_normal(9000), dtype)
+    b = rounded(np.array([1.0, -2.0, 3e38], np.float32), dtype)
+    for bad in (np.inf, -np.inf, None):
+        a[8500] = bad if bad is not None else 1
+        out, norm = be.clip_grad_norm([put(be, a, dtype), put(be, b, dtype)], float("inf"))
+        n = be.to_vec(norm)[0]
+        assert np.isinf(n) if bad is not None else abs(n / np.sqrt((a.astype(np.float64) ** 2).sum() + (b.astype(np.float64) ** 2).sum()) - 1) < 2 * E32
+        assert all(np.array_equal(be.to_vec(o), v) for o, v in zip(out, (a, b)))
+    a[3] = np.nan
+    out, norm = be.clip_grad_norm([put(be, a, dtype), put(be, b, dtype)], float("inf"))
+    assert np.isnan(be.to_vec(norm)[0]) and np.isnan(be.to_vec(out[0])).all() and np.isnan(be.to_vec(out[1])).all()
