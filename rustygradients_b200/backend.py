@@ -78,8 +78,14 @@ class Storage:
             check(status)
         return _capsule_new(m, b"dltensor", _capsule_gone_ptr)
 
-    def __dlpack__(self, stream=None, **_):
-        """`torch.from_dlpack(st)`: for consumers on the backend's own stream (BufferError elsewhere)."""
+    def __dlpack__(self, stream=None, *, max_version=None, dl_device=None, copy=None):
+        """`torch.from_dlpack(st)`: for consumers on the backend's own stream (BufferError elsewhere).  The tensor shares the
+        buffer: a copy, or another device, is a BufferError too.  Whatever `max_version` allows, the capsule is an unversioned
+        one."""
+        if copy:
+            raise BufferError("the tensor shares the storage's buffer: copy it after the export (torch.from_dlpack(st).clone())")
+        if dl_device is not None and tuple(int(v) for v in dl_device) != self.__dlpack_device__():
+            raise BufferError(f"the storage is on CUDA device {self._backend.device_index} and is not moved by an export")
         mine = self._backend.stream or 1          # 1 is the name of the default stream in the protocol
         if stream != -1 and (stream or 1) != mine:
             raise BufferError("the storage is ordered on its backend's stream: make the backend on the consumer's stream")

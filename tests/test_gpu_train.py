@@ -967,3 +967,17 @@ def test_clip_grad_norm_only_measures_with_an_infinite_maximum(backend, dtype):
     a[3] = np.nan
     out, norm = be.clip_grad_norm([put(be, a, dtype), put(be, b, dtype)], float("inf"))
     assert np.isnan(be.to_vec(norm)[0]) and np.isnan(be.to_vec(out[0])).all() and np.isnan(be.to_vec(out[1])).all()
+
+
+def test_an_exported_tensor_is_never_an_unasked_alias():
+    import torch
+    torch.cuda.set_device(0)
+    be = rg.B200Backend(0, stream=torch.cuda.current_stream().cuda_stream)
+    st = be.ones([4])
+    with pytest.raises(BufferError):
+        torch.from_dlpack(st, copy=True)
+    with pytest.raises(BufferError):
+        torch.from_dlpack(st, device="cpu")
+    mine = torch.from_dlpack(st).clone()
+    mine.add_(1)
+    assert np.array_equal(be.to_vec(st), np.ones(4, np.float32)) and torch.equal(torch.from_dlpack(st, copy=False), mine - 1)

@@ -35,6 +35,27 @@ def test_no_gpu_is_an_error_on_a_caller_stream_too():
         rg.B200Backend(0, stream=0)
 
 
+def test_dlpack_requests_that_an_alias_cannot_fulfil_are_refused():
+    import rustygradients_b200.backend as B
+
+    class Owner:
+        _ctx, stream, device_index = None, 0, 1
+
+    class Shared(B.Storage):
+        def to_dlpack(self):
+            return "capsule"
+
+    st = Shared(Owner(), 0)
+    assert st.__dlpack_device__() == (2, 1)
+    for asked in ({}, {"stream": 1}, {"stream": -1}, {"copy": None}, {"copy": False}, {"dl_device": (2, 1), "max_version": (1, 0)}):
+        assert st.__dlpack__(**asked) == "capsule"
+    for asked in ({"copy": True}, {"dl_device": (1, 0)}, {"dl_device": (2, 0)}, {"stream": 5}):
+        with pytest.raises(BufferError):
+            st.__dlpack__(**asked)
+    with pytest.raises(TypeError):
+        st.__dlpack__(something="else")
+
+
 def _bits(a):
     return np.ascontiguousarray(a, np.float32).view(np.uint32)
 
