@@ -58,7 +58,8 @@ RG_API int rg_device_count(void);
 RG_API rg_status rg_ctx_create(int device, rg_ctx** out);
 /* The same on a stream of the caller (a cudaStream_t of that device, NULL for its default stream), for the ops of this
  * header next to another owner of the GPU: every call enqueues on it, so arrays of that owner that are ordered on the
- * stream need no further synchronisation in either direction.  The stream must outlive the context and its storages.
+ * stream need no further synchronisation in either direction.  The stream must outlive the context and its storages.  Calls
+ * on such a context leave the thread's current device as it was.
  * Ops are not captured into a graph there, and rg_gpt_create refuses such a context (RG_ERR_UNSUPPORTED both). */
 RG_API rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** out);
 RG_API rg_status rg_ctx_destroy(rg_ctx* ctx);

@@ -33,9 +33,7 @@ rg_devbuf::~rg_devbuf() {
         life->small[small].push_back(ptr);  // capacity was reserved with the context
         return;
     }
-    int cur = 0;
-    cudaGetDevice(&cur);
-    if (cur != device) cudaSetDevice(device);
+    rg_on_device on(device, true);
     // the context's stream still exists: stream-ordered free; else (context destroyed first, which synchronised
     // the stream) a plain free.  A stream that is being captured takes no free of this buffer: it waits in `parked`.
     bool done = false;
@@ -57,7 +55,6 @@ rg_devbuf::~rg_devbuf() {
         cudaGetLastError();
         cudaFree(ptr);
     }
-    if (cur != device) cudaSetDevice(cur);
 }
 
 // ---------------------------------------------------------------------------
@@ -78,7 +75,8 @@ static rg_status ctx_create(int device, bool own_stream, cudaStream_t stream, rg
     int n = rg_device_count();
     if (device < 0 || device >= n)
         return rg_fail(RG_ERR_BACKEND, "Failed to initialize CUDA device %d: %d device(s) visible", device, n);
-    RG_CUDA(cudaSetDevice(device));
+    rg_on_device on(device, !own_stream);
+    RG_CUDA((cudaError_t)on.failed());
     cudaDeviceProp prop;
     RG_CUDA(cudaGetDeviceProperties(&prop, device));
     if (prop.major != 10)
@@ -125,7 +123,7 @@ extern "C" rg_status rg_ctx_destroy(rg_ctx* ctx) {
     if (!ctx) return RG_OK;
     {
         std::lock_guard<std::mutex> lock(ctx->life->mu);
-        cudaSetDevice(ctx->device);
+        rg_on_device on(ctx->device, !ctx->own_stream);
         cudaStreamSynchronize(ctx->stream);
         ctx->life->alive = false;
         for (void* p : ctx->life->parked) cudaFree(p);

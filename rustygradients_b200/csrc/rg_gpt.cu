@@ -477,7 +477,7 @@ extern "C" rg_status rg_gpt_create(rg_ctx* ctx, const rg_gpt_config* cfg, rg_gpt
 
 extern "C" rg_status rg_gpt_destroy(rg_gpt* m) {
     if (!m) return RG_OK;
-    cudaSetDevice(m->ctx->device);
+    rg_on_device on(m->ctx->device, false);
     cudaStreamSynchronize(m->ctx->stream);
     if (m->graph) cudaGraphExecDestroy(m->graph);
     tp_peer_close(m);

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/rg_b200.h"
+#include "rg_device_scope.h"
 
 // ---------------------------------------------------------------------------
 // errors
@@ -109,29 +110,26 @@ rg_status rg_alloc_storage(rg_ctx* ctx, const size_t* shape, int ndim, rg_storag
 rg_status rg_need_f32(const char* op, const rg_storage* a, const rg_storage* b = nullptr, const rg_storage* c = nullptr);
 rg_status rg_tc_wait_check(rg_ctx* ctx);  // after a synchronise: did a wait of a tensor-core kernel give up?
 
+struct rg_cuda_device {
+    static int get(int* d) { return (int)cudaGetDevice(d); }
+    static int set(int d) { return (int)cudaSetDevice(d); }
+};
+typedef rg_device_scope<rg_cuda_device> rg_on_device;
+
+// One call at a time per context, with the context's device current.  A context on a caller's stream works next to another
+// owner of the GPUs, so the thread's current device is put back.
 struct rg_ctx_guard {
-    rg_ctx* c;
-    explicit rg_ctx_guard(rg_ctx* ctx) : c(ctx) {
-        c->life->mu.lock();
-        cudaSetDevice(c->device);
-    }
-    ~rg_ctx_guard() { c->life->mu.unlock(); }
+    std::lock_guard<std::mutex> lock;
+    rg_on_device dev;
+    explicit rg_ctx_guard(rg_ctx* ctx) : rg_ctx_guard(ctx, !ctx->own_stream) {}
+
+  protected:
+    rg_ctx_guard(rg_ctx* ctx, bool put_back) : lock(ctx->life->mu), dev(ctx->device, put_back) {}
 };
 
-// The same for the ops that work next to another owner of the GPU (rg_ctx_create_on_stream): the thread's current
-// device is put back.
-struct rg_op_guard {
-    rg_ctx* c;
-    int before = -1;
-    explicit rg_op_guard(rg_ctx* ctx) : c(ctx) {
-        c->life->mu.lock();
-        cudaGetDevice(&before);
-        if (before != c->device) cudaSetDevice(c->device);
-    }
-    ~rg_op_guard() {
-        if (before >= 0 && before != c->device) cudaSetDevice(before);
-        c->life->mu.unlock();
-    }
+// The same for the ops that take and return other owners' arrays: put back on every context.
+struct rg_op_guard : rg_ctx_guard {
+    explicit rg_op_guard(rg_ctx* ctx) : rg_ctx_guard(ctx, true) {}
 };
 
 #define RG_LAUNCHED(ctx) ((ctx)->launches++)

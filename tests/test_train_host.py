@@ -146,11 +146,23 @@ def test_cpp_mirror_of_the_training_ops_runs():
     assert r.returncode == 0 and "OK" in r.stdout, r.stdout + r.stderr
 
 
-def test_few_row_reads_stay_inside_the_matrix(tmp_path):
-    """Every 16-byte read that the form for few rows makes without a guard, for matrices down to one column and one row."""
-    exe = str(tmp_path / "lce_plan_test")
+def _run_host_test(name, tmp_path):
+    exe = str(tmp_path / name)
     r = subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "rustygradients_b200", "csrc"),
-                        os.path.join(ROOT, "tests", "cpp", "lce_plan_test.cpp"), "-o", exe], capture_output=True, text=True)
+                        os.path.join(ROOT, "tests", "cpp", name + ".cpp"), "-o", exe], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "OK" in r.stdout, r.stdout
+
+
+def test_few_row_reads_stay_inside_the_matrix(tmp_path):
+    """Every 16-byte read that the form for few rows makes without a guard, for matrices down to one column and one row."""
+    _run_host_test("lce_plan_test", tmp_path)
+
+
+def test_the_current_device_is_put_back(tmp_path):
+    _run_host_test("device_scope_test", tmp_path)
+    # every entry point sets the device through that class
+    csrc = os.path.join(ROOT, "rustygradients_b200", "csrc")
+    calls = [f"{f}: {line.strip()}" for f in sorted(os.listdir(csrc)) for line in open(os.path.join(csrc, f)) if "cudaSetDevice(" in line]
+    assert calls == ["rg_internal.cuh: static int set(int d) { return (int)cudaSetDevice(d); }"]
