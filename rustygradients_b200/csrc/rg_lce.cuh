@@ -35,10 +35,10 @@ __device__ __forceinline__ lce_ms lce_merge(lce_ms a, lce_ms b) {
     return {m, a.s * expf(a.m - ref) + b.s * expf(b.m - ref)};
 }
 
-// out[i] = scale * sum over p of parts[p][i] (dx, or dw), fixed order; and, where dbias is given, dbias[c] = scale * sum over p
-// of dbparts[p][c]
+// out[i] = scale * sum over p of parts[p][i] (dx, or dw; i < count, which may be 0), fixed order; and, where dbias is given,
+// dbias[c] = scale * sum over p of dbparts[p][c], c < cols (rows dbpitch apart)
 void lce_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* out, int dtype,
-                          const float* dbparts, int dbrows, int V, float* dbias);
+                          const float* dbparts, int dbrows, int dbpitch, int cols, float* dbias);
 
 // The tensor-core form.
 rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c);

@@ -92,7 +92,7 @@ struct lt_args {
     const float* lse;         // LT_DZ
     __nv_bfloat16* dz;        // [plane][R][dz_pitch]: 1 plane for bf16, 3 for f32 inputs
     long long dz_pitch;
-    float* dbparts;           // [LT_BM / 32 * tiles_m][V] or NULL
+    float* dbparts;           // [LT_BM / 32 * tiles_m][dz_pitch] or NULL
     float* dxparts;           // LT_GRAD: [splits][R][D]
     int dx_add;               // add to what the pieces before left there
     int dx_t;                 // the first problem computes dx^T
@@ -380,7 +380,7 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
                         v[i] = keep + __shfl_xor_sync(RG_FULL_MASK, send, half);
                     }
                 }
-                if (lane < left) e.dbparts[(size_t)w.group * e.V + c + lane] = v[0];
+                if (lane < left) e.dbparts[(size_t)w.group * e.dz_pitch + col + lane] = v[0];
             }
         }
         return;
@@ -759,7 +759,7 @@ struct lm_args {
     float* tz;
     const float* lse;  // LT_DZ
     __nv_bfloat16* dz;  // [3][R][cols]
-    float* dbparts;  // [groups * db_rows][V] or NULL
+    float* dbparts;  // [groups * db_rows][cols] or NULL
     int db_rows;     // rows of dbparts for each group: the sums, then zeros
 };
 
@@ -1084,9 +1084,9 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
                     e.parts[(size_t)(t / e.groups) * e.R + row0 + r] = make_float2(a.m, a.s);
                 }
             } else if (e.dbparts && live) {
-                float* o = e.dbparts + (size_t)(t % e.groups) * e.db_rows * e.V + c;
+                float* o = e.dbparts + (size_t)(t % e.groups) * e.db_rows * e.cols + at + place;
                 o[0] = db;
-                for (int k = 1; k < e.db_rows; k++) o[(size_t)k * e.V] = 0.f;
+                for (int k = 1; k < e.db_rows; k++) o[(size_t)k * e.cols] = 0.f;
             }
         }
     }
@@ -1495,8 +1495,10 @@ rg_status lce_tc_forward(rg_ctx* ctx, lce_call& c) {
     return RG_OK;
 }
 
-// The gradient goes over pieces of the vocabulary: dz of a piece (at most LT_DZ_BYTES, whatever R and V are) is written as
-// bf16 planes, then one launch multiplies it with w and with x.
+// The gradient goes over pieces of the vocabulary: dz of a piece is written as bf16 planes, then one launch multiplies it with w
+// and with x.  A piece is as wide as LT_DZ_BYTES allow, but at least the 256 columns of a tile: beyond 1 Mi rows of bf16 (2^20)
+// or 349,525 of f32 its dz grows with the rows, 512 or 1,536 bytes each (x itself holds 2 or 4 bytes for each of its columns).
+// The partial sums of dbias are those of a piece too.
 #define LT_DZ_BYTES ((size_t)512 << 20)
 
 static int lt_piece(const lce_call& c) {
@@ -1541,7 +1543,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     if (cut_dw) RG_TRY(rg_alloc_storage(ctx, &wlen, 1, &o[3]));
     const int dbrows = mid ? rg_cdiv(c.R, 64) : LT_BM / 32 * rg_cdiv(c.R, LT_BM);
     if (c.dbias) {
-        const size_t blen = (size_t)dbrows * c.V;
+        const size_t blen = (size_t)dbrows * width;
         RG_TRY(rg_alloc_storage(ctx, &blen, 1, &o[2]));
     }
 
@@ -1584,8 +1586,12 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         e.p[1] = lt_problem(e.vn, c.D, c.R, bn, 1, 1);
         e.p[1].splits = splits_w, e.p[1].kb_per = run_w;
         RG_TRY(lt_run<LT_GRAD>(ctx, c, mg, e));
+        // the sums of dbias: with those of dx after the last piece, else in a launch of their own
+        const bool last = i + 1 == pieces;
+        if (last || c.dbias)
+            lce_finish_launch(ctx, o[1]->data(), splits, last ? (size_t)c.R * c.D : 0, c.scal, c.dx, c.dtype, e.dbparts, dbrows, width, e.vn,
+                              c.dbias ? c.dbias + e.v0 : nullptr);
     }
-    lce_finish_launch(ctx, o[1]->data(), splits, (size_t)c.R * c.D, c.scal, c.dx, c.dtype, c.dbias ? o[2]->data() : nullptr, dbrows, c.V, c.dbias);
-    if (cut_dw) lce_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, c.dw, c.dtype, nullptr, 0, 0, nullptr);
+    if (cut_dw) lce_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, c.dw, c.dtype, nullptr, 0, 0, 0, nullptr);
     return RG_OK;
 }

@@ -986,3 +986,31 @@ def test_an_exported_tensor_is_never_an_unasked_alias():
     mine = torch.from_dlpack(st).clone()
     mine.add_(1)
     assert np.array_equal(be.to_vec(st), np.ones(4, np.float32)) and torch.equal(torch.from_dlpack(st, copy=False), mine - 1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear_cross_entropy_gradient_scratch(backend, dtype):
+    """No scratch grows with rows times vocabulary: beside 512 MiB of dz, only what grows with one of them.  dbias comes out of
+    every piece."""
+    rt, driver = pytest.importorskip("cuda.bindings.runtime"), pytest.importorskip("cuda.bindings.driver")
+    be = backend
+    R, D, V = 300000, 8, 20003
+    x, w, b, t = ce_inputs(400, D, V, dtype, True, 0.1, 4)
+    xf, tf = np.zeros((R, D), np.float32), np.full(R, IGNORE, np.float32)
+    at = np.sort(np.random.default_rng(0).permutation(R)[:400])
+    xf[at], tf[at] = x, t
+    L, ex = np.zeros(R, np.float32), ce_exact(x, w, b, t)
+    L[at] = ex["lse"]
+    X, W, B, T, LS = put(be, xf, dtype), put(be, w, dtype), put(be, b), put(be, tf), put(be, L)
+    be.synchronize()
+    err, pool = rt.cudaDeviceGetDefaultMemPool(0)
+    high, used = rt.cudaMemPoolAttr.cudaMemPoolAttrUsedMemHigh, rt.cudaMemPoolAttr.cudaMemPoolAttrUsedMemCurrent
+    before = int(rt.cudaMemPoolGetAttribute(pool, used)[1])
+    assert int(rt.cudaMemPoolSetAttribute(pool, high, driver.cuuint64_t(0))[0]) == 0
+    _, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, LS)
+    be.synchronize()
+    grown = int(rt.cudaMemPoolGetAttribute(pool, high)[1]) - before
+    assert 256 << 20 <= grown <= (512 << 20) + R * D * 16 + D * V * 20 + (64 << 20), grown
+    _, _, _, tdw, tdb = ce_bounds(x, w, b, dtype, ex, t != IGNORE)
+    within(get(be, dw), ex["dw"], tdw + 1e-45, "dw")
+    within(get(be, db), ex["db"], tdb + 1e-45, "dbias")
