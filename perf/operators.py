@@ -211,15 +211,15 @@ def _clip(s):
 
 
 # ---- the same through the library
-_backend = None
+_backends = {}  # one for each device and stream that was current in a call
 
 
 def _run_own(s):
-    global _backend
-    if _backend is None:
+    where = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    if where not in _backends:
         import rustygradients_b200 as rg
-        _backend = rg.B200Backend(torch.cuda.current_device(), stream=torch.cuda.current_stream().cuda_stream)
-    be = _backend
+        _backends[where] = rg.B200Backend(where[0], stream=where[1])
+    be = _backends[where]
 
     def given(*names):
         return [None if s[n] is None else be.from_device(s[n]) for n in names]
