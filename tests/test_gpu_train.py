@@ -1014,3 +1014,26 @@ def test_linear_cross_entropy_gradient_scratch(backend, dtype):
     _, _, _, tdw, tdb = ce_bounds(x, w, b, dtype, ex, t != IGNORE)
     within(get(be, dw), ex["dw"], tdw + 1e-45, "dw")
     within(get(be, db), ex["db"], tdb + 1e-45, "dbias")
+
+
+def test_one_step_on_two_streams_in_turn():
+    """A backend per torch stream: every step is ordered with the inputs that its own stream made."""
+    import torch
+    torch.cuda.set_device(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    backends = [rg.B200Backend(0, stream=s.cuda_stream) for s in streams]
+    g, b = torch.ones(1600, device="cuda"), torch.zeros(1600, device="cuda")
+    torch.cuda.synchronize()
+    got = []
+    for k in range(8):
+        s, be = streams[k % 2], backends[k % 2]
+        with torch.cuda.stream(s):
+            x = torch.zeros(4000, 1600, device="cuda")
+            for _ in range(20):                            # the op must wait for these
+                x.add_(torch.arange(1600, device="cuda") * (k + 1.0))
+            y, mean, _ = be.layer_norm_fwd(be.from_device(x), be.from_device(g), be.from_device(b), EPS)
+            got.append((k, torch.from_dlpack(mean) + 0, torch.from_dlpack(y)[-1] + 0))
+    torch.cuda.synchronize()
+    for k, mean, y in got:
+        want = 20 * (k + 1.0) * 799.5                      # whole numbers: the sums are exact up to the last division
+        assert bool(((mean - want).abs() <= 60 * 2.0 ** -24 * want).all()) and abs(y[-1].item() / (1599 - 799.5) * 461.8802 - 1) < 1e-3

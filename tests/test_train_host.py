@@ -56,6 +56,38 @@ def test_dlpack_requests_that_an_alias_cannot_fulfil_are_refused():
         st.__dlpack__(something="else")
 
 
+def test_timing_cases_follow_the_current_stream_and_device(monkeypatch):
+    import importlib
+
+    import rustygradients_b200 as rg
+    P = importlib.import_module("perf.operators")
+    made = []
+
+    class Backend:
+        def __init__(self, device, stream):
+            self.at = (device, stream)
+            made.append(self.at)
+
+        def from_device(self, t):
+            return t
+
+        def layer_norm_fwd(self, x, gamma, beta, eps):
+            raise LookupError(self.at)
+
+    now = [0, 0]
+    monkeypatch.setattr(rg, "B200Backend", Backend)
+    monkeypatch.setattr(P, "_backends", {})
+    monkeypatch.setattr(P, "own", True)
+    monkeypatch.setattr(P.torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(P.torch.cuda, "current_stream", lambda: type("S", (), {"cuda_stream": now[1]})())
+    state = {"op": "ln_fwd", "x": 0, "gamma": 0, "beta": 0}
+    for now[:] in ([0, 0], [0, 7], [0, 0], [1, 0], [0, 7]):
+        with pytest.raises(LookupError) as at:
+            P.run(state)
+        assert at.value.args[0] == tuple(now)
+    assert made == [(0, 0), (0, 7), (1, 0)]
+
+
 def _bits(a):
     return np.ascontiguousarray(a, np.float32).view(np.uint32)
 
