@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict_
 // warps sharing the partials.  (A launch of its own for dbias cost 3 us.)
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) lce_finish_kernel(const float* __restrict__ parts, int nparts, size_t count, const float* __restrict__ scal,
-                                                         T* __restrict__ dx, int xblocks, const float* __restrict__ dbparts, int dbrows,
+                                                         const int* __restrict__ tgt, int D, T* __restrict__ dx, int xblocks, const float* __restrict__ dbparts, int dbrows,
                                                          int dbpitch, int cols, float* __restrict__ dbias) {
     __shared__ float red[8][32];
     rg_pdl_sync();
@@ -147,6 +147,9 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const float* __restrict
         dbias[c] = s * scale;
         return;
     }
+    // an upstream gradient that overflowed reaches the rows with a target only
+    const bool rows = tgt && !(fabsf(scale) <= 3.4028235e38f);
+    auto scaled = [&](float v, size_t at) { return rows && tgt[at / D] < 0 ? 0.f : v * scale; };
     const size_t stride = (size_t)xblocks * 256 * VEC;
     for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * VEC; i < count; i += stride) {
         if constexpr (VEC == 4) {
@@ -158,27 +161,28 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const float* __restrict
             }
             const float v[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) dx[i + k] = rg_from_float<T>(v[k] * scale);
+            for (int k = 0; k < 4; k++) dx[i + k] = rg_from_float<T>(scaled(v[k], i + k));
         } else {
-            dx[i] = rg_from_float<T>(rg_sum_parts(parts + i, nparts, count) * scale);
+            dx[i] = rg_from_float<T>(scaled(rg_sum_parts(parts + i, nparts, count), i));
         }
     }
 }
 template <typename T>
-static void lce_finish_typed(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, T* dx, const float* dbparts,
+static void lce_finish_typed(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, const int* tgt, int D, T* dx,
+                             const float* dbparts,
                              int dbrows, int dbpitch, int cols, float* dbias) {
     // four values a thread where every partial starts on a 16-byte boundary and there are threads enough (768 values and 50
     // partials: 15 us against 6; 6.5 million values and one partial: 9 us against 26)
     const bool vec = count % 4 == 0 && count >= ((size_t)1 << 19);
     const int xblocks = (int)std::min<size_t>((count + (vec ? 1023 : 255)) / (vec ? 1024 : 256), (size_t)ctx->sm_count * 16);
     rg_launch(true, vec ? lce_finish_kernel<T, 4> : lce_finish_kernel<T, 1>, dim3((unsigned)(xblocks + (dbias ? rg_cdiv(cols, 32) : 0))), dim3(256),
-              0, ctx->stream, parts, nparts, count, scal, dx, xblocks, dbparts, dbrows, dbpitch, cols, dbias);
+              0, ctx->stream, parts, nparts, count, scal, tgt, D, dx, xblocks, dbparts, dbrows, dbpitch, cols, dbias);
     RG_LAUNCHED(ctx);
 }
-void lce_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* out, int dtype,
+void lce_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, const int* tgt, int D, void* out, int dtype,
                           const float* dbparts, int dbrows, int dbpitch, int cols, float* dbias) {
-    if (dtype == RG_DTYPE_F32) lce_finish_typed(ctx, parts, nparts, count, scal, (float*)out, dbparts, dbrows, dbpitch, cols, dbias);
-    else lce_finish_typed(ctx, parts, nparts, count, scal, (__nv_bfloat16*)out, dbparts, dbrows, dbpitch, cols, dbias);
+    if (dtype == RG_DTYPE_F32) lce_finish_typed(ctx, parts, nparts, count, scal, tgt, D, (float*)out, dbparts, dbrows, dbpitch, cols, dbias);
+    else lce_finish_typed(ctx, parts, nparts, count, scal, tgt, D, (__nv_bfloat16*)out, dbparts, dbrows, dbpitch, cols, dbias);
 }
 
 // ---------------------------------------------------------------------------
@@ -678,7 +682,8 @@ extern "C" rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* 
             RG_TRY(rg_alloc_storage(ctx, &zlen, 1, &o[4]));
             RG_TRY(rg_alloc_storage(ctx, &plen, 1, &o[5]));
             lce_few_backward(ctx, c, o[4]->data(), o[5]->data());
-            lce_finish_launch(ctx, o[5]->data(), (int)nparts, (size_t)c.R * c.D, c.scal, c.dx, c.dtype, nullptr, 0, 0, 0, nullptr);
+            lce_finish_launch(ctx, o[5]->data(), (int)nparts, (size_t)c.R * c.D, c.scal, c.tgt, c.D, c.dx, c.dtype, nullptr, 0, 0, 0,
+                              nullptr);
         } else {
             RG_TRY(lce_tc_backward(ctx, c));
         }

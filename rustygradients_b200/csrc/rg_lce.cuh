@@ -36,8 +36,9 @@ __device__ __forceinline__ lce_ms lce_merge(lce_ms a, lce_ms b) {
 }
 
 // out[i] = scale * sum over p of parts[p][i] (dx, or dw; i < count, which may be 0), fixed order; and, where dbias is given,
-// dbias[c] = scale * sum over p of dbparts[p][c], c < cols (rows dbpitch apart)
-void lce_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, void* out, int dtype,
+// dbias[c] = scale * sum over p of dbparts[p][c], c < cols (rows dbpitch apart).  tgt (NULL for dw): the rows of D values without
+// a target are 0 whatever the scale is.
+void lce_finish_launch(rg_ctx* ctx, const float* parts, int nparts, size_t count, const float* scal, const int* tgt, int D, void* out, int dtype,
                           const float* dbparts, int dbrows, int dbpitch, int cols, float* dbias);
 
 // The tensor-core form.

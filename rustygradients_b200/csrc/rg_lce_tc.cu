@@ -1589,9 +1589,9 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         // the sums of dbias: with those of dx after the last piece, else in a launch of their own
         const bool last = i + 1 == pieces;
         if (last || c.dbias)
-            lce_finish_launch(ctx, o[1]->data(), splits, last ? (size_t)c.R * c.D : 0, c.scal, c.dx, c.dtype, e.dbparts, dbrows, width, e.vn,
-                              c.dbias ? c.dbias + e.v0 : nullptr);
+            lce_finish_launch(ctx, o[1]->data(), splits, last ? (size_t)c.R * c.D : 0, c.scal, c.tgt, c.D, c.dx, c.dtype, e.dbparts, dbrows,
+                              width, e.vn, c.dbias ? c.dbias + e.v0 : nullptr);
     }
-    if (cut_dw) lce_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, c.dw, c.dtype, nullptr, 0, 0, 0, nullptr);
+    if (cut_dw) lce_finish_launch(ctx, o[3]->data(), splits_w, (size_t)c.D * c.V, c.scal, nullptr, c.D, c.dw, c.dtype, nullptr, 0, 0, 0, nullptr);
     return RG_OK;
 }

@@ -1037,3 +1037,18 @@ def test_one_step_on_two_streams_in_turn():
     for k, mean, y in got:
         want = 20 * (k + 1.0) * 799.5                      # whole numbers: the sums are exact up to the last division
         assert bool(((mean - want).abs() <= 60 * 2.0 ** -24 * want).all()) and abs(y[-1].item() / (1599 - 799.5) * 461.8802 - 1) < 1e-3
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", [(3, 40, 300), (40, 40, 300), (300, 41, 300), (700, 768, 300)])
+def test_linear_cross_entropy_overflowed_upstream_gradient(backend, R, D, V, dtype):
+    """dloss of infinity or NaN: the rows without a target still have a gradient of 0, the others show it."""
+    be = backend
+    x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.0, 2)
+    t[::3] = IGNORE
+    X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t)
+    _, lse = be.linear_cross_entropy(X, W, B, T)
+    for bad in (np.inf, -np.inf, np.nan):
+        dx, dw, db = (be.to_array(s) for s in be.linear_cross_entropy_bwd(X, W, B, T, lse, put(be, np.array([bad], np.float32))))
+        assert not dx[::3].any() and not np.isfinite(np.delete(dx, np.arange(0, R, 3), 0)).any()
+        assert not np.isfinite(dw).all() and not np.isfinite(db).all()
