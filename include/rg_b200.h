@@ -56,7 +56,8 @@ typedef struct rg_gpt rg_gpt;         /* GPTModel, src/models/gpt.rs:17-24      
 RG_API int rg_device_count(void);
 /* CudaBackend::new(device_index), src/backend/cuda.rs:87-125; Device::cuda(index), src/backend/mod.rs:72-77 */
 RG_API rg_status rg_ctx_create(int device, rg_ctx** out);
-/* The same on a stream of the caller (a cudaStream_t of that device, NULL for its default stream), for the ops of this
+/* The same on a stream of the caller (a cudaStream_t of that device, NULL for its default stream; not
+ * cudaStreamPerThread, which is RG_ERR_UNSUPPORTED: it is another stream in each thread), for the ops of this
  * header next to another owner of the GPU: every call enqueues on it, so arrays of that owner that are ordered on the
  * stream need no further synchronisation in either direction.  The stream must outlive the context and its storages.  Calls
  * on such a context leave the thread's current device as it was.

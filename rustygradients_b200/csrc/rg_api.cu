@@ -116,6 +116,11 @@ static rg_status ctx_create(int device, bool own_stream, cudaStream_t stream, rg
 
 extern "C" rg_status rg_ctx_create(int device, rg_ctx** out) { return ctx_create(device, true, nullptr, out); }
 extern "C" rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** out) {
+    if (!out) return rg_fail(RG_ERR_INVALID_INPUT, "rg_ctx_create_on_stream: out is NULL");
+    *out = nullptr;
+    // that handle names another stream in each thread, and storages may be freed from any thread
+    if ((cudaStream_t)stream == cudaStreamPerThread)
+        return rg_fail(RG_ERR_UNSUPPORTED, "a context works on one stream: the per-thread default stream is another one in each thread");
     return ctx_create(device, false, (cudaStream_t)stream, out);
 }
 

@@ -88,6 +88,12 @@ def test_timing_cases_follow_the_current_stream_and_device(monkeypatch):
     assert made == [(0, 0), (0, 7), (1, 0)]
 
 
+def test_the_per_thread_default_stream_is_refused():
+    lib, p = _lib.load(), C.c_void_p()
+    assert lib.rg_ctx_create_on_stream(0, C.c_void_p(2), C.byref(p)) == _lib.RG_ERR_UNSUPPORTED and not p.value   # cudaStreamPerThread
+    assert b"per-thread" in lib.rg_last_error()
+
+
 def _bits(a):
     return np.ascontiguousarray(a, np.float32).view(np.uint32)
 
