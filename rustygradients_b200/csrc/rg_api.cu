@@ -148,12 +148,13 @@ extern "C" rg_status rg_ctx_destroy(rg_ctx* ctx) {
 }
 
 // The bounded waits of the tensor-core GEMM and attention kernels raise the second flag word when they give up (tiles or
-// split-k partials are then missing).  Called after a stream synchronise: reports it once and clears the word.
+// split-k partials are then missing).  Called after a stream synchronise: reports it once and clears the word.  On the context's
+// stream: a copy on the default stream would wait for the work that others have there.
 rg_status rg_tc_wait_check(rg_ctx* ctx) {
-    int v = 0;
-    RG_CUDA(cudaMemcpy(&v, ctx->d_flag + 1, sizeof(int), cudaMemcpyDeviceToHost));
-    if (v) {
-        RG_CUDA(cudaMemset(ctx->d_flag + 1, 0, sizeof(int)));
+    RG_CUDA(cudaMemcpyAsync(ctx->h_flag + 1, ctx->d_flag + 1, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
+    RG_CUDA(cudaStreamSynchronize(ctx->stream));
+    if (ctx->h_flag[1]) {
+        RG_CUDA(cudaMemsetAsync(ctx->d_flag + 1, 0, sizeof(int), ctx->stream));
         return rg_fail(RG_ERR_TIMEOUT, "a bounded wait inside a tensor-core kernel gave up; its output is incomplete");
     }
     return RG_OK;

@@ -1052,3 +1052,18 @@ def test_linear_cross_entropy_overflowed_upstream_gradient(backend, R, D, V, dty
         dx, dw, db = (be.to_array(s) for s in be.linear_cross_entropy_bwd(X, W, B, T, lse, put(be, np.array([bad], np.float32))))
         assert not dx[::3].any() and not np.isfinite(np.delete(dx, np.arange(0, R, 3), 0)).any()
         assert not np.isfinite(dw).all() and not np.isfinite(db).all()
+
+
+def test_a_synchronise_waits_for_its_own_stream_only():
+    import torch
+    torch.cuda.set_device(0)
+    side = torch.cuda.Stream()
+    be = rg.B200Backend(0, stream=side.cuda_stream)
+    be.to_vec(be.ones([3]))
+    torch.cuda.synchronize()
+    torch.cuda._sleep(2_000_000_000)            # about a second of the default stream
+    assert np.array_equal(be.to_vec(be.ones([3])), np.ones(3, np.float32))
+    be.synchronize()
+    busy = not torch.cuda.default_stream().query()
+    torch.cuda.synchronize()
+    assert busy
