@@ -61,7 +61,8 @@ RG_API rg_status rg_ctx_create(int device, rg_ctx** out);
  * header next to another owner of the GPU: every call enqueues on it, so arrays of that owner that are ordered on the
  * stream need no further synchronisation in either direction.  The stream must outlive the context and its storages.  Calls
  * on such a context leave the thread's current device as it was.
- * Ops are not captured into a graph there, and rg_gpt_create refuses such a context (RG_ERR_UNSUPPORTED both). */
+ * Ops are not captured into a graph there, and rg_gpt_create refuses such a context (RG_ERR_UNSUPPORTED both).  While the stream
+ * is being captured, rg_synchronize, rg_to_vec and rg_ctx_destroy are refused the same way, and do nothing. */
 RG_API rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** out);
 RG_API rg_status rg_ctx_destroy(rg_ctx* ctx);
 /* Backend::synchronize, src/backend/mod.rs:137-138 */

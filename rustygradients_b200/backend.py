@@ -145,7 +145,7 @@ class B200Backend:
 
     def close(self) -> None:
         if self._ctx:
-            self._lib.rg_ctx_destroy(self._ctx)
+            check(self._lib.rg_ctx_destroy(self._ctx))
             self._ctx = None
 
     def __del__(self):

@@ -124,8 +124,18 @@ extern "C" rg_status rg_ctx_create_on_stream(int device, void* stream, rg_ctx** 
     return ctx_create(device, false, (cudaStream_t)stream, out);
 }
 
+// A synchronise or a free inside a capture of the caller's stream would end that capture with an error.
+static rg_status not_in_callers_capture(const rg_ctx* ctx, const char* call) {
+    if (ctx->own_stream) return RG_OK;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &cs) == cudaSuccess && cs == cudaStreamCaptureStatusNone) return RG_OK;
+    cudaGetLastError();
+    return rg_fail(RG_ERR_UNSUPPORTED, "%s inside a capture of the caller's stream", call);
+}
+
 extern "C" rg_status rg_ctx_destroy(rg_ctx* ctx) {
     if (!ctx) return RG_OK;
+    RG_TRY(not_in_callers_capture(ctx, "rg_ctx_destroy"));
     {
         std::lock_guard<std::mutex> lock(ctx->life->mu);
         rg_on_device on(ctx->device, !ctx->own_stream);
@@ -163,6 +173,7 @@ rg_status rg_tc_wait_check(rg_ctx* ctx) {
 extern "C" rg_status rg_synchronize(rg_ctx* ctx) {
     if (!ctx) return rg_fail(RG_ERR_INVALID_INPUT, "rg_synchronize: ctx is NULL");
     rg_ctx_guard g(ctx);
+    RG_TRY(not_in_callers_capture(ctx, "rg_synchronize"));
     RG_CUDA(cudaStreamSynchronize(ctx->stream));
     return rg_tc_wait_check(ctx);
 }
@@ -281,6 +292,7 @@ extern "C" rg_status rg_from_slice(rg_ctx* ctx, const float* data, size_t len, c
 extern "C" rg_status rg_to_vec(rg_ctx* ctx, const rg_storage* st, float* outp, size_t cap) {
     if (!ctx || !st || (!outp && st->len)) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
     if (cap < st->len) return rg_fail(RG_ERR_SHAPE, "rg_to_vec: capacity %zu < %zu elements", cap, st->len);
+    RG_TRY(not_in_callers_capture(ctx, "rg_to_vec"));
     rg_storage* wide = nullptr;  // bf16 values are read as f32
     if (st->dtype != RG_DTYPE_F32) RG_TRY(rg_cast(ctx, st, RG_DTYPE_F32, &wide));
     rg_status rs = RG_OK;

@@ -1067,3 +1067,27 @@ def test_a_synchronise_waits_for_its_own_stream_only():
     busy = not torch.cuda.default_stream().query()
     torch.cuda.synchronize()
     assert busy
+
+
+def test_synchronising_calls_inside_a_capture_are_refused_and_leave_it_alone():
+    import torch
+    torch.cuda.set_device(0)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        be = rg.B200Backend(0, stream=stream.cuda_stream)
+        x = be.ones([5])
+        a = torch.zeros(4, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            a.add_(1)
+            for call in (be.synchronize, lambda: be.to_vec(x), be.close, lambda: be.from_slice([1.0], [1])):
+                with pytest.raises(rg.Unsupported):
+                    call()
+            a.add_(1)
+        graph.replay()
+        stream.synchronize()
+        assert a.tolist() == [2, 2, 2, 2] and np.array_equal(be.to_vec(x), np.ones(5, np.float32))
+        del x
+        be.close()
+        be.close()
