@@ -1370,9 +1370,11 @@ static rg_status lt_pack(rg_ctx* ctx, const lce_call& c, bool w_too, bool want_l
         const lt_rows& m = w->rows;
         if (want_logits) {
             const size_t n = (size_t)m.rows * m.cols, xn = (size_t)c.R * c.D;
-            auto blocks = [&](size_t k) { return (unsigned)std::max<size_t>(1, std::min<size_t>((k / 4 + 255) / 256, (size_t)ctx->sm_count * 8)); };
-            RG_CUDA(rg_launch(true, lt_max_kernel, dim3(blocks(n) + blocks(xn)), dim3(256), 0, ctx->stream, m.src, n, x->rows.src, xn,
-                              (int)blocks(xn), c.largest));
+            // one wave of blocks, shared by sizes (a wave each: 37 us instead of 30 for 4096x768x50257)
+            const size_t wave = (size_t)ctx->sm_count * 8;
+            auto blocks = [&](size_t k) { return std::max<size_t>(1, std::min((k / 4 + 255) / 256, wave * k / (n + xn))); };
+            RG_CUDA(rg_launch(true, lt_max_kernel, dim3((unsigned)(blocks(n) + blocks(xn))), dim3(256), 0, ctx->stream, m.src, n, x->rows.src,
+                              xn, (int)blocks(xn), c.largest));
             RG_LAUNCHED(ctx);
         }
         const unsigned grid = (unsigned)std::min<long long>(((long long)m.rows * (m.pitch / 8) + 255) / 256, (long long)ctx->sm_count * 16);
