@@ -1599,8 +1599,7 @@ extern "C" rg_status rg_debug_hook(rg_ctx* ctx, rg_gpt* m, int what, long long v
         case 1: {  // raise the flag word of the tensor-core kernels' waits, as a wait that gave up would
             if (!ctx) return rg_fail(RG_ERR_INVALID_INPUT, "NULL argument");
             rg_ctx_guard g(ctx);
-            const int one = 1;
-            RG_CUDA(cudaMemcpy(ctx->d_flag + 1, &one, sizeof(int), cudaMemcpyHostToDevice));
+            RG_CUDA(cudaMemsetAsync(ctx->d_flag + 1, 1, 1, ctx->stream));  // in the order in which the flag is read
             return RG_OK;
         }
         case 2:  // cluster token loop: head cluster 0 withholds its out-projection partial of layer `value` (-1: off)

@@ -1091,3 +1091,17 @@ def test_synchronising_calls_inside_a_capture_are_refused_and_leave_it_alone():
         del x
         be.close()
         be.close()
+
+
+def test_a_wait_that_gave_up_is_reported_once():
+    """The flag word of the bounded waits, raised as a wait that gave up would: the next synchronising call says so, once."""
+    be = rg.B200Backend(0)
+    x, w, b, t = ce_inputs(300, 40, 300, "f32", True, 0.1)
+    args = [put(be, a) for a in (x, w, b, t)]
+    want = be.to_vec(be.linear_cross_entropy(*args)[0])
+    assert be._lib.rg_debug_hook(be._ctx, None, 1, 0) == 0
+    loss, _ = be.linear_cross_entropy(*args)
+    with pytest.raises(rg.DeviceTimeout):
+        be.to_vec(loss)
+    assert np.array_equal(be.to_vec(loss), want)
+    be.synchronize()
