@@ -55,6 +55,8 @@ typedef struct rg_gpt rg_gpt;         /* GPTModel, src/models/gpt.rs:17-24      
 /* CudaBackend::device_count / is_available, src/backend/cuda.rs:128-135 */
 RG_API int rg_device_count(void);
 /* CudaBackend::new(device_index), src/backend/cuda.rs:87-125; Device::cuda(index), src/backend/mod.rs:72-77 */
+/* A context keeps up to 64 released buffers of each power of two from 512 bytes to 1 MiB for its next outputs (128 MiB at most),
+ * until it is destroyed. */
 RG_API rg_status rg_ctx_create(int device, rg_ctx** out);
 /* The same on a stream of the caller (a cudaStream_t of that device, NULL for its default stream; not
  * cudaStreamPerThread, which is RG_ERR_UNSUPPORTED: it is another stream in each thread), for the ops of this
@@ -142,7 +144,8 @@ RG_API rg_status rg_sparse_cross_entropy(rg_ctx* ctx, const rg_storage* logits, 
  * WasmGptTrainer::train_step (src/wasm_api.rs:62-94): final LayerNorm, LM head with its loss, their gradients, gradient
  * clipping.  Activations and matrices are f32 or bf16 (one type per call where not said otherwise); LayerNorm parameters,
  * biases, targets, statistics, losses and their gradients are f32, as in bf16-weight mode of the model below.  Every sum and
- * statistic is held in 32 bits or more; results do not depend on timing (no atomics on values).  These calls are not
+ * statistic is held in 32 bits or more (f32 accumulators of the tensor cores, which truncate, among them); results do not depend
+ * on timing (no atomics on values).  These calls are not
  * enqueued into a stream capture (RG_ERR_UNSUPPORTED).  A device-side wait that gives up is reported by the next
  * synchronising call (rg_synchronize, rg_to_vec: RG_ERR_TIMEOUT). -------------------------------------------------- */
 /* layer_norm that keeps its statistics for the gradient: y as rg_layer_norm (type of x), mean and rstd = 1/sqrt(var + eps)
@@ -165,7 +168,9 @@ RG_API rg_status rg_linear_cross_entropy(rg_ctx* ctx, const rg_storage* x, const
                                          const rg_storage* targets, int64_t ignore_index, rg_storage** loss, rg_storage** lse);
 /* Its gradient for an upstream gradient dloss ([1] f32, NULL for 1): with n the number of rows that have a target and
  * dz = (exp(z - lse) - onehot(target)) dloss / n (0 in ignored rows), dx = dz w^T and dw = x^T dz in the type of x,
- * dbias [V] = sum over rows of dz, f32 (NULL when bias is NULL; dbias may then be NULL).  lse is what the forward call returned. */
+ * dbias [V] = sum over rows of dz, f32 (NULL when bias is NULL; dbias may then be NULL).  lse is what the forward call returned.
+ * For bf16 inputs dz is rounded to bf16 before both products (not before dbias), except with a few rows; for f32 inputs the
+ * products keep 2^-21.  A row without a target takes part in dw with a weight of 0, so it has to be finite there. */
 RG_API rg_status rg_linear_cross_entropy_bwd(rg_ctx* ctx, const rg_storage* x, const rg_storage* w, const rg_storage* bias,
                                              const rg_storage* targets, int64_t ignore_index, const rg_storage* lse,
                                              const rg_storage* dloss, rg_storage** dx, rg_storage** dw, rg_storage** dbias);

@@ -243,8 +243,10 @@ struct lce_few {
 // z[k][j]: logit of row warp + 8 k and column lane + 32 j of the tile (-inf outside).  The 8 warps share the D axis.  Each lane
 // copies its four values of the warp's next rows of w asynchronously into a ring of its own in shared memory (kept in
 // registers they left too few warps: 3.5 TB/s), and multiplies them with the RB values of x, which lie in shared memory as
-// [d][row]: one or a few broadcast loads.  Rows of x are multiplied two at a time.  Bound by the bytes of w up to 8 rows of
-// f32 (38 us for [8,768] x [768,50257], 4.0 TB/s), by the multiplications and the loads of x above (16 rows: 64 us).
+// [d][row]: one or a few broadcast loads.  Rows of x are multiplied two at a time.  [8,768] x [768,50257] f32: 38 us, 4.0 TB/s, DRAM
+// active 46 %.  Neither the bytes nor the strips of 512 of them bound it: a kernel that only adds up the same strips takes 24 to
+// 26 us (6.0 to 6.4 TB/s).  What is left are the instructions of a row of w in each warp (16 paired multiplications, three shared
+// loads, a copy, its commit and its wait); 16 rows: 64 us.
 template <typename T, int RB>
 __device__ __forceinline__ void lce_few_logits(const lce_call& c, unsigned char* sm, float (&z)[RB / 8 > 0 ? RB / 8 : 1][4]) {
     typedef lce_few<T, RB> F;
@@ -498,7 +500,8 @@ __global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, con
     }
 }
 
-// The form for few rows, by what was measured at [R,768] x [768,50257] (us for the call; the other side for the same rows):
+// The form for few rows, by what was measured at [R,768] x [768,50257] (us for the call; the other side for the same rows; no
+// other width and vocabulary was measured, and with a few hundred classes this form has only as many CTAs as 124 go into them):
 //   forward   f32  8 rows 46, the tensor cores 57;  9 rows 67 and 55
 //             bf16 V aligned: 2 rows 34, the tensor cores 38; 3 rows 37 and 37
 //             bf16 V odd: the tensor cores, 34 for 1 to 16 rows (34 for 1, 38 for 4, 47 for 8 rows here)

@@ -11,7 +11,10 @@
 // brings 64-element wide boxes (128-byte swizzle) of three-dimensional arrays [plane][row][column]; what lies outside is
 // filled with zeros, which handles every ragged edge of R, D and V.
 //
-// bf16 inputs are one plane and are multiplied as they are.  f32 inputs are split into planes of 16 bits whose products are
+// bf16 inputs are one plane and are multiplied as they are, with one accumulator for all of K.  dz is one bf16 plane too: its
+// rounding (half a step, at most 2^-8 of each value) costs dx and dw about half of what their own rounding to
+// bf16 does (8e-4 of their norm at 4096x1600x50257); a second plane would double the products that are most of the gradient's
+// time.  The form for few rows, where no product is bound by the tensor cores, keeps dz in f32.  f32 inputs are split into planes of 16 bits whose products are
 // accumulated in f32:
 //  * logits: two f16 planes, x = 2^-a (x0 + x1) with a power of two per row of x and one for w that bring the largest
 //    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits, or what is above 2^-39 of that largest magnitude, whichever is less exact;
@@ -24,11 +27,13 @@
 //  * dx, dw: the sums run over the vocabulary and over the rows, where dz spans many orders of magnitude (a rare word's
 //    gradient is a sum of tiny ones), so f16's range is not enough: three bf16 planes hold all 24 bits (each the leading 8 bits
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
-// The tensor core truncates when it adds to its f32 accumulator, so a long chain loses about 2^-25 of the running sum per
-// step (measured: a relative error of 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32 inputs the chain is
-// therefore cut after every two k-blocks of 64: in each the small products come first and that of the leading planes last, and
-// the epilogue warps add the result to their f32 registers with rounding.  (A cut after every block: 907 instead of 852 us for
-// the loss of 4096x768x50257.)
+// The tensor core truncates when it adds to its f32 accumulator, always towards zero, so a long chain loses about 2^-25 of the
+// running sum per step (measured: a relative error of 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32
+// inputs the chain is therefore cut after every k-block of 64: in each the small products come first and that of the leading
+// planes last, and the epilogue warps add the result to their f32 registers with rounding.  Errors of the norm against 64 bits,
+// 600 rows, 128x300: dx 4.4e-7, dw 4.5e-7, dbias 2.2e-7, lse 7e-8 (f32 operations: 6.4e-7, 5.2e-7, 1.5e-7, 7e-8); cut after
+// every two blocks 1.4e-6, 1.4e-6, 6.5e-7, 2.0e-7, for a loss of 4096x768x50257 in 800 instead of 834 us and a gradient of
+// 2048 rows in 2,170 instead of 2,225 (858 and 862, 2,309 and 2,373 where the power limit holds the clock down).
 #include "rg_lce.cuh"
 
 #include <cuda.h>
@@ -38,7 +43,7 @@
 
 #define LT_BM 256  // rows of a tile: 128 in each CTA of a pair
 #define LT_BK 64
-#define LT_CHAIN 2  // k-blocks per accumulator for f32 inputs
+#define LT_CHAIN 1  // k-blocks per accumulator for f32 inputs
 #define LT_SPIN_LIMIT (1u << 22)
 #define LT_STAGE_ALL 196608   // bytes of the operand ring
 #define LT_MAX_STAGES 6
@@ -741,7 +746,7 @@ struct lm_shape {
     static constexpr int STAGES = PLANES == 3 ? 2 : 4;
     // accumulators of 64 columns: the tensor core goes on while the epilogue works on a tile's sums
     static constexpr int BUFFERS = (512 - STAGES * STAGE_COLS) / 64;
-    static constexpr int CHAIN = PLANES == 3 ? LT_CHAIN * LT_BK / LM_BK : 1 << 20;  // k-blocks per accumulator
+    static constexpr int CHAIN = PLANES == 3 ? 1 : 1 << 20;  // k-blocks per accumulator
     static constexpr int SMEM = STAGES * STAGE_BYTES + 2 * 4 * 64 * 8 + 1024 + 256;
 };
 
@@ -1389,7 +1394,8 @@ static rg_status lt_pack(rg_ctx* ctx, const lce_call& c, bool w_too, bool want_l
 static_assert(lt_shape<1>::BN == lt_shape<2>::BN, "the logits have one width of column tiles");
 #define LT_BN lt_shape<1>::BN
 
-// The form of lce_mid_kernel, by what was measured at [R,768] x [768,50257] (us for the call, and with packed or copied operands):
+// The form of lce_mid_kernel, by what was measured at [R,768] x [768,50257], at no other width and vocabulary (us for the call,
+// and with packed or copied operands):
 // f32 forward 17 rows 53 (153), 128 rows 86 (152), 256 rows 139 (154); gradient 17 rows 229 (309), 192 rows 385 (402), 256
 // rows 462 (434); bf16 with an odd vocabulary forward 17 rows 39 (65), 128 rows 56 (65), 192 rows 67 (66).  With an aligned
 // one bf16 is read as it lies by TMA.

@@ -1105,3 +1105,27 @@ def test_a_wait_that_gave_up_is_reported_once():
         be.to_vec(loss)
     assert np.array_equal(be.to_vec(loss), want)
     be.synchronize()
+
+
+def ce_norm_errors(be, R, D, V, dtype):
+    x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.1, 3)
+    ex = ce_exact(x, w, b, t)
+    X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t)
+    _, lse = be.linear_cross_entropy(X, W, B, T)
+    dx, dw, db = be.linear_cross_entropy_bwd(X, W, B, T, put(be, ex["lse"].astype(np.float32)))
+    # dbias adds dz of both signs (p, and p - 1 in the target's row): an error relative to the terms is relative to the sum of
+    # their magnitudes, which is larger than the sum
+    terms = ex["scale"] * np.abs(ex["dz"]).sum(0)
+    return {k: np.linalg.norm(get(be, g) - e) / np.linalg.norm(of) for k, g, e, of in
+            (("lse", lse, ex["lse"], ex["lse"]), ("dx", dx, ex["dx"], ex["dx"]), ("dw", dw, ex["dw"], ex["dw"]), ("dbias", db, ex["db"], terms))}
+
+
+@pytest.mark.parametrize("R,D,V", [(17, 8, 300), (64, 8, 300), (192, 8, 300), (64, 128, 300), (193, 128, 33), (600, 128, 300), (600, 1600, 33),
+                                   (2500, 128, 33), (2500, 512, 300), (600, 128, 3000)])
+def test_linear_cross_entropy_f32_keeps_f32(backend, R, D, V):
+    """The norm of the error, which sums that are truncated in one direction would fill.  A probability has an argument z - lse
+    of up to 16: lse rounded to f32, the difference, and its product with log2(e), each off by at most 2^-21 (2.8e-7 in the
+    mean square, the last one times ln 2), and 2 steps of the exponential: 4.5e-7 together; the logit itself half of that.  Twice
+    the sum of squares is 1e-6.  lse: the same over a logarithm of 4 to 9, an eighth."""
+    e = ce_norm_errors(backend, R, D, V, "f32")
+    assert e["dx"] <= 1e-6 and e["dw"] <= 1e-6 and e["dbias"] <= 1e-6 and e["lse"] <= 1.5e-7, e
