@@ -11,7 +11,8 @@
 // brings 64-element wide boxes (128-byte swizzle) of three-dimensional arrays [plane][row][column]; what lies outside is
 // filled with zeros, which handles every ragged edge of R, D and V.
 //
-// bf16 inputs are one plane and are multiplied as they are, with one accumulator for all of K.  dz is one bf16 plane too: its
+// bf16 inputs are one plane and are multiplied as they are, with accumulators of up to 768 of K for the loss and one for all of K
+// where the result is rounded to bf16 (lt_cuts).  dz is one bf16 plane too: its
 // rounding (half a step, at most 2^-8 of each value) costs dx and dw about half of what their own rounding to
 // bf16 does (8e-4 of their norm at 4096x1600x50257); a second plane would double the products that are most of the gradient's
 // time.  The form for few rows, where no product is bound by the tensor cores, keeps dz in f32.  f32 inputs are split into planes of 16 bits whose products are
@@ -43,7 +44,9 @@
 
 #define LT_BM 256  // rows of a tile: 128 in each CTA of a pair
 #define LT_BK 64
-#define LT_CHAIN 1  // k-blocks per accumulator for f32 inputs
+// k-blocks of 64 per accumulator for bf16 inputs, where it is cut: the loss, and dz where dbias is summed from it (lt_cuts)
+#define LT_CHAIN_FWD 12
+#define LT_CHAIN_DZ 6
 #define LT_SPIN_LIMIT (1u << 22)
 #define LT_STAGE_ALL 196608   // bytes of the operand ring
 #define LT_MAX_STAGES 6
@@ -56,18 +59,21 @@
 // logits of 4096x768x50257 f32 1.49 (640 us, tensor pipe active 80 %), of 8192x768x50257 bf16 1.26 (504 us, 63 %; 447 us when
 // nothing is brought from L2, 487 when the epilogue does nothing); gradient of 2048x768x50257 f32: dz 0.95 (502 us, 47 %; 340
 // without its planes and column sums), dx and dw 1.32 (68 %); of 4096x1600x50257 bf16: dz 1.28, dx and dw 1.21.
-// PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.
-template <int PLANES>
+// PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.  CUT: the accumulator is cut along K and the pieces are added in
+// registers (always for f32 inputs); else the epilogue works on the columns as they come from tensor memory.
+enum { LT_FWD = 0, LT_DZ = 1, LT_GRAD = 2 };
+template <int PLANES, int EPI = LT_GRAD, bool CUT = PLANES != 1>
 struct lt_shape {
     static constexpr int BN = PLANES == 3 ? 128 : 256;
     static constexpr int A_BYTES = 128 * LT_BK * 2, B_BYTES = BN / 2 * LT_BK * 2;  // of one CTA
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
     static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6, 3 or 2
     static constexpr int BUFFERS = 512 / BN;  // accumulators in tensor memory
-    // Warp 0 copies, warp 1 multiplies, FIRST.. the eight epilogue warps.  Pairs: a thread holds 128 columns in registers,
+    static constexpr int CHAIN = PLANES != 1 ? 1 : EPI == LT_FWD ? LT_CHAIN_FWD : LT_CHAIN_DZ;  // k-blocks per accumulator, at most
+    // Warp 0 copies, warp 1 multiplies, FIRST.. the eight epilogue warps.  256 columns in registers: a thread holds 128 columns in registers,
     // more than 12 warps get at launch, so registers move between whole groups of four warps: 384 threads x 168 at launch
     // = 128 x (56 + 224 + 224).
-    static constexpr bool MOVE_REGS = PLANES == 2;
+    static constexpr bool MOVE_REGS = CUT && BN == 256;
     static constexpr int FIRST = MOVE_REGS ? 4 : 2, THREADS = 32 * (FIRST + 8);
 };
 
@@ -78,8 +84,6 @@ struct lt_prob {
     int a_mn, b_mn;                        // 1: the M (N) axis is the contiguous one
     int a_k0, b_k0, b_n0;                  // where the piece of the vocabulary starts in A or B
 };
-
-enum { LT_FWD = 0, LT_DZ = 1, LT_GRAD = 2 };
 
 struct lt_args {
     lt_prob p[2];
@@ -442,11 +446,11 @@ __device__ __forceinline__ void lt_columns(const lt_args& e, const lt_tile& t, l
     __syncwarp();
 }
 
-template <int PLANES, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lt_shape<PLANES>::THREADS, 1)
+template <int PLANES, int EPI, bool CUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(lt_shape<PLANES, EPI, CUT>::THREADS, 1)
 lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmA1,
               const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ lt_args e) {
-    typedef lt_shape<PLANES> S;
+    typedef lt_shape<PLANES, EPI, CUT> S;
     extern __shared__ unsigned char lt_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(lt_raw) + 1023) & ~(uintptr_t)1023);
     float* stage_all = reinterpret_cast<float*>(ring + LT_STAGE_ALL);
@@ -579,15 +583,15 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t idesc = (1u << 4) | (PLANES == 2 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
                                        ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
-                // bf16: one accumulator for all of K; f32: one per LT_CHAIN k-blocks
-                const int segs = PLANES == 1 ? 1 : (nkb + LT_CHAIN - 1) / LT_CHAIN;
+                const int segs = CUT ? (nkb + S::CHAIN - 1) / S::CHAIN : 1;
+                const int chain = S::CHAIN == 1 ? 1 : (nkb + segs - 1) / segs;  // about the same for all pieces
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
                     const uint32_t buf = seg % S::BUFFERS;
                     ok = lt_wait(&acc_empty[buf], ((seg / S::BUFFERS) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d = tmem + buf * S::BN;
-                    for (int kb = 0; kb < (PLANES == 1 ? nkb : min(LT_CHAIN, nkb - sg * LT_CHAIN)); kb++, it++) {
+                    for (int kb = 0; kb < (CUT ? min(chain, nkb - sg * chain) : nkb); kb++, it++) {
                         const int s = it % S::STAGES;
                         ok = lt_wait(&full[s], (it / S::STAGES) & 1u, e.err);
                         if (!ok) break;
@@ -645,9 +649,9 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] * e.wscale[0] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
-            const int segs = PLANES == 1 ? 1 : (nkb + LT_CHAIN - 1) / LT_CHAIN;
-            float acc[PLANES == 1 ? 2 : HALF / 32][32];
-            if (PLANES != 1)
+            const int segs = CUT ? (nkb + S::CHAIN - 1) / S::CHAIN : 1;
+            float acc[CUT ? HALF / 32 : 2][32];
+            if (CUT)
 #pragma unroll
                 for (int c = 0; c < HALF / 32; c++)
 #pragma unroll
@@ -658,7 +662,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t ta = taddr + buf * S::BN;
-                if (PLANES == 1) {
+                if constexpr (!CUT) {
                     // the next 32 columns are on their way while these are worked on
                     lt_ld32(ta, acc[0]);
 #pragma unroll 1
@@ -697,7 +701,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 }
             }
             if (!ok) break;
-            if (PLANES != 1) {
+            if constexpr (CUT) {
                 // one copy of the epilogue's code: the next 32 columns move into its registers (four copies, 130 KB of
                 // instructions, took a single tile from 14 to 26 us)
 #pragma unroll 1
@@ -746,7 +750,7 @@ struct lm_shape {
     static constexpr int STAGES = PLANES == 3 ? 2 : 4;
     // accumulators of 64 columns: the tensor core goes on while the epilogue works on a tile's sums
     static constexpr int BUFFERS = (512 - STAGES * STAGE_COLS) / 64;
-    static constexpr int CHAIN = PLANES == 3 ? 1 : 1 << 20;  // k-blocks per accumulator
+    static constexpr int CHAIN = PLANES == 3 ? 1 : LT_CHAIN_DZ * LT_BK / LM_BK;  // k-blocks per accumulator
     static constexpr int SMEM = STAGES * STAGE_BYTES + 2 * 4 * 64 * 8 + 1024 + 256;
 };
 
@@ -1453,22 +1457,33 @@ static lt_prob lt_problem(int M, int N, int K, int bn, int a_mn, int b_mn) {
     return p;
 }
 
-template <int PLANES, int EPI>
+template <int PLANES, int EPI, bool CUT>
 static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
-    RG_CUDA(cudaFuncSetAttribute(lce_tc_kernel<PLANES, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_SMEM_BYTES));
+    RG_CUDA(cudaFuncSetAttribute(lce_tc_kernel<PLANES, EPI, CUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_SMEM_BYTES));
     long long total = 0;
     for (int i = 0; i < e.nprobs; i++) total += (long long)e.p[i].tiles_m * e.p[i].tiles_n * e.p[i].splits;
     if (total > 0x3fffffff) return rg_fail(RG_ERR_SHAPE, "linear_cross_entropy: too many tiles");
     const int grid = 2 * (int)std::min<long long>(total, ctx->sm_count / 2);
-    RG_CUDA(rg_launch(true, lce_tc_kernel<PLANES, EPI>, dim3(grid), dim3(lt_shape<PLANES>::THREADS), LT_SMEM_BYTES, ctx->stream, maps[0], maps[1],
-                      maps[2], maps[3], e));
+    RG_CUDA(rg_launch(true, lce_tc_kernel<PLANES, EPI, CUT>, dim3(grid), dim3(lt_shape<PLANES, EPI, CUT>::THREADS), LT_SMEM_BYTES, ctx->stream,
+                      maps[0], maps[1], maps[2], maps[3], e));
     RG_LAUNCHED(ctx);
     e.counter++;  // each launch hands out its tiles from a counter of its own
     return RG_OK;
 }
+// bf16 logits in pieces along D.  lse, the loss and dbias are f32, and a chain that truncates shows in them: off by up to 1.1e-6
+// (lse) and 4.4e-6 (dbias) of the norm at D = 1600, 5.7e-6 and 2e-5 at 9000, against 4.5e-7 and 8.4e-7 with chains of 768 and
+// 384.  dx and dw are rounded to bf16, so dz is only cut where dbias is asked for.  Cost: loss of 4096x1600x50257 537 -> 560 us, gradients
+// with a bias of 2048x768x50257 479 -> 491 and of 4096x1600x50257 1,700 -> 1,785 (in pieces always: loss of 4096x192x50257 160 -> 221).
+template <int EPI>
+static bool lt_cuts(const lce_call& c) {
+    return EPI == LT_FWD ? c.D > LT_CHAIN_FWD * LT_BK : c.D > LT_CHAIN_DZ * LT_BK && c.dbias;
+}
 template <int EPI>
 static rg_status lt_run(rg_ctx* ctx, const lce_call& c, const CUtensorMap* maps, lt_args& e) {
-    return c.dtype == RG_DTYPE_F32 ? lt_launch<EPI == LT_GRAD ? 3 : 2, EPI>(ctx, maps, e) : lt_launch<1, EPI>(ctx, maps, e);
+    if (c.dtype == RG_DTYPE_F32) return lt_launch<EPI == LT_GRAD ? 3 : 2, EPI, true>(ctx, maps, e);
+    if constexpr (EPI != LT_GRAD)
+        if (lt_cuts<EPI>(c)) return lt_launch<1, EPI, true>(ctx, maps, e);
+    return lt_launch<1, EPI, false>(ctx, maps, e);
 }
 
 static void lt_common(rg_ctx* ctx, const lce_call& c, int* counter, lt_args* e) {

@@ -1129,3 +1129,13 @@ def test_linear_cross_entropy_f32_keeps_f32(backend, R, D, V):
     the sum of squares is 1e-6.  lse: the same over a logarithm of 4 to 9, an eighth."""
     e = ce_norm_errors(backend, R, D, V, "f32")
     assert e["dx"] <= 1e-6 and e["dw"] <= 1e-6 and e["dbias"] <= 1e-6 and e["lse"] <= 1.5e-7, e
+
+
+@pytest.mark.parametrize("R,D,V", [(17, 768, 33), (17, 1600, 33), (64, 1600, 301), (300, 800, 72), (300, 9000, 33), (64, 9000, 301), (2500, 416, 96)])
+def test_linear_cross_entropy_f32_results_of_bf16_inputs(backend, R, D, V):
+    """lse and dbias are f32 whatever the matrices are, also for a wide D: accumulators of at most 768 (lse) and 384 of K (dbias), 48
+    and 24 steps that truncate by half a step (2^-24) in the mean, of a partial sum that is half of the logit in the mean.  A
+    logit of magnitude 2.5 is then off by 3.6e-6 and 1.8e-6: 1.4e-6 of lse, and 1.8e-6 of each term of dbias; 1e-6 for the
+    arguments of the exponentials as in f32."""
+    e = ce_norm_errors(backend, R, D, V, "bf16")
+    assert e["lse"] <= 1.5e-6 and e["dbias"] <= 2.1e-6, e
