@@ -30,11 +30,10 @@
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
 // The tensor core truncates when it adds to its f32 accumulator, always towards zero, so a long chain loses about 2^-25 of the
 // running sum per step (measured: a relative error of 7e-7 at K = 768 and 1.4e-5 at K = 50304 for random signs).  For f32
-// inputs the chain is therefore cut after every k-block of 64: in each the small products come first and that of the leading
-// planes last, and the epilogue warps add the result to their f32 registers with rounding.  Errors of the norm against 64 bits,
-// 600 rows, 128x300: dx 4.4e-7, dw 4.5e-7, dbias 2.2e-7, lse 7e-8 (f32 operations: 6.4e-7, 5.2e-7, 1.5e-7, 7e-8); cut after
-// every two blocks 1.4e-6, 1.4e-6, 6.5e-7, 2.0e-7, for a loss of 4096x768x50257 in 800 instead of 834 us and a gradient of
-// 2048 rows in 2,170 instead of 2,225 (858 and 862, 2,309 and 2,373 where the power limit holds the clock down).
+// inputs the chain is therefore cut after every k-block of 64 (lt_seg): in each the small products come first and that of the
+// leading planes last, and the epilogue warps add the result to their f32 registers with rounding.  Errors of the norm against
+// 64 bits, 600 rows, 128x300: dx 4.4e-7, dw 4.5e-7, dbias 2.2e-7, lse 7e-8 (f32 operations: 6.4e-7, 5.2e-7, 1.5e-7, 7e-8); cut
+// after every two blocks 1.4e-6, 1.4e-6, 6.5e-7, 2.0e-7, at the same speed for the loss and 1 % faster for the gradient.
 #include "rg_lce.cuh"
 
 #include <cuda.h>
@@ -69,10 +68,10 @@ struct lt_shape {
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
     static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6, 3 or 2
     static constexpr int BUFFERS = 512 / BN;  // accumulators in tensor memory
-    static constexpr int CHAIN = PLANES != 1 ? 1 : EPI == LT_FWD ? LT_CHAIN_FWD : LT_CHAIN_DZ;  // k-blocks per accumulator, at most
-    // Warp 0 copies, warp 1 multiplies, FIRST.. the eight epilogue warps.  256 columns in registers: a thread holds 128 columns in registers,
-    // more than 12 warps get at launch, so registers move between whole groups of four warps: 384 threads x 168 at launch
-    // = 128 x (56 + 224 + 224).
+    static constexpr int CHAIN = PLANES != 1 ? 1 : EPI == LT_FWD ? LT_CHAIN_FWD : LT_CHAIN_DZ;  // k-blocks per accumulator (lt_seg)
+    // Warp 0 copies, warp 1 multiplies, FIRST.. the eight epilogue warps.  Where pieces of 256 columns are added, a thread holds
+    // 128 of them in registers, more than 12 warps get at launch, so registers move between whole groups of four warps: 384
+    // threads x 168 at launch = 128 x (56 + 224 + 224).
     static constexpr bool MOVE_REGS = CUT && BN == 256;
     static constexpr int FIRST = MOVE_REGS ? 4 : 2, THREADS = 32 * (FIRST + 8);
 };
@@ -266,6 +265,23 @@ __device__ __forceinline__ lt_tile lt_decode(const lt_args& e, int t) {
 template <int PLANES>
 __device__ __forceinline__ int lt_width(const lt_prob& p, int n) {
     return min(lt_shape<PLANES>::BN, (p.N - n * lt_shape<PLANES>::BN + 31) & ~31);
+}
+
+// How the nkb k-blocks of a tile are cut into accumulators: their number, and the k-blocks of accumulator sg.  Pairs have two
+// accumulators in tensor memory, and the epilogue of the tile before (3,500 cycles) lasts longer than the products of two k-blocks
+// (3,072); so of 8 k-blocks and more the first two accumulators take two each: loss of 1024x768x50257
+// 280 -> 266 us, of 4096 rows 818 to 857 -> 752 to 781; dx 4.0e-7 -> 6.5e-7 at worst (2500x512x300; f32 operations 9.9e-7).
+template <typename S, int PLANES, bool CUT>
+__device__ __forceinline__ int lt_segs(int nkb) {
+    if (!CUT) return 1;
+    return PLANES == 2 ? nkb - (nkb >= 8 ? 2 : 0) : (nkb + S::CHAIN - 1) / S::CHAIN;
+}
+template <typename S, int PLANES, bool CUT>
+__device__ __forceinline__ int lt_seg(int nkb, int segs, int sg) {
+    if (!CUT) return nkb;
+    if (PLANES == 2) return nkb >= 8 && sg < 2 ? 2 : 1;
+    const int chain = S::CHAIN == 1 ? 1 : (nkb + segs - 1) / segs;  // about the same for all
+    return min(chain, nkb - sg * chain);
 }
 
 // What a thread keeps of its row while the columns of a tile pass by.
@@ -583,15 +599,15 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t idesc = (1u << 4) | (PLANES == 2 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
                                        ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
-                const int segs = CUT ? (nkb + S::CHAIN - 1) / S::CHAIN : 1;
-                const int chain = S::CHAIN == 1 ? 1 : (nkb + segs - 1) / segs;  // about the same for all pieces
+                const int segs = lt_segs<S, PLANES, CUT>(nkb);
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
                     const uint32_t buf = seg % S::BUFFERS;
                     ok = lt_wait(&acc_empty[buf], ((seg / S::BUFFERS) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d = tmem + buf * S::BN;
-                    for (int kb = 0; kb < (CUT ? min(chain, nkb - sg * chain) : nkb); kb++, it++) {
+                    const int blocks = lt_seg<S, PLANES, CUT>(nkb, segs, sg);
+                    for (int kb = 0; kb < blocks; kb++, it++) {
                         const int s = it % S::STAGES;
                         ok = lt_wait(&full[s], (it / S::STAGES) & 1u, e.err);
                         if (!ok) break;
@@ -649,7 +665,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] * e.wscale[0] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
-            const int segs = CUT ? (nkb + S::CHAIN - 1) / S::CHAIN : 1;
+            const int segs = lt_segs<S, PLANES, CUT>(nkb);
             float acc[CUT ? HALF / 32 : 2][32];
             if (CUT)
 #pragma unroll
