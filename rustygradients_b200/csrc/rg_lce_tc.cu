@@ -1564,7 +1564,8 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
     // dx or its transpose: whichever pads less (a row tile is 256, a column tile as narrow as 32)
     auto pad = [](long long m, long long n) { return (m + 255) / 256 * 256 * ((n + 31) / 32 * 32); };
     const bool dx_t = pad(c.D, c.R) < pad(c.R, c.D);
-    lt_prob pdx = dx_t ? lt_problem(c.D, c.R, piece, bn, 0, 0) : lt_problem(c.R, c.D, piece, bn, 0, 0);
+    const int first = std::min(piece, c.V);  // columns of the first piece; it writes every partial dx that is added in the end
+    lt_prob pdx = dx_t ? lt_problem(c.D, c.R, first, bn, 0, 0) : lt_problem(c.R, c.D, first, bn, 0, 0);
     lt_prob pdw = lt_problem(piece, c.D, c.R, bn, 1, 1);
     // The K axes are cut where tiles are fewer or longer than makes an even load: runs of `run` k-blocks, none of them empty.  A
     // smaller last piece has fewer runs of dx and leaves the other sums alone; dw is only cut when there is one piece.
@@ -1574,7 +1575,7 @@ rg_status lce_tc_backward(rg_ctx* ctx, lce_call& c) {
         p.kb_per = rg_cdiv(p.kb_per, std::min(16, rg_cdiv(p.kb_per, fair)));
         return p.kb_per;
     };
-    const int run = cut(pdx), splits = rg_cdiv(rg_cdiv(piece, LT_BK), run);
+    const int run = cut(pdx), splits = rg_cdiv(rg_cdiv(first, LT_BK), run);
     const bool cut_dw = pieces == 1 && pdw.tiles_m * pdw.tiles_n < clusters && pdw.kb_per > fair;
     const int run_w = cut_dw ? cut(pdw) : pdw.kb_per, splits_w = rg_cdiv(rg_cdiv(c.R, LT_BK), run_w);
     const size_t plen = (size_t)splits * c.R * c.D, wlen = (size_t)splits_w * c.D * c.V;

@@ -1139,3 +1139,63 @@ def test_linear_cross_entropy_f32_results_of_bf16_inputs(backend, R, D, V):
     arguments of the exponentials as in f32."""
     e = ce_norm_errors(backend, R, D, V, "bf16")
     assert e["lse"] <= 1.5e-6 and e["dbias"] <= 2.1e-6, e
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# memory that was something else before
+# ---------------------------------------------------------------------------------------------------------------------
+def poison(be):
+    """What the context and the device's pool hand out next is full of NaN."""
+    held = [be.from_slice(np.full(n, np.nan, np.float32), [n]) for size in range(9, 21) for n in [2 ** size // 4] for _ in range(24)]
+    held += [be.from_slice(np.full(n << 18, np.nan, np.float32), [n << 18]) for n in (2, 3, 5, 8, 16, 32, 64) for _ in range(4)]
+    be.synchronize()
+    del held
+
+
+def bits(be, storages):
+    return [be.to_vec(s).copy() for s in storages if s is not None]
+
+
+# (10, 8, 8548): the K axis of dx in 15 pieces where a vocabulary rounded up to whole tiles would have 16
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", [(10, 8, 8548), (23, 9, 8472), (12, 12, 12379), (16, 9, 8598), (300, 40, 5700), (3, 70, 5000), (5, 8, 2), (17, 8, 33), (64, 192, 97),
+                                   (200, 100, 1000), (193, 60, 131), (511, 257, 775), (700, 768, 300), (1025, 40, 2049), (8000, 128, 97)])
+def test_linear_cross_entropy_in_memory_of_nan(backend, R, D, V, dtype):
+    """No result depends on what its scratch held before."""
+    be = backend
+    x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.2, 1)
+    ex = ce_exact(x, w, b, t)
+    X, W, B, T, L = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t), put(be, ex["lse"].astype(np.float32))
+    _, _, tdx, tdw, tdb = ce_bounds(x, w, b, dtype, ex, t != IGNORE)
+    for turn in range(2):
+        poison(be)
+        loss, lse = bits(be, be.linear_cross_entropy(X, W, B, T))
+        poison(be)
+        dx, dw, db = (get(be, s) for s in be.linear_cross_entropy_bwd(X, W, B, T, L))
+        assert np.isfinite(loss).all() and np.isfinite(lse).all()
+        within(dx, ex["dx"], tdx + 1e-45, "dx")
+        within(dw, ex["dw"], tdw + 1e-45, "dw")
+        within(db, ex["db"], tdb + 1e-45, "dbias")
+
+
+def test_linear_cross_entropy_wide_values_in_memory_of_nan(backend):
+    for R, D, V in ((200, 64, 1000), (300, 30, 8548), (193, 9, 8590)):
+        poison(backend)
+        ce_one_large_value(backend, R, D, V, "f32", "dead channel", 1e10)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_other_training_ops_in_memory_of_nan(backend, dtype):
+    be = backend
+    for rows, n in ((1, 1), (3, 7), (256, 192), (37, 1023), (650, 1600), (5, 4097), (2, 16386), (3000, 768)):
+        x, dy, g, b = ln_inputs(rows, n, dtype)
+        X, DY, G, B = put(be, x, dtype), put(be, dy, dtype), put(be, g), put(be, b)
+        y, m, r = be.layer_norm_fwd(X, G, B, EPS)
+        want = bits(be, (y, m, r, *be.layer_norm_bwd(DY, X, G, m, r), *be.clip_grad_norm([X, DY, G], 0.5)[0]))
+        poison(be)
+        y, m, r = be.layer_norm_fwd(X, G, B, EPS)
+        poison(be)
+        got = bits(be, (y, m, r, *be.layer_norm_bwd(DY, X, G, m, r), *be.clip_grad_norm([X, DY, G], 0.5)[0]))
+        assert all(np.isfinite(a).all() and np.array_equal(a, b) for a, b in zip(got, want)), (rows, n)
+    poison(be)
+    assert np.array_equal(be.to_vec(be.cast(put(be, x, dtype), "f32")).reshape(x.shape), x)
