@@ -11,8 +11,8 @@
 // brings 64-element wide boxes (128-byte swizzle) of three-dimensional arrays [plane][row][column]; what lies outside is
 // filled with zeros, which handles every ragged edge of R, D and V.
 //
-// bf16 inputs are one plane and are multiplied as they are, with accumulators of up to 768 of K for the loss and one for all of K
-// where the result is rounded to bf16 (lt_cuts).  dz is one bf16 plane too: its
+// bf16 inputs are one plane and are multiplied as they are, with accumulators of 256 to 768 of K for the loss and one for all of
+// K where the result is rounded to bf16 (lt_chain).  dz is one bf16 plane too: its
 // rounding (half a step, at most 2^-8 of each value) costs dx and dw about half of what their own rounding to
 // bf16 does (8e-4 of their norm at 4096x1600x50257); a second plane would double the products that are most of the gradient's
 // time.  The form for few rows, where no product is bound by the tensor cores, keeps dz in f32.  f32 inputs are split into planes of 16 bits whose products are
@@ -43,9 +43,11 @@
 
 #define LT_BM 256  // rows of a tile: 128 in each CTA of a pair
 #define LT_BK 64
-// k-blocks of 64 per accumulator for bf16 inputs, where it is cut: the loss, and dz where dbias is summed from it (lt_cuts)
+// k-blocks of 64 per accumulator for logits of bf16 inputs, where it is cut (lt_chain): the loss, dz where dbias is summed from it,
+// and both where there is no more than one tile for each pair of CTAs
 #define LT_CHAIN_FWD 12
 #define LT_CHAIN_DZ 6
+#define LT_CHAIN_ONE 4
 #define LT_SPIN_LIMIT (1u << 22)
 #define LT_STAGE_ALL 196608   // bytes of the operand ring
 #define LT_MAX_STAGES 6
@@ -68,7 +70,6 @@ struct lt_shape {
     static constexpr int STAGE_BYTES = PLANES * (A_BYTES + B_BYTES);
     static constexpr int STAGES = LT_STAGE_ALL / STAGE_BYTES;  // 6, 3 or 2
     static constexpr int BUFFERS = 512 / BN;  // accumulators in tensor memory
-    static constexpr int CHAIN = PLANES != 1 ? 1 : EPI == LT_FWD ? LT_CHAIN_FWD : LT_CHAIN_DZ;  // k-blocks per accumulator (lt_seg)
     // Warp 0 copies, warp 1 multiplies, FIRST.. the eight epilogue warps.  Where pieces of 256 columns are added, a thread holds
     // 128 of them in registers, more than 12 warps get at launch, so registers move between whole groups of four warps: 384
     // threads x 168 at launch = 128 x (56 + 224 + 224).
@@ -108,6 +109,7 @@ struct lt_args {
     float* dwparts;           // [splits][D][V], or NULL: the second problem's K axis is not cut
     int dw_bf16;
     const float* scal;
+    int chain;                // PLANES 1, CUT: k-blocks per accumulator, at most
 };
 
 // f32 logits: do the largest finite magnitudes of w and x ask for more range than a pair of f16 has?  (A product beyond f32 is
@@ -271,16 +273,16 @@ __device__ __forceinline__ int lt_width(const lt_prob& p, int n) {
 // accumulators in tensor memory, and the epilogue of the tile before (3,500 cycles) lasts longer than the products of two k-blocks
 // (3,072); so of 8 k-blocks and more the first two accumulators take two each: loss of 1024x768x50257
 // 280 -> 266 us, of 4096 rows 818 to 857 -> 752 to 781; dx 4.0e-7 -> 6.5e-7 at worst (2500x512x300; f32 operations 9.9e-7).
-template <typename S, int PLANES, bool CUT>
-__device__ __forceinline__ int lt_segs(int nkb) {
+template <int PLANES, bool CUT>
+__device__ __forceinline__ int lt_segs(const lt_args& e, int nkb) {
     if (!CUT) return 1;
-    return PLANES == 2 ? nkb - (nkb >= 8 ? 2 : 0) : (nkb + S::CHAIN - 1) / S::CHAIN;
+    return PLANES == 3 ? nkb : PLANES == 2 ? nkb - (nkb >= 8 ? 2 : 0) : (nkb + e.chain - 1) / e.chain;
 }
-template <typename S, int PLANES, bool CUT>
+template <int PLANES, bool CUT>
 __device__ __forceinline__ int lt_seg(int nkb, int segs, int sg) {
     if (!CUT) return nkb;
-    if (PLANES == 2) return nkb >= 8 && sg < 2 ? 2 : 1;
-    const int chain = S::CHAIN == 1 ? 1 : (nkb + segs - 1) / segs;  // about the same for all
+    if (PLANES != 1) return PLANES == 2 && nkb >= 8 && sg < 2 ? 2 : 1;
+    const int chain = (nkb + segs - 1) / segs;  // about the same for all
     return min(chain, nkb - sg * chain);
 }
 
@@ -599,14 +601,14 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
                 const uint32_t idesc = (1u << 4) | (PLANES == 2 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)p.a_mn << 15) | ((uint32_t)p.b_mn << 16) |
                                        ((uint32_t)(lt_width<PLANES>(p, t.n) >> 3) << 17) | ((uint32_t)(LT_BM >> 4) << 24);
                 const uint32_t astep = p.a_mn ? 2048 : 32, bstep = p.b_mn ? 2048 : 32;  // 16 elements of K
-                const int segs = lt_segs<S, PLANES, CUT>(nkb);
+                const int segs = lt_segs<PLANES, CUT>(e, nkb);
                 for (int sg = 0; sg < segs && ok; sg++, seg++) {
                     const uint32_t buf = seg % S::BUFFERS;
                     ok = lt_wait(&acc_empty[buf], ((seg / S::BUFFERS) & 1u) ^ 1u, e.err);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d = tmem + buf * S::BN;
-                    const int blocks = lt_seg<S, PLANES, CUT>(nkb, segs, sg);
+                    const int blocks = lt_seg<PLANES, CUT>(nkb, segs, sg);
                     for (int kb = 0; kb < blocks; kb++, it++) {
                         const int s = it % S::STAGES;
                         ok = lt_wait(&full[s], (it / S::STAGES) & 1u, e.err);
@@ -665,7 +667,7 @@ lce_tc_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ 
             w.scale = (PLANES == 2 && w.live) ? e.xscale[w.row] * e.wscale[0] : 0.f;
             const int c0 = t.n * S::BN + half * HALF;
             const int kb0 = t.split * p.kb_per, nkb = min(p.kb_per, (p.K + LT_BK - 1) / LT_BK - kb0);
-            const int segs = lt_segs<S, PLANES, CUT>(nkb);
+            const int segs = lt_segs<PLANES, CUT>(e, nkb);
             float acc[CUT ? HALF / 32 : 2][32];
             if (CUT)
 #pragma unroll
@@ -766,7 +768,7 @@ struct lm_shape {
     static constexpr int STAGES = PLANES == 3 ? 2 : 4;
     // accumulators of 64 columns: the tensor core goes on while the epilogue works on a tile's sums
     static constexpr int BUFFERS = (512 - STAGES * STAGE_COLS) / 64;
-    static constexpr int CHAIN = PLANES == 3 ? 1 : LT_CHAIN_DZ * LT_BK / LM_BK;  // k-blocks per accumulator
+    static constexpr int CHAIN = PLANES == 3 ? 1 : LT_CHAIN_ONE * LT_BK / LM_BK;  // k-blocks per accumulator
     static constexpr int SMEM = STAGES * STAGE_BYTES + 2 * 4 * 64 * 8 + 1024 + 256;
 };
 
@@ -1486,19 +1488,27 @@ static rg_status lt_launch(rg_ctx* ctx, const CUtensorMap* maps, lt_args& e) {
     e.counter++;  // each launch hands out its tiles from a counter of its own
     return RG_OK;
 }
-// bf16 logits in pieces along D.  lse, the loss and dbias are f32, and a chain that truncates shows in them: off by up to 1.1e-6
-// (lse) and 4.4e-6 (dbias) of the norm at D = 1600, 5.7e-6 and 2e-5 at 9000, against 4.5e-7 and 8.4e-7 with chains of 768 and
-// 384.  dx and dw are rounded to bf16, so dz is only cut where dbias is asked for.  Cost: loss of 4096x1600x50257 537 -> 560 us, gradients
-// with a bias of 2048x768x50257 479 -> 491 and of 4096x1600x50257 1,700 -> 1,785 (in pieces always: loss of 4096x192x50257 160 -> 221).
+// bf16 logits in pieces along D: k-blocks per accumulator, 0 for one accumulator.  lse, the loss and dbias are f32, and a chain that
+// truncates shows in them: off by up to 1.1e-6 (lse) and 4.4e-6 (dbias) of the norm at D = 1600, 5.7e-6 and 2e-5 at 9000, against
+// 6.4e-7 with chains of 768, 1.3e-6 of 384 and 9e-7 of 256 for dbias.  dx and dw are rounded to bf16, so dz is only cut where
+// dbias is asked for.  Cost of the long chains: loss of 4096x1600x50257 537 -> 553 us, gradients with a bias of 2048x768x50257 479
+// -> 490 and of 4096x1600x50257 1,700 -> 1,765 (256 for all: 520 and 1,795); loss of 4096x192x50257 in pieces 221 instead of 160.
+// With one tile for a pair of CTAs nothing waits for the epilogue, and 256 costs nothing (200x768x3000, 1000x768x4000: the same
+// within 1 %).
 template <int EPI>
-static bool lt_cuts(const lce_call& c) {
-    return EPI == LT_FWD ? c.D > LT_CHAIN_FWD * LT_BK : c.D > LT_CHAIN_DZ * LT_BK && c.dbias;
+static int lt_chain(rg_ctx* ctx, const lce_call& c, const lt_prob& p) {
+    if (EPI == LT_DZ && !c.dbias) return 0;
+    const bool one = (long long)p.tiles_m * p.tiles_n <= ctx->sm_count / 2;
+    const int chain = one ? LT_CHAIN_ONE : EPI == LT_FWD ? LT_CHAIN_FWD : LT_CHAIN_DZ;
+    return c.D > chain * LT_BK ? chain : 0;
 }
 template <int EPI>
 static rg_status lt_run(rg_ctx* ctx, const lce_call& c, const CUtensorMap* maps, lt_args& e) {
     if (c.dtype == RG_DTYPE_F32) return lt_launch<EPI == LT_GRAD ? 3 : 2, EPI, true>(ctx, maps, e);
-    if constexpr (EPI != LT_GRAD)
-        if (lt_cuts<EPI>(c)) return lt_launch<1, EPI, true>(ctx, maps, e);
+    if constexpr (EPI != LT_GRAD) {
+        e.chain = lt_chain<EPI>(ctx, c, e.p[0]);
+        if (e.chain) return lt_launch<1, EPI, true>(ctx, maps, e);
+    }
     return lt_launch<1, EPI, false>(ctx, maps, e);
 }
 
