@@ -51,9 +51,8 @@ __global__ void __launch_bounds__(1024) lce_check_kernel(const float* __restrict
 // lse of 8 rows per CTA: 32 threads share the slices of a row, lanes of 8 rows read 64 contiguous bytes.  The maximum of
 // all slices comes first, so the sum is one exponential per slice with no chain between them.  Then the loss: the sum of a
 // CTA's rows in f64; the last CTA to finish adds the CTAs in order and divides.
-__global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict__ parts, int nparts, int R, const int* __restrict__ tgt,
-                                                       const float* __restrict__ tz, const float* __restrict__ scal,
-                                                       int* __restrict__ ticket, double* __restrict__ sums, float* __restrict__ lse_out,
+__global__ void __launch_bounds__(256) lce_loss_kernel(const float2* parts, int nparts, int R, const int* tgt, const float* tz,
+                                                       const float* scal, int* ticket, double* sums, float* __restrict__ lse_out,
                                                        float* __restrict__ loss) {
     __shared__ float red[32][9];
     __shared__ double rows_s[8];
@@ -126,9 +125,9 @@ __global__ void __launch_bounds__(256) lce_loss_kernel(const float2* __restrict_
 // The final sums of the gradient: the first `xblocks` blocks those of dx (or dw), the others 32 columns of dbias each, eight
 // warps sharing the partials.  (A launch of its own for dbias cost 3 us.)
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) lce_finish_kernel(const float* __restrict__ parts, int nparts, size_t count, const float* __restrict__ scal,
-                                                         const int* __restrict__ tgt, int D, T* __restrict__ dx, int xblocks, const float* __restrict__ dbparts, int dbrows,
-                                                         int dbpitch, int cols, float* __restrict__ dbias) {
+__global__ void __launch_bounds__(256) lce_finish_kernel(const float* parts, int nparts, size_t count, const float* scal, const int* tgt, int D,
+                                                         T* __restrict__ dx, int xblocks, const float* dbparts, int dbrows, int dbpitch,
+                                                         int cols, float* __restrict__ dbias) {
     __shared__ float red[8][32];
     rg_pdl_sync();
     const float scale = scal[1];
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(256, RB <= 4 ? 4 : RB <= 8 ? 3 : 2) lce_few_dz
 // out: 81 us for 8 rows of [768,50257] f32, 3.8 TB/s; 128 us for 16, bound by the exchanges.
 #define LCE_DG 32
 template <typename T, int RB>
-__global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, const float* __restrict__ dz, float* __restrict__ dxparts) {
+__global__ void __launch_bounds__(256) lce_few_grad_kernel(const lce_call c, const float* dz, float* __restrict__ dxparts) {
     constexpr int PAIRS = (RB + 1) / 2;
     __shared__ __align__(16) float xs[LCE_DG][RB];
     __shared__ float dxs[8][LCE_DG][RB];

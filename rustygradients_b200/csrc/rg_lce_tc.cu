@@ -1040,7 +1040,7 @@ __global__ void __launch_bounds__(LM_THREADS, 1) lce_mid_kernel(const __grid_con
                 float(&v)[32] = acc[0];
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] += bias;
-                const int tgt = lane < left ? __ldg(e.tgt + r0 + lane) : -1;  // of row `lane`
+                const int tgt = lane < left ? e.tgt[r0 + lane] : -1;  // of row `lane`
                 const bool hits = __any_sync(RG_FULL_MASK, tgt >= v0 && tgt < v0 + e.tile);  // a row has its target in the tile
                 if (EPI == LT_FWD) {
                     if (hits) {
@@ -1257,7 +1257,7 @@ __global__ void __launch_bounds__(256) lt_max_kernel(const float* __restrict__ w
 // launch of 4 to 8 us of its own.
 template <bool PAIR, bool TRIPLE>
 __global__ void __launch_bounds__(256) lt_pack_kernel(const float* __restrict__ src, int rows, int cols, int pitch,
-                                                      const unsigned* __restrict__ largest, uint16_t* __restrict__ pair,
+                                                      const unsigned* largest, uint16_t* __restrict__ pair,
                                                       uint16_t* __restrict__ triple, float* __restrict__ scale_out, const lt_rows x) {
     rg_pdl_sync();
     const int xblocks = (x.rows + 7) / 8, block = (int)blockIdx.x - xblocks;

@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256) rg_ln_bwd_long_cols_kernel(const T* __res
 }
 
 // out[c] = sum over p of parts[p][c], c < cols, in a fixed order: a CTA takes 32 columns, its 32 warps every 32nd partial.
-__global__ void __launch_bounds__(1024) rg_colsum_kernel(const float* __restrict__ parts, int nparts, long long cols,
+__global__ void __launch_bounds__(1024) rg_colsum_kernel(const float* parts, int nparts, long long cols,
                                                          float* __restrict__ out0, float* __restrict__ out1, long long split) {
     __shared__ float red[32][33];
     rg_pdl_sync();
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(256) rg_clip_sumsq_kernel(const __grid_constan
     if (threadIdx.x == 0) parts[blockIdx.x] = acc;
 }
 
-__global__ void __launch_bounds__(256) rg_clip_scale_kernel(const __grid_constant__ clip_table t, const double* __restrict__ parts,
+__global__ void __launch_bounds__(256) rg_clip_scale_kernel(const __grid_constant__ clip_table t, const double* parts,
                                                             int nparts, float max_norm, float* __restrict__ norm_out) {
     __shared__ double red[8];
     asm volatile("griddepcontrol.wait;" ::: "memory");

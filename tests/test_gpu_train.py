@@ -1199,3 +1199,67 @@ def test_other_training_ops_in_memory_of_nan(backend, dtype):
         assert all(np.isfinite(a).all() and np.array_equal(a, b) for a, b in zip(got, want)), (rows, n)
     poison(be)
     assert np.array_equal(be.to_vec(be.cast(put(be, x, dtype), "f32")).reshape(x.shape), x)
+
+
+def backlogged(call, room=[]):
+    """`call` is enqueued behind work that lasts and empties the caches, so that all of its launches are there when the first one
+    starts, and the first one has to fetch everything from memory."""
+    import torch
+    room[:] = room or [torch.empty(1 << 29, device="cuda")]
+    for _ in range(3):
+        room[0].fill_(0)
+    return call()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("R,D,V", [(1, 64, 1000), (4, 64, 1000), (16, 96, 1003), (40, 64, 304), (150, 64, 301), (200, 64, 304), (300, 72, 304), (1390, 24, 152),
+                                   (1243, 176, 232), (509, 480, 776), (476, 176, 184), (1500, 40, 1001)])
+def test_linear_cross_entropy_enqueued_behind_other_work(R, D, V, dtype):
+    """The launches of a call start behind one another early; none may read what the one before has not written.  In memory of NaN,
+    with all launches waiting in the stream."""
+    import torch
+    torch.cuda.set_device(0)
+    be = rg.B200Backend(0, stream=torch.cuda.current_stream().cuda_stream)
+    x, w, b, t = ce_inputs(R, D, V, dtype, True, 0.2, 1)
+    X, W, B, T = put(be, x, dtype), put(be, w, dtype), put(be, b), put(be, t)
+    loss, lse = be.linear_cross_entropy(X, W, B, T)
+    L = put(be, be.to_vec(lse))
+    want = bits(be, (loss, lse)), bits(be, be.linear_cross_entropy_bwd(X, W, B, T, L))
+    nan = torch.full((1 << 18,), float("nan"), device="cuda").bfloat16()
+    N = {n: be.from_device(nan[:n]) for n in (128, 256, 512, 1024, 2048, 4096, 8192, 16384, 32768, 65536, 131072, 262144)}
+    for turn in range(40):
+        held = [be.cast(s, "f32") for s in N.values() for _ in range(8)]       # f32 NaN in buffers of every small size
+        torch.cuda.synchronize()
+        del held
+        got = backlogged(lambda: be.linear_cross_entropy(X, W, B, T))
+        assert all(np.array_equal(p, q) for p, q in zip(bits(be, got), want[0])), turn
+        held = [be.cast(s, "f32") for s in N.values() for _ in range(8)]
+        torch.cuda.synchronize()
+        del held, got
+        got = backlogged(lambda: be.linear_cross_entropy_bwd(X, W, B, T, L))
+        assert all(np.array_equal(p, q) for p, q in zip(bits(be, got), want[1])), turn
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_other_training_ops_enqueued_behind_other_work(dtype):
+    import torch
+    torch.cuda.set_device(0)
+    be = rg.B200Backend(0, stream=torch.cuda.current_stream().cuda_stream)
+    nan = torch.full((1 << 18,), float("nan"), device="cuda").bfloat16()
+    N = {n: be.from_device(nan[:n]) for n in (128, 256, 512, 1024, 2048, 4096, 8192, 16384, 32768, 65536, 131072, 262144)}
+    for rows, n in ((1, 64), (256, 192), (40, 1023), (300, 1600), (5, 16400)):
+        x, dy, g, b = ln_inputs(rows, n, dtype)
+        X, DY, G, B = put(be, x, dtype), put(be, dy, dtype), put(be, g), put(be, b)
+        y, m, r = be.layer_norm_fwd(X, G, B, EPS)
+
+        def step():
+            out = be.layer_norm_bwd(DY, X, G, m, r)
+            clipped, norm = be.clip_grad_norm([X, DY, G, B], 0.5)
+            return (*out, *clipped, norm)
+
+        want = bits(be, step())
+        for turn in range(20):
+            held = [be.cast(s, "f32") for s in N.values() for _ in range(8)]
+            torch.cuda.synchronize()
+            del held
+            assert all(np.array_equal(p, q) for p, q in zip(bits(be, backlogged(step)), want)), (rows, n, turn)
