@@ -207,9 +207,9 @@ __global__ void __launch_bounds__(256) rg_gemv_kernel(rg_gemv_args p) {
 // the step reads.
 // ---------------------------------------------------------------------------
 template <typename WT>
-__global__ void rg_embed_step_kernel(const uint32_t* __restrict__ tokens, int C, const WT* __restrict__ wte,
+__global__ void rg_embed_step_kernel(const uint32_t* tokens, int C, const WT* __restrict__ wte,
                                      const WT* __restrict__ wpe, int D, long long ldt, float* __restrict__ x,
-                                     const int* __restrict__ pos_next, int* __restrict__ pos) {
+                                     const int* pos_next, int* pos) {
     rg_pdl_sync();
     const int t = *pos_next;
     const int b = blockIdx.x;
@@ -472,7 +472,7 @@ static __global__ void __launch_bounds__(1024) rg_pick_kernel(rg_pick_args p) {
 
 // Merge of the split-context attention partials into finished head outputs:
 // out[b][h*hd + d] = sum_s w_s o_s[d] / sum_s w_s l_s with w_s = exp(m_s - max m).
-static __global__ void rg_attn_merge_kernel(const float* __restrict__ ap, float* __restrict__ out, int B, int H, int hd, int NS,
+static __global__ void rg_attn_merge_kernel(const float* ap, float* __restrict__ out, int B, int H, int hd, int NS,
                                             __nv_bfloat16* __restrict__ out16 = nullptr) {
     rg_pdl_sync();
     const int i = blockIdx.x * blockDim.x + threadIdx.x;

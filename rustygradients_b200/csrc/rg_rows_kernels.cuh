@@ -22,7 +22,7 @@ __device__ __forceinline__ float rg_block_sum_256(float v, float* sm8) {
 
 // v = x + bias + sum of the k-split partials (all optional but x); x <- v when store_x; out16 <- LN(v; gamma, beta).
 // Two-pass statistics on the values held in registers: mean, then the biased variance of (v - mean).
-static __global__ void __launch_bounds__(256) rg_rows_res_ln_bf16_kernel(const float* __restrict__ parts, int nparts, size_t pstride,
+static __global__ void __launch_bounds__(256) rg_rows_res_ln_bf16_kernel(const float* parts, int nparts, size_t pstride,
                                                                          const float* __restrict__ bias, float* __restrict__ x,
                                                                          int store_x, const float* __restrict__ gamma,
                                                                          const float* __restrict__ beta,
@@ -61,7 +61,7 @@ static __global__ void __launch_bounds__(256) rg_rows_res_ln_bf16_kernel(const f
 }
 
 // out16[m][n] = act(bias[n] + sum of the partials)
-static __global__ void rg_rows_act_bf16_kernel(const float* __restrict__ parts, int nparts, size_t pstride,
+static __global__ void rg_rows_act_bf16_kernel(const float* parts, int nparts, size_t pstride,
                                                const float* __restrict__ bias, int N, size_t total, int act,
                                                __nv_bfloat16* __restrict__ out16) {
     rg_pdl_sync();

@@ -204,3 +204,23 @@ def test_the_current_device_is_put_back(tmp_path):
     csrc = os.path.join(ROOT, "rustygradients_b200", "csrc")
     calls = [f"{f}: {line.strip()}" for f in sorted(os.listdir(csrc)) for line in open(os.path.join(csrc, f)) if "cudaSetDevice(" in line]
     assert calls == ["rg_internal.cuh: static int set(int d) { return (int)cudaSetDevice(d); }"]
+
+
+def test_kernels_that_start_early_read_only_finished_data_as_constant():
+    """A `const __restrict__` parameter of a kernel that waits for its predecessor may be read in front of the wait: only what was
+    complete before the chain began (a caller's matrices, weights, LayerNorm parameters) is passed that way."""
+    import re
+    csrc = os.path.join(ROOT, "rustygradients_b200", "csrc")
+    found = set()
+    for f in sorted(os.listdir(csrc)):
+        text = open(os.path.join(csrc, f)).read()
+        text = re.sub(r"__launch_bounds__\((?:[^()]|\([^()]*\))*\)|__cluster_dims__\([^()]*\)", "", text)
+        for m in re.finditer(r"__global__[^;{]*?(\w+)\(([^;{]*?)\)\s*\{", text):
+            end = text.find("\n}", m.end())
+            if re.search(r"rg_pdl_sync\(\)|griddepcontrol\.wait", text[m.end():end]):
+                found |= {(m.group(1), p) for p in re.findall(r"const [\w:]+\s*\*\s*__restrict__ (\w+)", m.group(2))}
+    assert found == {("lt_align_kernel", "src"), ("lt_max_kernel", "w"), ("lt_max_kernel", "x"), ("lt_pack_kernel", "src"),
+                     ("rg_embed_step_kernel", "wte"), ("rg_embed_step_kernel", "wpe"),
+                     ("rg_rows_res_ln_bf16_kernel", "bias"), ("rg_rows_res_ln_bf16_kernel", "gamma"), ("rg_rows_res_ln_bf16_kernel", "beta"),
+                     ("rg_rows_act_bf16_kernel", "bias"), ("rg_rows_res_ln_tp_bf16_kernel", "bias"),
+                     ("rg_rows_res_ln_tp_bf16_kernel", "gamma"), ("rg_rows_res_ln_tp_bf16_kernel", "beta")}
