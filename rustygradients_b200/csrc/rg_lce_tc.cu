@@ -57,9 +57,9 @@
 // of its 128 rows.  A k-block then costs an SM 128 x 64 + BN/2 x 64 values from L2 instead of 128 x 64 + BN x 64, which
 // bounded the one-SM form (12.5 TB/s from L2, 1.09 PFLOP/s in bf16).
 // Measured (PFLOP/s of the products that are multiplied; a library product of bf16 reaches 1.6, 1.37 for seconds on end):
-// logits of 4096x768x50257 f32 1.49 (640 us, tensor pipe active 80 %), of 8192x768x50257 bf16 1.26 (504 us, 63 %; 447 us when
-// nothing is brought from L2, 487 when the epilogue does nothing); gradient of 2048x768x50257 f32: dz 0.95 (502 us, 47 %; 340
-// without its planes and column sums), dx and dw 1.32 (68 %); of 4096x1600x50257 bf16: dz 1.28, dx and dw 1.21.
+// logits of 4096x768x50257 f32 1.50 (634 us, tensor pipe active 79 %), of 8192x768x50257 bf16 1.26 (503 us, 64 %; 447 us when
+// nothing is brought from L2, 487 when the epilogue does nothing); gradient of 2048x768x50257 f32: dz 1.00 (474 us, 47 %; 340
+// without its planes and column sums), dx and dw 1.33 (1,430 us, 62 to 66 %); of 4096x1600x50257 bf16: dz 1.37, dx and dw 1.24.
 // PLANES: 1 bf16 values, 2 pairs of f16, 3 triples of bf16.  CUT: the accumulator is cut along K and the pieces are added in
 // registers (always for f32 inputs); else the epilogue works on the columns as they come from tensor memory.
 enum { LT_FWD = 0, LT_DZ = 1, LT_GRAD = 2 };
