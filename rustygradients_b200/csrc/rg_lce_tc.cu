@@ -12,19 +12,20 @@
 // filled with zeros, which handles every ragged edge of R, D and V.
 //
 // bf16 inputs are one plane and are multiplied as they are, with accumulators of 256 to 768 of K for the loss and one for all of
-// K where the result is rounded to bf16 (lt_chain).  dz is one bf16 plane too: its
-// rounding (half a step, at most 2^-8 of each value) costs dx and dw about half of what their own rounding to
-// bf16 does (8e-4 of their norm at 4096x1600x50257); a second plane would double the products that are most of the gradient's
-// time.  The form for few rows, where no product is bound by the tensor cores, keeps dz in f32.  f32 inputs are split into planes of 16 bits whose products are
-// accumulated in f32:
+// K where the result is rounded to bf16 (lt_chain).  dz is one bf16 plane too: its rounding (half a step, at most 2^-8 of each
+// value) costs dx and dw about half of what their own rounding to bf16 does (8e-4 of their norm at 4096x1600x50257); a second
+// plane would double the products that are most of the gradient's time.  The form for few rows, where no product is bound by the
+// tensor cores, keeps dz in f32.
+// f32 inputs are split into planes of 16 bits whose products are accumulated in f32:
 //  * logits: two f16 planes, x = 2^-a (x0 + x1) with a power of two per row of x and one for w that bring the largest
 //    magnitude to 2^14..2^15.  x0 + x1 holds 22 bits, or what is above 2^-39 of that largest magnitude, whichever is less exact;
 //    three of the four products are taken, the fourth is below 2^-22 of the magnitudes.  The scales leave in the epilogue.
 //    A logit is then off by up to 2^-38 D max|x| max|w| beside the 2^-21 of its own products, and only its absolute error counts
-//    in a softmax: pairs are used while that stays below 2^-16 (lt_wide; roundings that do not all go the same way leave some 2^-23).  A single
-//    huge value - in a class that a bias of -inf takes out, or a channel that the other side leaves at zero - would cost all
-//    other logits their digits; where the largest magnitudes allow that, lce_mid_kernel multiplies triples of bf16 instead,
-//    which have f32's range.  Both launches are enqueued and the device decides, so the host does not wait for the maxima.
+//    in a softmax: pairs are used while that stays below 2^-16 (lt_wide; roundings that do not all go the same way leave some
+//    2^-23).  A single huge value - in a class that a bias of -inf takes out, or a channel that the other side leaves at zero -
+//    would cost all other logits their digits; where the largest magnitudes allow that, lce_mid_kernel multiplies triples of
+//    bf16 instead, which have f32's range.  Both launches are enqueued and the device decides, so the host does not wait for
+//    the maxima.
 //  * dx, dw: the sums run over the vocabulary and over the rows, where dz spans many orders of magnitude (a rare word's
 //    gradient is a sum of tiny ones), so f16's range is not enough: three bf16 planes hold all 24 bits (each the leading 8 bits
 //    of what the planes before leave), and six of the nine products are taken; the others are below 2^-21.
@@ -271,8 +272,8 @@ __device__ __forceinline__ int lt_width(const lt_prob& p, int n) {
 
 // How the nkb k-blocks of a tile are cut into accumulators: their number, and the k-blocks of accumulator sg.  Pairs have two
 // accumulators in tensor memory, and the epilogue of the tile before (3,500 cycles) lasts longer than the products of two k-blocks
-// (3,072); so of 8 k-blocks and more the first two accumulators take two each: loss of 1024x768x50257
-// 280 -> 266 us, of 4096 rows 818 to 857 -> 752 to 781; dx 4.0e-7 -> 6.5e-7 at worst (2500x512x300; f32 operations 9.9e-7).
+// (1,536 each); so of 8 k-blocks and more the first two accumulators take two each: loss of 1024x768x50257 280 -> 266 us, of 4096
+// rows 818 to 857 -> 752 to 781; dx 4.0e-7 -> 6.5e-7 at worst (2500x512x300; f32 operations 9.9e-7).
 template <int PLANES, bool CUT>
 __device__ __forceinline__ int lt_segs(const lt_args& e, int nkb) {
     if (!CUT) return 1;
